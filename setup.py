@@ -37,6 +37,9 @@ setup(
             name="mia_train_b200._C",
             sources=sources,
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+            # The shared C++ runtime that PyTorch itself uses. A toolchain that finds only the static one
+            # would link a second copy, whose streams crash as soon as an error message formats a number.
+            extra_link_args=["-l:libstdc++.so.6"],
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
