@@ -93,6 +93,8 @@ void koleo_bwd(at::Tensor x, at::Tensor xn, at::Tensor nn, at::Tensor dist, doub
 at::Tensor axial_angles_fwd(at::Tensor coords, std::vector<at::Tensor> freqs);
 void axial_angles_bwd(at::Tensor dangles, at::Tensor coords, std::vector<at::Tensor> freqs,
                       std::vector<at::Tensor> dfreqs);
+void dropout_apply(at::Tensor x, c10::optional<at::Tensor> residual, at::Tensor y, int64_t dropped,
+                   c10::optional<at::Tensor> rng, c10::optional<at::Tensor> record);
 }  // namespace mia
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -157,5 +159,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_gemm_pair_mode", &mia::set_gemm_pair_mode, "0: single-CTA GEMM tiles; else CTA pairs when M >= 256; returns the previous mode");
   m.def("axial_angles_fwd", &mia::axial_angles_fwd, "angles[r, p] = coords[r, axis(p)] * freq(p)");
   m.def("axial_angles_bwd", &mia::axial_angles_bwd, "accumulate the frequency gradients of axial_angles_fwd");
+  m.def("dropout_apply", &mia::dropout_apply, "counter-based dropout (+ residual); no mask is stored");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }
