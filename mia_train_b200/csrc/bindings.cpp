@@ -95,6 +95,12 @@ void axial_angles_bwd(at::Tensor dangles, at::Tensor coords, std::vector<at::Ten
                       std::vector<at::Tensor> dfreqs);
 void dropout_apply(at::Tensor x, c10::optional<at::Tensor> residual, at::Tensor y, int64_t dropped,
                    c10::optional<at::Tensor> rng, c10::optional<at::Tensor> record);
+void qk_norm_fwd(at::Tensor q, at::Tensor k, c10::optional<at::Tensor> qw, c10::optional<at::Tensor> kw,
+                 c10::optional<at::Tensor> angles, at::Tensor pairs, at::Tensor yq, at::Tensor yk, double eps);
+void qk_norm_bwd(at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k, c10::optional<at::Tensor> qw,
+                 c10::optional<at::Tensor> kw, c10::optional<at::Tensor> angles, at::Tensor pairs, at::Tensor dq,
+                 at::Tensor dk, c10::optional<at::Tensor> dqw, c10::optional<at::Tensor> dkw, int64_t accumulate,
+                 c10::optional<at::Tensor> dangles, double eps);
 }  // namespace mia
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -160,5 +166,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("axial_angles_fwd", &mia::axial_angles_fwd, "angles[r, p] = coords[r, axis(p)] * freq(p)");
   m.def("axial_angles_bwd", &mia::axial_angles_bwd, "accumulate the frequency gradients of axial_angles_fwd");
   m.def("dropout_apply", &mia::dropout_apply, "counter-based dropout (+ residual); no mask is stored");
+  m.def("qk_norm_fwd", &mia::qk_norm_fwd, "RMS norm of q and k heads + position rotation");
+  m.def("qk_norm_bwd", &mia::qk_norm_bwd, "gradients of qk_norm_fwd (q, k, weights, angles); dq / dk may alias the incoming gradients");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }

@@ -1,0 +1,448 @@
+// RMS norm of every query and key head with its learned weight, and the position rotation, in one
+// pass; forward and backward.
+//
+//   r = 1 / sqrt(mean_c x[c]^2 + eps),  n[c] = x[c] r w[c]
+//   y[i] = n[i] cos a_p - n[j] sin a_p,  y[j] = n[j] cos a_p + n[i] sin a_p     for pair p = (i, j)
+//   y[c] = n[c]                                                                for unpaired channels
+//
+// With C[c] = cos a_p and S[c] = -sin a_p (c first of its pair) or +sin a_p (second), and c' the
+// partner of c (C = 1, S = 0 when there is none): y[c] = n[c] C[c] + n[c'] S[c]. Backward:
+//   dn[c] = dy[c] C[c] - dy[c'] S[c]
+//   dw[c] += dn[c] x[c] r                       (over all heads of all tokens)
+//   dx[c] = r (g[c] - x[c] r mean_c(g x r)),    g = dn w
+//   da_p  = n[i] dn[j] - n[j] dn[i], summed over the token's query and key heads; dn[c'] needs only
+//           dy[c'] C[c] + dy[c] S[c], which the lane of c has, so each lane adds +-n[c] dn[c'] alone
+//
+// One warp per token. The sine and cosine of the token's angles are computed once and kept by every
+// lane for its eight channels; the warp then walks the token's query and key heads, 256 / D' of them
+// at a time (D' = D rounded up to a power of two, D' / 8 lanes a head), 16 bytes a lane. Partners are
+// exchanged through shared memory at index c + c / 8, which spreads the stride of eight between lanes
+// over all banks. Each element is read once and written once: the kernels are bound by HBM.
+// Weight gradients: registers over a warp's tokens, one partial a CTA, summed in a fixed order by a
+// second kernel, so the result does not depend on the order in which CTAs run.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "common.cuh"
+#include "vec8.cuh"
+
+namespace mia {
+
+constexpr int kQkWarps = 4;
+constexpr int kQkMaxD = 256;
+
+struct HeadView {  // (B, T, H, D) with unit channel stride; strides in elements
+  void* p;
+  int64_t sb, st, sh;
+  int heads;
+};
+
+struct QkNormParams {
+  HeadView x[2];   // q, k (input)
+  HeadView dy[2];  // gradients of the outputs (backward)
+  HeadView y[2];   // outputs (forward: rotated; backward: dx)
+  const float* w[2];
+  const float* angles;  // (1 or B, T, P) or nullptr
+  int64_t angle_bstride;
+  const int* pairs;  // (P, 2)
+  int P;
+  float* dangles;   // (B, T, P) or nullptr
+  float* dw_parts;  // (CTAs, 2, D) or nullptr
+  int B, T, D;
+  float eps;
+};
+
+__device__ __forceinline__ int qk_pad(int c) { return c + (c >> 3); }
+
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T* head_ptr(const HeadView& v, int64_t b, int64_t t, int h) {
+  return reinterpret_cast<T*>(v.p) + b * v.sb + t * v.st + h * v.sh;
+}
+
+// Shared memory of one CTA: the partner of each channel and the sign of its contribution to the
+// angle gradient, then per warp the token's (C, S) table and the exchange rows.
+template <int LPR>
+struct QkSmem {
+  static constexpr int kRows = 32 / LPR;             // heads a warp holds at a time
+  static constexpr int kCh = LPR * 8;                // channels of a head, rounded up
+  static constexpr int kRowFloats = kCh + LPR;       // padded exchange row
+  float2 cs[kQkWarps][kCh];
+  float ex[kQkWarps][kRows][kRowFloats];
+  int partner[kCh];
+  float sign[kCh];
+};
+
+// Fills partner / sign; a pair that names a channel outside the head is left out.
+template <int LPR>
+__device__ __forceinline__ void qk_partners(QkSmem<LPR>& sm, const QkNormParams& p) {
+  for (int c = threadIdx.x; c < QkSmem<LPR>::kCh; c += blockDim.x) {
+    sm.partner[c] = c;
+    sm.sign[c] = 0.f;
+  }
+  __syncthreads();
+  if (p.angles != nullptr)
+    for (int i = threadIdx.x; i < p.P; i += blockDim.x) {
+      const int a = p.pairs[2 * i], b = p.pairs[2 * i + 1];
+      if ((unsigned)a < (unsigned)p.D && (unsigned)b < (unsigned)p.D && a != b) {
+        sm.partner[a] = b;
+        sm.partner[b] = a;
+        sm.sign[a] = 1.f;
+        sm.sign[b] = -1.f;
+      }
+    }
+  __syncthreads();
+}
+
+// The (C, S) table of token (b, t), by one warp.
+template <int LPR>
+__device__ __forceinline__ void qk_table(QkSmem<LPR>& sm, const QkNormParams& p, int warp, int lane, int64_t b,
+                                         int64_t t) {
+  __syncwarp();
+  for (int c = lane; c < QkSmem<LPR>::kCh; c += 32) sm.cs[warp][c] = make_float2(1.f, 0.f);
+  __syncwarp();
+  if (p.angles != nullptr) {
+    const float* ang = p.angles + b * p.angle_bstride + t * p.P;
+    for (int i = lane; i < p.P; i += 32) {
+      const int a = p.pairs[2 * i], c = p.pairs[2 * i + 1];
+      if ((unsigned)a < (unsigned)p.D && (unsigned)c < (unsigned)p.D && a != c) {
+        float s, co;
+        sincosf(ang[i], &s, &co);
+        sm.cs[warp][a] = make_float2(co, -s);
+        sm.cs[warp][c] = make_float2(co, s);
+      }
+    }
+  }
+  __syncwarp();
+}
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_fwd_kernel(const QkNormParams p) {
+  using S = QkSmem<LPR>;
+  __shared__ S sm;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int row = lane / LPR, cg = lane % LPR;
+  const bool on = cg * 8 < p.D;
+  qk_partners<LPR>(sm, p);
+  const int64_t token = (int64_t)blockIdx.x * kQkWarps + warp;
+  if (token >= (int64_t)p.B * p.T) return;
+  const int64_t b = token / p.T, t = token % p.T;
+  qk_table<LPR>(sm, p, warp, lane, b, t);
+  float C[8], Sn[8];
+  int part[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 v = sm.cs[warp][cg * 8 + j];
+    C[j] = v.x;
+    Sn[j] = v.y;
+    part[j] = qk_pad(sm.partner[cg * 8 + j]);
+  }
+  const float inv_d = 1.f / (float)p.D;
+  float* ex = sm.ex[warp][row];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
+    for (int h0 = 0; h0 < p.x[s].heads; h0 += S::kRows) {
+      const int h = h0 + row;
+      const bool live = on && h < p.x[s].heads;
+      float v[8] = {};
+      if (live) unpack8(load_raw8(head_ptr<const T>(p.x[s], b, t, h) + cg * 8), v);
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+      const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = v[j] * r * w[j];
+        ex[cg * 9 + j] = v[j];
+      }
+      __syncwarp();
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = fmaf(ex[part[j]], Sn[j], v[j] * C[j]);
+      __syncwarp();
+      if (live) store8(head_ptr<T>(p.y[s], b, t, h) + cg * 8, o);
+    }
+  }
+}
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_bwd_kernel(const QkNormParams p) {
+  using S = QkSmem<LPR>;
+  __shared__ S sm;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int row = lane / LPR, cg = lane % LPR;
+  const bool on = cg * 8 < p.D;
+  qk_partners<LPR>(sm, p);
+  int part[8];
+  float sign[8], w[2][8], dw[2][8] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    part[j] = qk_pad(sm.partner[cg * 8 + j]);
+    sign[j] = sm.sign[cg * 8 + j];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) w[s][j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
+  }
+  const float inv_d = 1.f / (float)p.D;
+  float* ex = sm.ex[warp][row];
+  const int64_t tokens = (int64_t)p.B * p.T;
+  for (int64_t token = (int64_t)blockIdx.x * kQkWarps + warp; token < tokens; token += (int64_t)gridDim.x * kQkWarps) {
+    const int64_t b = token / p.T, t = token % p.T;
+    qk_table<LPR>(sm, p, warp, lane, b, t);
+    float C[8], Sn[8], da[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 v = sm.cs[warp][cg * 8 + j];
+      C[j] = v.x;
+      Sn[j] = v.y;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      for (int h0 = 0; h0 < p.x[s].heads; h0 += S::kRows) {
+        const int h = h0 + row;
+        const bool live = on && h < p.x[s].heads;
+        float v[8] = {}, g[8] = {};
+        if (live) {
+          const Raw8<T> xr = load_raw8(head_ptr<const T>(p.x[s], b, t, h) + cg * 8);
+          unpack8(load_raw8(head_ptr<const T>(p.dy[s], b, t, h) + cg * 8), g);
+          unpack8(xr, v);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          ss = fmaf(v[j], v[j], ss);
+          ex[cg * 9 + j] = g[j];
+        }
+        const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
+        __syncwarp();
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float other = ex[part[j]];
+          const float dn = fmaf(-other, Sn[j], g[j] * C[j]);
+          const float dn_other = fmaf(g[j], Sn[j], other * C[j]);
+          v[j] *= r;  // normalised
+          da[j] = fmaf(sign[j] * v[j] * w[s][j], dn_other, da[j]);
+          dw[s][j] = fmaf(dn, v[j], dw[s][j]);
+          g[j] = dn * w[s][j];
+          dot = fmaf(g[j], v[j], dot);
+        }
+        const float m = group_sum<LPR>(dot) * inv_d;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = r * fmaf(-v[j], m, g[j]);
+        __syncwarp();
+        if (live) store8(head_ptr<T>(p.y[s], b, t, h) + cg * 8, g);
+      }
+    }
+    if (p.dangles != nullptr) {
+      // the rows of the warp hold parts of the same channels: add them, then the two channels of a pair
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int o = LPR; o < 32; o <<= 1) da[j] += __shfl_xor_sync(0xffffffffu, da[j], o);
+        if (row == 0) sm.ex[warp][0][cg * 9 + j] = da[j];
+      }
+      __syncwarp();
+      float* out = p.dangles + token * p.P;
+      for (int i = lane; i < p.P; i += 32) {
+        const int a = p.pairs[2 * i], c = p.pairs[2 * i + 1];
+        const bool ok = (unsigned)a < (unsigned)p.D && (unsigned)c < (unsigned)p.D && a != c;
+        out[i] = ok ? sm.ex[warp][0][qk_pad(a)] + sm.ex[warp][0][qk_pad(c)] : 0.f;
+      }
+    }
+  }
+  if (p.dw_parts != nullptr) {
+    // rows of a warp by shuffles, warps through shared memory in warp order
+    float* red = reinterpret_cast<float*>(&sm.cs[0][0]);  // kQkWarps x kCh floats of the table's float2s
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int o = LPR; o < 32; o <<= 1) dw[s][j] += __shfl_xor_sync(0xffffffffu, dw[s][j], o);
+        if (row == 0) red[warp * S::kCh + cg * 8 + j] = dw[s][j];
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.D; c += blockDim.x) {
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < kQkWarps; ++k) a += red[k * S::kCh + c];
+        p.dw_parts[((int64_t)blockIdx.x * 2 + s) * p.D + c] = a;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// out[s][c] (+)= sum over CTAs of parts[cta][s][c], in a fixed order. One CTA of 32 x 8 threads for
+// 32 channels of one of the two weights.
+__global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ parts, int ctas, int D, float* dq,
+                                                         float* dk, int accumulate) {
+  __shared__ float red[8][32];
+  const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const int c = blockIdx.x * 32 + lane, s = blockIdx.y;
+  float a = 0.f;
+  if (c < D)
+    for (int k = slice; k < ctas; k += 8) a += parts[((int64_t)k * 2 + s) * D + c];
+  red[slice][lane] = a;
+  __syncthreads();
+  float* out = s == 0 ? dq : dk;
+  if (slice == 0 && c < D && out != nullptr) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) a += red[k][lane];
+    out[c] = (accumulate >> s & 1) ? out[c] + a : a;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+static HeadView head_view(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 4 && t.scalar_type() == like.scalar_type() &&
+                  t.size(0) == like.size(0) && t.size(1) == like.size(1) && t.size(3) == like.size(3),
+              "qk_norm: ", what, " must be a (B, T, H, D) tensor of the query's batch, length, head size and type");
+  const int64_t e = 16 / (int64_t)t.element_size();
+  auto vec = [&](int64_t stride, int64_t size) { return size <= 1 || stride % e == 0; };
+  TORCH_CHECK(t.stride(3) == 1 && vec(t.stride(0), t.size(0)) && vec(t.stride(1), t.size(1)) &&
+                  vec(t.stride(2), t.size(2)) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+              "qk_norm: ", what, " must have 16-byte aligned heads of contiguous channels");
+  return HeadView{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), (int)t.size(2)};
+}
+
+static QkNormParams qk_params(const torch::Tensor& q, const torch::Tensor& k, const c10::optional<torch::Tensor>& qw,
+                              const c10::optional<torch::Tensor>& kw, const c10::optional<torch::Tensor>& angles,
+                              const torch::Tensor& pairs, double eps) {
+  QkNormParams p{};
+  TORCH_CHECK(q.dim() == 4 && q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= kQkMaxD,
+              "qk_norm: head size must be a multiple of 8 up to ", kQkMaxD);
+  TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "qk_norm: batch or length too large");
+  p.x[0] = head_view(q, q, "q");
+  p.x[1] = head_view(k, q, "k");
+  p.B = (int)q.size(0);
+  p.T = (int)q.size(1);
+  p.D = (int)q.size(3);
+  p.eps = (float)eps;
+  const c10::optional<torch::Tensor>* ws[2] = {&qw, &kw};
+  for (int s = 0; s < 2; ++s) {
+    if (!ws[s]->has_value()) continue;
+    const torch::Tensor& w = **ws[s];
+    TORCH_CHECK(w.device() == q.device() && w.scalar_type() == at::kFloat && w.is_contiguous() && w.numel() == p.D,
+                "qk_norm: weights must be contiguous fp32 vectors of the head size");
+    p.w[s] = w.data_ptr<float>();
+  }
+  TORCH_CHECK(pairs.device() == q.device() && pairs.scalar_type() == at::kInt && pairs.is_contiguous() &&
+                  pairs.dim() == 2 && pairs.size(1) == 2,
+              "qk_norm: pairs must be a contiguous int32 (P, 2) tensor");
+  p.P = (int)pairs.size(0);
+  TORCH_CHECK(p.P <= p.D / 2, "qk_norm: at most D / 2 pairs");
+  p.pairs = pairs.data_ptr<int>();
+  if (angles.has_value() && p.P > 0) {
+    TORCH_CHECK(angles->device() == q.device() && angles->scalar_type() == at::kFloat && angles->is_contiguous() &&
+                    angles->dim() == 3 && (angles->size(0) == 1 || angles->size(0) == p.B) &&
+                    angles->size(1) == p.T && angles->size(2) == p.P,
+                "qk_norm: angles must be contiguous fp32 (1 or B, T, P)");
+    p.angles = angles->data_ptr<float>();
+    p.angle_bstride = angles->size(0) == 1 ? 0 : (int64_t)p.T * p.P;
+  }
+  return p;
+}
+
+template <typename F>
+static void qk_dispatch(const torch::Tensor& q, int D, F&& f) {
+  auto by_lanes = [&](auto type) {
+    if (D <= 32) f(type, std::integral_constant<int, 4>{});
+    else if (D <= 64) f(type, std::integral_constant<int, 8>{});
+    else if (D <= 128) f(type, std::integral_constant<int, 16>{});
+    else f(type, std::integral_constant<int, 32>{});
+  };
+  if (q.scalar_type() == at::kBFloat16) by_lanes(__nv_bfloat16{});
+  else if (q.scalar_type() == at::kHalf) by_lanes(__half{});
+  else if (q.scalar_type() == at::kFloat) by_lanes(float{});
+  else TORCH_CHECK(false, "qk_norm: bf16, fp16 or fp32 expected");
+}
+
+void qk_norm_fwd(torch::Tensor q, torch::Tensor k, c10::optional<torch::Tensor> qw, c10::optional<torch::Tensor> kw,
+                 c10::optional<torch::Tensor> angles, torch::Tensor pairs, torch::Tensor yq, torch::Tensor yk,
+                 double eps) {
+  QkNormParams p = qk_params(q, k, qw, kw, angles, pairs, eps);
+  p.y[0] = head_view(yq, q, "the output of q");
+  p.y[1] = head_view(yk, q, "the output of k");
+  TORCH_CHECK(p.y[0].heads == p.x[0].heads && p.y[1].heads == p.x[1].heads, "qk_norm: output head counts");
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t tokens = (int64_t)p.B * p.T;
+  if (tokens == 0) return;
+  const int64_t blocks = (tokens + kQkWarps - 1) / kQkWarps;
+  TORCH_CHECK(blocks <= INT32_MAX, "qk_norm: too many tokens");
+  qk_dispatch(q, p.D, [&](auto type, auto lanes) {
+    qk_norm_fwd_kernel<decltype(type), decltype(lanes)::value><<<(unsigned)blocks, 32 * kQkWarps, 0, stream>>>(p);
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// dq / dk may be the very tensors dyq / dyk (each lane reads its channels before it writes them).
+// dqw / dkw (fp32, D) are overwritten, or added to where `accumulate` has bit 0 / bit 1.
+void qk_norm_bwd(torch::Tensor dyq, torch::Tensor dyk, torch::Tensor q, torch::Tensor k,
+                 c10::optional<torch::Tensor> qw, c10::optional<torch::Tensor> kw, c10::optional<torch::Tensor> angles,
+                 torch::Tensor pairs, torch::Tensor dq, torch::Tensor dk, c10::optional<torch::Tensor> dqw,
+                 c10::optional<torch::Tensor> dkw, int64_t accumulate, c10::optional<torch::Tensor> dangles,
+                 double eps) {
+  QkNormParams p = qk_params(q, k, qw, kw, angles, pairs, eps);
+  p.dy[0] = head_view(dyq, q, "the gradient of q's output");
+  p.dy[1] = head_view(dyk, q, "the gradient of k's output");
+  p.y[0] = head_view(dq, q, "dq");
+  p.y[1] = head_view(dk, q, "dk");
+  for (int s = 0; s < 2; ++s)
+    TORCH_CHECK(p.dy[s].heads == p.x[s].heads && p.y[s].heads == p.x[s].heads, "qk_norm: gradient head counts");
+  float* dws[2] = {nullptr, nullptr};
+  const c10::optional<torch::Tensor>* dwt[2] = {&dqw, &dkw};
+  for (int s = 0; s < 2; ++s) {
+    if (!dwt[s]->has_value()) continue;
+    const torch::Tensor& w = **dwt[s];
+    TORCH_CHECK(w.device() == q.device() && w.scalar_type() == at::kFloat && w.is_contiguous() && w.numel() == p.D,
+                "qk_norm: weight gradients must be contiguous fp32 vectors of the head size");
+    dws[s] = w.data_ptr<float>();
+  }
+  if (dangles.has_value() && p.angles != nullptr) {
+    TORCH_CHECK(dangles->device() == q.device() && dangles->scalar_type() == at::kFloat && dangles->is_contiguous() &&
+                    dangles->numel() == (int64_t)p.B * p.T * p.P,
+                "qk_norm: dangles must be contiguous fp32 (B, T, P)");
+    p.dangles = dangles->data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t tokens = (int64_t)p.B * p.T;
+  const bool want_dw = dws[0] != nullptr || dws[1] != nullptr;
+  if (tokens == 0) {
+    for (int s = 0; s < 2; ++s)
+      if (dws[s] != nullptr && !(accumulate >> s & 1)) C10_CUDA_CHECK(cudaMemsetAsync(dws[s], 0, 4 * p.D, stream));
+    return;
+  }
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int blocks = (int)std::min<int64_t>((tokens + kQkWarps - 1) / kQkWarps, 4 * sms);
+  torch::Tensor parts;
+  if (want_dw) {
+    parts = torch::empty({blocks, 2, p.D}, q.options().dtype(at::kFloat));
+    p.dw_parts = parts.data_ptr<float>();
+  }
+  qk_dispatch(q, p.D, [&](auto type, auto lanes) {
+    qk_norm_bwd_kernel<decltype(type), decltype(lanes)::value><<<blocks, 32 * kQkWarps, 0, stream>>>(p);
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (want_dw) {
+    qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, stream>>>(p.dw_parts, blocks, p.D, dws[0], dws[1],
+                                                                    (int)accumulate);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+}
+
+}  // namespace mia
