@@ -101,6 +101,12 @@ void qk_norm_bwd(at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k, c10
                  c10::optional<at::Tensor> kw, c10::optional<at::Tensor> angles, at::Tensor pairs, at::Tensor dq,
                  at::Tensor dk, c10::optional<at::Tensor> dqw, c10::optional<at::Tensor> dkw, int64_t accumulate,
                  c10::optional<at::Tensor> dangles, double eps);
+void fp8_quantize(at::Tensor x, c10::optional<at::Tensor> aux, c10::optional<at::Tensor> gamma, bool block, bool e5m2,
+                  c10::optional<at::Tensor> q, c10::optional<at::Tensor> q_scale, c10::optional<at::Tensor> qt,
+                  c10::optional<at::Tensor> qt_scale, c10::optional<at::Tensor> sums, bool accumulate);
+void fp8_gemm(at::Tensor a, at::Tensor a_scale, bool a_block, at::Tensor b, at::Tensor b_scale, bool b_block, int64_t k,
+              at::Tensor d, c10::optional<at::Tensor> bias, c10::optional<at::Tensor> residual,
+              c10::optional<at::Tensor> gamma, c10::optional<at::Tensor> aux_out, int64_t act, bool accumulate);
 }  // namespace mia
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -168,5 +174,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout_apply", &mia::dropout_apply, "counter-based dropout (+ residual); no mask is stored");
   m.def("qk_norm_fwd", &mia::qk_norm_fwd, "RMS norm of q and k heads + position rotation");
   m.def("qk_norm_bwd", &mia::qk_norm_bwd, "gradients of qk_norm_fwd (q, k, weights, angles); dq / dk may alias the incoming gradients");
+  m.def("fp8_quantize", &mia::fp8_quantize, "8-bit values with power-of-two block scales, row- and column-wise, + column sums");
+  m.def("fp8_gemm", &mia::fp8_gemm, "8-bit tcgen05 GEMM with a scale per block of 128 along K and fused epilogue");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }

@@ -505,14 +505,15 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// 2-D bf16 tensor map over a row-major (rows x inner) matrix with row stride `ld` elements.
-static CUtensorMap make_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows) {
+// 2-D tensor map over a row-major (rows x inner) matrix with row stride `ld` elements of `esize` bytes.
+static CUtensorMap make_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows,
+                            CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, int esize = 2) {
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * esize)};
   cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+  CUresult r = encode_fn()(&map, type, 2, const_cast<void*>(base), dims, strides, box,
                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with ", (int)r);
@@ -523,6 +524,10 @@ static int num_sms(int device);
 
 CUtensorMap make_bf16_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows) {
   return make_map(base, inner, rows, ld, box_inner, box_rows);
+}
+
+CUtensorMap make_u8_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows) {
+  return make_map(base, inner, rows, ld, box_inner, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
 int sm_count(int device) { return num_sms(device); }

@@ -123,7 +123,7 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, int m, int n
     }
     return;
   }
-  const bool full = (n + 32 <= p.N);
+  const bool full = n + 32 <= p.N && p.N % 8 == 0;  // 16-byte accesses (other widths: 8-bit GEMMs only)
   const size_t row = (size_t)m * p.N;
   if (p.bias != nullptr) {
     if (full) {
@@ -265,6 +265,8 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, int m, int n
 // 2-D bf16 tensor map over a row-major (rows x inner) matrix with row stride `ld` elements,
 // 128-byte swizzle, box (box_inner x box_rows). Defined in gemm.cu.
 CUtensorMap make_bf16_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows);
+// The same over 8-bit elements.
+CUtensorMap make_u8_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows);
 int sm_count(int device);
 
 }  // namespace mia

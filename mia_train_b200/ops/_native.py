@@ -91,6 +91,9 @@ ERROR_CODES = {
     101: "GEMM TMA producer wait",
     102: "GEMM MMA issuer wait",
     103: "GEMM epilogue wait",
+    111: "8-bit GEMM TMA producer wait",
+    112: "8-bit GEMM MMA issuer wait",
+    113: "8-bit GEMM epilogue wait",
     201: "attention barrier wait",
     301: "collective flag wait",
     401: "sharded-optimizer reduce-scatter barrier",
