@@ -107,6 +107,7 @@ void fp8_quantize(at::Tensor x, c10::optional<at::Tensor> aux, c10::optional<at:
 void fp8_gemm(at::Tensor a, at::Tensor a_scale, bool a_block, at::Tensor b, at::Tensor b_scale, bool b_block, int64_t k,
               at::Tensor d, c10::optional<at::Tensor> bias, c10::optional<at::Tensor> residual,
               c10::optional<at::Tensor> gamma, c10::optional<at::Tensor> aux_out, int64_t act, bool accumulate);
+int64_t set_fp8_tile(int64_t tile);
 }  // namespace mia
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -176,5 +177,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_bwd", &mia::qk_norm_bwd, "gradients of qk_norm_fwd (q, k, weights, angles); dq / dk may alias the incoming gradients");
   m.def("fp8_quantize", &mia::fp8_quantize, "8-bit values with power-of-two block scales, row- and column-wise, + column sums");
   m.def("fp8_gemm", &mia::fp8_gemm, "8-bit tcgen05 GEMM with a scale per block of 128 along K and fused epilogue");
+  m.def("set_fp8_tile", &mia::set_fp8_tile, "-1: tile of the 8-bit GEMM by its rule; 0: 128 x 128, 1: 256 x 256; returns the previous");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }

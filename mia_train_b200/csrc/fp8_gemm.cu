@@ -5,16 +5,22 @@
 // A (M, K) and B (N, K) are e4m3 or e5m2, both K-major, rows padded to 16 bytes. sA has one scale per
 // row and K block (or per 128 rows), sB one per 128 rows (weights) or one per row (weight gradients).
 //
-// CTA = 4 control warps (two idle) + 8 epilogue warps, one CTA per SM, persistent over 128 x 128 tiles:
-//   warp 0     TMA producer: 128 x 128-byte tiles of A and B into a ring of shared-memory stages.
-//   warp 1     MMA issuer: four K = 32 steps of tcgen05.mma (kind::f8f6f4) per K block into one of two
-//              TMEM accumulators, which holds the products of that K block alone.
-//   warps 4..  epilogue: read each K block's products with tcgen05.ld, multiply by the scales and add in
-//              fp32 registers (a warp owns 32 rows x 64 columns), while the tensor core fills the other
-//              accumulator; after the last block bias / GELU / LayerScale / residual / accumulate and
-//              the stores (`epilogue_chunk`). A lane prefetches its row's scale of the next K block; with
-//              a scale per row of B also its share of the warp's column scales, which the lanes pass on
-//              through a small double-buffered strip of shared memory that belongs to the warp alone.
+// CTA = 4 control warps (two idle) + 8 epilogue warps, one CTA per SM, persistent over output tiles of
+// 128 x 128, or 256 x 256 by a pair of CTAs (cta_group::2: each CTA holds its 128 rows of A and half of
+// B in its shared memory and its 128 rows of the products in its TMEM; the even CTA issues the MMAs):
+//   warp 0     TMA producer: 128-byte wide tiles of A and B into a ring of shared-memory stages.
+//   warp 1     MMA issuer: four K = 32 steps of tcgen05.mma (kind::f8f6f4) per K block into one of the
+//              TMEM units, which holds the products of that K block alone. One thread issues everything,
+//              so its instructions count: descriptors advance by additions.
+//   warps 4..  epilogue: read a unit with tcgen05.ld, multiply by the scales and add in fp32 registers
+//              (a warp owns 32 rows x BN / 2 columns) while the tensor core fills the other units. A lane
+//              fetches its row's scale two K blocks ahead; with a scale per row of B also its share
+//              of the warp's column scales, which the lanes pass on through a small double-buffered strip
+//              of shared memory that belongs to the warp alone.
+//              After the last block the warp adds the bias, applies GELU, rounds into 128-byte swizzled rows
+//              of shared memory and leaves the stores (or, to accumulate, the additions) to TMA while it goes
+//              on with the next tile. LayerScale, residual and odd widths take a second form, which turns
+//              the sums through shared memory so that four lanes hold 16 columns of one row.
 // The scales are applied in fp32 outside the tensor core, so they may be any fp32 numbers, and no sum
 // longer than 128 products is left to the tensor core's own accumulation.
 //
@@ -24,7 +30,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cfloat>
+#include <type_traits>
 
 #include "common.cuh"
 #include "errors.h"
@@ -47,72 +55,230 @@ struct Fp8Operands {
   int a_format, b_format;  // 0 = e4m3, 1 = e5m2
 };
 
-template <int BN, int STAGES>
+template <int CG, int BN, int STAGES>
 struct F8Smem {
-  static constexpr int kBTile = BN * kF8K;
+  static constexpr int kBTile = BN / CG * kF8K;
   static constexpr int kStage = kF8ATile + kBTile;
-  static constexpr int kScales = 2 * 4 * BN * 4;  // two strips of BN / 2 floats for each epilogue warp
-  static constexpr int kBytes = STAGES * kStage + kScales + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int kScales = kF8EpiWarps * 2 * (BN / 2) * 4;  // two strips for each epilogue warp
+  // Staging of the stores: BN / 128 boxes of 32 rows x 128 bytes for each epilogue warp.
+  static constexpr int kWarpStaging = BN / 128 * 4096;
+  static constexpr int kStaging = kF8EpiWarps * kWarpStaging;
+  static constexpr int kBytes = STAGES * kStage + kStaging + kScales + 1024 /*align*/ + 256 /*barriers*/;
 };
 
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t pack_u32x2(uint32_t a, uint32_t b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
+// One lane of a converged warp. Unlike a test of the lane index, the compiler knows that a single thread
+// passes it, and keeps the operands of the TMA and tcgen05 instructions behind it in uniform registers:
+// the four MMAs of a K block then issue in their execution time instead of about 140 cycles each.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 
-// mbar_wait by a whole warp. The lanes poll the barrier one by one and may see it complete in different
-// polls; the vote brings them together again before the warp-wide TMEM loads that follow.
+// A load that stays where it is written: the compiler would move a plain one down to its first use, behind
+// the waits it is meant to overlap.
+__device__ __forceinline__ float load_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+// A staged box to global memory (clipped at the tensor's edges), stored or added; bulk groups belong to
+// the thread that issues them.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// 16 lanes x 32 columns: thread t receives, of every eight columns g, columns 2 (t % 4) and + 1 of row t / 4
+// in r[4 g], r[4 g + 1] and of row t / 4 + 8 in r[4 g + 2], r[4 g + 3].
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) { tmem_ld_wait_regs(r); }
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) { tmem_ld_wait_regs16(r); }
+
+// Whether `bar` has completed phase `parity`, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait for a whole warp: one lane polls, the others take its answer and with it the ordering. Polling
+// with all lanes costs 32 barrier operations a try, and lanes that see the barrier complete in different
+// tries would have to be brought together before the warp-wide TMEM loads that follow.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
                                                int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+  int ok = 0;
+  if (threadIdx.x % 32 == 0) ok = mbar_wait(bar, parity, abort_flag, err, code) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-template <int BN, int STAGES, bool SB_ROW>
+// One K block: four steps of 32, the first of which overwrites D. A step of 32 bytes along the swizzled rows
+// adds 2 to the address field of either descriptor.
+#define MIA_MMA_F8_BLOCK(GROUP)                                                          \
+  asm volatile(                                                                          \
+      "{\n\t.reg .pred f, t;\n\t.reg .b64 a, b;\n\t"                                     \
+      "setp.ne.b32 f, 0, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"                                 \
+      "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %1, %2, %3, f;\n\t"           \
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"                                       \
+      "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a, b, %3, t;\n\t"             \
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"                                       \
+      "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a, b, %3, t;\n\t"             \
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"                                       \
+      "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a, b, %3, t;\n\t}" ::"r"(d_tmem), \
+      "l"(a_desc), "l"(b_desc), "r"(idesc))
+
+template <int CG>
+__device__ __forceinline__ void tc_mma_f8_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+  if constexpr (CG == 2) MIA_MMA_F8_BLOCK("2");
+  else MIA_MMA_F8_BLOCK("1");
+}
+
+// 128 accumulators a thread (BN = 256) need more than the 168 registers that 384 threads can start with:
+// the four control warps hand theirs down. 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kF8ControlRegs = 40, kF8EpilogueRegs = 232;
+static_assert(128 * kF8ControlRegs + 32 * kF8EpiWarps * kF8EpilogueRegs <= kF8Threads * 168, "register split");
+
+// Four columns n .. n + 3 of row m: bias, GELU (keeping the pre-activation), LayerScale, residual,
+// accumulation, store. `vec`: N % 4 == 0 and all four columns exist.
+__device__ __forceinline__ void fp8_store4(const GemmParams& p, int64_t m, int n, float4 acc, bool vec) {
+  float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  const int64_t at = m * p.N + n;
+  const int count = vec ? 4 : min(4, p.N - n);
+  auto vec_f32 = [&](const float* src, float (&o)[4]) {
+    if (vec) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(src));
+      o[0] = f.x; o[1] = f.y; o[2] = f.z; o[3] = f.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = j < count ? src[j] : 0.f;
+    }
+  };
+  auto load_bf16 = [&](const __nv_bfloat16* src, float (&o)[4]) {
+    if (vec) {
+      const uint2 u = *reinterpret_cast<const uint2*>(src);
+      o[0] = bf16_lo(u.x); o[1] = bf16_hi(u.x); o[2] = bf16_lo(u.y); o[3] = bf16_hi(u.y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = j < count ? __bfloat162float(src[j]) : 0.f;
+    }
+  };
+  auto store_bf16 = [&](__nv_bfloat16* dst) {
+    if (vec) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < count) dst[j] = __float2bfloat16_rn(v[j]);
+    }
+  };
+  float t[4];
+  if (p.bias != nullptr) {
+    vec_f32(p.bias + n, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += t[j];
+  }
+  if (p.act == kActGelu) {
+    if (p.aux_out != nullptr) store_bf16(p.aux_out + at);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = gelu_erf(v[j]);
+  }
+  if (p.gamma != nullptr) {
+    vec_f32(p.gamma + n, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= t[j];
+  }
+  if (p.residual != nullptr) {
+    load_bf16(p.residual + at, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += t[j];
+  }
+  if (p.d_fp32) {
+    float* dst = reinterpret_cast<float*>(p.D) + at;
+    if (vec) {
+      float4* d4 = reinterpret_cast<float4*>(dst);
+      if (p.accumulate) {
+        const float4 old = *d4;
+        v[0] += old.x; v[1] += old.y; v[2] += old.z; v[3] += old.w;
+      }
+      *d4 = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < count) dst[j] = p.accumulate ? dst[j] + v[j] : v[j];
+    }
+  } else {
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.D) + at;
+    if (p.accumulate) {
+      load_bf16(dst, t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += t[j];
+    }
+    store_bf16(dst);
+  }
+}
+
+template <int CG, int BN, int HALVES, int STAGES, bool SB_ROW, bool FULL>
 __global__ void __launch_bounds__(kF8Threads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux,
                     const GemmParams p, const Fp8Operands o) {
-  using L = F8Smem<BN, STAGES>;
+  using L = F8Smem<CG, BN, STAGES>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smA = smem;
   uint8_t* smB = smem + STAGES * kF8ATile;
-  float* smS = reinterpret_cast<float*>(smem + STAGES * L::kStage);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * L::kStage + L::kScales);
+  uint8_t* smT = smem + STAGES * L::kStage;
+  float* smS = reinterpret_cast<float*>(smT + L::kStaging);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smT + L::kStaging + L::kScales);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* tfull_bar = empty_bar + STAGES;           // [2]
-  uint64_t* tempty_bar = tfull_bar + 2;               // [2]
-  uint64_t* drain_bar = tempty_bar + 2;               // [1]
+  uint64_t* tfull_bar = empty_bar + STAGES;  // [kUnits]
+  uint64_t* tempty_bar = tfull_bar + 4;      // [kUnits]
+  uint64_t* drain_bar = tempty_bar + 4;      // [1]
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
-  constexpr uint32_t kTmemCols = 2 * BN;
+  const int rank = CG == 2 ? (int)cluster_ctarank() : 0;
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+  constexpr int kUnitCols = BN / HALVES;
+  constexpr int kUnits = 512 / kUnitCols < 4 ? 512 / kUnitCols : 4;
+  constexpr uint32_t kTmemCols = kUnits * kUnitCols;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], 1);
+      mbar_init(&full_bar[s], 1);   // the even CTA's producer announces the bytes of the pair
+      mbar_init(&empty_bar[s], 1);  // one commit of the MMA issuer, to both CTAs
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < kUnits; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], kF8EpiWarps);
+      mbar_init(&tempty_bar[a], CG * kF8EpiWarps / HALVES);  // the unit's epilogue warps of the pair, on the even CTA
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -121,31 +287,44 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     prefetch_tensormap(&tmB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_base_slot, kTmemCols);
-    tmem_relinquish();
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(tmem_base_slot, kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_base_slot, kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
   const int num_k = (p.K + kF8K - 1) / kF8K;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < kF8FirstEpi) {
+    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8ControlRegs));
+    if (warp == 0 && elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
-        const int m0 = (tile % p.num_m_tiles) * 128, n0 = (tile / p.num_m_tiles) * BN;
+      for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
+        const int m0 = (tile % p.num_m_tiles) * (128 * CG) + 128 * rank;
+        const int n0 = (tile / p.num_m_tiles) * BN + BN / CG * rank;
         for (int kb = 0; kb < num_k; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.err, kErrFp8ProducerWait)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full_bar[stage], L::kStage);
-          tma_load_2d(smA + stage * kF8ATile, &tmA, &full_bar[stage], kb * kF8K, m0);
-          tma_load_2d(smB + stage * L::kBTile, &tmB, &full_bar[stage], kb * kF8K, n0);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], CG * L::kStage);
+          if constexpr (CG == 2) {
+            tma_load_2d_pair(smA + stage * kF8ATile, &tmA, &full_bar[stage], kb * kF8K, m0);
+            tma_load_2d_pair(smB + stage * L::kBTile, &tmB, &full_bar[stage], kb * kF8K, n0);
+          } else {
+            tma_load_2d(smA + stage * kF8ATile, &tmA, &full_bar[stage], kb * kF8K, m0);
+            tma_load_2d(smB + stage * L::kBTile, &tmB, &full_bar[stage], kb * kF8K, n0);
+          }
           ++issued;
           if (++stage == STAGES) {
             stage = 0;
@@ -153,7 +332,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           }
         }
       }
-      if (!ok) {
+      if (!ok && rank == 0) {  // let the copies in flight land before this CTA's shared memory goes away
         int s = stage, ph = phase;
         for (int i = 0; i < STAGES && i < issued; ++i) {
           if (--s < 0) {
@@ -163,161 +342,403 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           mbar_wait(&full_bar[s], ph, nullptr, nullptr, 0);
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = make_idesc_f8(128, BN, o.a_format, o.b_format);
+    } else if (warp == 1 && rank == 0 && elect_one()) {
+      const uint32_t idesc = make_idesc_f8(128 * CG, kUnitCols, o.a_format, o.b_format);
+      const uint64_t a_desc0 = make_sdesc_sw128(smem_u32(smA), 16, 1024);
+      const uint64_t b_desc0 = make_sdesc_sw128(smem_u32(smB), 16, 1024);
+      uint64_t a_desc = a_desc0, b_desc = b_desc0;
+      uint32_t d_tmem = tmem_base;
       int stage = 0;
       uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
+      int unit = 0;
+      uint32_t unit_phase = 0;
       bool ok = true;
       bool any_mma = false;
-      for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < num_k; ++kb) {
-          if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.err, kErrFp8MmaWait) ||
-              !mbar_wait(&full_bar[stage], phase, abort_flag, p.err, kErrFp8MmaWait)) {
+      for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
+        for (int kb = 0; kb < num_k && ok; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.err, kErrFp8MmaWait)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t d_tmem = tmem_base + acc * BN;
-          const uint32_t a_base = smem_u32(smA + stage * kF8ATile);
-          const uint32_t b_base = smem_u32(smB + stage * L::kBTile);
 #pragma unroll
-          for (int k = 0; k < kF8K / 32; ++k)
-            tc_mma_f8(d_tmem, make_sdesc_sw128(a_base + k * 32, 16, 1024), make_sdesc_sw128(b_base + k * 32, 16, 1024),
-                      idesc, k > 0 ? 1u : 0u);
-          any_mma = true;
-          tc_commit(&empty_bar[stage]);
-          tc_commit(&tfull_bar[acc]);
+          for (int h = 0; h < HALVES; ++h) {
+            if (!mbar_wait(&tempty_bar[unit], unit_phase ^ 1, abort_flag, p.err, kErrFp8MmaWait)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            tc_mma_f8_block<CG>(d_tmem, a_desc, b_desc + h * ((kUnitCols / CG * kF8K) >> 4), idesc);
+            any_mma = true;
+            if constexpr (CG == 2) tc_commit_pair_both(&tfull_bar[unit]);
+            else tc_commit(&tfull_bar[unit]);
+            d_tmem += kUnitCols;
+            if (++unit == kUnits) {
+              unit = 0;
+              unit_phase ^= 1;
+              d_tmem = tmem_base;
+            }
+          }
+          if (!ok) break;
+          if constexpr (CG == 2) tc_commit_pair_both(&empty_bar[stage]);
+          else tc_commit(&empty_bar[stage]);
+          a_desc += kF8ATile >> 4;
+          b_desc += L::kBTile >> 4;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
+            a_desc = a_desc0;
+            b_desc = b_desc0;
           }
-          acc ^= 1;
-          if (acc == 0) acc_phase ^= 1;
         }
       }
       if (!ok && any_mma) {
-        tc_commit(drain_bar);
+        if constexpr (CG == 2) tc_commit_pair_both(drain_bar);
+        else tc_commit(drain_bar);
         mbar_wait(drain_bar, 0, nullptr, nullptr, 0);
       }
     }
-  } else if (warp >= kF8FirstEpi) {
-    const int lane_group = warp % 4;                     // TMEM lanes 32 * lane_group .. + 31
-    const int col_part = (warp - kF8FirstEpi) / 4;       // half of the tile's columns
+  } else {
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8EpilogueRegs));
+    const int lane_group = warp % 4;                // TMEM lanes 32 * lane_group .. + 31
+    const int part = (warp - kF8FirstEpi) / 4;
     constexpr int kCols = BN / 2;
-    constexpr int kChunks = kCols / 32;
+    // How a warp's 32 rows x kCols columns lie in its registers. With a scale per block: lane = row, 32 columns
+    // a load, so that a thread multiplies everything by one number. With a scale per column that layout would
+    // read kCols scales a thread from shared memory (at 128 bytes a cycle the whole SM twice the time of the
+    // MMAs), so a load brings 16 rows x 32 columns instead: a thread has two columns of every eight, in four rows.
+    constexpr int kWidth = SB_ROW ? 16 : 32;  // registers a load fills: two loads in flight fit beside the sums
+    constexpr int kChunks = kCols / kWidth;
+    constexpr int kRowsT = SB_ROW ? 4 : 1;    // rows a thread holds: 8 i + lane / 4, or its lane
+    const int row_t = SB_ROW ? lane / 4 : lane;
+    auto chunk_at = [](int c) { return SB_ROW ? (c / 2) * 32 + ((uint32_t)(c % 2 * 16) << 16) : c * 32; };  // TMEM offset
     constexpr int kLaneCols = kCols / 32;
+    // One unit: the warps' halves are its two column ranges. Two units (a 256-wide tile of a pair): unit h
+    // holds columns 64 h .. + 63 of the even CTA's 128 rows of B, then the same of the odd CTA's.
+    const int half = HALVES == 2 ? part : 0;
+    const int t_col = HALVES == 2 ? 0 : part * kCols;
+    const int n_col = HALVES == 2 ? half * 64 : part * kCols;
+    auto column = [](int c) { return HALVES == 2 && c >= 64 ? c + 64 : c; };  // of the warp's kCols
     float* strip = smS + (warp - kF8FirstEpi) * 2 * kCols;
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < p.num_tiles && ok; tile += gridDim.x) {
-      const int m = (tile % p.num_m_tiles) * 128 + lane_group * 32 + lane;
-      const int n0 = (tile / p.num_m_tiles) * BN + col_part * kCols;
-      const uint32_t t_row = tmem_base + ((uint32_t)(lane_group * 32) << 16) + col_part * kCols;
-      uint64_t sum[kCols / 2];
+    uint8_t* const staging = smT + (warp - kF8FirstEpi) * L::kWarpStaging;
+    int unit = half;
+    uint32_t unit_phase = 0;
+    bool ok = true, ready = false;
+    for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
+      const int m_warp = (tile % p.num_m_tiles) * (128 * CG) + 128 * rank + lane_group * 32;
+      const int n0 = (tile / p.num_m_tiles) * BN + n_col;
+      const uint32_t t_row = tmem_base + ((uint32_t)(lane_group * 32) << 16) + t_col;
+      float sum[kCols];
 #pragma unroll
-      for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
-      const bool live = m < p.M;
-      const float* sa = o.sa + (live ? (m >> o.sa_shift) : 0);
-      // SB_ROW: this lane fetches the scales of columns n0 + lane + 32 i
-      const float* sb = o.sb + (SB_ROW ? n0 + lane : min(n0, p.N - 1) >> 7);
-      float sa_next = live ? __ldg(sa) : 0.f;
-      float sb_next[kLaneCols];
+      for (int j = 0; j < kCols; ++j) sum[j] = 0.f;
+      // Scales: this row's, and of B either one per block the warp's columns lie in (one, or two with HALVES
+      // == 2) or, with a scale per row of B, those of columns n0 + column(32 i) + lane. Rows and columns past
+      // the edge fetch the last one: their sums are never stored.
+      constexpr int kSb = SB_ROW ? kLaneCols : HALVES;
+      const float* sa = o.sa;
+      int sa_at[kRowsT];
 #pragma unroll
-      for (int i = 0; i < kLaneCols; ++i)
-        sb_next[i] = SB_ROW ? (n0 + lane + 32 * i < p.N ? __ldg(sb + 32 * i) : 0.f) : (i == 0 ? __ldg(sb) : 0.f);
+      for (int i = 0; i < kRowsT; ++i) sa_at[i] = min(m_warp + row_t + 8 * i, p.M - 1) >> o.sa_shift;
+      const float* sb = o.sb;
+      int sb_at[kSb];
+#pragma unroll
+      for (int i = 0; i < kSb; ++i)
+        sb_at[i] = SB_ROW ? min(n0 + column(32 * i) + lane, p.N - 1) : min(n0 + 128 * i, p.N - 1) >> 7;
+      float sa_ahead[2][kRowsT], sb_ahead[2][kSb];  // of K blocks kb and kb + 1
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+#pragma unroll
+        for (int i = 0; i < kRowsT; ++i) sa_ahead[d][i] = load_now(sa + sa_at[i]);
+#pragma unroll
+        for (int i = 0; i < kSb; ++i) sb_ahead[d][i] = load_now(sb + sb_at[i]);
+        if (d + 1 < num_k) {
+          sa += o.sa_ld;
+          sb += o.sb_ld;
+        }
+      }
       for (int kb = 0; kb < num_k; ++kb) {
-        const float sa_now = sa_next, sb_now = sb_next[0];
-        const float* sbv = strip + (kb & 1) * kCols;
-        if (SB_ROW) {
-          // the strip of two K blocks ago: every lane has passed the barrier after reading it
-#pragma unroll
-          for (int i = 0; i < kLaneCols; ++i) strip[(kb & 1) * kCols + lane + 32 * i] = sb_next[i];
-          __syncwarp();
-        }
-        if (kb + 1 < num_k) {
-          if (live) sa_next = __ldg(sa + (kb + 1) * o.sa_ld);
-#pragma unroll
-          for (int i = 0; i < kLaneCols; ++i)
-            if (SB_ROW ? n0 + lane + 32 * i < p.N : i == 0) sb_next[i] = __ldg(sb + (kb + 1) * o.sb_ld + 32 * i);
-        }
-        if (!mbar_wait_warp(&tfull_bar[acc], acc_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
+        if (!ready && !mbar_wait_warp(&tfull_bar[unit], unit_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        float s = sa_now;
-        if (!SB_ROW) {
-          s = sa_now * sb_now;
-          s = s > FLT_MAX ? FLT_MAX : s;  // two huge scales over a zero product stay zero; NaN stays NaN
+        uint32_t r[2][kWidth];  // the next columns are on their way while these are added
+        const uint32_t t_unit = t_row + unit * kUnitCols;
+        tmem_load(t_unit, r[0]);
+        // behind the first load: this block's scales into place, those of two blocks on under way
+        float s1[SB_ROW ? kRowsT : kSb];
+        float* const sbv = strip + (kb & 1) * kCols;
+        if (SB_ROW) {
+#pragma unroll
+          for (int i = 0; i < kRowsT; ++i) s1[i] = sa_ahead[0][i];
+          // the strip of two K blocks ago: every lane has passed the barrier after reading it
+#pragma unroll
+          for (int i = 0; i < kSb; ++i) sbv[lane + 32 * i] = sb_ahead[0][i];
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (int i = 0; i < kSb; ++i) {
+            const float s = sa_ahead[0][0] * sb_ahead[0][i];
+            s1[i] = s > FLT_MAX ? FLT_MAX : s;  // two huge scales over a zero product stay zero; NaN stays NaN
+          }
         }
-        const uint64_t s2 = pack_f32x2(s, s);
+#pragma unroll
+        for (int i = 0; i < kRowsT; ++i) {
+          sa_ahead[0][i] = sa_ahead[1][i];
+          sa_ahead[1][i] = load_now(sa + sa_at[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kSb; ++i) {
+          sb_ahead[0][i] = sb_ahead[1][i];
+          sb_ahead[1][i] = load_now(sb + sb_at[i]);
+        }
+        if (kb + 3 < num_k) {
+          sa += o.sa_ld;
+          sb += o.sb_ld;
+        }
+        int next = unit + HALVES;
+        const uint32_t next_phase = next >= kUnits ? unit_phase ^ 1 : unit_phase;
+        next = next >= kUnits ? next - kUnits : next;
+        int seen = 0;
+        float2 bs[2][4];  // scales of this thread's columns of 32, fetched one step ahead as well
+        const float2* const my_scales = reinterpret_cast<const float2*>(sbv) + (lane & 3);
+        if (SB_ROW) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) bs[0][g] = my_scales[g * 4];
+        }
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(t_row + acc * BN + c * 32, r);
-          tmem_ld_wait_regs(r);
-          if (c == kChunks - 1) {
+          uint32_t(&now)[kWidth] = r[c & 1];
+          tmem_wait(now);
+          if (c + 1 < kChunks) {
+            tmem_load(t_unit + chunk_at(c + 1), r[(c + 1) & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty_bar[acc]);
+            if (lane == 0) {
+              if constexpr (CG == 2) mbar_arrive_cluster(&tempty_bar[unit], 0);
+              else mbar_arrive(&tempty_bar[unit]);
+              seen = mbar_test(&tfull_bar[next], next_phase) ? 1 : 0;  // answered while the last columns are added
+            }
           }
+          float* const x = sum + c * kWidth;
           if (SB_ROW) {
+            if (c % 2 == 0 && c + 2 < kChunks) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float4 b = reinterpret_cast<const float4*>(sbv)[c * 8 + q];
-              uint64_t& x = sum[c * 16 + 2 * q];
-              uint64_t& y = sum[c * 16 + 2 * q + 1];
-              x = fma_f32x2(mul_f32x2(pack_u32x2(r[4 * q], r[4 * q + 1]), s2), pack_f32x2(b.x, b.y), x);
-              y = fma_f32x2(mul_f32x2(pack_u32x2(r[4 * q + 2], r[4 * q + 3]), s2), pack_f32x2(b.z, b.w), y);
+              for (int g = 0; g < 4; ++g) bs[(c / 2 + 1) & 1][g] = my_scales[(c / 2 + 1) * 16 + g * 4];
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 b = bs[(c / 2) & 1][g];
+              const float lo = s1[(c % 2 * 2) % kRowsT], hi = s1[(c % 2 * 2 + 1) % kRowsT];
+              x[4 * g] = fmaf(__uint_as_float(now[(4 * g) % kWidth]) * lo, b.x, x[4 * g]);
+              x[4 * g + 1] = fmaf(__uint_as_float(now[(4 * g + 1) % kWidth]) * lo, b.y, x[4 * g + 1]);
+              x[4 * g + 2] = fmaf(__uint_as_float(now[(4 * g + 2) % kWidth]) * hi, b.x, x[4 * g + 2]);
+              x[4 * g + 3] = fmaf(__uint_as_float(now[(4 * g + 3) % kWidth]) * hi, b.y, x[4 * g + 3]);
             }
           } else {
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-              sum[c * 16 + q] = fma_f32x2(pack_u32x2(r[2 * q], r[2 * q + 1]), s2, sum[c * 16 + q]);
+            for (int q = 0; q < kWidth; ++q)
+              x[q] = fmaf(__uint_as_float(now[q]), s1[!SB_ROW && kSb == 2 ? c * kWidth / 64 : 0], x[q]);
           }
         }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        ready = __shfl_sync(0xffffffffu, seen, 0) != 0;
+        unit = next;
+        unit_phase = next_phase;
       }
       if (!ok) break;
+      if constexpr (!FULL) {
+        if (p.bias != nullptr) {
+          if (SB_ROW) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        uint32_t r[32];
+            for (int g = 0; g < kCols / 8; ++g) {  // eight columns: registers 32 (g / 4) + 4 (g % 4) .. + 3, and 16 on
+              const int n = n0 + column(g * 8) + (lane & 3) * 2;
+              const float2 v = n < p.N ? __ldg(reinterpret_cast<const float2*>(p.bias + n)) : make_float2(0.f, 0.f);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          r[2 * q] = (uint32_t)sum[c * 16 + q];
-          r[2 * q + 1] = (uint32_t)(sum[c * 16 + q] >> 32);
+              for (int i = 0; i < 4; ++i) {
+                float* x = sum + g / 4 * 32 + i / 2 * 16 + g % 4 * 4 + i % 2 * 2;
+                x[0] += v.x;
+                x[1] += v.y;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 4) {
+              const int n = n0 + column(c);
+              const float4 v = n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              sum[c] += v.x; sum[c + 1] += v.y; sum[c + 2] += v.z; sum[c + 3] += v.w;
+            }
+          }
         }
-        epilogue_chunk<kEpiAll>(p, m, n0 + c * 32, r);
+        // Boxes of 64 bf16 or 32 fp32 columns into 128-byte rows whose 16-byte pieces are XOR-swizzled with the
+        // row's low three bits, as the tensor maps expect, from column `first` of the warp's on.
+        constexpr int kBoxes = L::kWarpStaging / 4096;
+        auto stage = [&](const CUtensorMap* map, int first, auto wide, bool add) {
+          constexpr bool kF32 = decltype(wide)::value;
+          constexpr int kBoxCols = kF32 ? 32 : 64;
+          if (elect_one()) bulk_wait_read();  // the staging rows are free again
+          __syncwarp();
+#pragma unroll
+          for (int box = 0; box < kBoxes; ++box) {
+            uint8_t* const at = staging + box * 4096;
+            const float* const src = sum + first + box * kBoxCols;
+            if constexpr (SB_ROW) {
+#pragma unroll
+              for (int g = 0; g < kBoxCols / 8; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int row = i * 8 + lane / 4;
+                  const float* x = src + g / 4 * 32 + i / 2 * 16 + g % 4 * 4 + i % 2 * 2;
+                  if constexpr (kF32)
+                    *reinterpret_cast<float2*>(at + row * 128 + (((2 * g + (lane & 3) / 2) ^ (row & 7)) << 4) +
+                                               (lane & 1) * 8) = make_float2(x[0], x[1]);
+                  else
+                    *reinterpret_cast<uint32_t*>(at + row * 128 + ((g ^ (row & 7)) << 4) + (lane & 3) * 4) =
+                        pack_bf16x2(x[0], x[1]);
+                }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                uint4 u;
+                if constexpr (kF32) {
+                  const float* x = src + j * 4;
+                  u = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                } else {
+                  const float* x = src + j * 8;
+                  u = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                 pack_bf16x2(x[6], x[7]));
+                }
+                *reinterpret_cast<uint4*>(at + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+#pragma unroll
+            for (int box = 0; box < kBoxes; ++box) {
+              const int n = n0 + column(first + box * kBoxCols);
+              if (n < p.N && m_warp < p.M) {
+                if (add) tma_add_2d(map, staging + box * 4096, n, m_warp);
+                else tma_store_2d(map, staging + box * 4096, n, m_warp);
+              }
+            }
+            bulk_commit();
+          }
+        };
+        if (p.act == kActGelu) {
+          if (p.aux_out != nullptr) stage(&tmAux, 0, std::false_type{}, false);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) sum[c] = gelu_erf(sum[c]);
+        }
+        if (p.d_fp32) {
+          stage(&tmD, 0, std::true_type{}, p.accumulate != 0);
+          stage(&tmD, kCols / 2, std::true_type{}, p.accumulate != 0);
+        } else {
+          stage(&tmD, 0, std::false_type{}, false);
+        }
+      } else {
+        // 16 columns at a time as 64-byte rows, their 16-byte pieces XOR-swizzled so that no access meets a bank
+        // conflict; then lane = (row of eight, four columns)
+        const bool n_vec = p.N % 4 == 0;
+        const int row0 = m_warp + lane / 4, rows_left = p.M - row0;
+        const float4* const take =
+            reinterpret_cast<const float4*>(staging) + (lane / 4) * 4 + ((lane & 3) ^ ((lane >> 3) & 3));
+        const int n_lane = n0 + (lane & 3) * 4;
+#pragma unroll
+        for (int c = 0; c < kCols / 16; ++c) {
+          __syncwarp();
+          if constexpr (SB_ROW) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = i * 8 + lane / 4;
+                const float* x = sum + c / 2 * 32 + i / 2 * 16 + (c % 2 * 2 + g) * 4 + i % 2 * 2;
+                *reinterpret_cast<float2*>(staging + row * 64 + (((2 * g + (lane & 3) / 2) ^ ((row >> 1) & 3)) << 4) +
+                                           (lane & 1) * 8) = make_float2(x[0], x[1]);
+              }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float* x = sum + c * 16 + 4 * q;
+              reinterpret_cast<float4*>(staging)[lane * 4 + (q ^ ((lane >> 1) & 3))] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          __syncwarp();
+          float4 v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = take[q * 32];
+          const int n = n_lane + column(c * 16);
+          if (n >= p.N) continue;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q)
+            if (8 * q < rows_left) fp8_store4(p, row0 + 8 * q, n, q == 0 ? v[0] : q == 1 ? v[1] : q == 2 ? v[2] : v[3], n_vec);
+        }
       }
     }
+    if (!FULL && elect_one()) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the peer no longer reads this CTA's shared memory or signals its barriers
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, kTmemCols);
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, kTmemCols);
+    else tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
 // ------------------------------------------------------------------------------------------ host
 
-template <int BN, int STAGES, bool SB_ROW>
-static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, GemmParams& p, const Fp8Operands& o, int device,
+template <int CG, int BN, int HALVES, int STAGES, bool SB_ROW, bool FULL>
+static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
+                       const CUtensorMap& taux, GemmParams& p, const Fp8Operands& o, int device,
                        cudaStream_t stream) {
-  using L = F8Smem<BN, STAGES>;
-  auto kern = fp8_gemm_kernel<BN, STAGES, SB_ROW>;
+  using L = F8Smem<CG, BN, STAGES>;
+  auto kern = fp8_gemm_kernel<CG, BN, HALVES, STAGES, SB_ROW, FULL>;
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-  p.num_m_tiles = (p.M + 127) / 128;
+  p.num_m_tiles = (p.M + 128 * CG - 1) / (128 * CG);
   p.num_n_tiles = (p.N + BN - 1) / BN;
   p.num_tiles = p.num_m_tiles * p.num_n_tiles;
-  kern<<<std::min(p.num_tiles, sm_count(device)), kF8Threads, L::kBytes, stream>>>(ta, tb, p, o);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CG * std::min(p.num_tiles, sm_count(device) / CG), 1, 1);
+  cfg.blockDim = dim3(kF8Threads, 1, 1);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, td, taux, p, o));
+}
+
+// Tile shape: the share of the SMs' time that goes into real output (waves of tiles over the SMs, rows and
+// columns past the edge) counts for each shape, and a 256 x 256 tile runs about 1.4 times the rate of four
+// 128 x 128 ones. Measured, 256 against 128, bf16 out, scales per weight block: 16384 x 1280 x 5120 (M x N
+// x K) 125 / 205 us, 16384 x 5120 x 1280 122 / 143 us, 2048 x 4096 x 1024 16.5 / 18.6 us; with half of the
+// SMs idle 2048 x 1024 x 4096 22.7 / 16.5 us, 1029 x 640 x 1712 14.4 / 12.4 us.
+enum Fp8Tile : int { kTile128 = 0, kTile256 = 1 };
+
+// -1: by the rule below; otherwise every call takes this tile (`set_fp8_tile`, tests and measurements).
+static std::atomic<int> g_fp8_tile{-1};
+
+int64_t set_fp8_tile(int64_t tile) {
+  TORCH_CHECK(tile >= -1 && tile <= kTile256, "set_fp8_tile: -1 (automatic), 0 or 1");
+  return g_fp8_tile.exchange((int)tile);
+}
+
+static int choose_tile(int64_t M, int64_t N, int sms) {
+  const int forced = g_fp8_tile.load(std::memory_order_relaxed);
+  if (forced >= 0) return forced;
+  auto eff = [&](int cg, int bn) {
+    const int64_t tiles = (M + 128 * cg - 1) / (128 * cg) * ((N + bn - 1) / bn);
+    const int64_t workers = sms / cg, waves = (tiles + workers - 1) / workers;
+    return (double)M * N / ((double)waves * workers * 128 * cg * bn);
+  };
+  return M > 128 && eff(2, 256) >= 0.7 * eff(1, 128) ? kTile256 : kTile128;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -395,10 +816,24 @@ void fp8_gemm(torch::Tensor a, torch::Tensor a_scale, bool a_block, torch::Tenso
   p.residual = check_mat(residual, "residual");
   p.aux_out = check_mat(aux_out, "aux_out");
   TORCH_CHECK(act == kActNone || act == kActGelu, "fp8_gemm: act must be none or GELU");
+  const int tile = choose_tile(M, N, sm_count(device));
   const CUtensorMap ta = make_u8_map(a.data_ptr(), k, M, a.stride(0), kF8K, 128);
   const CUtensorMap tb = make_u8_map(b.data_ptr(), k, N, b.stride(0), kF8K, 128);
-  if (b_block) launch_fp8<128, 6, false>(ta, tb, p, o, device, stream);
-  else launch_fp8<128, 6, true>(ta, tb, p, o, device, stream);
+  // TMA stores take rows of a multiple of 16 bytes, and the accumulation a fp32 output.
+  const bool full = p.gamma != nullptr || p.residual != nullptr || N % (p.d_fp32 && p.aux_out == nullptr ? 4 : 8) != 0 ||
+                    (accumulate && !p.d_fp32);
+  CUtensorMap td = ta, taux = ta;
+  if (!full) {
+    td = make_store_map(d.data_ptr(), N, M, p.d_fp32);
+    if (p.aux_out != nullptr) taux = make_store_map(p.aux_out, N, M, false);
+  }
+  auto run = [&](auto row, auto rest) {
+    constexpr bool kRow = decltype(row)::value, kFull = decltype(rest)::value;
+    if (tile == kTile256) launch_fp8<2, 256, 2, 4, kRow, kFull>(ta, tb, td, taux, p, o, device, stream);
+    else launch_fp8<1, 128, 1, 5, kRow, kFull>(ta, tb, td, taux, p, o, device, stream);
+  };
+  if (b_block) full ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
+  else full ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
 }
 
 }  // namespace mia

@@ -526,6 +526,11 @@ CUtensorMap make_bf16_map(const void* base, int64_t inner, int64_t rows, int64_t
   return make_map(base, inner, rows, ld, box_inner, box_rows);
 }
 
+CUtensorMap make_store_map(const void* base, int64_t inner, int64_t rows, bool fp32) {
+  return make_map(base, inner, rows, inner, fp32 ? 32 : 64, 32,
+                  fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, fp32 ? 4 : 2);
+}
+
 CUtensorMap make_u8_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows) {
   return make_map(base, inner, rows, ld, box_inner, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }

@@ -265,7 +265,9 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, int m, int n
 // 2-D bf16 tensor map over a row-major (rows x inner) matrix with row stride `ld` elements,
 // 128-byte swizzle, box (box_inner x box_rows). Defined in gemm.cu.
 CUtensorMap make_bf16_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows);
-// The same over 8-bit elements.
+// 128-byte swizzled boxes of 32 rows x 128 bytes of a contiguous (rows x inner) bf16 or fp32 output.
+CUtensorMap make_store_map(const void* base, int64_t inner, int64_t rows, bool fp32);
+// Over 8-bit elements.
 CUtensorMap make_u8_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows);
 int sm_count(int device);
 

@@ -22,6 +22,13 @@ E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+@pytest.fixture(params=[0, 1], ids=["128x128", "256x256"])
+def tile(request):
+    previous = _native.native().set_fp8_tile(request.param)
+    yield request.param
+    _native.native().set_fp8_tile(previous)
+
+
 def _no_errors():
     torch.cuda.synchronize()
     assert _native.native().check_errors(0) == 0
@@ -126,7 +133,7 @@ GEMMS = [(1, 1, 1), (1, 8, 16), (5, 33, 130), (128, 128, 128), (129, 257, 384), 
 
 @pytest.mark.parametrize("b_block", [True, False])
 @pytest.mark.parametrize("m,n,k", GEMMS)
-def test_products(m, n, k, b_block):
+def test_products(m, n, k, b_block, tile):
     a, b = _operands(m, n, k, b_block)
     da, db = a.dequantize(), b.dequantize()
     exact = da.double() @ db.double().t()
@@ -139,7 +146,7 @@ def test_products(m, n, k, b_block):
 
 @pytest.mark.parametrize("fa,fb", [(E4M3, E5M2), (E5M2, E4M3), (E5M2, E5M2)])
 @pytest.mark.parametrize("b_block", [True, False])
-def test_product_formats(fa, fb, b_block):
+def test_product_formats(fa, fb, b_block, tile):
     a, b = _operands(200, 264, 400, b_block, fa, fb)
     da, db = a.dequantize(), b.dequantize()
     y = fp8_gemm(a, b, out_dtype=F32)
@@ -147,7 +154,7 @@ def test_product_formats(fa, fb, b_block):
     _no_errors()
 
 
-def test_block_scales_of_the_left_operand():
+def test_block_scales_of_the_left_operand(tile):
     a = quantize_fp8(_loud(300, 256, BF16, 1), block_rows=BLOCK)
     b = quantize_fp8(_loud(200, 256, BF16, 2))
     da, db = a.dequantize(), b.dequantize()
@@ -158,7 +165,7 @@ def test_block_scales_of_the_left_operand():
 
 @pytest.mark.parametrize("m,n,k", [(130, 264, 300), (70, 77, 200), (1030, 1544, 640)])
 @pytest.mark.parametrize("b_block", [True, False])
-def test_epilogue(m, n, k, b_block):
+def test_epilogue(m, n, k, b_block, tile):
     a, b = _operands(m, n, k, b_block)
     torch.manual_seed(3)
     bias, gamma = torch.randn(n, device=DEV), torch.rand(n, device=DEV)
@@ -179,7 +186,7 @@ def test_epilogue(m, n, k, b_block):
     _no_errors()
 
 
-def test_extreme_scales_and_non_finite_blocks():
+def test_extreme_scales_and_non_finite_blocks(tile):
     x = torch.ones(130, 300, device=DEV)
     x[1] *= 2.0**100
     x[2] *= 2.0**-120
@@ -201,7 +208,7 @@ def test_extreme_scales_and_non_finite_blocks():
         assert (fp8_gemm(quantize_fp8(pair), quantize_fp8(other, block_rows=block), out_dtype=F32) == 0).all()
 
 
-def test_writes_only_its_output():
+def test_writes_only_its_output(tile):
     a, b = _operands(130, 72, 200, True)
     out = torch.full((134, 72), 7.0, device=DEV, dtype=BF16)
     fp8_gemm(a, b, out=out[2:132])
@@ -216,7 +223,7 @@ def test_strided_scales_are_taken():
     assert torch.equal(fp8_gemm(a, b), fp8_gemm(a, Fp8Matrix(b.data, wide[:, :77], b.cols, 1)))
 
 
-def test_repeats_are_identical():
+def test_repeats_are_identical(tile):
     # the last size gives every SM several tiles
     for m, n, k in ((1000, 776, 1536), (8192, 1280, 5120)):
         for b_block in (False, True):
