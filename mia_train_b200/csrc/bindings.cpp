@@ -1,6 +1,7 @@
 // Python bindings of the mia_train_b200._C extension (all kernels are sm_100a).
 #include <torch/extension.h>
 
+#include "block_ops.h"
 #include "errors.h"
 
 namespace mia {
@@ -93,20 +94,16 @@ void koleo_bwd(at::Tensor x, at::Tensor xn, at::Tensor nn, at::Tensor dist, doub
 at::Tensor axial_angles_fwd(at::Tensor coords, std::vector<at::Tensor> freqs);
 void axial_angles_bwd(at::Tensor dangles, at::Tensor coords, std::vector<at::Tensor> freqs,
                       std::vector<at::Tensor> dfreqs);
-void dropout_apply(at::Tensor x, c10::optional<at::Tensor> residual, at::Tensor y, int64_t dropped,
-                   c10::optional<at::Tensor> rng, c10::optional<at::Tensor> record);
-void qk_norm_fwd(at::Tensor q, at::Tensor k, c10::optional<at::Tensor> qw, c10::optional<at::Tensor> kw,
-                 c10::optional<at::Tensor> angles, at::Tensor pairs, at::Tensor yq, at::Tensor yk, double eps);
-void qk_norm_bwd(at::Tensor dyq, at::Tensor dyk, at::Tensor q, at::Tensor k, c10::optional<at::Tensor> qw,
-                 c10::optional<at::Tensor> kw, c10::optional<at::Tensor> angles, at::Tensor pairs, at::Tensor dq,
-                 at::Tensor dk, c10::optional<at::Tensor> dqw, c10::optional<at::Tensor> dkw, int64_t accumulate,
-                 c10::optional<at::Tensor> dangles, double eps);
-void fp8_quantize(at::Tensor x, c10::optional<at::Tensor> aux, c10::optional<at::Tensor> gamma, bool block, bool e5m2,
-                  c10::optional<at::Tensor> q, c10::optional<at::Tensor> q_scale, c10::optional<at::Tensor> qt,
-                  c10::optional<at::Tensor> qt_scale, c10::optional<at::Tensor> sums, bool accumulate);
-void fp8_gemm(at::Tensor a, at::Tensor a_scale, bool a_block, at::Tensor b, at::Tensor b_scale, bool b_block, int64_t k,
-              at::Tensor d, c10::optional<at::Tensor> bias, c10::optional<at::Tensor> residual,
-              c10::optional<at::Tensor> gamma, c10::optional<at::Tensor> aux_out, int64_t act, bool accumulate);
+at::Tensor dropout(const at::Tensor& x, const OptTensor& residual, int64_t dropped, const OptTensor& rng);
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
+                                                const OptTensor& kw, const OptTensor& angles, const OptTensor& pairs,
+                                                double eps, const OptTensor& q_sink, const OptTensor& k_sink);
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                      const OptTensor& gamma, int64_t act, bool bf16, const OptTensor& shadow, const OptTensor& w_sink,
+                      const OptTensor& b_sink);
+at::Tensor fp8_linear_quantized(const at::Tensor& x, const at::Tensor& data, const at::Tensor& scale, bool block,
+                                int64_t K, const OptTensor& bias, const OptTensor& residual, const OptTensor& gamma,
+                                int64_t act, bool bf16);
 int64_t set_fp8_tile(int64_t tile);
 }  // namespace mia
 
@@ -177,6 +174,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_bwd", &mia::qk_norm_bwd, "gradients of qk_norm_fwd (q, k, weights, angles); dq / dk may alias the incoming gradients");
   m.def("fp8_quantize", &mia::fp8_quantize, "8-bit values with power-of-two block scales, row- and column-wise, + column sums");
   m.def("fp8_gemm", &mia::fp8_gemm, "8-bit tcgen05 GEMM with a scale per block of 128 along K and fused epilogue");
+  m.def("dropout", &mia::dropout, "dropout (+ residual) as an autograd node");
+  m.def("qk_norm_rope", &mia::qk_norm_rope, "RMS norm of q and k heads + rotation as an autograd node");
+  m.def("fp8_linear", &mia::fp8_linear, "linear layer on 8-bit products as an autograd node");
+  m.def("fp8_linear_quantized", &mia::fp8_linear_quantized, "8-bit linear layer on a weight quantised once");
   m.def("set_fp8_tile", &mia::set_fp8_tile, "-1: tile of the 8-bit GEMM by its rule; 0: 128 x 128, 1: 256 x 256; returns the previous");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }

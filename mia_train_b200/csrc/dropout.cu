@@ -19,6 +19,7 @@
 
 #include <mutex>
 
+#include "block_ops.h"
 #include "common.cuh"
 #include "vec8.cuh"
 

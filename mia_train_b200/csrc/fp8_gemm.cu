@@ -34,6 +34,7 @@
 #include <cfloat>
 #include <type_traits>
 
+#include "block_ops.h"
 #include "common.cuh"
 #include "errors.h"
 #include "gemm_common.cuh"
@@ -696,7 +697,11 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
                        cudaStream_t stream) {
   using L = F8Smem<CG, BN, STAGES>;
   auto kern = fp8_gemm_kernel<CG, BN, HALVES, STAGES, SB_ROW, FULL>;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  static std::atomic<bool> configured[64] = {};
+  if (!configured[device].load(std::memory_order_acquire)) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    configured[device].store(true, std::memory_order_release);
+  }
   p.num_m_tiles = (p.M + 128 * CG - 1) / (128 * CG);
   p.num_n_tiles = (p.N + BN - 1) / BN;
   p.num_tiles = p.num_m_tiles * p.num_n_tiles;

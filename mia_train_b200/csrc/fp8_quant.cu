@@ -23,6 +23,7 @@
 #include <cuda_fp8.h>
 #include <torch/extension.h>
 
+#include "block_ops.h"
 #include "common.cuh"
 #include "vec8.cuh"
 

@@ -24,6 +24,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include "block_ops.h"
 #include "common.cuh"
 #include "vec8.cuh"
 

@@ -65,34 +65,21 @@ def _draw(device: torch.device) -> torch.Tensor:
 
 
 class _Dropout(torch.autograd.Function):
+    """The PyTorch path; on CUDA `csrc/block_ops.cpp` holds the same node."""
+
     @staticmethod
     def forward(ctx, x, residual, dropped, rng):  # type: ignore[override]
-        xc = x.contiguous()
-        res = residual.contiguous() if residual is not None else None
+        # the pair is copied, as the kernel does: the caller may advance its own before the backward pass
+        used = _draw(x.device) if rng is None else rng.clone()
         ctx.dropped = dropped
-        if use_native(x) and x.dtype in _DTYPES:
-            used = torch.empty(2, dtype=torch.int64, device=x.device)
-            y = torch.empty_like(xc)
-            native().dropout_apply(xc, res, y, dropped, rng.contiguous() if rng is not None else None, used)
-        else:
-            # copied, as the kernel does: the caller may advance its pair before the backward pass
-            used = _draw(x.device) if rng is None else rng.clone()
-            y = dropout_reference(xc, dropped, used, res)
         ctx.save_for_backward(used)
-        return y
+        return dropout_reference(x, dropped, used, residual)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):  # type: ignore[override]
         (used,) = ctx.saved_tensors
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dyc = dy.contiguous()
-            if use_native(dy) and dy.dtype in _DTYPES:
-                dx = torch.empty_like(dyc)
-                native().dropout_apply(dyc, None, dx, ctx.dropped, used, None)
-            else:
-                dx = dropout_reference(dyc, ctx.dropped, used)
+        dx = dropout_reference(dy, ctx.dropped, used) if ctx.needs_input_grad[0] else None
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None
 
 
@@ -122,4 +109,6 @@ def dropout(
     dropped = round(p * STEPS) if training else 0
     if dropped == 0:
         return x if residual is None else residual + x
+    if x.dtype in _DTYPES and use_native(x):
+        return native().dropout(x, residual, dropped, rng)
     return _Dropout.apply(x, residual, dropped, rng)

@@ -31,7 +31,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._native import native, use_native
-from ._params import compute_weight, grad_sink
+from ._params import grad_sink
 from .linear import _ACTS, ACT_GELU, compute_dtype, gelu_grad_reference, gelu_reference
 
 BLOCK = 128
@@ -196,27 +196,19 @@ def fp8_gemm(
     return out
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _vec(t: torch.Tensor | None) -> torch.Tensor | None:
-    return _aligned(t.detach().float()) if t is not None else None
-
-
 class _Fp8Linear(torch.autograd.Function):
+    """The PyTorch path; on CUDA `csrc/block_ops.cpp` holds the same node."""
+
     @staticmethod
     def forward(ctx, x2, weight, bias, residual, gamma, act, cdtype):  # type: ignore[override]
         e4m3 = torch.float8_e4m3fn
         need_x, need_w, need_g = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[4]
         n = weight.shape[0]
-        w = compute_weight(weight, weight.dtype if weight.dtype in _DTYPES else torch.float32)
         shadow = getattr(weight, "_mia_shadow", None)  # under a sharded optimizer only the bf16 copy is current
-        w = (shadow if shadow is not None else w).detach().reshape(n, -1).contiguous()
+        w = (shadow if shadow is not None else weight).detach().reshape(n, -1)
         xq, xt = _quantize(x2, 1, e4m3, True, need_w)
         wq, wt = _quantize(w, BLOCK, e4m3, True, need_x)
-        g, bf = _vec(gamma), _vec(bias)
+        g, bf = (t.detach().float() if t is not None else None for t in (gamma, bias))
         pre = torch.empty((x2.shape[0], n), device=x2.device, dtype=cdtype) if act == ACT_GELU else None
         y = fp8_gemm(xq, wq, out_dtype=cdtype, bias=bf, residual=residual, gamma=g, act=act, aux_out=pre)
         keep = {"xt": xt, "wt": wt, "xq": xq if need_g else None, "wq": wq if need_g else None}
@@ -237,7 +229,6 @@ class _Fp8Linear(torch.autograd.Function):
         act, wdtype, wshape, gdtype, bdtype = ctx.meta
         need_x, need_w, need_b, need_r, need_g = ctx.needs_input_grad[:5]
         n = dy.shape[1]
-        dy = dy if dy.stride(1) == 1 and dy.stride(0) >= n else dy.contiguous()
         dgamma = None
         if need_g:
             # d(gamma * h) / d gamma needs h = act(x W^T + b): recomputed once, from the saved operands
@@ -292,20 +283,27 @@ def fp8_linear(
         t is not None and t.requires_grad for t in (x, bias, residual, gamma)
     ):
         raise ValueError("a weight quantised once has no backward; pass the weight tensor to train")
-    x2 = x.reshape(-1, k)
-    if x2.dtype not in _DTYPES:
-        x2 = x2.to(cdtype)
-    if x2.stride(1) != 1:
-        x2 = x2.contiguous()
     fused = cdtype == torch.bfloat16
-    res2 = _aligned(residual.reshape(-1, n).to(cdtype)) if residual is not None and fused else None
-    f_act, f_gamma = (act, gamma) if fused else (0, None)
-    if quantised:
-        xq, _ = _quantize(x2.detach(), 1, torch.float8_e4m3fn, True, False)
-        y = fp8_gemm(xq, weight, out_dtype=cdtype, bias=_vec(bias), residual=res2, gamma=_vec(f_gamma), act=f_act)
+    f_act, f_gamma, f_res = (act, gamma, residual) if fused else (0, None, None)
+    if x.dtype not in _DTYPES:
+        x = x.to(cdtype)
+    if use_native(x):
+        if quantised:
+            y = native().fp8_linear_quantized(x, weight.data, weight.scale, weight.block_rows != 1, k, bias, f_res, f_gamma,
+                                              f_act, fused)
+        else:
+            # under a sharded optimizer only the bf16 copy of a weight is current
+            y = native().fp8_linear(x, weight, bias, f_res, f_gamma, f_act, fused, getattr(weight, "_mia_shadow", None),
+                                    grad_sink(weight), grad_sink(bias))
     else:
-        y = _Fp8Linear.apply(x2, weight, bias, res2, f_gamma, f_act, cdtype)
-    y = y.reshape(*x.shape[:-1], n)
+        x2 = x.reshape(-1, k)
+        res2 = f_res.reshape(-1, n).to(cdtype) if f_res is not None else None
+        if quantised:
+            y = fp8_gemm(_quantize(x2.detach(), 1, torch.float8_e4m3fn, True, False)[0], weight, out_dtype=cdtype,
+                         bias=bias, residual=res2, gamma=f_gamma, act=f_act)
+        else:
+            y = _Fp8Linear.apply(x2, weight, bias, res2, f_gamma, f_act, cdtype)
+        y = y.reshape(*x.shape[:-1], n)
     if fused:
         return y
     if act == ACT_GELU:

@@ -53,14 +53,6 @@ def _native_norm_ok(q: torch.Tensor, k: torch.Tensor) -> bool:
     return q.dtype in _DTYPES and k.dtype == q.dtype and d % 8 == 0 and 8 <= d <= MAX_HEAD_DIM and use_native(q, k)
 
 
-def _heads(x: torch.Tensor) -> torch.Tensor:
-    """x itself when its heads can be read 16 bytes at a time, else a contiguous copy."""
-    e = 16 // x.element_size()
-    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0
-    ok = ok and all(x.stride(i) % e == 0 or x.shape[i] <= 1 for i in range(3))
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
 def _prepared(angles: torch.Tensor | None, pairs: torch.Tensor | None, device: torch.device):
     if angles is None or pairs is None or pairs.numel() == 0:
         return None, torch.zeros((0, 2), dtype=torch.int32, device=device)
@@ -68,7 +60,7 @@ def _prepared(angles: torch.Tensor | None, pairs: torch.Tensor | None, device: t
 
 
 class _Norms:
-    """What forward and backward share: fp32 weights, their sinks, and the gradient buffers."""
+    """Weight and angle gradients of the attention node."""
 
     @staticmethod
     def weight(w: torch.Tensor | None) -> torch.Tensor | None:
@@ -102,43 +94,6 @@ class _Norms:
         if shape[0] == 1 and dangles.shape[0] != 1:
             dangles = dangles.sum(0, keepdim=True)
         return dangles.to(dtype)
-
-
-class _NativeQKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, qw, kw, angles, pairs, eps):  # type: ignore[override]
-        b, t, hq, d = q.shape
-        hk = k.shape[2]
-        qc, kc = _heads(q), _heads(k)
-        ang, pr = _prepared(angles, pairs, q.device)
-        qwf, kwf = _Norms.weight(qw), _Norms.weight(kw)
-        out = torch.empty((b, t, hq + hk, d), device=q.device, dtype=q.dtype)
-        yq, yk = out[:, :, :hq], out[:, :, hq:]
-        native().qk_norm_fwd(qc, kc, qwf, kwf, ang, pr, yq, yk, float(eps))
-        ctx.save_for_backward(qc, kc, qwf, kwf, ang, pr)
-        ctx.eps = float(eps)
-        ctx.sinks = (grad_sink(qw), grad_sink(kw))
-        ctx.w_dtypes = tuple(w.dtype if w is not None else None for w in (qw, kw))
-        ctx.angles_meta = (angles.shape, angles.dtype) if angles is not None else None
-        return yq, yk
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dyq, dyk):  # type: ignore[override]
-        q, k, qw, kw, ang, pairs = ctx.saved_tensors
-        b, t, hq, d = q.shape
-        dyq, dyk = _heads(dyq), _heads(dyk)
-        ctx.want_w = ctx.needs_input_grad[2:4]
-        buf = torch.empty((b, t, hq + k.shape[2], d), device=q.device, dtype=q.dtype)
-        dq, dk = buf[:, :, :hq], buf[:, :, hq:]
-        dws, bits = _Norms.grads(ctx, d, q.device)
-        dangles = None
-        if ang is not None and ctx.needs_input_grad[4]:
-            dangles = torch.empty((b, t, pairs.shape[0]), device=q.device, dtype=torch.float32)
-        native().qk_norm_bwd(dyq, dyk, q, k, qw, kw, ang, pairs, dq, dk, dws[0], dws[1], bits, dangles, ctx.eps)
-        if ctx.angles_meta is not None:
-            dangles = _Norms.angle_grad(dangles, *ctx.angles_meta)
-        return dq, dk, *_Norms.returned(ctx, dws), dangles, None, None
 
 
 def _check(q, k, q_weight, k_weight, angles, pairs) -> None:
@@ -175,7 +130,8 @@ def qk_norm_rope(
     """Normalised and rotated (q, k); see the module docstring."""
     _check(q, k, q_weight, k_weight, angles, pairs)
     if _native_norm_ok(q, k):
-        return _NativeQKNormRope.apply(q, k, q_weight, k_weight, angles, pairs, eps)
+        return native().qk_norm_rope(q, k, q_weight, k_weight, angles, pairs, float(eps), grad_sink(q_weight),
+                                     grad_sink(k_weight))
     pairs = pairs.to(q.device) if pairs is not None else None
     return (head_norm_rope_reference(q, q_weight, angles, pairs, eps),
             head_norm_rope_reference(k, k_weight, angles, pairs, eps))
