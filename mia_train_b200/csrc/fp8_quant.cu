@@ -18,10 +18,15 @@
 // Thread (tx, ty) holds rows 8 ty .. 8 ty + 7 of columns 8 tx .. 8 tx + 7, so that it owns eight
 // consecutive bytes of both q and q^T; q^T goes through shared memory in 8-byte units, XOR-swizzled
 // by tx so that neither side meets a bank conflict, and leaves as 16-byte stores.
+// Instructions, not bytes, are scarce (ncu: 15 a value for q alone in a first version that kept fp32
+// values): bf16 input stays packed, its magnitudes are compared two at a time as 16-bit integers (their
+// order as numbers, NaN above infinity above the rest), and rows are reduced in pairs.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 #include <torch/extension.h>
+
+#include <type_traits>
 
 #include "block_ops.h"
 #include "common.cuh"
@@ -38,7 +43,6 @@ struct QuantParams {
   const float* gamma;        // (C), or nullptr
   int64_t R;
   int64_t C;
-  int e5m2;
   uint8_t* q;  // (R, q_ld)
   int64_t q_ld;
   float* q_scale;  // 1 x 128: [c / 128][r], row stride q_scale_ld; block: [c / 128][r / 128]
@@ -51,148 +55,216 @@ struct QuantParams {
   int col_tiles;
 };
 
-// Scale for a block whose largest |v| has the given bits, and its reciprocal.
-__device__ __forceinline__ void pow2_scale(uint32_t amax_bits, int e5m2, float& scale, float& inv) {
-  if (amax_bits >= 0x7F800000u) {
-    scale = inv = __uint_as_float(0x7FC00000u);
-    return;
-  }
-  int e = (int)(amax_bits >> 23) - (e5m2 ? 15 : 8) + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  e = e < 1 ? 1 : e;
-  scale = __uint_as_float((uint32_t)e << 23);
-  inv = __uint_as_float((uint32_t)(254 - e) << 23);
+// Scale for a block whose largest |v| has the given fp32 bits, and its reciprocal. A mantissa above 1.75
+// carries into the exponent.
+template <bool E5M2>
+__device__ __forceinline__ void pow2_scale(uint32_t amax_bits, float& scale, float& inv) {
+  const int e = max((int)((amax_bits + 0x1FFFFFu) >> 23) - (E5M2 ? 15 : 8), 1);
+  const bool finite = amax_bits < 0x7F800000u;
+  scale = __uint_as_float(finite ? (uint32_t)e << 23 : 0x7FC00000u);
+  inv = __uint_as_float(finite ? (uint32_t)(254 - e) << 23 : 0x7FC00000u);
 }
 
-__device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d, int e5m2) {
-  const __nv_fp8_interpretation_t f = e5m2 ? __NV_E5M2 : __NV_E4M3;
+template <bool E5M2>
+__device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
+  constexpr __nv_fp8_interpretation_t f = E5M2 ? __NV_E5M2 : __NV_E4M3;
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, f);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, f);
   return lo | hi << 16;
 }
 
+// A thread's 8 x 8 values: fp32 in general.
+template <typename T, bool PACKED>
+struct QuantTile {
+  float v[8][8];
+  __device__ __forceinline__ float get(int i, int j) const { return v[i][j]; }
+  __device__ __forceinline__ void load(const T* src, int64_t ld, int rows, int cols, bool vec) {
+    if (vec) {
+      Raw8<T> raw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = i < rows ? load_raw8(src + i * ld) : Raw8<T>{};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) unpack8(raw[i], v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = (i < rows && j < cols) ? to_f32(src[i * ld + j]) : 0.f;
+    }
+  }
+  static __device__ __forceinline__ uint32_t mag(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
+  // fp32 bits of the largest magnitude of row i over the 16 threads of the row
+  __device__ __forceinline__ void row_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m[i] = max(m[i], mag(v[i][j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+    }
+  }
+  // of column j over the warp's 16 rows
+  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[j] = max(m[j], mag(v[i][j]));
+      m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    }
+  }
+};
+
+// bf16 pairs as they come.
+template <>
+struct QuantTile<__nv_bfloat16, true> {
+  uint32_t w[8][4];
+  __device__ __forceinline__ float get(int i, int j) const { return j & 1 ? bf16_hi(w[i][j / 2]) : bf16_lo(w[i][j / 2]); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* src, int64_t ld, int rows, int cols, bool vec) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (vec) {
+        if (i < rows) u = *reinterpret_cast<const uint4*>(src + i * ld);
+      } else if (i < rows) {
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(src + i * ld);
+        uint32_t t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          t[k] = (2 * k < cols ? e[2 * k] : 0u) | (2 * k + 1 < cols ? (uint32_t)e[2 * k + 1] << 16 : 0u);
+        u = make_uint4(t[0], t[1], t[2], t[3]);
+      }
+      w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+    }
+  }
+  __device__ __forceinline__ uint32_t mag2(int i, int k) const { return w[i][k] & 0x7FFF7FFFu; }
+  __device__ __forceinline__ void row_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t a = __vmaxu2(__vmaxu2(mag2(i, 0), mag2(i, 1)), __vmaxu2(mag2(i, 2), mag2(i, 3)));
+      const uint32_t b = __vmaxu2(__vmaxu2(mag2(i + 1, 0), mag2(i + 1, 1)), __vmaxu2(mag2(i + 1, 2), mag2(i + 1, 3)));
+      uint32_t two = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));  // row i low, row i + 1 high
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, o));
+      m[i] = two << 16;
+      m[i + 1] = two & 0xFFFF0000u;
+    }
+  }
+  __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t two = mag2(0, k);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) two = __vmaxu2(two, mag2(i, k));
+      two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, 16));
+      m[2 * k] = two << 16;
+      m[2 * k + 1] = two & 0xFFFF0000u;
+    }
+  }
+};
+
 enum QuantMode : int { kQuantRows = 1, kQuantCols = 2, kQuantBlock = 4, kQuantSums = 8 };
 
-template <typename T, int MODE, bool AUX>
-__global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
+template <typename T, int MODE, bool AUX, bool E5M2>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && !AUX ? 3 : 2) quant_kernel(const QuantParams p) {
   constexpr bool kBlock = (MODE & kQuantBlock) != 0;
   constexpr bool kRows = (MODE & kQuantRows) != 0;
   constexpr bool kCols = (MODE & kQuantCols) != 0;
   constexpr bool kSums = (MODE & kQuantSums) != 0;
   __shared__ __align__(16) uint32_t col_red[8][kQBlk];
-  __shared__ __align__(16) float col_scale[2][kQBlk];
+  __shared__ __align__(16) float col_inv[kQBlk];
   __shared__ __align__(16) uint2 tile[kCols ? kQBlk * 16 : 1];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int tx = tid % 16, ty = tid / 16;
   const int64_t rb = blockIdx.x / p.col_tiles, cb = blockIdx.x % p.col_tiles;
   const int64_t r0 = rb * kQBlk + ty * 8, c0 = cb * kQBlk + tx * 8;
-  float v[8][8];
-  const T* src = reinterpret_cast<const T*>(p.x) + r0 * p.x_ld + c0;
-  const bool vec = c0 + 8 <= p.C && p.x_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
-  if (vec) {
-    Raw8<T> raw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (r0 + i < p.R) raw[i] = load_raw8(src + i * p.x_ld);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (r0 + i < p.R) {
-        unpack8(raw[i], v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = (r0 + i < p.R && c0 + j < p.C) ? to_f32(src[i * p.x_ld + j]) : 0.f;
-  }
+  const int rows = (int)min((int64_t)8, p.R - r0), cols = (int)min((int64_t)8, p.C - c0);  // may be negative: none
+  QuantTile<T, std::is_same_v<T, __nv_bfloat16> && !AUX> t;
+  const bool vec = cols == 8 && p.x_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0;
+  t.load(reinterpret_cast<const T*>(p.x) + r0 * p.x_ld + c0, p.x_ld, rows, cols, vec);
   if constexpr (AUX) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (r0 + i < p.R && c0 + j < p.C) {
-          if (p.aux != nullptr) v[i][j] *= gelu_erf_grad(__bfloat162float(p.aux[(r0 + i) * p.C + c0 + j]));
-          if (p.gamma != nullptr) v[i][j] *= p.gamma[c0 + j];
+        if (i < rows && j < cols) {
+          if (p.aux != nullptr) t.v[i][j] *= gelu_erf_grad(__bfloat162float(p.aux[(r0 + i) * p.C + c0 + j]));
+          if (p.gamma != nullptr) t.v[i][j] *= p.gamma[c0 + j];
         }
   }
-  auto mag = [](float f) { return __float_as_uint(f) & 0x7FFFFFFFu; };
 
-  // largest magnitudes: per row over the 16 threads of the row, per column over the tile's 16 row
-  // groups, or over the tile
-  float row_inv[8], blk_scale = 0.f, blk_inv = 0.f;
+  float blk_inv = 0.f;
   if constexpr (kBlock) {
-    uint32_t m = 0;
+    uint32_t m8[8];
+    t.col_max(m8);
+    uint32_t m = m8[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int j = 1; j < 8; ++j) m = max(m, m8[j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mag(v[i][j]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) col_red[0][warp] = m;
     __syncthreads();
     m = col_red[0][0];
 #pragma unroll
     for (int k = 1; k < 8; ++k) m = max(m, col_red[0][k]);
-    pow2_scale(m, p.e5m2, blk_scale, blk_inv);
+    float blk_scale;
+    pow2_scale<E5M2>(m, blk_scale, blk_inv);
     if (tid == 0) {
       if (kRows) p.q_scale[cb * p.q_scale_ld + rb] = blk_scale;
       if (kCols) p.qt_scale[rb * p.qt_scale_ld + cb] = blk_scale;
     }
-  } else {
-    if constexpr (kRows) {
+  } else if constexpr (kCols) {
+    uint32_t m[8];
+    t.col_max(m);
+    if (lane < 16) {
+      *reinterpret_cast<uint4*>(&col_red[warp][tx * 8]) = make_uint4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<uint4*>(&col_red[warp][tx * 8 + 4]) = make_uint4(m[4], m[5], m[6], m[7]);
+    }
+  }
+  if constexpr (kRows) {
+    float inv[8], scale[8];
+    if constexpr (!kBlock) {
+      uint32_t m[8];
+      t.row_max(m);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t m = 0;
+      for (int i = 0; i < 8; ++i) pow2_scale<E5M2>(m[i], scale[i], inv[i]);
+      if (tx < 8 && tx < rows) {  // lane tx of a row group writes the scale of row tx: eight in one sector
+        float mine = scale[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, mag(v[i][j]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float s;
-        pow2_scale(m, p.e5m2, s, row_inv[i]);
-        if (tx == 0 && r0 + i < p.R) p.q_scale[cb * p.q_scale_ld + r0 + i] = s;
+        for (int i = 1; i < 8; ++i) mine = tx == i ? scale[i] : mine;
+        p.q_scale[cb * p.q_scale_ld + r0 + tx] = mine;
       }
     }
-    if constexpr (kCols) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, mag(v[i][j]));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if (lane < 16) col_red[warp][tx * 8 + j] = m;
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float k = kBlock ? blk_inv : inv[i];
+      if (i < rows && c0 < p.q_ld)
+        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) =
+            make_uint2(cvt4<E5M2>(t.get(i, 0) * k, t.get(i, 1) * k, t.get(i, 2) * k, t.get(i, 3) * k),
+                       cvt4<E5M2>(t.get(i, 4) * k, t.get(i, 5) * k, t.get(i, 6) * k, t.get(i, 7) * k));
+    }
+  }
+  if constexpr (kCols) {
+    if constexpr (!kBlock) {
       __syncthreads();
       if (tid < kQBlk) {
         uint32_t m = col_red[0][tid];
 #pragma unroll
         for (int k = 1; k < 8; ++k) m = max(m, col_red[k][tid]);
         float s, inv;
-        pow2_scale(m, p.e5m2, s, inv);
-        col_scale[0][tid] = inv;
+        pow2_scale<E5M2>(m, s, inv);
+        col_inv[tid] = inv;
         if (cb * kQBlk + tid < p.C) p.qt_scale[rb * p.qt_scale_ld + cb * kQBlk + tid] = s;
       }
       __syncthreads();
     }
-  }
-  if constexpr (kRows) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float k = kBlock ? blk_inv : row_inv[i];
-      if (r0 + i < p.R && c0 < p.q_ld)
-        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) =
-            make_uint2(cvt4(v[i][0] * k, v[i][1] * k, v[i][2] * k, v[i][3] * k, p.e5m2),
-                       cvt4(v[i][4] * k, v[i][5] * k, v[i][6] * k, v[i][7] * k, p.e5m2));
-    }
-  }
-  if constexpr (kCols) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float k = kBlock ? blk_inv : col_scale[0][tx * 8 + j];
-      tile[(tx * 8 + j) * 16 + (ty ^ tx)] = make_uint2(cvt4(v[0][j] * k, v[1][j] * k, v[2][j] * k, v[3][j] * k, p.e5m2),
-                                                       cvt4(v[4][j] * k, v[5][j] * k, v[6][j] * k, v[7][j] * k, p.e5m2));
+      const float k = kBlock ? blk_inv : col_inv[tx * 8 + j];
+      tile[(tx * 8 + j) * 16 + (ty ^ tx)] =
+          make_uint2(cvt4<E5M2>(t.get(0, j) * k, t.get(1, j) * k, t.get(2, j) * k, t.get(3, j) * k),
+                     cvt4<E5M2>(t.get(4, j) * k, t.get(5, j) * k, t.get(6, j) * k, t.get(7, j) * k));
     }
     __syncthreads();
     const int64_t t0 = rb * kQBlk;
@@ -211,7 +283,7 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
     for (int j = 0; j < 8; ++j) {
       float a = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a += v[i][j];
+      for (int i = 0; i < 8; ++i) a += t.get(i, j);
       a += __shfl_xor_sync(0xffffffffu, a, 16);
       if (lane < 16) col_red[warp][tx * 8 + j] = __float_as_uint(a);
     }
@@ -243,11 +315,11 @@ __global__ void __launch_bounds__(256) quant_sums_kernel(const float* __restrict
   }
 }
 
-template <typename T, bool AUX>
+template <typename T, bool AUX, bool E5M2>
 static void launch_quant(const QuantParams& p, int mode, unsigned blocks, cudaStream_t stream) {
   switch (mode) {
 #define MIA_QUANT_CASE(M) \
-  case M: quant_kernel<T, M, AUX><<<blocks, 256, 0, stream>>>(p); break;
+  case M: quant_kernel<T, M, AUX, E5M2><<<blocks, 256, 0, stream>>>(p); break;
     MIA_QUANT_CASE(kQuantRows)
     MIA_QUANT_CASE(kQuantCols)
     MIA_QUANT_CASE(kQuantRows | kQuantCols)
@@ -288,7 +360,6 @@ void fp8_quantize(torch::Tensor x, c10::optional<torch::Tensor> aux, c10::option
   p.x_ld = x.stride(0);
   p.R = x.size(0);
   p.C = x.size(1);
-  p.e5m2 = e5m2 ? 1 : 0;
   const int64_t rb = (p.R + kQBlk - 1) / kQBlk, cb = (p.C + kQBlk - 1) / kQBlk;
   int mode = block ? kQuantBlock : 0;
   TORCH_CHECK(q.has_value() == q_scale.has_value() && qt.has_value() == qt_scale.has_value(),
@@ -339,8 +410,9 @@ void fp8_quantize(torch::Tensor x, c10::optional<torch::Tensor> aux, c10::option
     const bool extra = p.aux != nullptr || p.gamma != nullptr;
     auto run = [&](auto type) {
       using T = decltype(type);
-      if (extra) launch_quant<T, true>(p, mode, (unsigned)(rb * cb), stream);
-      else launch_quant<T, false>(p, mode, (unsigned)(rb * cb), stream);
+      const unsigned blocks = (unsigned)(rb * cb);
+      if (e5m2) extra ? launch_quant<T, true, true>(p, mode, blocks, stream) : launch_quant<T, false, true>(p, mode, blocks, stream);
+      else extra ? launch_quant<T, true, false>(p, mode, blocks, stream) : launch_quant<T, false, false>(p, mode, blocks, stream);
     };
     if (x.scalar_type() == at::kBFloat16) run(__nv_bfloat16{});
     else if (x.scalar_type() == at::kHalf) run(__half{});
