@@ -301,7 +301,16 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
-  const int num_k = (p.K + kF8K - 1) / kF8K;
+  // Work unit -> output tile (m fastest, so that concurrent CTAs share tiles of B) and its K blocks.
+  const int total_k = (p.K + kF8K - 1) / kF8K;
+  struct Unit {
+    int m0, n0, kb0, num_k;
+  };
+  auto work_unit = [&](int index) {
+    const int tiles = p.num_m_tiles * p.num_n_tiles, tile = index % tiles;
+    const int kb0 = index / tiles * p.k_blocks_per_split;
+    return Unit{tile % p.num_m_tiles * (128 * CG), tile / p.num_m_tiles * BN, kb0, min(p.k_blocks_per_split, total_k - kb0)};
+  };
 
   if (warp < kF8FirstEpi) {
     if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8ControlRegs));
@@ -311,9 +320,9 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       int issued = 0;
       bool ok = true;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
-        const int m0 = (tile % p.num_m_tiles) * (128 * CG) + 128 * rank;
-        const int n0 = (tile / p.num_m_tiles) * BN + BN / CG * rank;
-        for (int kb = 0; kb < num_k; ++kb) {
+        const Unit u = work_unit(tile);
+        const int m0 = u.m0 + 128 * rank, n0 = u.n0 + BN / CG * rank;
+        for (int kb = u.kb0; kb < u.kb0 + u.num_k; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.err, kErrFp8ProducerWait)) {
             ok = false;
             break;
@@ -356,6 +365,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       bool ok = true;
       bool any_mma = false;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
+        const int num_k = work_unit(tile).num_k;
         for (int kb = 0; kb < num_k && ok; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.err, kErrFp8MmaWait)) {
             ok = false;
@@ -425,8 +435,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     uint32_t unit_phase = 0;
     bool ok = true, ready = false;
     for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
-      const int m_warp = (tile % p.num_m_tiles) * (128 * CG) + 128 * rank + lane_group * 32;
-      const int n0 = (tile / p.num_m_tiles) * BN + n_col;
+      const Unit u = work_unit(tile);
+      const int num_k = u.num_k;
+      const int m_warp = u.m0 + 128 * rank + lane_group * 32;
+      const int n0 = u.n0 + n_col;
       const uint32_t t_row = tmem_base + ((uint32_t)(lane_group * 32) << 16) + t_col;
       float sum[kCols];
 #pragma unroll
@@ -435,11 +447,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       // == 2) or, with a scale per row of B, those of columns n0 + column(32 i) + lane. Rows and columns past
       // the edge fetch the last one: their sums are never stored.
       constexpr int kSb = SB_ROW ? kLaneCols : HALVES;
-      const float* sa = o.sa;
+      const float* sa = o.sa + u.kb0 * o.sa_ld;
       int sa_at[kRowsT];
 #pragma unroll
       for (int i = 0; i < kRowsT; ++i) sa_at[i] = min(m_warp + row_t + 8 * i, p.M - 1) >> o.sa_shift;
-      const float* sb = o.sb;
+      const float* sb = o.sb + u.kb0 * o.sb_ld;
       int sb_at[kSb];
 #pragma unroll
       for (int i = 0; i < kSb; ++i)
@@ -632,8 +644,9 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           for (int c = 0; c < kCols; ++c) sum[c] = gelu_erf(sum[c]);
         }
         if (p.d_fp32) {
-          stage(&tmD, 0, std::true_type{}, p.accumulate != 0);
-          stage(&tmD, kCols / 2, std::true_type{}, p.accumulate != 0);
+          const bool add = p.accumulate != 0 || p.splits > 1;
+          stage(&tmD, 0, std::true_type{}, add);
+          stage(&tmD, kCols / 2, std::true_type{}, add);
         } else {
           stage(&tmD, 0, std::false_type{}, false);
         }
@@ -693,8 +706,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
 template <int CG, int BN, int HALVES, int STAGES, bool SB_ROW, bool FULL>
 static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
-                       const CUtensorMap& taux, GemmParams& p, const Fp8Operands& o, int device,
-                       cudaStream_t stream) {
+                       const CUtensorMap& taux, GemmParams& p, const Fp8Operands& o, bool may_split,
+                       int device, cudaStream_t stream) {
   using L = F8Smem<CG, BN, STAGES>;
   auto kern = fp8_gemm_kernel<CG, BN, HALVES, STAGES, SB_ROW, FULL>;
   static std::atomic<bool> configured[64] = {};
@@ -704,9 +717,17 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   }
   p.num_m_tiles = (p.M + 128 * CG - 1) / (128 * CG);
   p.num_n_tiles = (p.N + BN - 1) / BN;
-  p.num_tiles = p.num_m_tiles * p.num_n_tiles;
+  const int tiles = p.num_m_tiles * p.num_n_tiles, num_k = (p.K + kF8K - 1) / kF8K, workers = sm_count(device) / CG;
+  // Two halves of K where the last wave of whole tiles would leave many SMs idle (weight gradients: a long K and
+  // few tiles). Both halves are added to a cleared fp32 output; a sum of two does not depend on their order. Measured
+  // at 5120 x 1280 x 16384 (100 tiles of 256 x 256 for 74 pairs): 217 -> 181 us.
+  auto waves = [&](int units) { return (units + workers - 1) / workers; };
+  p.splits = may_split && num_k >= 16 && 0.85 * 2 * waves(tiles) >= waves(2 * tiles) ? 2 : 1;
+  p.k_blocks_per_split = (num_k + p.splits - 1) / p.splits;
+  p.num_tiles = tiles * p.splits;
+  if (p.splits > 1) C10_CUDA_CHECK(cudaMemsetAsync(p.D, 0, (size_t)p.M * p.N * sizeof(float), stream));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(CG * std::min(p.num_tiles, sm_count(device) / CG), 1, 1);
+  cfg.gridDim = dim3(CG * std::min(p.num_tiles, workers), 1, 1);
   cfg.blockDim = dim3(kF8Threads, 1, 1);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = stream;
@@ -800,7 +821,6 @@ void fp8_gemm(torch::Tensor a, torch::Tensor a_scale, bool a_block, torch::Tenso
   p.d_fp32 = d.scalar_type() == at::kFloat;
   p.act = (int)act;
   p.accumulate = accumulate ? 1 : 0;
-  p.splits = 1;
   p.err = error_word(device);
   auto check_vec = [&](const c10::optional<torch::Tensor>& t, const char* name) -> const float* {
     if (!t.has_value()) return nullptr;
@@ -832,10 +852,11 @@ void fp8_gemm(torch::Tensor a, torch::Tensor a_scale, bool a_block, torch::Tenso
     td = make_store_map(d.data_ptr(), N, M, p.d_fp32);
     if (p.aux_out != nullptr) taux = make_store_map(p.aux_out, N, M, false);
   }
+  const bool may_split = !full && p.d_fp32 && !accumulate && act == kActNone && p.bias == nullptr;
   auto run = [&](auto row, auto rest) {
     constexpr bool kRow = decltype(row)::value, kFull = decltype(rest)::value;
-    if (tile == kTile256) launch_fp8<2, 256, 2, 4, kRow, kFull>(ta, tb, td, taux, p, o, device, stream);
-    else launch_fp8<1, 128, 1, 5, kRow, kFull>(ta, tb, td, taux, p, o, device, stream);
+    if (tile == kTile256) launch_fp8<2, 256, 2, 4, kRow, kFull>(ta, tb, td, taux, p, o, may_split, device, stream);
+    else launch_fp8<1, 128, 1, 5, kRow, kFull>(ta, tb, td, taux, p, o, may_split, device, stream);
   };
   if (b_block) full ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
   else full ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
