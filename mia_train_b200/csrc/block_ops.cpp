@@ -25,6 +25,16 @@ void once_differentiable(const at::Tensor& grad, const char* what) {
               ": the backward pass is differentiable once only");
 }
 
+// A parameter's `main_grad`. Not a saved variable: it is written between forward and backward (cleared, or added to
+// by other layers), which saved variables may not be.
+void keep_sink(AutogradContext* ctx, const char* name, const OptTensor& sink) {
+  if (sink.has_value()) ctx->saved_data[name] = *sink;
+}
+at::Tensor kept_sink(AutogradContext* ctx, const char* name) {
+  const auto it = ctx->saved_data.find(name);
+  return it == ctx->saved_data.end() ? at::Tensor() : it->second.toTensor();
+}
+
 bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
 at::Tensor aligned(const at::Tensor& t) {
@@ -89,7 +99,9 @@ struct QkNormNode : Function<QkNormNode> {
     at::Tensor out = at::empty({B, T, Hq + Hk, D}, q.options());
     at::Tensor yq = out.narrow(2, 0, Hq), yk = out.narrow(2, Hq, Hk);
     qk_norm_fwd(qc, kc, qf, kf, ang, pr, yq, yk, eps);
-    ctx->save_for_backward({qc, kc, value(qf), value(kf), value(ang), pr, value(q_sink), value(k_sink)});
+    ctx->save_for_backward({qc, kc, value(qf), value(kf), value(ang), pr});
+    keep_sink(ctx, "q_sink", q_sink);
+    keep_sink(ctx, "k_sink", k_sink);
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["need_qw"] = wants(qw);
     ctx->saved_data["need_kw"] = wants(kw);
@@ -114,11 +126,12 @@ struct QkNormNode : Function<QkNormNode> {
     at::Tensor dq = buf.narrow(2, 0, Hq), dk = buf.narrow(2, Hq, Hk);
     const char* need[2] = {"need_qw", "need_kw"};
     const char* type[2] = {"qw_type", "kw_type"};
+    const at::Tensor sinks[2] = {kept_sink(ctx, "q_sink"), kept_sink(ctx, "k_sink")};
     OptTensor dw[2];
     int64_t accumulate = 0;
     for (int s = 0; s < 2; ++s) {
       if (!ctx->saved_data[need[s]].toBool()) continue;
-      const at::Tensor sink = saved[6 + s];
+      const at::Tensor sink = sinks[s];
       if (sink.defined()) accumulate |= 1 << s;
       dw[s] = sink.defined() ? sink.view({D}) : at::empty({D}, q.options().dtype(at::kFloat));
     }
@@ -196,7 +209,9 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     fp8_gemm(xq.data, xq.scale, false, wq.data, wq.scale, true, K, y, b, res, g, pre, act, false);
     if (!need_g) xq = wq = Q8();
     ctx->save_for_backward({value(pre), value(g), value(b), xt.data, xt.scale, wt.data, wt.scale, xq.data, xq.scale,
-                            wq.data, wq.scale, value(w_sink), value(b_sink)});
+                            wq.data, wq.scale});
+    keep_sink(ctx, "w_sink", w_sink);
+    keep_sink(ctx, "b_sink", b_sink);
     auto& d = ctx->saved_data;
     d["act"] = act;
     d["need_x"] = need_x;
@@ -232,7 +247,7 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
       fp8_gemm(s[7], s[8], false, s[9], s[10], true, K, h, opt(s[2]), {}, {}, {}, act, false);
       dgamma = dz.to(at::kFloat).mul_(h).sum(0).to((at::ScalarType)d["g_type"].toInt());
     }
-    const at::Tensor w_sink = s[11], b_sink = s[12];
+    const at::Tensor w_sink = kept_sink(ctx, "w_sink"), b_sink = kept_sink(ctx, "b_sink");
     at::Tensor db;
     OptTensor sums;
     if (need_b) {

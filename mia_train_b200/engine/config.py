@@ -171,6 +171,9 @@ class TrainerConfig:
     # Data parallelism of the graph step across the dp ranks: "p2p" (sharded optimizer over peer
     # memory), "nccl" (the same over NCCL collectives) or "allreduce" (replicated optimizer).
     graph_dp: str = "p2p"
+    # Products of the transformer blocks' projections: "bf16", or "fp8" (e4m3 with a scale per block of 128,
+    # `ops/fp8.py`; forward and both gradients). "fp8" needs precision = "bf16".
+    linear_precision: str = "bf16"
 
     def __post_init__(self) -> None:
         checks = [
@@ -241,6 +244,14 @@ class TrainerConfig:
             (
                 self.graph_dp in ("p2p", "nccl", "allreduce"),
                 f"graph_dp must be 'p2p', 'nccl' or 'allreduce', got {self.graph_dp!r}",
+            ),
+            (
+                self.linear_precision in ("bf16", "fp8"),
+                f"linear_precision must be 'bf16' or 'fp8', got {self.linear_precision!r}",
+            ),
+            (
+                self.linear_precision != "fp8" or self.precision == "bf16",
+                f"linear_precision = 'fp8' needs precision = 'bf16', got {self.precision!r}",
             ),
         ]
         for ok, message in checks:

@@ -48,6 +48,7 @@ from ..utils.metrics import MetricLogger, reduce_metrics
 from .activation_checkpoint import apply_activation_checkpointing
 from .checkpoint import CheckpointManager
 from .config import TrainerConfig
+from .fp8 import apply_fp8_linears
 from .mfu import ThroughputMeter, measure_step_flops
 from .optimizer import build_lr_scheduler, build_optimizer, clip_grad_norm_, is_stem
 from .profiler import StepProfiler, annotate, current_rank, should_profile
@@ -111,6 +112,8 @@ class Trainer:
         self.output_dir = Path(output_dir)
         self.device = device or torch.device("cpu")
         torch.manual_seed(config.seed)
+        if config.linear_precision == "fp8":
+            apply_fp8_linears(algorithm, self.dims.tp)
         if config.activation_checkpointing:
             apply_activation_checkpointing(algorithm)
         algorithm = algorithm.to(self.device)

@@ -26,8 +26,10 @@ import torch.nn as nn
 
 from ...ops._native import reference_math
 from ...ops.attention import attention, attention_reference, rope_attention
+from ...ops.qk_norm import qk_norm_rope, qk_norm_rope_attention
 from ...parallel.tensor_parallel import rope_to_tp
 from .lora import apply_linear
+from .rms_norm import RMSNorm
 from .rope import RotaryTables
 
 BACKENDS = ("auto", "sdpa", "native", "flash4")
@@ -64,11 +66,24 @@ class _AttentionBase(nn.Module):
         return "sdpa"
 
 
+def head_norms(attn: nn.Module) -> tuple[torch.Tensor, torch.Tensor, float]:
+    """Query and key norm weights and eps of an attention module. Under tensor parallelism they see this
+    rank's heads only, so their gradients are summed over the group, like the rotary angles'."""
+    return rope_to_tp(attn.q_norm.weight, attn), rope_to_tp(attn.k_norm.weight, attn), attn.q_norm.eps
+
+
 class SelfAttention(_AttentionBase):
-    def __init__(self, dim: int, num_heads: int, backend: str = "auto", qkv_bias: bool = True) -> None:
+    """`qk_norm` adds an RMS norm over every query and key head (`q_norm`, `k_norm`, one learned weight of the
+    head size each), applied with the rotation in one kernel."""
+
+    def __init__(
+        self, dim: int, num_heads: int, backend: str = "auto", qkv_bias: bool = True, qk_norm: bool = False
+    ) -> None:
         super().__init__(dim, num_heads, backend)
         self.qkv = nn.Linear(dim, 3 * dim, bias=qkv_bias)
         self.proj = nn.Linear(dim, dim)
+        self.q_norm = RMSNorm(self.head_dim) if qk_norm else None
+        self.k_norm = RMSNorm(self.head_dim) if qk_norm else None
 
     def forward(
         self, x: torch.Tensor, rope: Any = None, residual: torch.Tensor | None = None
@@ -87,8 +102,14 @@ class SelfAttention(_AttentionBase):
         if rope is None or isinstance(rope, RotaryTables):
             angles = rope_to_tp(rope.angles, self) if rope is not None else None
             pairs = rope.pairs if rope is not None else None
+            if self.q_norm is not None:
+                qw, kw, eps = head_norms(self)
+                return qk_norm_rope_attention(qkv, qw, kw, angles, pairs, self.scale, eps)
             return rope_attention(qkv, angles, pairs, self.scale)
         q, k, v = qkv.unbind(dim=2)
+        if self.q_norm is not None:
+            qw, kw, eps = head_norms(self)
+            q, k = qk_norm_rope(q, k, qw, kw, eps=eps)
         return attention(rope(q), rope(k), v, self.scale)
 
 

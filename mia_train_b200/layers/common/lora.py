@@ -7,7 +7,8 @@ to the base. `merge_lora()` folds the delta into the weight and reverts the clas
 
 `apply_linear(module, x, ...)` is how every layer here calls a projection: it runs the native
 fused-epilogue GEMM on the base weight and, for an adapted module, adds the low-rank delta
-`(x A^T) B^T * scaling` (two rank-r GEMMs).
+`(x A^T) B^T * scaling` (two rank-r GEMMs). A module marked by `use_fp8` runs its products in 8-bit
+floating point (`ops.fp8.fp8_linear`).
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ...ops.fp8 import fp8_linear
 from ...ops.linear import linear
 
 
@@ -122,7 +124,20 @@ def apply_linear(
         if gamma is not None:
             y = y * gamma
         return y if residual is None else residual + y
+    if is_fp8(module):
+        return fp8_linear(x, module.weight, b, activation=activation, residual=residual, gamma=gamma)
     return linear(x, module.weight, b, activation=activation, residual=residual, gamma=gamma)
+
+
+def use_fp8(module: nn.Linear) -> None:
+    """Run this projection's products in 8-bit floating point from now on."""
+    if isinstance(module, LoRAMixin) or hasattr(module, "_tp_mode"):
+        raise ValueError("a LoRA-adapted or tensor-parallel layer has no 8-bit products")
+    module._fp8 = True  # type: ignore[assignment]
+
+
+def is_fp8(module: nn.Module) -> bool:
+    return bool(getattr(module, "_fp8", False))
 
 
 def is_adapted(module: nn.Module) -> bool:
@@ -130,5 +145,5 @@ def is_adapted(module: nn.Module) -> bool:
 
 
 def needs_per_layer(module: nn.Module) -> bool:
-    """LoRA-adapted or tensor-parallel: the layer must run through `apply_linear`, not a fused op."""
-    return isinstance(module, LoRAMixin) or hasattr(module, "_tp_mode")
+    """LoRA-adapted, tensor-parallel or 8-bit: the layer must run through `apply_linear`, not a fused op."""
+    return isinstance(module, LoRAMixin) or hasattr(module, "_tp_mode") or is_fp8(module)

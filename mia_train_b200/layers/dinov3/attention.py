@@ -10,6 +10,9 @@ residual add fused into the output projection's epilogue when the block passes t
 attention core the native fused RoPE+attention kernel; the rotation pairs channels (i, i + D/2),
 i.e. `rope_rotate_half`. `use_fa4` is accepted for config compatibility; FlashAttention-4 is not
 part of this framework, so requesting it is an error.
+
+`qk_norm` adds an RMS norm over every query and key head (`q_norm`, `k_norm`), applied with the rotation in
+one kernel. `proj_drop` > 0 drops elements of the projected output in training, fused with the residual add.
 """
 
 from __future__ import annotations
@@ -25,10 +28,13 @@ import torch.nn.functional as F
 
 from ...ops._native import reference_math
 from ...ops.attention import rope_attention
+from ...ops.dropout import dropout
+from ...ops.qk_norm import qk_norm_rope_attention
 from ...parallel.tensor_parallel import rope_to_tp
-from ..common.attention import flash4_status
+from ..common.attention import flash4_status, head_norms
 from ..common.batched_tokens import cat_keep_shapes, uncat_with_shapes
 from ..common.lora import apply_linear
+from ..common.rms_norm import RMSNorm
 from .rope import RopeTables
 
 
@@ -80,6 +86,7 @@ class SelfAttention(nn.Module):
         proj_drop: float = 0.0,
         mask_k_bias: bool = False,
         use_fa4: bool = False,
+        qk_norm: bool = False,
         device=None,
     ) -> None:
         super().__init__()
@@ -94,6 +101,8 @@ class SelfAttention(nn.Module):
         self.attn_drop = nn.Dropout(attn_drop)
         self.proj = nn.Linear(dim, dim, bias=proj_bias, device=device)
         self.proj_drop = nn.Dropout(proj_drop)
+        self.q_norm = RMSNorm(self.head_dim).to(device) if qk_norm else None
+        self.k_norm = RMSNorm(self.head_dim).to(device) if qk_norm else None
         self._pairs: torch.Tensor | None = None
 
     # -- projections ----------------------------------------------------------------------
@@ -128,12 +137,24 @@ class SelfAttention(nn.Module):
             if angles.dim() == 2:
                 angles = angles.unsqueeze(0)
         pairs = self._pairs_on(qkv.device) if angles is not None else None
-        out = rope_attention(qkv, angles, pairs, self.scale)
+        if self.q_norm is not None:
+            qw, kw, eps = head_norms(self)
+            out = qk_norm_rope_attention(qkv, qw, kw, angles, pairs, self.scale, eps)
+        else:
+            out = rope_attention(qkv, angles, pairs, self.scale)
         return out.reshape(b, n, c)
+
+    def project(self, out: torch.Tensor, residual=None, gamma=None) -> torch.Tensor:
+        """`residual + gamma * dropout(proj(out))`."""
+        p = self.proj_drop.p if self.training else 0.0
+        if p == 0.0:
+            return apply_linear(self.proj, out, residual=residual, gamma=gamma)
+        y = apply_linear(self.proj, out, gamma=gamma)  # the per-channel scale commutes with dropout
+        return dropout(y, p, residual=residual.to(y.dtype) if residual is not None else None)
 
     def forward(self, x: torch.Tensor, attn_bias=None, rope=None, residual=None, gamma=None) -> torch.Tensor:
         out = self.compute_attention(self._qkv(x), attn_bias=attn_bias, rope=rope)
-        return apply_linear(self.proj, out, residual=residual, gamma=gamma)
+        return self.project(out, residual=residual, gamma=gamma)
 
     def forward_list(self, x_list, attn_bias=None, rope_list=None, residual_list=None, gamma=None) -> list[torch.Tensor]:
         assert len(x_list) == len(rope_list)
@@ -144,4 +165,4 @@ class SelfAttention(nn.Module):
         res = None
         if residual_list is not None:
             res, _, _ = cat_keep_shapes(residual_list)
-        return uncat_with_shapes(apply_linear(self.proj, flat, residual=res, gamma=gamma), shapes, counts)
+        return uncat_with_shapes(self.project(flat, residual=res, gamma=gamma), shapes, counts)

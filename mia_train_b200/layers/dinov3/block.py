@@ -53,13 +53,14 @@ class SelfAttentionBlock(nn.Module):
         ffn_layer: Callable[..., Mlp | SwiGLUFFN] = Mlp,
         mask_k_bias: bool = False,
         use_fa4: bool = False,
+        qk_norm: bool = False,
         device=None,
     ) -> None:
         super().__init__()
         self.norm1 = norm_layer(dim)
         self.attn: SelfAttention = attn_class(
             dim, num_heads=num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias, attn_drop=attn_drop,
-            proj_drop=drop, mask_k_bias=mask_k_bias, use_fa4=use_fa4, device=device,
+            proj_drop=drop, mask_k_bias=mask_k_bias, use_fa4=use_fa4, qk_norm=qk_norm, device=device,
         )
         self.ls1: nn.Module = LayerScale(dim, init_values=init_values, device=device) if init_values else nn.Identity()
         self.norm2 = norm_layer(dim)
@@ -126,9 +127,7 @@ class SelfAttentionBlock(nn.Module):
             raise NotImplementedError("blocks with a custom attention core do not support drop_path > 0")
         h = _norm(self.norm1, x)
         out = attention(self.attn, self.attn._qkv(h))
-        from ..common.lora import apply_linear
-
-        x_attn = apply_linear(self.attn.proj, out, residual=x, gamma=self._gamma(self.ls1))
+        x_attn = self.attn.project(out, residual=x, gamma=self._gamma(self.ls1))
         return self.mlp.forward(_norm(self.norm2, x_attn), residual=x_attn, gamma=self._gamma(self.ls2))
 
     def forward(self, x_or_x_list, rope_or_rope_list=None, *, attention: Callable | None = None, sp=None,

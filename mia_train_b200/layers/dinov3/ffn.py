@@ -3,7 +3,8 @@
 `Mlp` (fc1 -> GELU -> fc2) and `SwiGLUFFN` (w3(silu(w1 x) * w2 x), hidden = ceil(2/3 h) aligned),
 with `forward_list` over concatenated crops. `forward(x, residual=, gamma=)` fuses the block's
 LayerScale and residual add into the last projection's epilogue; `Mlp` runs fc1+GELU+fc2 as one
-native MLP node when neither projection is LoRA-adapted.
+native MLP node when neither projection is LoRA-adapted. With `drop` > 0 in training, both layers drop
+elements of the hidden activations and of the output (fused with the residual add).
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ...ops.dropout import dropout
 from ...ops.mlp import mlp
 from ..common.batched_tokens import cat_keep_shapes, uncat_with_shapes
 from ..common.lora import apply_linear, needs_per_layer
@@ -27,6 +29,12 @@ class ListForwardMixin:
         flat, shapes, counts = cat_keep_shapes(x_list)
         res = cat_keep_shapes(residual_list)[0] if residual_list is not None else None
         return uncat_with_shapes(self.forward(flat, residual=res, gamma=gamma), shapes, counts)
+
+
+def _dropped(last: nn.Linear, h: torch.Tensor, p: float, residual, gamma) -> torch.Tensor:
+    """`residual + gamma * dropout(last(h))`; the per-channel scale commutes with dropout."""
+    y = apply_linear(last, h, gamma=gamma)
+    return dropout(y, p, residual=residual.to(y.dtype) if residual is not None else None)
 
 
 class Mlp(nn.Module, ListForwardMixin):
@@ -49,12 +57,10 @@ class Mlp(nn.Module, ListForwardMixin):
         self.drop = nn.Dropout(drop)
 
     def forward(self, x: torch.Tensor, residual=None, gamma=None) -> torch.Tensor:
-        if self.training and self.drop.p > 0:  # dropout between the layers: unfused
-            y = self.drop(apply_linear(self.fc2, self.drop(self.act(apply_linear(self.fc1, x)))))
-            if gamma is not None:
-                y = y * gamma
-            return y if residual is None else residual + y
         exact_gelu = isinstance(self.act, nn.GELU) and getattr(self.act, "approximate", "none") == "none"
+        if self.training and self.drop.p > 0:
+            h = apply_linear(self.fc1, x, activation="gelu") if exact_gelu else self.act(apply_linear(self.fc1, x))
+            return _dropped(self.fc2, dropout(h, self.drop.p), self.drop.p, residual, gamma)
         if exact_gelu and gamma is None and not (needs_per_layer(self.fc1) or needs_per_layer(self.fc2)):
             return mlp(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, residual=residual)
         h = apply_linear(self.fc1, x, activation="gelu") if exact_gelu else self.act(apply_linear(self.fc1, x))
@@ -81,7 +87,10 @@ class SwiGLUFFN(nn.Module, ListForwardMixin):
         self.w1 = nn.Linear(in_features, hidden, bias=bias, device=device)
         self.w2 = nn.Linear(in_features, hidden, bias=bias, device=device)
         self.w3 = nn.Linear(hidden, out_features, bias=bias, device=device)
+        self.drop = nn.Dropout(drop)
 
     def forward(self, x: torch.Tensor, residual=None, gamma=None) -> torch.Tensor:
         hidden = F.silu(apply_linear(self.w1, x)) * apply_linear(self.w2, x)
+        if self.training and self.drop.p > 0:
+            return _dropped(self.w3, dropout(hidden, self.drop.p), self.drop.p, residual, gamma)
         return apply_linear(self.w3, hidden, residual=residual, gamma=gamma)

@@ -18,7 +18,9 @@ import torch
 import torch.nn.functional as F
 
 from ...ops.attention import attention, rope_attention
+from ...ops.qk_norm import qk_norm_rope
 from ...parallel.tensor_parallel import rope_to_tp
+from ..common.attention import head_norms
 from .block import SelfAttentionBlock
 from .rope import RopeTables
 
@@ -55,6 +57,11 @@ def windowed_attention(
     b, n_tok, _ = qkv.shape
     heads, hd = attn.num_heads, attn.head_dim
     c = heads * hd
+    if attn.q_norm is not None:  # norm per token and head: the same in every window
+        qw, kw, eps = head_norms(attn)
+        q, k, v = qkv.reshape(b, n_tok, 3, heads, hd).unbind(2)
+        q, k = qk_norm_rope(q, k, qw, kw, eps=eps)
+        qkv = torch.stack([q, k, v], dim=2).reshape(b, n_tok, 3 * c)
     pre, pat = qkv[:, :n_prefix], qkv[:, n_prefix:]
     nwin = (grid[0] // w) * (grid[1] // w) * (grid[2] // w)
     win = window_partition(pat, grid, w)  # (B*nw, w^3, 3C)

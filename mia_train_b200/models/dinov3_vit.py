@@ -52,6 +52,8 @@ class DinoVisionTransformer(DinoVisionTransformer3D):
         use_fa4: bool = False,
         untie_cls_and_patch_norms: bool = False,
         untie_global_and_local_cls_norm: bool = False,
+        qk_norm: bool = False,
+        drop_rate: float = 0.0,
         device: Any | None = None,
     ) -> None:
         super().__init__(
@@ -66,7 +68,8 @@ class DinoVisionTransformer(DinoVisionTransformer3D):
             drop_path_rate=drop_path_rate, layerscale_init=layerscale_init, norm_layer=norm_layer,
             ffn_layer=ffn_layer, ffn_bias=ffn_bias, proj_bias=proj_bias, n_storage_tokens=n_storage_tokens,
             mask_k_bias=mask_k_bias, use_fa4=use_fa4, untie_cls_and_patch_norms=untie_cls_and_patch_norms,
-            untie_global_and_local_cls_norm=untie_global_and_local_cls_norm, device=device,
+            untie_global_and_local_cls_norm=untie_global_and_local_cls_norm, qk_norm=qk_norm, drop_rate=drop_rate,
+            device=device,
         )
 
     def _make_patch_embed(self, img_size, patch_size, in_chans, embed_dim) -> nn.Module:

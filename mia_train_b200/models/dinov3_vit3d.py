@@ -99,6 +99,8 @@ class DinoVisionTransformer3D(BaseModel):
         untie_global_and_local_cls_norm: bool = False,
         window_size: int = 0,
         global_every: int = 0,
+        qk_norm: bool = False,
+        drop_rate: float = 0.0,
         device: Any | None = None,
     ) -> None:
         super().__init__()
@@ -110,6 +112,8 @@ class DinoVisionTransformer3D(BaseModel):
             raise ValueError(f"unknown pos_embed_rope_dtype {pos_embed_rope_dtype!r}; expected one of {sorted(dtype_dict)}")
         if pos_embed_rope_type not in ROPE_TYPES:
             raise ValueError(f"unknown pos_embed_rope_type {pos_embed_rope_type!r}; expected one of {list(ROPE_TYPES)}")
+        if not 0.0 <= drop_rate < 1.0:
+            raise ValueError(f"drop_rate must be in [0, 1), got {drop_rate}")
         if window_size < 0 or global_every < 0:
             raise ValueError("window_size and global_every must be >= 0")
         norm_cls = norm_layer_dict[norm_layer]
@@ -140,7 +144,7 @@ class DinoVisionTransformer3D(BaseModel):
                 dim=embed_dim, num_heads=num_heads, ffn_ratio=ffn_ratio, qkv_bias=qkv_bias, proj_bias=proj_bias,
                 ffn_bias=ffn_bias, drop_path=drop_path_rate, norm_layer=norm_cls, act_layer=nn.GELU,
                 ffn_layer=ffn_cls, init_values=layerscale_init, mask_k_bias=mask_k_bias, use_fa4=use_fa4,
-                device=device,
+                qk_norm=qk_norm, drop=drop_rate, device=device,
             )
             for _ in range(depth)
         )

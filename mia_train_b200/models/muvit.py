@@ -40,6 +40,8 @@ class MuViT3D(BaseModel):
         mlp_ratio: float = 2.0,
         attention_backend: str = "auto",
         rotary_base: float = 10000.0,
+        qk_norm: bool = False,
+        dropout: float = 0.0,
     ) -> None:
         super().__init__()
         levels = tuple(levels)
@@ -76,7 +78,7 @@ class MuViT3D(BaseModel):
         nn.init.trunc_normal_(self.level_embed, std=0.02)
         self.blocks = nn.ModuleList(
             TransformerBlock(embed_dim, num_heads, mlp_ratio, attention_backend, spatial_rank=SPATIAL_RANK,
-                             rotary_base=rotary_base)
+                             rotary_base=rotary_base, qk_norm=qk_norm, dropout=dropout)
             for _ in range(depth)
         )
         self.norm = nn.LayerNorm(embed_dim)

@@ -12,6 +12,8 @@ Differences:
 * `pos_embed = "rope" | "sincos" | "learned"`. The reference has RoPE only (the default here);
   "sincos" adds a fixed 3D sin-cos table and "learned" a trainable one (`pos_embed` parameter) to
   the tokens instead of rotating attention.
+* `qk_norm` normalises query and key heads; `dropout` drops hidden activations and branch outputs in
+  training. Both default to off, as in the reference.
 """
 
 from __future__ import annotations
@@ -66,6 +68,8 @@ class ViT3D(BaseModel):
         attention_backend: str = "auto",
         rotary_base: float = 10000.0,
         pos_embed: str = "rope",
+        qk_norm: bool = False,
+        dropout: float = 0.0,
     ) -> None:
         super().__init__()
         img_size = tuple(img_size)  # type: ignore[assignment]
@@ -93,7 +97,7 @@ class ViT3D(BaseModel):
         self.blocks = nn.ModuleList(
             TransformerBlock(
                 embed_dim, num_heads, mlp_ratio, attention_backend,
-                spatial_rank=SPATIAL_RANK, rotary_base=rotary_base, rotary=use_rope,
+                spatial_rank=SPATIAL_RANK, rotary_base=rotary_base, rotary=use_rope, qk_norm=qk_norm, dropout=dropout,
             )
             for _ in range(depth)
         )

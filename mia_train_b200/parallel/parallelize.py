@@ -54,6 +54,14 @@ def _apply_tensor_parallel(model: nn.Module, mesh: DeviceMesh, dims: ParallelDim
             f"tensor parallelism (tp = {dims.tp}, tp_comm = {dims.tp_comm!r}): set [model] drop_path_rate = 0, "
             "use tp_comm = \"allreduce\", or train with data parallelism"
         )
+    dropped = [name for name, m in model.named_modules()
+               if getattr(m, "dropout", 0.0) or (isinstance(m, nn.Dropout) and m.p > 0.0)]
+    if dropped:
+        # every rank would have to draw the mask of the elements it holds
+        raise ValueError(
+            f"dropout ({dropped[0]}, ... {len(dropped)} modules) cannot be combined with tensor parallelism "
+            f"(tp = {dims.tp}): set the model's dropout to 0 or train with data parallelism"
+        )
     plan = model.tensor_parallel_plan() if isinstance(model, BaseModel) else None
     if plan is None:
         raise ValueError(
