@@ -13,11 +13,16 @@
 //   da_p  = n[i] dn[j] - n[j] dn[i], summed over the token's query and key heads; dn[c'] needs only
 //           dy[c'] C[c] + dy[c] S[c], which the lane of c has, so each lane adds +-n[c] dn[c'] alone
 //
-// One warp per token. The sine and cosine of the token's angles are computed once and kept by every
-// lane for its eight channels; the warp then walks the token's query and key heads, 256 / D' of them
-// at a time (D' = D rounded up to a power of two, D' / 8 lanes a head), 16 bytes a lane. Partners are
-// exchanged through shared memory at index c + c / 8, which spreads the stride of eight between lanes
-// over all banks. Each element is read once and written once: the kernels are bound by HBM.
+// A warp walks whole tokens (forward: query and key heads in turn; backward: one warp of a pair the query
+// heads, the other the key heads, their parts of da_p joined in shared memory). The sine and cosine of the
+// token's angles are computed once and kept by every lane for its eight channels; the heads then pass
+// 256 / D' at a time (D' = D rounded up to a power of two, D' / 8 lanes a head), 16 bytes a lane. The grid
+// is as large as fits on the SMs at once; a warp loads several such steps together, the next ones (of the
+// next token as well) while it works on the last, and the next token's angles with them.
+// Partners: where every lane's eight channels are paired with eight channels of one other lane (rotation
+// by halves of a head of a power-of-two size), by shuffles; otherwise (axial chunks) through shared memory
+// at index c + c / 8, which spreads the stride of eight between lanes over all banks. Each element is read
+// once and written once: the kernels are bound by HBM.
 // Weight gradients: registers over a warp's tokens, one partial a CTA, summed in a fixed order by a
 // second kernel, so the result does not depend on the order in which CTAs run.
 #include <ATen/cuda/CUDAContext.h>
@@ -50,7 +55,8 @@ struct QkNormParams {
   int P;
   float* dangles;   // (B, T, P) or nullptr
   float* dw_parts;  // (CTAs, 2, D) or nullptr
-  int B, T, D;
+  unsigned B, T;
+  int D;
   float eps;
 };
 
@@ -63,13 +69,14 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// Head h of token `token` of the flattened (B, T); tokens are counted in 32 bits (64-bit division is slow).
 template <typename T>
-__device__ __forceinline__ T* head_ptr(const HeadView& v, int64_t b, int64_t t, int h) {
-  return reinterpret_cast<T*>(v.p) + b * v.sb + t * v.st + h * v.sh;
+__device__ __forceinline__ T* head_ptr(const HeadView& v, unsigned token, unsigned length, int h) {
+  const unsigned b = token / length, t = token - b * length;
+  return reinterpret_cast<T*>(v.p) + (int64_t)b * v.sb + (int64_t)t * v.st + (int64_t)h * v.sh;
 }
 
-// Shared memory of one CTA: the partner of each channel and the sign of its contribution to the
-// angle gradient, then per warp the token's (C, S) table and the exchange rows.
+// Shared memory of one CTA: per warp the token's (C, S) table and the exchange rows; the partner of each channel.
 template <int LPR>
 struct QkSmem {
   static constexpr int kRows = 32 / LPR;             // heads a warp holds at a time
@@ -78,127 +85,206 @@ struct QkSmem {
   float2 cs[kQkWarps][kCh];
   float ex[kQkWarps][kRows][kRowFloats];
   int partner[kCh];
-  float sign[kCh];
+  int2 pairs[kCh / 2];  // x < 0: left out
+  float da[kQkWarps][kRowFloats];  // backward: each warp's part of the token's angle gradient
+  int scattered;  // not 0: some lane's channels are paired with channels of several lanes
 };
 
-// Fills partner / sign; a pair that names a channel outside the head is left out.
+constexpr int kQkAhead = 4;  // steps whose loads are in flight together (backward: half of them, for x and dy)
+
+// Fills partner and pairs; a pair that names a channel outside the head is left out.
 template <int LPR>
 __device__ __forceinline__ void qk_partners(QkSmem<LPR>& sm, const QkNormParams& p) {
+  if (threadIdx.x == 0) sm.scattered = 0;
   for (int c = threadIdx.x; c < QkSmem<LPR>::kCh; c += blockDim.x) {
     sm.partner[c] = c;
-    sm.sign[c] = 0.f;
   }
   __syncthreads();
+  for (int c = threadIdx.x; c < kQkWarps * QkSmem<LPR>::kCh; c += blockDim.x) (&sm.cs[0][0])[c] = make_float2(1.f, 0.f);
   if (p.angles != nullptr)
     for (int i = threadIdx.x; i < p.P; i += blockDim.x) {
       const int a = p.pairs[2 * i], b = p.pairs[2 * i + 1];
+      sm.pairs[i] = make_int2(-1, -1);
       if ((unsigned)a < (unsigned)p.D && (unsigned)b < (unsigned)p.D && a != b) {
         sm.partner[a] = b;
         sm.partner[b] = a;
-        sm.sign[a] = 1.f;
-        sm.sign[b] = -1.f;
+        sm.pairs[i] = make_int2(a, b);
       }
     }
   __syncthreads();
+  for (int c = threadIdx.x; c < QkSmem<LPR>::kCh; c += blockDim.x)
+    if (sm.partner[c] != (sm.partner[c & ~7] & ~7) + (c & 7)) sm.scattered = 1;
+  __syncthreads();
 }
 
-// The (C, S) table of token (b, t), by one warp.
+// The values of this lane's partner channels.
 template <int LPR>
-__device__ __forceinline__ void qk_table(QkSmem<LPR>& sm, const QkNormParams& p, int warp, int lane, int64_t b,
-                                         int64_t t) {
-  __syncwarp();
-  for (int c = lane; c < QkSmem<LPR>::kCh; c += 32) sm.cs[warp][c] = make_float2(1.f, 0.f);
+__device__ __forceinline__ void qk_exchange(const float (&v)[8], float (&o)[8], float* ex, int cg, const int (&part)[8],
+                                            bool scattered, int source) {
+  if (scattered) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ex[cg * 9 + j] = v[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = ex[part[j]];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = __shfl_sync(0xffffffffu, v[j], source);
+  }
+}
+
+// A token's angles, lane i holding i, i + 32, ...
+constexpr int kQkAngles = kQkMaxD / 2 / 32;
+__device__ __forceinline__ void qk_fetch_angles(const QkNormParams& p, unsigned token, int lane, float (&ang)[kQkAngles]) {
+  if (p.angles == nullptr) return;
+  const unsigned b = token / p.T, t = token - b * p.T;
+  const float* a = p.angles + (int64_t)b * p.angle_bstride + (int64_t)t * p.P;
+#pragma unroll
+  for (int k = 0; k < kQkAngles; ++k)
+    if (lane + 32 * k < p.P) ang[k] = a[lane + 32 * k];
+}
+
+// The (C, S) table of a token, by one warp; entries of unpaired channels stay (1, 0) from the start.
+template <int LPR>
+__device__ __forceinline__ void qk_table(float2* cs, const QkNormParams& p, const int2* pairs, int lane,
+                                         const float (&ang)[kQkAngles]) {
   __syncwarp();
   if (p.angles != nullptr) {
-    const float* ang = p.angles + b * p.angle_bstride + t * p.P;
-    for (int i = lane; i < p.P; i += 32) {
-      const int a = p.pairs[2 * i], c = p.pairs[2 * i + 1];
-      if ((unsigned)a < (unsigned)p.D && (unsigned)c < (unsigned)p.D && a != c) {
+#pragma unroll
+    for (int k = 0; k < kQkAngles; ++k) {
+      const int i = lane + 32 * k;
+      if (i < p.P && pairs[i].x >= 0) {
         float s, co;
-        sincosf(ang[i], &s, &co);
-        sm.cs[warp][a] = make_float2(co, -s);
-        sm.cs[warp][c] = make_float2(co, s);
+        sincosf(ang[k], &s, &co);
+        cs[pairs[i].x] = make_float2(co, -s);
+        cs[pairs[i].y] = make_float2(co, s);
       }
     }
   }
   __syncwarp();
 }
 
-template <typename T, int LPR>
-__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_fwd_kernel(const QkNormParams p) {
-  using S = QkSmem<LPR>;
-  __shared__ S sm;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int row = lane / LPR, cg = lane % LPR;
-  const bool on = cg * 8 < p.D;
-  qk_partners<LPR>(sm, p);
-  const int64_t token = (int64_t)blockIdx.x * kQkWarps + warp;
-  if (token >= (int64_t)p.B * p.T) return;
-  const int64_t b = token / p.T, t = token % p.T;
-  qk_table<LPR>(sm, p, warp, lane, b, t);
-  float C[8], Sn[8];
-  int part[8];
+// Loads of kAhead steps of a warp's walk: heads h0 + row, h0 + row + kRows, ...
+template <typename T, int LPR, int AHEAD>
+__device__ __forceinline__ void qk_load(const HeadView& v, const QkNormParams& p, unsigned token, int h0, int row, int cg,
+                                        bool on, Raw8<T> (&raw)[AHEAD]) {
+  const T* src = head_ptr<const T>(v, token, p.T, h0 + row) + cg * 8;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float2 v = sm.cs[warp][cg * 8 + j];
-    C[j] = v.x;
-    Sn[j] = v.y;
-    part[j] = qk_pad(sm.partner[cg * 8 + j]);
-  }
-  const float inv_d = 1.f / (float)p.D;
-  float* ex = sm.ex[warp][row];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
-    for (int h0 = 0; h0 < p.x[s].heads; h0 += S::kRows) {
-      const int h = h0 + row;
-      const bool live = on && h < p.x[s].heads;
-      float v[8] = {};
-      if (live) unpack8(load_raw8(head_ptr<const T>(p.x[s], b, t, h) + cg * 8), v);
-      float ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-      const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = v[j] * r * w[j];
-        ex[cg * 9 + j] = v[j];
-      }
-      __syncwarp();
-      float o[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = fmaf(ex[part[j]], Sn[j], v[j] * C[j]);
-      __syncwarp();
-      if (live) store8(head_ptr<T>(p.y[s], b, t, h) + cg * 8, o);
-    }
+  for (int u = 0; u < AHEAD; ++u) {
+    const int h = u * (32 / LPR);
+    raw[u] = on && h0 + h + row < v.heads ? load_raw8(src + h * v.sh) : Raw8<T>{};
   }
 }
 
 template <typename T, int LPR>
-__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_bwd_kernel(const QkNormParams p) {
+__global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_fwd_kernel(const QkNormParams p) {
   using S = QkSmem<LPR>;
+  constexpr int kAhead = sizeof(T) == 2 ? kQkAhead : kQkAhead / 2;
   __shared__ S sm;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int row = lane / LPR, cg = lane % LPR;
   const bool on = cg * 8 < p.D;
+  const unsigned tokens = p.B * p.T, stride = gridDim.x * kQkWarps;
+  unsigned token = blockIdx.x * kQkWarps + warp;
+  float ang[kQkAngles] = {};
+  Raw8<T> next[kAhead];
+  if (token < tokens) {
+    qk_fetch_angles(p, token, lane, ang);
+    qk_load<T, LPR>(p.x[0], p, token, 0, row, cg, on, next);
+  }
   qk_partners<LPR>(sm, p);
+  if (token >= tokens) return;
+  float w[2][8], C[8], Sn[8];
   int part[8];
-  float sign[8], w[2][8], dw[2][8] = {};
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     part[j] = qk_pad(sm.partner[cg * 8 + j]);
-    sign[j] = sm.sign[cg * 8 + j];
 #pragma unroll
     for (int s = 0; s < 2; ++s) w[s][j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
   }
+  const bool scattered = sm.scattered != 0;
+  const int source = row * LPR + sm.partner[cg * 8] / 8;
   const float inv_d = 1.f / (float)p.D;
   float* ex = sm.ex[warp][row];
-  const int64_t tokens = (int64_t)p.B * p.T;
-  for (int64_t token = (int64_t)blockIdx.x * kQkWarps + warp; token < tokens; token += (int64_t)gridDim.x * kQkWarps) {
-    const int64_t b = token / p.T, t = token % p.T;
-    qk_table<LPR>(sm, p, warp, lane, b, t);
+  for (; token < tokens; token += stride) {
+    qk_table<LPR>(sm.cs[warp], p, sm.pairs, lane, ang);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 v = sm.cs[warp][cg * 8 + j];
+      C[j] = v.x;
+      Sn[j] = v.y;
+    }
+    const unsigned after = token + stride;
+    if (after < tokens) qk_fetch_angles(p, after, lane, ang);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      T* const dst = head_ptr<T>(p.y[s], token, p.T, row) + cg * 8;
+      const int heads = p.x[s].heads;
+      for (int h0 = 0; h0 < heads; h0 += kAhead * S::kRows) {
+        Raw8<T> raw[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
+        if (h0 + kAhead * S::kRows < heads) qk_load<T, LPR>(p.x[s], p, token, h0 + kAhead * S::kRows, row, cg, on, next);
+        else if (s == 0 && p.x[1].heads > 0) qk_load<T, LPR>(p.x[1], p, token, 0, row, cg, on, next);
+        else if (after < tokens) qk_load<T, LPR>(p.x[0], p, after, 0, row, cg, on, next);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int h = h0 + u * S::kRows;
+          if (h >= heads) break;
+          float v[8], o[8];
+          unpack8(raw[u], v);
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+          const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[s][j];
+          qk_exchange<LPR>(v, o, ex, cg, part, scattered, source);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], Sn[j], v[j] * C[j]);
+          if (on && h + row < heads) store8(dst + h * p.y[s].sh, o);
+        }
+      }
+    }
+  }
+}
+
+// Warps 2 i and 2 i + 1 walk the same tokens, the first their query heads, the second their key heads.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkNormParams p) {
+  using S = QkSmem<LPR>;
+  constexpr int kAhead = sizeof(T) == 2 ? kQkAhead / 2 : 1;
+  constexpr int kPairs = kQkWarps / 2;
+  __shared__ S sm;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int pair = warp / 2, s = warp % 2;
+  const int row = lane / LPR, cg = lane % LPR;
+  const bool on = cg * 8 < p.D;
+  const unsigned tokens = p.B * p.T, stride = gridDim.x * kPairs;
+  unsigned token = blockIdx.x * kPairs + pair;
+  const HeadView xv = p.x[s], gv = p.dy[s], yv = p.y[s];
+  float ang[kQkAngles] = {};
+  Raw8<T> next_x[kAhead], next_g[kAhead];
+  if (token < tokens) {
+    qk_fetch_angles(p, token, lane, ang);
+    qk_load<T, LPR>(xv, p, token, 0, row, cg, on, next_x);
+    qk_load<T, LPR>(gv, p, token, 0, row, cg, on, next_g);
+  }
+  qk_partners<LPR>(sm, p);
+  int part[8];
+  float w[8], dw[8] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    part[j] = qk_pad(sm.partner[cg * 8 + j]);
+    w[j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
+  }
+  const bool scattered = sm.scattered != 0;
+  const int source = row * LPR + sm.partner[cg * 8] / 8;
+  const float inv_d = 1.f / (float)p.D;
+  float* ex = sm.ex[warp][row];
+  for (; token < tokens; token += stride) {
+    qk_table<LPR>(sm.cs[warp], p, sm.pairs, lane, ang);
     float C[8], Sn[8], da[8] = {};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -206,81 +292,88 @@ __global__ void __launch_bounds__(32 * kQkWarps) qk_norm_bwd_kernel(const QkNorm
       C[j] = v.x;
       Sn[j] = v.y;
     }
+    const unsigned after = token + stride;
+    if (after < tokens) qk_fetch_angles(p, after, lane, ang);
+    // dx may overwrite dy: a lane has loaded all it needs of a head before it stores there
+    T* const dst = head_ptr<T>(yv, token, p.T, row) + cg * 8;
+    for (int h0 = 0; h0 < xv.heads; h0 += kAhead * S::kRows) {
+      Raw8<T> xr[kAhead], gr[kAhead];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      for (int h0 = 0; h0 < p.x[s].heads; h0 += S::kRows) {
-        const int h = h0 + row;
-        const bool live = on && h < p.x[s].heads;
-        float v[8] = {}, g[8] = {};
-        if (live) {
-          const Raw8<T> xr = load_raw8(head_ptr<const T>(p.x[s], b, t, h) + cg * 8);
-          unpack8(load_raw8(head_ptr<const T>(p.dy[s], b, t, h) + cg * 8), g);
-          unpack8(xr, v);
-        }
+      for (int u = 0; u < kAhead; ++u) {
+        xr[u] = next_x[u];
+        gr[u] = next_g[u];
+      }
+      const bool more = h0 + kAhead * S::kRows < xv.heads;
+      if (more || after < tokens) {
+        qk_load<T, LPR>(xv, p, more ? token : after, more ? h0 + kAhead * S::kRows : 0, row, cg, on, next_x);
+        qk_load<T, LPR>(gv, p, more ? token : after, more ? h0 + kAhead * S::kRows : 0, row, cg, on, next_g);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int h = h0 + u * S::kRows;
+        if (h >= xv.heads) break;
+        float v[8], g[8], other[8];
+        unpack8(xr[u], v);
+        unpack8(gr[u], g);
         float ss = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ss = fmaf(v[j], v[j], ss);
-          ex[cg * 9 + j] = g[j];
-        }
+        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
         const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
-        __syncwarp();
+        qk_exchange<LPR>(g, other, ex, cg, part, scattered, source);
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float other = ex[part[j]];
-          const float dn = fmaf(-other, Sn[j], g[j] * C[j]);
-          const float dn_other = fmaf(g[j], Sn[j], other * C[j]);
+          const float dn = fmaf(-other[j], Sn[j], g[j] * C[j]);
+          const float dn_other = fmaf(g[j], Sn[j], other[j] * C[j]);
           v[j] *= r;  // normalised
-          da[j] = fmaf(sign[j] * v[j] * w[s][j], dn_other, da[j]);
-          dw[s][j] = fmaf(dn, v[j], dw[s][j]);
-          g[j] = dn * w[s][j];
+          da[j] = fmaf(v[j] * w[j], dn_other, da[j]);
+          dw[j] = fmaf(dn, v[j], dw[j]);
+          g[j] = dn * w[j];
           dot = fmaf(g[j], v[j], dot);
         }
         const float m = group_sum<LPR>(dot) * inv_d;
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = r * fmaf(-v[j], m, g[j]);
-        __syncwarp();
-        if (live) store8(head_ptr<T>(p.y[s], b, t, h) + cg * 8, g);
+        if (on && h + row < xv.heads) store8(dst + h * yv.sh, g);
       }
     }
     if (p.dangles != nullptr) {
-      // the rows of the warp hold parts of the same channels: add them, then the two channels of a pair
+      // the rows of a warp, then the pair's two warps, hold parts of the same channels; then the two channels of
+      // a rotated pair, with opposite signs
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
 #pragma unroll
         for (int o = LPR; o < 32; o <<= 1) da[j] += __shfl_xor_sync(0xffffffffu, da[j], o);
-        if (row == 0) sm.ex[warp][0][cg * 9 + j] = da[j];
+        if (row == 0) sm.da[warp][cg * 9 + j] = da[j];
       }
-      __syncwarp();
-      float* out = p.dangles + token * p.P;
-      for (int i = lane; i < p.P; i += 32) {
-        const int a = p.pairs[2 * i], c = p.pairs[2 * i + 1];
-        const bool ok = (unsigned)a < (unsigned)p.D && (unsigned)c < (unsigned)p.D && a != c;
-        out[i] = ok ? sm.ex[warp][0][qk_pad(a)] + sm.ex[warp][0][qk_pad(c)] : 0.f;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory");
+      float* out = p.dangles + (int64_t)token * p.P;
+      const float *dq = sm.da[warp - s], *dk = sm.da[warp - s + 1];
+      for (int i = lane + 32 * s; i < p.P; i += 64) {
+        const int2 ch = sm.pairs[i];
+        const int a = qk_pad(max(ch.x, 0)), c = qk_pad(max(ch.y, 0));
+        out[i] = ch.x < 0 ? 0.f : (dq[a] + dk[a]) - (dq[c] + dk[c]);
       }
+      asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory");
     }
   }
   if (p.dw_parts != nullptr) {
-    // rows of a warp by shuffles, warps through shared memory in warp order
+    // rows of a warp by shuffles, the CTA's warps of one kind through shared memory in warp order
     float* red = reinterpret_cast<float*>(&sm.cs[0][0]);  // kQkWarps x kCh floats of the table's float2s
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int j = 0; j < 8; ++j) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int o = LPR; o < 32; o <<= 1) dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], o);
+      if (row == 0) red[warp * S::kCh + cg * 8 + j] = dw[j];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * p.D; c += blockDim.x) {
+      const int kind = c / p.D, ch = c % p.D;
+      float a = 0.f;
 #pragma unroll
-        for (int o = LPR; o < 32; o <<= 1) dw[s][j] += __shfl_xor_sync(0xffffffffu, dw[s][j], o);
-        if (row == 0) red[warp * S::kCh + cg * 8 + j] = dw[s][j];
-      }
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.D; c += blockDim.x) {
-        float a = 0.f;
-#pragma unroll
-        for (int k = 0; k < kQkWarps; ++k) a += red[k * S::kCh + c];
-        p.dw_parts[((int64_t)blockIdx.x * 2 + s) * p.D + c] = a;
-      }
-      __syncthreads();
+      for (int k = 0; k < kPairs; ++k) a += red[(2 * k + kind) * S::kCh + ch];
+      p.dw_parts[((int64_t)blockIdx.x * 2 + kind) * p.D + ch] = a;
     }
   }
 }
@@ -325,11 +418,12 @@ static QkNormParams qk_params(const torch::Tensor& q, const torch::Tensor& k, co
   QkNormParams p{};
   TORCH_CHECK(q.dim() == 4 && q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= kQkMaxD,
               "qk_norm: head size must be a multiple of 8 up to ", kQkMaxD);
-  TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX, "qk_norm: batch or length too large");
+  TORCH_CHECK(q.size(0) * q.size(1) < (1ll << 30), "qk_norm: too many tokens");
+  TORCH_CHECK(q.size(2) >= 1 && k.size(2) >= 1, "qk_norm: at least one query and one key head");
   p.x[0] = head_view(q, q, "q");
   p.x[1] = head_view(k, q, "k");
-  p.B = (int)q.size(0);
-  p.T = (int)q.size(1);
+  p.B = (unsigned)q.size(0);
+  p.T = (unsigned)q.size(1);
   p.D = (int)q.size(3);
   p.eps = (float)eps;
   const c10::optional<torch::Tensor>* ws[2] = {&qw, &kw};
@@ -382,10 +476,10 @@ void qk_norm_fwd(torch::Tensor q, torch::Tensor k, c10::optional<torch::Tensor> 
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int64_t tokens = (int64_t)p.B * p.T;
   if (tokens == 0) return;
-  const int64_t blocks = (tokens + kQkWarps - 1) / kQkWarps;
-  TORCH_CHECK(blocks <= INT32_MAX, "qk_norm: too many tokens");
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int blocks = (int)std::min<int64_t>((tokens + kQkWarps - 1) / kQkWarps, 4 * sms);
   qk_dispatch(q, p.D, [&](auto type, auto lanes) {
-    qk_norm_fwd_kernel<decltype(type), decltype(lanes)::value><<<(unsigned)blocks, 32 * kQkWarps, 0, stream>>>(p);
+    qk_norm_fwd_kernel<decltype(type), decltype(lanes)::value><<<blocks, 32 * kQkWarps, 0, stream>>>(p);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -429,7 +523,7 @@ void qk_norm_bwd(torch::Tensor dyq, torch::Tensor dyk, torch::Tensor q, torch::T
     return;
   }
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int blocks = (int)std::min<int64_t>((tokens + kQkWarps - 1) / kQkWarps, 4 * sms);
+  const int blocks = (int)std::min<int64_t>((tokens + kQkWarps / 2 - 1) / (kQkWarps / 2), 4 * sms);
   torch::Tensor parts;
   if (want_dw) {
     parts = torch::empty({blocks, 2, p.D}, q.options().dtype(at::kFloat));
