@@ -162,8 +162,8 @@ __device__ __forceinline__ void tc_mma_f8_block(uint32_t d_tmem, uint64_t a_desc
 
 // 128 accumulators a thread (BN = 256) need more than the 168 registers that 384 threads can start with:
 // the four control warps hand theirs down. 128 * 40 + 256 * 232 = 384 * 168.
-constexpr int kF8ControlRegs = 40, kF8EpilogueRegs = 232;
-static_assert(128 * kF8ControlRegs + 32 * kF8EpiWarps * kF8EpilogueRegs <= kF8Threads * 168, "register split");
+constexpr int kF8LaunchRegs = 168, kF8ControlRegs = 40, kF8EpilogueRegs = 232;
+static_assert(128 * kF8ControlRegs + 32 * kF8EpiWarps * kF8EpilogueRegs <= kF8Threads * kF8LaunchRegs, "register split");
 
 // Four columns n .. n + 3 of row m: bias, GELU (keeping the pre-activation), LayerScale, residual,
 // accumulation, store. `vec`: N % 4 == 0 and all four columns exist.
@@ -713,10 +713,16 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   static std::atomic<bool> configured[64] = {};
   if (!configured[device].load(std::memory_order_acquire)) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    cudaFuncAttributes attr;
+    C10_CUDA_CHECK(cudaFuncGetAttributes(&attr, kern));
+    // the epilogue warps' larger share comes out of the block's own registers: with fewer they would wait for good
+    TORCH_CHECK(BN < 256 || attr.numRegs >= kF8LaunchRegs, "fp8_gemm: built with ", attr.numRegs, " registers a thread, ",
+                kF8LaunchRegs, " needed");
     configured[device].store(true, std::memory_order_release);
   }
   p.num_m_tiles = (p.M + 128 * CG - 1) / (128 * CG);
   p.num_n_tiles = (p.N + BN - 1) / BN;
+  TORCH_CHECK((int64_t)p.num_m_tiles * p.num_n_tiles < (1ll << 30), "fp8_gemm: output too large");
   const int tiles = p.num_m_tiles * p.num_n_tiles, num_k = (p.K + kF8K - 1) / kF8K, workers = sm_count(device) / CG;
   // Two halves of K where the last wave of whole tiles would leave many SMs idle (weight gradients: a long K and
   // few tiles). Both halves are added to a cleared fp32 output; a sum of two does not depend on their order. Measured

@@ -40,7 +40,8 @@ constexpr int kQkMaxD = 256;
 
 struct HeadView {  // (B, T, H, D) with unit channel stride; strides in elements
   void* p;
-  int64_t sb, st, sh;
+  int64_t sb, st;
+  int sh;
   int heads;
 };
 
@@ -73,7 +74,7 @@ __device__ __forceinline__ float group_sum(float v) {
 template <typename T>
 __device__ __forceinline__ T* head_ptr(const HeadView& v, unsigned token, unsigned length, int h) {
   const unsigned b = token / length, t = token - b * length;
-  return reinterpret_cast<T*>(v.p) + (int64_t)b * v.sb + (int64_t)t * v.st + (int64_t)h * v.sh;
+  return reinterpret_cast<T*>(v.p) + (int64_t)b * v.sb + (int64_t)t * v.st + h * v.sh;
 }
 
 // Shared memory of one CTA: per warp the token's (C, S) table and the exchange rows; the partner of each channel.
@@ -117,10 +118,10 @@ __device__ __forceinline__ void qk_partners(QkSmem<LPR>& sm, const QkNormParams&
   __syncthreads();
 }
 
-// The values of this lane's partner channels.
-template <int LPR>
-__device__ __forceinline__ void qk_exchange(const float (&v)[8], float (&o)[8], float* ex, int cg, const int (&part)[8],
-                                            bool scattered, int source) {
+// The values of this lane's partner channels: `raw` as loaded, `v` its eight values.
+template <int LPR, typename T>
+__device__ __forceinline__ void qk_exchange(const Raw8<T>& raw, const float (&v)[8], float (&o)[8], float* ex, int cg,
+                                            const int (&part)[8], bool scattered, int source) {
   if (scattered) {
     __syncwarp();
 #pragma unroll
@@ -129,8 +130,15 @@ __device__ __forceinline__ void qk_exchange(const float (&v)[8], float (&o)[8], 
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = ex[part[j]];
   } else {
+    Raw8<T> other;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = __shfl_sync(0xffffffffu, v[j], source);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      other.u[i].x = __shfl_sync(0xffffffffu, raw.u[i].x, source);
+      other.u[i].y = __shfl_sync(0xffffffffu, raw.u[i].y, source);
+      other.u[i].z = __shfl_sync(0xffffffffu, raw.u[i].z, source);
+      other.u[i].w = __shfl_sync(0xffffffffu, raw.u[i].w, source);
+    }
+    unpack8(other, o);
   }
 }
 
@@ -165,15 +173,14 @@ __device__ __forceinline__ void qk_table(float2* cs, const QkNormParams& p, cons
   __syncwarp();
 }
 
-// Loads of kAhead steps of a warp's walk: heads h0 + row, h0 + row + kRows, ...
+// Loads of AHEAD steps of a warp's walk over one token's heads: src is this lane's place in head `row`, the steps
+// are heads h0, h0 + 32 / LPR, ... on from there; `left` = heads - row, or none for a lane past the channels.
 template <typename T, int LPR, int AHEAD>
-__device__ __forceinline__ void qk_load(const HeadView& v, const QkNormParams& p, unsigned token, int h0, int row, int cg,
-                                        bool on, Raw8<T> (&raw)[AHEAD]) {
-  const T* src = head_ptr<const T>(v, token, p.T, h0 + row) + cg * 8;
+__device__ __forceinline__ void qk_load(const T* src, int sh, int h0, int left, Raw8<T> (&raw)[AHEAD]) {
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u) {
-    const int h = u * (32 / LPR);
-    raw[u] = on && h0 + h + row < v.heads ? load_raw8(src + h * v.sh) : Raw8<T>{};
+    const int h = h0 + u * (32 / LPR);
+    raw[u] = h < left ? load_raw8(src + h * sh) : Raw8<T>{};
   }
 }
 
@@ -191,17 +198,21 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_fwd_kernel(const QkN
   Raw8<T> next[kAhead];
   if (token < tokens) {
     qk_fetch_angles(p, token, lane, ang);
-    qk_load<T, LPR>(p.x[0], p, token, 0, row, cg, on, next);
+    qk_load<T, LPR>(head_ptr<const T>(p.x[0], token, p.T, row) + cg * 8, p.x[0].sh, 0, on ? p.x[0].heads - row : 0, next);
   }
   qk_partners<LPR>(sm, p);
   if (token >= tokens) return;
-  float w[2][8], C[8], Sn[8];
+  // y[c] = r (x[c] (w[c] C[c]) + x[c'] (w[c'] S[c])): both factors are made once a token, x itself is exchanged
+  float w[2][8], w_other[2][8], C[8], Sn[8];
   int part[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     part[j] = qk_pad(sm.partner[cg * 8 + j]);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) w[s][j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
+    for (int s = 0; s < 2; ++s) {
+      w[s][j] = (on && p.w[s] != nullptr) ? p.w[s][cg * 8 + j] : 1.f;
+      w_other[s][j] = (on && p.w[s] != nullptr) ? p.w[s][sm.partner[cg * 8 + j]] : 1.f;
+    }
   }
   const bool scattered = sm.scattered != 0;
   const int source = row * LPR + sm.partner[cg * 8] / 8;
@@ -219,31 +230,43 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_fwd_kernel(const QkN
     if (after < tokens) qk_fetch_angles(p, after, lane, ang);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+      const int heads = p.x[s].heads, sh = p.x[s].sh, left = on ? heads - row : 0;
+      const T* const src = head_ptr<const T>(p.x[s], token, p.T, row) + cg * 8;
       T* const dst = head_ptr<T>(p.y[s], token, p.T, row) + cg * 8;
-      const int heads = p.x[s].heads;
+      float a[8], b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a[j] = w[s][j] * C[j];
+        b[j] = w_other[s][j] * Sn[j];
+      }
       for (int h0 = 0; h0 < heads; h0 += kAhead * S::kRows) {
         Raw8<T> raw[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
-        if (h0 + kAhead * S::kRows < heads) qk_load<T, LPR>(p.x[s], p, token, h0 + kAhead * S::kRows, row, cg, on, next);
-        else if (s == 0 && p.x[1].heads > 0) qk_load<T, LPR>(p.x[1], p, token, 0, row, cg, on, next);
-        else if (after < tokens) qk_load<T, LPR>(p.x[0], p, after, 0, row, cg, on, next);
+        if (h0 + kAhead * S::kRows < heads) {
+          qk_load<T, LPR>(src, sh, h0 + kAhead * S::kRows, left, next);
+        } else if (s == 0) {
+          qk_load<T, LPR>(head_ptr<const T>(p.x[1], token, p.T, row) + cg * 8, p.x[1].sh, 0, on ? p.x[1].heads - row : 0, next);
+        } else if (after < tokens) {
+          qk_load<T, LPR>(head_ptr<const T>(p.x[0], after, p.T, row) + cg * 8, p.x[0].sh, 0, on ? p.x[0].heads - row : 0, next);
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           const int h = h0 + u * S::kRows;
           if (h >= heads) break;
           float v[8], o[8];
           unpack8(raw[u], v);
+          qk_exchange<LPR>(raw[u], v, o, ex, cg, part, scattered, source);
           float ss = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+          for (int j = 0; j < 8; ++j) {
+            ss = fmaf(v[j], v[j], ss);
+            o[j] = fmaf(o[j], b[j], v[j] * a[j]);
+          }
           const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[s][j];
-          qk_exchange<LPR>(v, o, ex, cg, part, scattered, source);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], Sn[j], v[j] * C[j]);
-          if (on && h + row < heads) store8(dst + h * p.y[s].sh, o);
+          for (int j = 0; j < 8; ++j) o[j] *= r;
+          if (h < left) store8(dst + h * p.y[s].sh, o);
         }
       }
     }
@@ -264,12 +287,13 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
   const unsigned tokens = p.B * p.T, stride = gridDim.x * kPairs;
   unsigned token = blockIdx.x * kPairs + pair;
   const HeadView xv = p.x[s], gv = p.dy[s], yv = p.y[s];
+  const int left = on ? xv.heads - row : 0;
   float ang[kQkAngles] = {};
   Raw8<T> next_x[kAhead], next_g[kAhead];
   if (token < tokens) {
     qk_fetch_angles(p, token, lane, ang);
-    qk_load<T, LPR>(xv, p, token, 0, row, cg, on, next_x);
-    qk_load<T, LPR>(gv, p, token, 0, row, cg, on, next_g);
+    qk_load<T, LPR>(head_ptr<const T>(xv, token, p.T, row) + cg * 8, xv.sh, 0, left, next_x);
+    qk_load<T, LPR>(head_ptr<const T>(gv, token, p.T, row) + cg * 8, gv.sh, 0, left, next_g);
   }
   qk_partners<LPR>(sm, p);
   int part[8];
@@ -296,6 +320,8 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
     if (after < tokens) qk_fetch_angles(p, after, lane, ang);
     // dx may overwrite dy: a lane has loaded all it needs of a head before it stores there
     T* const dst = head_ptr<T>(yv, token, p.T, row) + cg * 8;
+    const T* const xs = head_ptr<const T>(xv, token, p.T, row) + cg * 8;
+    const T* const gs = head_ptr<const T>(gv, token, p.T, row) + cg * 8;
     for (int h0 = 0; h0 < xv.heads; h0 += kAhead * S::kRows) {
       Raw8<T> xr[kAhead], gr[kAhead];
 #pragma unroll
@@ -303,10 +329,12 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
         xr[u] = next_x[u];
         gr[u] = next_g[u];
       }
-      const bool more = h0 + kAhead * S::kRows < xv.heads;
-      if (more || after < tokens) {
-        qk_load<T, LPR>(xv, p, more ? token : after, more ? h0 + kAhead * S::kRows : 0, row, cg, on, next_x);
-        qk_load<T, LPR>(gv, p, more ? token : after, more ? h0 + kAhead * S::kRows : 0, row, cg, on, next_g);
+      if (h0 + kAhead * S::kRows < xv.heads) {
+        qk_load<T, LPR>(xs, xv.sh, h0 + kAhead * S::kRows, left, next_x);
+        qk_load<T, LPR>(gs, gv.sh, h0 + kAhead * S::kRows, left, next_g);
+      } else if (after < tokens) {
+        qk_load<T, LPR>(head_ptr<const T>(xv, after, p.T, row) + cg * 8, xv.sh, 0, left, next_x);
+        qk_load<T, LPR>(head_ptr<const T>(gv, after, p.T, row) + cg * 8, gv.sh, 0, left, next_g);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
@@ -319,14 +347,14 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
         const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
-        qk_exchange<LPR>(g, other, ex, cg, part, scattered, source);
+        qk_exchange<LPR>(gr[u], g, other, ex, cg, part, scattered, source);
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float dn = fmaf(-other[j], Sn[j], g[j] * C[j]);
           const float dn_other = fmaf(g[j], Sn[j], other[j] * C[j]);
           v[j] *= r;  // normalised
-          da[j] = fmaf(v[j] * w[j], dn_other, da[j]);
+          da[j] = fmaf(v[j], dn_other, da[j]);  // times w[j], after the last head
           dw[j] = fmaf(dn, v[j], dw[j]);
           g[j] = dn * w[j];
           dot = fmaf(g[j], v[j], dot);
@@ -334,7 +362,7 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
         const float m = group_sum<LPR>(dot) * inv_d;
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = r * fmaf(-v[j], m, g[j]);
-        if (on && h + row < xv.heads) store8(dst + h * yv.sh, g);
+        if (h < left) store8(dst + h * yv.sh, g);
       }
     }
     if (p.dangles != nullptr) {
@@ -342,6 +370,7 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
       // a rotated pair, with opposite signs
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        da[j] *= w[j];
 #pragma unroll
         for (int o = LPR; o < 32; o <<= 1) da[j] += __shfl_xor_sync(0xffffffffu, da[j], o);
         if (row == 0) sm.da[warp][cg * 9 + j] = da[j];
@@ -378,24 +407,26 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
   }
 }
 
-// out[s][c] (+)= sum over CTAs of parts[cta][s][c], in a fixed order. One CTA of 32 x 8 threads for
-// 32 channels of one of the two weights.
-__global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ parts, int ctas, int D, float* dq,
-                                                         float* dk, int accumulate) {
-  __shared__ float red[8][32];
+// out[s][c] (+)= sum over CTAs of parts[cta][s][c], in a fixed order: a CTA of 32 slices of the list for 32
+// channels of one of the two weights, eight loads of a thread in flight.
+__global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restrict__ parts, int ctas, int D, float* dq,
+                                                          float* dk, int accumulate) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
   const int c = blockIdx.x * 32 + lane, s = blockIdx.y;
   float a = 0.f;
-  if (c < D)
-    for (int k = slice; k < ctas; k += 8) a += parts[((int64_t)k * 2 + s) * D + c];
+  if (c < D) {
+#pragma unroll 8
+    for (int k = slice; k < ctas; k += 32) a += parts[((int64_t)k * 2 + s) * D + c];
+  }
   red[slice][lane] = a;
   __syncthreads();
-  float* out = s == 0 ? dq : dk;
-  if (slice == 0 && c < D && out != nullptr) {
+  a = red[lane][slice];  // warp `slice` adds the 32 slices of channel `slice`
 #pragma unroll
-    for (int k = 1; k < 8; ++k) a += red[k][lane];
-    out[c] = (accumulate >> s & 1) ? out[c] + a : a;
-  }
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  const int mine = blockIdx.x * 32 + slice;
+  float* out = s == 0 ? dq : dk;
+  if (lane == 0 && mine < D && out != nullptr) out[mine] = (accumulate >> s & 1) ? out[mine] + a : a;
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -409,7 +440,8 @@ static HeadView head_view(const torch::Tensor& t, const torch::Tensor& like, con
   TORCH_CHECK(t.stride(3) == 1 && vec(t.stride(0), t.size(0)) && vec(t.stride(1), t.size(1)) &&
                   vec(t.stride(2), t.size(2)) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
               "qk_norm: ", what, " must have 16-byte aligned heads of contiguous channels");
-  return HeadView{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), (int)t.size(2)};
+  TORCH_CHECK(std::abs(t.stride(2)) * t.size(2) < (1ll << 31), "qk_norm: ", what, " has too large a head stride");
+  return HeadView{t.data_ptr(), t.stride(0), t.stride(1), (int)t.stride(2), (int)t.size(2)};
 }
 
 static QkNormParams qk_params(const torch::Tensor& q, const torch::Tensor& k, const c10::optional<torch::Tensor>& qw,
@@ -534,7 +566,7 @@ void qk_norm_bwd(torch::Tensor dyq, torch::Tensor dyk, torch::Tensor q, torch::T
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_dw) {
-    qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, stream>>>(p.dw_parts, blocks, p.D, dws[0], dws[1],
+    qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 1024, 0, stream>>>(p.dw_parts, blocks, p.D, dws[0], dws[1],
                                                                     (int)accumulate);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }

@@ -7,7 +7,7 @@ the channel pairs by the token's angles (`ops/attention.py` states that form):
     n = x * rsqrt(mean(x^2) + eps) * weight,   y = rotate_pairs(n, angles, pairs)
 
 in fp32, rounded once. The inputs may be strided views of a packed projection; the outputs share one
-contiguous buffer. `angles` (1 or B, T, P) and `pairs` (P, 2) may be None: norm only. Each channel is
+contiguous buffer. `angles` (1 or B, T, P), read in fp32, and `pairs` (P, 2) may be None: norm only. Each channel is
 in one pair at most; a pair that names a channel outside the head is skipped on CUDA. The backward pass
 recomputes the norm from q and k (nothing else is kept) and returns the gradients of q, k, both
 weights and the angles.
@@ -63,6 +63,14 @@ class _Norms:
     """Weight and angle gradients of the attention node."""
 
     @staticmethod
+    def sinks(qw: torch.Tensor | None, kw: torch.Tensor | None):
+        """Both weights' `main_grad`. The kernel writes both gradients at once, so one parameter used as both weights
+        gets them through autograd, which adds them."""
+        if qw is not None and qw is kw:
+            return None, None
+        return grad_sink(qw), grad_sink(kw)
+
+    @staticmethod
     def weight(w: torch.Tensor | None) -> torch.Tensor | None:
         return w.float().contiguous() if w is not None else None
 
@@ -97,13 +105,14 @@ class _Norms:
 
 
 def _check(q, k, q_weight, k_weight, angles, pairs) -> None:
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"q and k must be (B, T, H, D) of one batch, length and head size, got {tuple(q.shape)} and "
-                         f"{tuple(k.shape)}")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or (qs[0], qs[1], qs[3]) != (ks[0], ks[1], ks[3]) or not qs[2] or not ks[2]:
+        raise ValueError(f"q and k must be (B, T, H, D) of one batch, length and head size, got {tuple(qs)} and "
+                         f"{tuple(ks)}")
     if q.dtype != k.dtype or q.device != k.device or not q.is_floating_point():
         raise ValueError(f"q and k must share a floating-point dtype and a device, got {q.dtype} on {q.device} and "
                          f"{k.dtype} on {k.device}")
-    b, t, _, d = q.shape
+    b, t, _, d = qs
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (w.shape != (d,) or w.device != q.device):
             raise ValueError(f"{name} must be a vector of the head size {d} on {q.device}, got {tuple(w.shape)} on {w.device}")
@@ -130,8 +139,8 @@ def qk_norm_rope(
     """Normalised and rotated (q, k); see the module docstring."""
     _check(q, k, q_weight, k_weight, angles, pairs)
     if _native_norm_ok(q, k):
-        return native().qk_norm_rope(q, k, q_weight, k_weight, angles, pairs, float(eps), grad_sink(q_weight),
-                                     grad_sink(k_weight))
+        q_sink, k_sink = _Norms.sinks(q_weight, k_weight)
+        return native().qk_norm_rope(q, k, q_weight, k_weight, angles, pairs, float(eps), q_sink, k_sink)
     pairs = pairs.to(q.device) if pairs is not None else None
     return (head_norm_rope_reference(q, q_weight, angles, pairs, eps),
             head_norm_rope_reference(k, k_weight, angles, pairs, eps))
@@ -152,7 +161,7 @@ class _NativeNormRopeAttention(torch.autograd.Function):
         native().attention_fwd_strided(q, k, v, o, lse, float(scale))
         ctx.save_for_backward(qkv, qk, o, lse, qwf, kwf, ang, pr)
         ctx.scale, ctx.eps = float(scale), float(eps)
-        ctx.sinks = (grad_sink(qw), grad_sink(kw))
+        ctx.sinks = _Norms.sinks(qw, kw)
         ctx.w_dtypes = tuple(w.dtype if w is not None else None for w in (qw, kw))
         ctx.angles_meta = (angles.shape, angles.dtype) if angles is not None else None
         return o

@@ -186,6 +186,44 @@ def test_epilogue(m, n, k, b_block, tile):
     _no_errors()
 
 
+@pytest.mark.parametrize("b_block", [True, False])
+def test_epilogue_over_many_tiles(b_block, tile):
+    """Several tiles an SM through each form of the epilogue: the staging buffers are used again and again."""
+    m, n, k = 4096, 2568, 256
+    a, b = _operands(m, n, k, b_block)
+    torch.manual_seed(5)
+    bias, gamma, res = torch.randn(n, device=DEV), torch.rand(n, device=DEV), torch.randn(m, n, device=DEV).bfloat16()
+    da, db = a.dequantize(), b.dequantize()
+    acc = da.double() @ db.double().t() + bias.double()
+    slack = _product_bound(da, db, k) * 1.2 + acc.abs() * 2.0**-22
+    pre = torch.empty(m, n, device=DEV, dtype=BF16)
+    y = fp8_gemm(a, b, bias=bias, act=ACT_GELU, aux_out=pre)
+    assert ((pre.double() - acc).abs() <= slack + acc.abs() * 2.0**-8 * 1.01).all()
+    assert ((y.double() - F.gelu(acc)).abs() <= slack + 4e-6 * (1 + acc.abs()) + F.gelu(acc).abs() * 2.0**-8 * 1.01).all()
+    y = fp8_gemm(a, b, bias=bias, gamma=gamma, residual=res)
+    want = res.double() + gamma.double() * acc
+    assert ((y.double() - want).abs() <= slack + want.abs() * 2.0**-8 * 1.01 + (res.double().abs() + acc.abs()) * 2.0**-23).all()
+    out = torch.ones(m, n, device=DEV)
+    fp8_gemm(a, b, out=out, accumulate=True)
+    want = 1 + acc - bias.double()
+    assert ((out.double() - want).abs() <= slack + (want.abs() + acc.abs() + bias.double().abs() + 1) * 2.0**-23).all()
+    _no_errors()
+
+
+def test_long_sum_into_few_tiles(tile):
+    """The two halves of K that fill the SMs: same numbers on every run, and no halves when adding to a gradient."""
+    a, b = _operands(640, 520, 8200, False)
+    da, db = a.dequantize(), b.dequantize()
+    exact = da.double() @ db.double().t()
+    first = fp8_gemm(a, b, out_dtype=F32)
+    assert ((first.double() - exact).abs() <= _product_bound(da, db, 8200)).all()
+    assert all(torch.equal(fp8_gemm(a, b, out_dtype=F32), first) for _ in range(4))
+    sums = [fp8_gemm(a, b, out=torch.ones(640, 520, device=DEV), accumulate=True) for _ in range(4)]
+    assert all(torch.equal(s, sums[0]) for s in sums)
+    assert ((sums[0].double() - 1 - exact).abs() <= _product_bound(da, db, 8200) + (1 + exact.abs()) * 2.0**-23).all()
+    _no_errors()
+
+
 def test_extreme_scales_and_non_finite_blocks(tile):
     x = torch.ones(130, 300, device=DEV)
     x[1] *= 2.0**100

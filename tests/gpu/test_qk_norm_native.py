@@ -211,6 +211,19 @@ def test_main_grad_accumulates():
     torch.testing.assert_close(p.main_grad, full[2] + 1, rtol=2 * U, atol=2 * U)
 
 
+def test_one_parameter_as_both_weights():
+    q, k, qw, kw, ang, pairs, dq, dk = _case(1, 300, 4, 4, 64, "half", True, BF16)
+    full = _run(q, k, qw, qw.clone(), ang, pairs, dq, dk)[2]
+    for sink in (False, True):
+        p = torch.nn.Parameter(qw.clone())
+        if sink:
+            p.main_grad = torch.zeros_like(qw)
+        yq, yk = qk_norm_rope(q, k, p, p, ang, pairs, eps=EPS)
+        torch.autograd.backward((yq, yk), (dq, dk))
+        torch.testing.assert_close(p.grad, full[2] + full[3], rtol=2 * U, atol=2 * U)
+        assert not sink or (p.main_grad == 0).all()
+
+
 def test_attention_on_normed_heads_matches_the_separate_calls():
     from mia_train_b200.ops.attention import rope_attention
 
