@@ -20,7 +20,9 @@
 // by tx so that neither side meets a bank conflict, and leaves as 16-byte stores.
 // Instructions, not bytes, are scarce (ncu: 15 a value for q alone in a first version that kept fp32
 // values): bf16 input stays packed, its magnitudes are compared two at a time as 16-bit integers (their
-// order as numbers, NaN above infinity above the rest), and rows are reduced in pairs.
+// order as numbers, NaN above infinity above the rest), and rows are reduced in pairs. Measured: 16384 x
+// 5120 bf16 to q 51 us (4.97 TB/s of all bytes read and written), to q^T 48 us, to both 68 us, with column
+// sums 83 us; 5120 x 1280 fp32 with one scale a tile to both 15 us.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
