@@ -16,6 +16,10 @@ using torch::autograd::variable_list;
 
 namespace {
 
+// Inside a node nothing is recorded: views, copies and allocations go past the autograd dispatch keys. In a backward
+// pass only once the saved variables are there: fetching them may run a checkpointed forward pass again.
+using BelowAutograd = at::AutoDispatchBelowADInplaceOrView;
+
 at::Tensor value(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 bool wants(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
@@ -47,6 +51,7 @@ at::Tensor aligned(const at::Tensor& t) {
 struct DropoutNode : Function<DropoutNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& residual, int64_t dropped,
                             const OptTensor& rng) {
+    BelowAutograd below;
     const at::Tensor xc = x.contiguous();
     const OptTensor res = residual.has_value() ? OptTensor(residual->contiguous()) : OptTensor();
     at::Tensor used = at::empty({2}, x.options().dtype(at::kLong));
@@ -61,11 +66,13 @@ struct DropoutNode : Function<DropoutNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const at::Tensor dy = grads[0];
     once_differentiable(dy, "dropout");
+    const at::Tensor used = ctx->get_saved_variables()[0];
+    BelowAutograd below;
     at::Tensor dx;
     if (ctx->saved_data["need_x"].toBool()) {
       const at::Tensor dyc = dy.contiguous();
       dx = at::empty_like(dyc);
-      dropout_apply(dyc, {}, dx, ctx->saved_data["dropped"].toInt(), ctx->get_saved_variables()[0], {});
+      dropout_apply(dyc, {}, dx, ctx->saved_data["dropped"].toInt(), used, {});
     }
     return {dx, ctx->saved_data["need_r"].toBool() ? dy : at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -89,6 +96,7 @@ struct QkNormNode : Function<QkNormNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
                                const OptTensor& kw, const OptTensor& angles, const OptTensor& pairs, double eps,
                                const OptTensor& q_sink, const OptTensor& k_sink) {
+    BelowAutograd below;
     const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
     const at::Tensor qc = heads(q), kc = heads(k);
     const OptTensor qf = fp32_vector(qw), kf = fp32_vector(kw);
@@ -118,6 +126,7 @@ struct QkNormNode : Function<QkNormNode> {
     once_differentiable(grads[0], "qk_norm_rope");
     once_differentiable(grads[1], "qk_norm_rope");
     const variable_list saved = ctx->get_saved_variables();
+    BelowAutograd below;
     const at::Tensor q = saved[0], k = saved[1], pairs = saved[5];
     const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
     const at::Tensor dyq = grads[0].defined() ? heads(grads[0]) : at::zeros_like(q, at::MemoryFormat::Contiguous);
@@ -191,6 +200,7 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
                             const OptTensor& residual, const OptTensor& gamma, int64_t act, bool bf16,
                             const OptTensor& shadow, const OptTensor& w_sink, const OptTensor& b_sink, bool grad) {
+    BelowAutograd below;
     const int64_t N = weight.size(0), K = weight.numel() / N;
     const at::ScalarType type = bf16 ? at::kBFloat16 : at::kFloat;
     const at::Tensor x2 = matrix(x, K);
@@ -232,6 +242,7 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     const at::Tensor dy = grads[0];
     once_differentiable(dy, "fp8_linear");
     const variable_list s = ctx->get_saved_variables();
+    BelowAutograd below;
     auto& d = ctx->saved_data;
     const std::vector<int64_t> x_shape = d["x_shape"].toIntVector(), w_shape = d["w_shape"].toIntVector();
     const int64_t N = w_shape[0], K = x_shape.back();
@@ -299,6 +310,7 @@ at::Tensor fp8_linear_quantized(const at::Tensor& x, const at::Tensor& data, con
                                 int64_t K, const OptTensor& bias, const OptTensor& residual, const OptTensor& gamma,
                                 int64_t act, bool bf16) {
   at::NoGradGuard no_grad;
+  BelowAutograd below;
   const at::ScalarType type = bf16 ? at::kBFloat16 : at::kFloat;
   const at::Tensor x2 = matrix(x, K);
   const int64_t M = x2.size(0), N = data.size(0);

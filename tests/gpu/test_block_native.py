@@ -166,3 +166,32 @@ def test_captured_training_step_uses_all_three(tmp_path):
         if "inv_freqs" not in n:
             assert not torch.equal(p, before[n]), n
     _no_errors()
+
+
+def test_second_derivatives_are_refused():
+    from mia_train_b200.ops.dropout import dropout
+    from mia_train_b200.ops.fp8 import fp8_linear
+    from mia_train_b200.ops.qk_norm import qk_norm_rope
+
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    heads = torch.randn(1, 4, 2, 64, device=DEV, requires_grad=True)
+    w = torch.randn(32, 64, device=DEV)
+    for leaf, f in ((x, lambda t: dropout(t, 0.5)), (x, lambda t: fp8_linear(t, w)),
+                    (heads, lambda t: qk_norm_rope(t, t, None, None)[0])):
+        y = f(leaf)
+        dy = torch.ones_like(y).requires_grad_(True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y, leaf, dy, create_graph=True)
+
+
+def test_no_grad_keeps_nothing():
+    from mia_train_b200.ops.fp8 import fp8_linear
+
+    x, w = torch.randn(512, 1024, device=DEV).bfloat16(), torch.randn(1024, 1024, device=DEV, requires_grad=True)
+    with torch.no_grad():
+        y = fp8_linear(x, w)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        z = fp8_linear(x, w)
+        assert torch.cuda.memory_allocated() - before == z.numel() * 2 and torch.equal(y, z)
+    assert not z.requires_grad
