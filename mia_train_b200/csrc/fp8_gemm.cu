@@ -17,14 +17,16 @@
 //              fetches its row's scale two K blocks ahead; with a scale per row of B also its share
 //              of the warp's column scales, which the lanes pass on through a small double-buffered strip
 //              of shared memory that belongs to the warp alone.
-//              After the last block the warp adds the bias, applies GELU, rounds into 128-byte swizzled rows
-//              of shared memory and leaves the stores (or, to accumulate, the additions) to TMA while it goes
-//              on with the next tile. LayerScale, residual and odd widths take a second form, which turns
-//              the sums through shared memory so that four lanes hold 16 columns of one row.
+//              After the last block the warp applies bias, GELU, LayerScale and residual, rounds into 128-byte
+//              swizzled rows of shared memory and leaves the stores (or, to accumulate, the additions) to TMA
+//              while it goes on with the next tile; the residual came into the same rows by TMA during the K
+//              loop. Odd widths and a few combinations take a second form, which turns the sums through
+//              shared memory so that four lanes hold 16 columns of one row.
 // What bounds it: the additions. 128 x 256 sums a K block and CTA are 256 FMA cycles of the SM at best, with a
 // scale per column twice that, against 512 cycles of MMA; with both emptied of arithmetic the same pipeline runs
 // at 2590 TFLOP/s. Measured (bf16 out): 8192^3 2010 TFLOP/s with scales per weight block, 1400 with a scale per
-// row of both; 16384 x 1280 x 5120 (M x N x K) 125 us (1715 TFLOP/s), 16384 x 5120 x 1280 123 us.
+// row of both; 16384 x 1280 x 5120 (M x N x K) 127 us (1690 TFLOP/s), with a residual 138 us (228 us when the
+// lanes fetched it), 16384 x 5120 x 1280 124 us, with GELU and its pre-activation 230 us.
 // Tried and slower: sums by packed f32x2 FMAs (1620 at 8192^3), 16 epilogue warps of 64 columns (1315), stores by
 // the lanes instead of TMA (16384 x 5120 x 1280: 155 us).
 // The scales are applied in fp32 outside the tensor core, so they may be any fp32 numbers, and no sum
@@ -254,6 +256,7 @@ template <int CG, int BN, int HALVES, int STAGES, bool SB_ROW, bool FULL>
 __global__ void __launch_bounds__(kF8Threads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux,
+                    const __grid_constant__ CUtensorMap tmRes,
                     const GemmParams p, const Fp8Operands o) {
   using L = F8Smem<CG, BN, STAGES>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -267,7 +270,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   uint64_t* tfull_bar = empty_bar + STAGES;  // [kUnits]
   uint64_t* tempty_bar = tfull_bar + 4;      // [kUnits]
   uint64_t* drain_bar = tempty_bar + 4;      // [1]
-  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* res_bar = drain_bar + 1;         // [kF8EpiWarps]
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(res_bar + kF8EpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
 
   const int warp = threadIdx.x / 32;
@@ -288,6 +292,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       mbar_init(&tempty_bar[a], CG * kF8EpiWarps / HALVES);  // the unit's epilogue warps of the pair, on the even CTA
     }
     mbar_init(drain_bar, 1);
+    for (int w = 0; w < kF8EpiWarps; ++w) mbar_init(&res_bar[w], 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tensormap(&tmA);
@@ -440,6 +445,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     int unit = half;
     uint32_t unit_phase = 0;
     bool ok = true, ready = false;
+    constexpr int kBoxes = L::kWarpStaging / 4096;  // of 32 rows x 64 bf16 columns
+    uint64_t* const my_res = &res_bar[warp - kF8FirstEpi];
+    uint32_t res_phase = 0;
+    bool res_pending = false;
     for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
       const Unit u = work_unit(tile);
       const int num_k = u.num_k;
@@ -473,6 +482,19 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           sa += o.sa_ld;
           sb += o.sb_ld;
         }
+      }
+      if (!FULL && p.residual != nullptr) {
+        // this warp's part of the residual, into the staging rows its outputs will leave from; outside the K loop,
+        // where the test alone cost the calls without a residual a tenth of their time
+        if (elect_one()) {
+          bulk_wait_read();  // the last tile's stores have read them
+          mbar_arrive_expect_tx(my_res, kBoxes * 4096);
+#pragma unroll
+          for (int box = 0; box < kBoxes; ++box)
+            tma_load_2d(staging + box * 4096, &tmRes, my_res, n0 + column(box * 64), m_warp);
+        }
+        __syncwarp();
+        res_pending = true;
       }
       for (int kb = 0; kb < num_k; ++kb) {
         if (!ready && !mbar_wait_warp(&tfull_bar[unit], unit_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
@@ -566,31 +588,35 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       }
       if (!ok) break;
       if constexpr (!FULL) {
-        if (p.bias != nullptr) {
+        // sum = op(sum, vec[n]) for a vector over the columns
+        auto per_column = [&](const float* vec, auto op) {
           if (SB_ROW) {
 #pragma unroll
             for (int g = 0; g < kCols / 8; ++g) {  // eight columns: registers 32 (g / 4) + 4 (g % 4) .. + 3, and 16 on
               const int n = n0 + column(g * 8) + (lane & 3) * 2;
-              const float2 v = n < p.N ? __ldg(reinterpret_cast<const float2*>(p.bias + n)) : make_float2(0.f, 0.f);
+              const float2 v = n < p.N ? __ldg(reinterpret_cast<const float2*>(vec + n)) : make_float2(0.f, 0.f);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float* x = sum + g / 4 * 32 + i / 2 * 16 + g % 4 * 4 + i % 2 * 2;
-                x[0] += v.x;
-                x[1] += v.y;
+                op(x[0], v.x);
+                op(x[1], v.y);
               }
             }
           } else {
 #pragma unroll
             for (int c = 0; c < kCols; c += 4) {
               const int n = n0 + column(c);
-              const float4 v = n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
-              sum[c] += v.x; sum[c + 1] += v.y; sum[c + 2] += v.z; sum[c + 3] += v.w;
+              const float4 v = n < p.N ? __ldg(reinterpret_cast<const float4*>(vec + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              op(sum[c], v.x);
+              op(sum[c + 1], v.y);
+              op(sum[c + 2], v.z);
+              op(sum[c + 3], v.w);
             }
           }
-        }
+        };
+        if (p.bias != nullptr) per_column(p.bias, [](float& x, float v) { x += v; });
         // Boxes of 64 bf16 or 32 fp32 columns into 128-byte rows whose 16-byte pieces are XOR-swizzled with the
         // row's low three bits, as the tensor maps expect, from column `first` of the warp's on.
-        constexpr int kBoxes = L::kWarpStaging / 4096;
         auto stage = [&](const CUtensorMap* map, int first, auto wide, bool add) {
           constexpr bool kF32 = decltype(wide)::value;
           constexpr int kBoxCols = kF32 ? 32 : 64;
@@ -649,6 +675,45 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 #pragma unroll
           for (int c = 0; c < kCols; ++c) sum[c] = gelu_erf(sum[c]);
         }
+        if (p.gamma != nullptr) per_column(p.gamma, [](float& x, float v) { x *= v; });
+        if (p.residual != nullptr) {
+          res_pending = false;
+          if (!mbar_wait_warp(my_res, res_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
+            res_pending = true;
+            ok = false;
+            break;
+          }
+          res_phase ^= 1;
+#pragma unroll
+          for (int box = 0; box < kBoxes; ++box) {
+            const uint8_t* const at = staging + box * 4096;
+            float* const x0 = sum + box * 64;
+            if constexpr (SB_ROW) {
+#pragma unroll
+              for (int g = 0; g < 8; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int row = i * 8 + lane / 4;
+                  float* x = x0 + g / 4 * 32 + i / 2 * 16 + g % 4 * 4 + i % 2 * 2;
+                  const uint32_t u = *reinterpret_cast<const uint32_t*>(at + row * 128 + ((g ^ (row & 7)) << 4) + (lane & 3) * 4);
+                  x[0] += bf16_lo(u);
+                  x[1] += bf16_hi(u);
+                }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint4 u = *reinterpret_cast<const uint4*>(at + lane * 128 + ((j ^ (lane & 7)) << 4));
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  x0[j * 8 + 2 * h] += bf16_lo(w[h]);
+                  x0[j * 8 + 2 * h + 1] += bf16_hi(w[h]);
+                }
+              }
+            }
+          }
+          __syncwarp();
+        }
         if (p.d_fp32) {
           const bool add = p.accumulate != 0 || p.splits > 1;
           stage(&tmD, 0, std::true_type{}, add);
@@ -696,7 +761,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
       }
     }
-    if (!FULL && elect_one()) bulk_wait_all();
+    if (!FULL && elect_one()) {
+      if (res_pending) mbar_wait(my_res, res_phase, nullptr, nullptr, 0);  // given up on: let it land all the same
+      bulk_wait_all();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -712,7 +780,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
 template <int CG, int BN, int HALVES, int STAGES, bool SB_ROW, bool FULL>
 static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
-                       const CUtensorMap& taux, GemmParams& p, const Fp8Operands& o, bool may_split,
+                       const CUtensorMap& taux, const CUtensorMap& tres, GemmParams& p, const Fp8Operands& o, bool may_split,
                        int device, cudaStream_t stream) {
   using L = F8Smem<CG, BN, STAGES>;
   auto kern = fp8_gemm_kernel<CG, BN, HALVES, STAGES, SB_ROW, FULL>;
@@ -750,7 +818,7 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 1 : 0;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, td, taux, p, o));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, td, taux, tres, p, o));
 }
 
 // Tile shape: the share of the SMs' time that goes into real output (waves of tiles over the SMs, rows and
@@ -856,19 +924,23 @@ void fp8_gemm(torch::Tensor a, torch::Tensor a_scale, bool a_block, torch::Tenso
   const int tile = choose_tile(M, N, sm_count(device));
   const CUtensorMap ta = make_u8_map(a.data_ptr(), k, M, a.stride(0), kF8K, 128);
   const CUtensorMap tb = make_u8_map(b.data_ptr(), k, N, b.stride(0), kF8K, 128);
-  // TMA stores take rows of a multiple of 16 bytes, and the accumulation a fp32 output.
-  const bool full = p.gamma != nullptr || p.residual != nullptr || N % (p.d_fp32 && p.aux_out == nullptr ? 4 : 8) != 0 ||
-                    (accumulate && !p.d_fp32);
-  CUtensorMap td = ta, taux = ta;
+  // TMA moves rows of a multiple of 16 bytes and adds in fp32 only; the pre-activation and the residual would
+  // want the staging rows at the same time.
+  const bool bf16_rows = !p.d_fp32 || p.aux_out != nullptr || p.residual != nullptr;
+  const bool full = N % (bf16_rows ? 8 : 4) != 0 || (accumulate && !p.d_fp32) ||
+                    (p.aux_out != nullptr && p.residual != nullptr);
+  CUtensorMap td = ta, taux = ta, tres = ta;
   if (!full) {
     td = make_store_map(d.data_ptr(), N, M, p.d_fp32);
     if (p.aux_out != nullptr) taux = make_store_map(p.aux_out, N, M, false);
+    if (p.residual != nullptr) tres = make_store_map(p.residual, N, M, false);
   }
-  const bool may_split = !full && p.d_fp32 && !accumulate && act == kActNone && p.bias == nullptr;
+  const bool may_split = !full && p.d_fp32 && !accumulate && act == kActNone && p.bias == nullptr &&
+                         p.gamma == nullptr && p.residual == nullptr;
   auto run = [&](auto row, auto rest) {
     constexpr bool kRow = decltype(row)::value, kFull = decltype(rest)::value;
-    if (tile == kTile256) launch_fp8<2, 256, 2, 4, kRow, kFull>(ta, tb, td, taux, p, o, may_split, device, stream);
-    else launch_fp8<1, 128, 1, 5, kRow, kFull>(ta, tb, td, taux, p, o, may_split, device, stream);
+    if (tile == kTile256) launch_fp8<2, 256, 2, 4, kRow, kFull>(ta, tb, td, taux, tres, p, o, may_split, device, stream);
+    else launch_fp8<1, 128, 1, 5, kRow, kFull>(ta, tb, td, taux, tres, p, o, may_split, device, stream);
   };
   if (b_block) full ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
   else full ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
