@@ -317,25 +317,33 @@ __global__ void __launch_bounds__(256) quant_sums_kernel(const float* __restrict
   }
 }
 
+// The combinations that exist: 1 x 128 blocks either way or both, for e4m3 with the column sums of a gradient as
+// well; 128 x 128 blocks of a weight, alone or both ways; the factors of a gradient (AUX) are bf16 and e4m3.
 template <typename T, bool AUX, bool E5M2>
-static void launch_quant(const QuantParams& p, int mode, unsigned blocks, cudaStream_t stream) {
-  switch (mode) {
+static bool launch_quant(const QuantParams& p, int mode, unsigned blocks, cudaStream_t stream) {
 #define MIA_QUANT_CASE(M) \
-  case M: quant_kernel<T, M, AUX, E5M2><<<blocks, 256, 0, stream>>>(p); break;
+  case M: quant_kernel<T, M, AUX, E5M2><<<blocks, 256, 0, stream>>>(p); return true;
+  switch (mode) {
     MIA_QUANT_CASE(kQuantRows)
     MIA_QUANT_CASE(kQuantCols)
     MIA_QUANT_CASE(kQuantRows | kQuantCols)
-    MIA_QUANT_CASE(kQuantSums)
-    MIA_QUANT_CASE(kQuantRows | kQuantSums)
-    MIA_QUANT_CASE(kQuantCols | kQuantSums)
-    MIA_QUANT_CASE(kQuantRows | kQuantCols | kQuantSums)
-    MIA_QUANT_CASE(kQuantBlock | kQuantRows)
-    MIA_QUANT_CASE(kQuantBlock | kQuantCols)
-    MIA_QUANT_CASE(kQuantBlock | kQuantRows | kQuantCols)
-#undef MIA_QUANT_CASE
-    default: TORCH_CHECK(false, "fp8_quantize: unsupported combination of outputs ", mode);
   }
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if constexpr (!E5M2) {
+    switch (mode) {
+      MIA_QUANT_CASE(kQuantSums)
+      MIA_QUANT_CASE(kQuantRows | kQuantSums)
+      MIA_QUANT_CASE(kQuantCols | kQuantSums)
+      MIA_QUANT_CASE(kQuantRows | kQuantCols | kQuantSums)
+    }
+  }
+  if constexpr (!AUX) {
+    switch (mode) {
+      MIA_QUANT_CASE(kQuantBlock | kQuantRows)
+      MIA_QUANT_CASE(kQuantBlock | kQuantRows | kQuantCols)
+    }
+  }
+#undef MIA_QUANT_CASE
+  return false;
 }
 
 static void check_fp8(const torch::Tensor& q, const torch::Tensor& scale, int64_t rows, int64_t cols, int64_t scale_cols,
@@ -410,16 +418,22 @@ void fp8_quantize(torch::Tensor x, c10::optional<torch::Tensor> aux, c10::option
     TORCH_CHECK(rb * cb <= INT32_MAX, "fp8_quantize: matrix too large");
     p.col_tiles = (int)cb;
     const bool extra = p.aux != nullptr || p.gamma != nullptr;
+    const unsigned blocks = (unsigned)(rb * cb);
     auto run = [&](auto type) {
       using T = decltype(type);
-      const unsigned blocks = (unsigned)(rb * cb);
-      if (e5m2) extra ? launch_quant<T, true, true>(p, mode, blocks, stream) : launch_quant<T, false, true>(p, mode, blocks, stream);
-      else extra ? launch_quant<T, true, false>(p, mode, blocks, stream) : launch_quant<T, false, false>(p, mode, blocks, stream);
+      if (extra) {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) return !e5m2 && launch_quant<T, true, false>(p, mode, blocks, stream);
+        return false;
+      }
+      return e5m2 ? launch_quant<T, false, true>(p, mode, blocks, stream) : launch_quant<T, false, false>(p, mode, blocks, stream);
     };
-    if (x.scalar_type() == at::kBFloat16) run(__nv_bfloat16{});
-    else if (x.scalar_type() == at::kHalf) run(__half{});
-    else if (x.scalar_type() == at::kFloat) run(float{});
+    bool ran = false;
+    if (x.scalar_type() == at::kBFloat16) ran = run(__nv_bfloat16{});
+    else if (x.scalar_type() == at::kHalf) ran = run(__half{});
+    else if (x.scalar_type() == at::kFloat) ran = run(float{});
     else TORCH_CHECK(false, "fp8_quantize: bf16, fp16 or fp32 expected");
+    TORCH_CHECK(ran, "fp8_quantize: unsupported combination of type, format, factors and outputs (", mode, ")");
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   if (sums.has_value()) {
     quant_sums_kernel<<<(unsigned)((p.C + 31) / 32), 256, 0, stream>>>(p.sums, rb, p.C, sums->data_ptr<float>(),
