@@ -123,7 +123,7 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams& p, int m, int n
     }
     return;
   }
-  const bool full = n + 32 <= p.N && p.N % 8 == 0;  // 16-byte accesses (other widths: 8-bit GEMMs only)
+  const bool full = (n + 32 <= p.N);
   const size_t row = (size_t)m * p.N;
   if (p.bias != nullptr) {
     if (full) {
