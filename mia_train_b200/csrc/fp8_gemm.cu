@@ -137,14 +137,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// mbar_wait for a whole warp: one lane polls, the others take its answer and with it the ordering. Polling
-// with all lanes costs 32 barrier operations a try, and lanes that see the barrier complete in different
-// tries would have to be brought together before the warp-wide TMEM loads that follow.
+// mbar_wait for a whole warp: one lane polls, a shuffle gives the others its answer, and __syncwarp what the
+// barrier ordered: a shuffle alone orders no memory. Polling with all lanes costs 32 barrier operations a
+// try, and lanes that see the barrier complete in different tries would have to be brought together before the
+// warp-wide TMEM loads that follow.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
                                                int code) {
   int ok = 0;
   if (threadIdx.x % 32 == 0) ok = mbar_wait(bar, parity, abort_flag, err, code) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
 }
 
 // One K block: four steps of 32, the first of which overwrites D. A step of 32 bytes along the swizzled rows
@@ -583,6 +586,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           }
         }
         ready = __shfl_sync(0xffffffffu, seen, 0) != 0;
+        __syncwarp();  // as in mbar_wait_warp
         unit = next;
         unit_phase = next_phase;
       }
