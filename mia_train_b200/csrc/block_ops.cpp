@@ -88,8 +88,11 @@ at::Tensor heads(const at::Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-OptTensor fp32_vector(const OptTensor& w) {
-  return w.has_value() ? OptTensor(w->detach().to(at::kFloat).contiguous()) : OptTensor();
+// fp32 values of an operand that is kept for the backward pass: the operand itself where nothing needs converting,
+// never a detached alias. Below the autograd keys an alias has a version counter of its own, and a change of the
+// operand between forward and backward would go unseen.
+OptTensor fp32_values(const OptTensor& w) {
+  return w.has_value() ? OptTensor(w->to(at::kFloat).contiguous()) : OptTensor();
 }
 
 struct QkNormNode : Function<QkNormNode> {
@@ -99,9 +102,9 @@ struct QkNormNode : Function<QkNormNode> {
     BelowAutograd below;
     const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
     const at::Tensor qc = heads(q), kc = heads(k);
-    const OptTensor qf = fp32_vector(qw), kf = fp32_vector(kw);
+    const OptTensor qf = fp32_values(qw), kf = fp32_values(kw);
     const bool rotate = angles.has_value() && pairs.has_value() && pairs->numel() > 0;
-    const OptTensor ang = rotate ? OptTensor(angles->detach().to(at::kFloat).contiguous()) : OptTensor();
+    const OptTensor ang = rotate ? fp32_values(angles) : OptTensor();
     const at::Tensor pr = rotate ? pairs->to(q.device(), at::kInt).contiguous()
                                  : at::empty({0, 2}, q.options().dtype(at::kInt));
     at::Tensor out = at::empty({B, T, Hq + Hk, D}, q.options());
@@ -192,8 +195,8 @@ at::Tensor matrix(const at::Tensor& x, int64_t cols) {
   return m.stride(1) == 1 || cols == 1 ? m : m.contiguous();
 }
 
-OptTensor aligned_vector(const OptTensor& v) {
-  return v.has_value() ? OptTensor(aligned(v->detach().to(at::kFloat))) : OptTensor();
+OptTensor aligned_vector(const OptTensor& v) {  // not detached: see fp32_values
+  return v.has_value() ? OptTensor(aligned(v->to(at::kFloat))) : OptTensor();
 }
 
 struct Fp8LinearNode : Function<Fp8LinearNode> {
@@ -206,7 +209,8 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     const at::Tensor x2 = matrix(x, K);
     const at::Tensor w = matrix((shadow.has_value() ? *shadow : weight).detach(), K);
     // under no_grad nothing is kept for a backward pass
-    const bool need_x = grad && x.requires_grad(), need_w = grad && weight.requires_grad(), need_g = grad && wants(gamma);
+    const bool need_x = grad && x.requires_grad(), need_w = grad && weight.requires_grad();
+    const bool need_b = grad && wants(bias), need_g = grad && wants(gamma);
     Q8 xq, xt, wq, wt;
     quantize_both(x2, false, true, need_w, xq, xt);
     quantize_both(w, true, true, need_x, wq, wt);
@@ -218,7 +222,10 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     at::Tensor y = at::empty({M, N}, x.options().dtype(type));
     fp8_gemm(xq.data, xq.scale, false, wq.data, wq.scale, true, K, y, b, res, g, pre, act, false);
     if (!need_g) xq = wq = Q8();
-    ctx->save_for_backward({value(pre), value(g), value(b), xt.data, xt.scale, wt.data, wt.scale, xq.data, xq.scale,
+    // gamma scales the gradient of the product; the bias is in the activation that gamma's own gradient recomputes
+    const at::Tensor kept_g = need_x || need_w || need_b ? value(g) : at::Tensor();
+    const at::Tensor kept_b = need_g ? value(b) : at::Tensor();
+    ctx->save_for_backward({value(pre), kept_g, kept_b, xt.data, xt.scale, wt.data, wt.scale, xq.data, xq.scale,
                             wq.data, wq.scale});
     keep_sink(ctx, "w_sink", w_sink);
     keep_sink(ctx, "b_sink", b_sink);
@@ -226,7 +233,7 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     d["act"] = act;
     d["need_x"] = need_x;
     d["need_w"] = need_w;
-    d["need_b"] = wants(bias);
+    d["need_b"] = need_b;
     d["need_r"] = wants(residual);
     d["need_g"] = need_g;
     d["x_shape"] = x.sizes().vec();

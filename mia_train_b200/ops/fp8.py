@@ -214,7 +214,8 @@ class _Fp8Linear(torch.autograd.Function):
         keep = {"xt": xt, "wt": wt, "xq": xq if need_g else None, "wq": wq if need_g else None}
         ctx.held = {k: (m.cols, m.block_rows) for k, m in keep.items() if m is not None}
         flat = [t for m in keep.values() if m is not None for t in (m.data, m.scale)]
-        ctx.save_for_backward(pre, g, bf, *flat)
+        # gamma scales the gradient of the product; the bias is in the activation that gamma's own gradient recomputes
+        ctx.save_for_backward(pre, g if any(ctx.needs_input_grad[:3]) else None, bf if need_g else None, *flat)
         ctx.meta = (act, weight.dtype, weight.shape, gamma.dtype if gamma is not None else None,
                     bias.dtype if bias is not None else None)
         ctx.sinks = (grad_sink(weight), grad_sink(bias))

@@ -1,0 +1,107 @@
+"""What the native nodes keep between forward and backward: seen by autograd's checks, and no more than is read."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover - collected on CPU, skipped there
+    pytest.skip("needs CUDA", allow_module_level=True)
+
+from mia_train_b200.ops.fp8 import fp8_linear  # noqa: E402
+from mia_train_b200.ops.qk_norm import qk_norm_rope, qk_norm_rope_attention  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+BF16 = torch.bfloat16
+CHANGED = "modified by an inplace operation"
+
+
+def _half_pairs(d):
+    i = torch.arange(d // 2)
+    return torch.stack([i, i + d // 2], 1).int().to(DEV)
+
+
+def _heads():
+    torch.manual_seed(0)
+    pairs = _half_pairs(64)
+    t = {"q": torch.randn(2, 5, 3, 64, device=DEV).bfloat16(), "k": torch.randn(2, 5, 3, 64, device=DEV).bfloat16(),
+         "qw": torch.rand(64, device=DEV), "kw": torch.rand(64, device=DEV),
+         "angles": torch.randn(1, 5, 32, device=DEV), "pairs": pairs}
+    for key in ("q", "k", "qw", "kw", "angles"):
+        t[key].requires_grad_(True)
+    return t
+
+
+@pytest.mark.parametrize("name", ["q", "k", "qw", "kw", "angles", "pairs"])
+@pytest.mark.parametrize("entry", ["norm", "attention"])
+def test_head_norm_refuses_operands_changed_before_backward(name, entry):
+    t = _heads()
+    if entry == "norm":
+        y = qk_norm_rope(t["q"], t["k"], t["qw"], t["kw"], t["angles"], t["pairs"])[0]
+    else:
+        packed = torch.stack([t["q"], t["k"], t["k"]], 2).detach().requires_grad_(True)
+        t["q"] = t["k"] = packed
+        y = qk_norm_rope_attention(packed, t["qw"], t["kw"], t["angles"], t["pairs"], 0.125)
+    with torch.no_grad():
+        t[name].add_(1)
+    with pytest.raises(RuntimeError, match=CHANGED):
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_head_norm_takes_converted_weights_as_they_were(dtype):
+    """A weight in another type is converted in the forward pass; the copy is what backward differentiates with."""
+    t = _heads()
+    qw = t["qw"].detach().to(dtype)
+    dy = torch.randn_like(t["q"])
+
+    def grads(change):
+        w = qw.clone().requires_grad_(True)
+        y = qk_norm_rope(t["q"], t["k"], w, None, t["angles"], t["pairs"])[0]
+        if change:
+            with torch.no_grad():
+                w.mul_(3)
+        return torch.autograd.grad(y, (t["q"], w, t["angles"]), dy)
+
+    if dtype == torch.float32:
+        with pytest.raises(RuntimeError, match=CHANGED):
+            grads(True)
+        return
+    for a, b in zip(grads(False), grads(True), strict=True):
+        assert torch.equal(a, b)
+
+
+def _linear(act=None, gamma=True, n=64):
+    torch.manual_seed(1)
+    t = {"x": torch.randn(40, 32, device=DEV).bfloat16(), "weight": torch.randn(n, 32, device=DEV),
+         "bias": torch.randn(n, device=DEV), "gamma": torch.rand(n, device=DEV) if gamma else None}
+    t = {k: v.requires_grad_(True) for k, v in t.items() if v is not None}
+    return t, lambda: fp8_linear(t["x"], t["weight"], t["bias"], activation=act, gamma=t.get("gamma"))
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("name", ["gamma", "bias"])
+def test_linear_refuses_vectors_changed_before_backward(name, act):
+    """gamma scales the gradient of the product, bias is in the recomputed activation behind gamma's own gradient."""
+    t, run = _linear(act)
+    y = run()
+    with torch.no_grad():
+        t[name].add_(1)
+    with pytest.raises(RuntimeError, match=CHANGED):
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "bias"])
+def test_linear_allows_changes_of_what_backward_does_not_read(name):
+    """x and weight are kept as 8-bit copies, and without gamma nothing in the backward pass depends on the bias."""
+    t, run = _linear("gelu", gamma=False)
+    dy = torch.randn(40, 64, device=DEV).bfloat16()
+    leaves = list(t.values())
+    want = torch.autograd.grad(run(), leaves, dy)
+    y = run()
+    with torch.no_grad():
+        t[name].mul_(3)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want, strict=True):
+        assert torch.equal(a, b)

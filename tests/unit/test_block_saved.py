@@ -1,0 +1,41 @@
+"""What the CPU path of the 8-bit linear layer keeps between forward and backward."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mia_train_b200.ops.fp8 import fp8_linear
+
+
+def _linear(act=None, gamma=True):
+    torch.manual_seed(1)
+    t = {"x": torch.randn(5, 32).bfloat16(), "weight": torch.randn(8, 32), "bias": torch.randn(8)}
+    if gamma:
+        t["gamma"] = torch.rand(8)
+    t = {k: v.requires_grad_(True) for k, v in t.items()}
+    return t, lambda: fp8_linear(t["x"], t["weight"], t["bias"], activation=act, gamma=t.get("gamma"))
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("name", ["gamma", "bias"])
+def test_vectors_changed_before_backward_are_refused(name, act):
+    t, run = _linear(act)
+    y = run()
+    with torch.no_grad():
+        t[name].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "bias"])
+def test_changes_of_what_backward_does_not_read_are_allowed(name):
+    t, run = _linear("gelu", gamma=False)
+    dy = torch.randn(5, 8).bfloat16()
+    leaves = list(t.values())
+    want = torch.autograd.grad(run(), leaves, dy)
+    y = run()
+    with torch.no_grad():
+        t[name].mul_(3)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want, strict=True):
+        assert torch.equal(a, b)
