@@ -218,7 +218,8 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     const int64_t M = x2.size(0);
     OptTensor res, pre;
     if (residual.has_value()) res = aligned(residual->detach().reshape({M, N}).to(type));
-    if (act != 0) pre = at::empty({M, N}, x.options().dtype(type));
+    // the pre-activation is read by the gradients of the product alone; without it the epilogue also stages one output less
+    if (act != 0 && (need_x || need_w || need_b)) pre = at::empty({M, N}, x.options().dtype(type));
     at::Tensor y = at::empty({M, N}, x.options().dtype(type));
     fp8_gemm(xq.data, xq.scale, false, wq.data, wq.scale, true, K, y, b, res, g, pre, act, false);
     if (!need_g) xq = wq = Q8();

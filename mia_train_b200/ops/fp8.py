@@ -200,22 +200,23 @@ class _Fp8Linear(torch.autograd.Function):
     """The PyTorch path; on CUDA `csrc/block_ops.cpp` holds the same node."""
 
     @staticmethod
-    def forward(ctx, x2, weight, bias, residual, gamma, act, cdtype):  # type: ignore[override]
+    def forward(ctx, x2, weight, bias, residual, gamma, act, cdtype, grad):  # type: ignore[override]
         e4m3 = torch.float8_e4m3fn
-        need_x, need_w, need_g = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[4]
+        need_x, need_w, need_b, _, need_g = (grad and n for n in ctx.needs_input_grad[:5])
+        product = need_x or need_w or need_b  # some gradient goes through the activation
         n = weight.shape[0]
         shadow = getattr(weight, "_mia_shadow", None)  # under a sharded optimizer only the bf16 copy is current
         w = (shadow if shadow is not None else weight).detach().reshape(n, -1)
         xq, xt = _quantize(x2, 1, e4m3, True, need_w)
         wq, wt = _quantize(w, BLOCK, e4m3, True, need_x)
         g, bf = (t.detach().float() if t is not None else None for t in (gamma, bias))
-        pre = torch.empty((x2.shape[0], n), device=x2.device, dtype=cdtype) if act == ACT_GELU else None
+        pre = torch.empty((x2.shape[0], n), device=x2.device, dtype=cdtype) if act == ACT_GELU and product else None
         y = fp8_gemm(xq, wq, out_dtype=cdtype, bias=bf, residual=residual, gamma=g, act=act, aux_out=pre)
         keep = {"xt": xt, "wt": wt, "xq": xq if need_g else None, "wq": wq if need_g else None}
         ctx.held = {k: (m.cols, m.block_rows) for k, m in keep.items() if m is not None}
         flat = [t for m in keep.values() if m is not None for t in (m.data, m.scale)]
         # gamma scales the gradient of the product; the bias is in the activation that gamma's own gradient recomputes
-        ctx.save_for_backward(pre, g if any(ctx.needs_input_grad[:3]) else None, bf if need_g else None, *flat)
+        ctx.save_for_backward(pre, g if product else None, bf if need_g else None, *flat)
         ctx.meta = (act, weight.dtype, weight.shape, gamma.dtype if gamma is not None else None,
                     bias.dtype if bias is not None else None)
         ctx.sinks = (grad_sink(weight), grad_sink(bias))
@@ -249,7 +250,7 @@ class _Fp8Linear(torch.autograd.Function):
             else:
                 dw = fp8_gemm(dzt, held["xt"], out_dtype=torch.float32).to(wdtype).view(wshape)
         db = sums.to(bdtype) if need_b and b_sink is None else None
-        return dx, dw, db, (dy if need_r else None), dgamma, None, None
+        return dx, dw, db, (dy if need_r else None), dgamma, None, None, None
 
 
 def fp8_linear(
@@ -303,7 +304,7 @@ def fp8_linear(
             y = fp8_gemm(_quantize(x2.detach(), 1, torch.float8_e4m3fn, True, False)[0], weight, out_dtype=cdtype,
                          bias=bias, residual=res2, gamma=f_gamma, act=f_act)
         else:
-            y = _Fp8Linear.apply(x2, weight, bias, res2, f_gamma, f_act, cdtype)
+            y = _Fp8Linear.apply(x2, weight, bias, res2, f_gamma, f_act, cdtype, torch.is_grad_enabled())
         y = y.reshape(*x.shape[:-1], n)
     if fused:
         return y

@@ -105,3 +105,60 @@ def test_linear_allows_changes_of_what_backward_does_not_read(name):
         t[name].mul_(3)
     for a, b in zip(torch.autograd.grad(y, leaves, dy), want, strict=True):
         assert torch.equal(a, b)
+
+
+M, K, N = 512, 1024, 1024
+# 8-bit x and weight with their scales (the allocator hands out multiples of 512 bytes), and y
+OPERANDS = M * K + 4 * M * K // 128 + N * K + 512
+OUTPUT = 2 * M * N
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "inference_mode", "constants", "residual_only"])
+def test_gelu_without_a_backward_writes_no_preactivation(mode):
+    torch.manual_seed(2)
+    x, w = torch.randn(M, K, device=DEV).bfloat16(), torch.randn(N, K, device=DEV)
+    b, res = torch.randn(N, device=DEV), torch.randn(M, N, device=DEV).bfloat16()
+    train = mode in ("no_grad", "inference_mode")
+    for t in (x, w, b):
+        t.requires_grad_(train)
+    res.requires_grad_(mode == "residual_only")
+    grad = {"no_grad": torch.no_grad(), "inference_mode": torch.inference_mode()}.get(mode, torch.enable_grad())
+
+    def run():
+        with grad:
+            return fp8_linear(x, w, b, activation="gelu", residual=res)
+
+    first = run()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = run()
+    assert torch.cuda.max_memory_allocated() - before == OPERANDS + OUTPUT
+    assert torch.equal(y, first) and y.requires_grad == (mode == "residual_only")
+
+
+def test_gelu_output_does_not_depend_on_grad_mode():
+    """With its pre-activation the residual takes another form of the epilogue: the numbers stay the same."""
+    torch.manual_seed(3)
+    x, w = torch.randn(300, 256, device=DEV).bfloat16(), torch.randn(264, 256, device=DEV, requires_grad=True)
+    b, g = torch.randn(264, device=DEV), torch.rand(264, device=DEV)
+    res = torch.randn(300, 264, device=DEV).bfloat16()
+    for kw in (dict(), dict(gamma=g), dict(residual=res), dict(gamma=g, residual=res)):
+        y = fp8_linear(x, w, b, activation="gelu", **kw)
+        with torch.no_grad():
+            z = fp8_linear(x, w, b, activation="gelu", **kw)
+        # the same fp32 terms, but product and sum may be one rounding or two (half a step, 2^-24, of either term):
+        # that moves a rounding to bf16 by a step (at most 2^-7) where it falls between two, one time in 2^14 or so
+        gap = (y.detach().double() - z.double()).abs()
+        term = res.double().abs() if "residual" in kw else torch.zeros_like(gap)
+        assert (gap <= z.double().abs() * 2.0**-7 + (2 * term + z.double().abs()) * 2.0**-23).all()
+        assert (gap > 0).double().mean() < 2.0**-8
+
+
+def test_gamma_alone_needs_no_preactivation():
+    t, run = _linear("gelu")
+    dy = torch.randn(40, 64, device=DEV).bfloat16()
+    want = torch.autograd.grad(run(), t["gamma"], dy)[0]
+    for k, v in t.items():
+        v.requires_grad_(k == "gamma")
+    assert torch.equal(torch.autograd.grad(run(), t["gamma"], dy)[0], want)

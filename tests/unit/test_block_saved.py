@@ -39,3 +39,26 @@ def test_changes_of_what_backward_does_not_read_are_allowed(name):
         t[name].mul_(3)
     for a, b in zip(torch.autograd.grad(y, leaves, dy), want, strict=True):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "constants", "gamma_only"])
+def test_gelu_without_a_product_gradient_keeps_no_preactivation(mode, monkeypatch):
+    import mia_train_b200.ops.fp8 as fp8
+
+    asked = []
+    real = fp8.fp8_gemm
+    monkeypatch.setattr(fp8, "fp8_gemm", lambda *a, **kw: asked.append(kw.get("aux_out")) or real(*a, **kw))
+    quantised = []
+    both = fp8._quantize
+    monkeypatch.setattr(fp8, "_quantize", lambda *a, **kw: quantised.append(a[4]) or both(*a, **kw))
+    t, run = _linear("gelu")
+    for k, v in t.items():
+        v.requires_grad_(mode == "no_grad" or (mode == "gamma_only" and k == "gamma"))
+    with torch.set_grad_enabled(mode != "no_grad"):
+        y = run()
+    assert asked == [None] and quantised == [False, False]
+    if mode == "gamma_only":
+        (g,) = torch.autograd.grad(y.float().sum(), t["gamma"])
+        for v in t.values():
+            v.requires_grad_(True)
+        assert torch.equal(g, torch.autograd.grad(run().float().sum(), t["gamma"])[0])
