@@ -2,7 +2,8 @@
 // small calls are bound by the host: a Python autograd.Function costs 40 to 100 us for forward and backward, more
 // than these kernels run for below some ten million elements.
 //
-// Every backward pass is differentiable once: it refuses gradients that need a graph themselves.
+// Every backward pass is differentiable once: with create_graph it refuses to run where its result depends on
+// anything that wants a gradient, the incoming gradient or an operand.
 #include <ATen/ATen.h>
 #include <torch/extension.h>
 
@@ -24,8 +25,10 @@ at::Tensor value(const OptTensor& t) { return t.has_value() ? *t : at::Tensor();
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 bool wants(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
-void once_differentiable(const at::Tensor& grad, const char* what) {
-  TORCH_CHECK(!(at::GradMode::is_enabled() && grad.defined() && grad.requires_grad()), what,
+// `open`: whether the gradients depend on an operand that itself wants a gradient. Without create_graph nothing is
+// missed; with it, even a constant incoming gradient would leave the result without the graph it should have.
+void once_differentiable(const at::Tensor& grad, bool open, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (open || (grad.defined() && grad.requires_grad()))), what,
               ": the backward pass is differentiable once only");
 }
 
@@ -65,7 +68,7 @@ struct DropoutNode : Function<DropoutNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const at::Tensor dy = grads[0];
-    once_differentiable(dy, "dropout");
+    once_differentiable(dy, false, "dropout");  // linear in dy, and of x it knows only the place
     const at::Tensor used = ctx->get_saved_variables()[0];
     BelowAutograd below;
     at::Tensor dx;
@@ -114,6 +117,8 @@ struct QkNormNode : Function<QkNormNode> {
     keep_sink(ctx, "q_sink", q_sink);
     keep_sink(ctx, "k_sink", k_sink);
     ctx->saved_data["eps"] = eps;
+    // each gradient depends on q, k and the angles; the weights' own are constant in the weights
+    ctx->saved_data["open"] = q.requires_grad() || k.requires_grad() || (rotate && wants(angles));
     ctx->saved_data["need_qw"] = wants(qw);
     ctx->saved_data["need_kw"] = wants(kw);
     ctx->saved_data["need_angles"] = rotate && wants(angles);
@@ -126,8 +131,9 @@ struct QkNormNode : Function<QkNormNode> {
     return {yq, yk};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable(grads[0], "qk_norm_rope");
-    once_differentiable(grads[1], "qk_norm_rope");
+    const bool open = ctx->saved_data["open"].toBool();
+    once_differentiable(grads[0], open, "qk_norm_rope");
+    once_differentiable(grads[1], open, "qk_norm_rope");
     const variable_list saved = ctx->get_saved_variables();
     BelowAutograd below;
     const at::Tensor q = saved[0], k = saved[1], pairs = saved[5];
@@ -232,6 +238,8 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
     keep_sink(ctx, "b_sink", b_sink);
     auto& d = ctx->saved_data;
     d["act"] = act;
+    // y is linear in x, weight, bias and gamma alone, but not in two that are multiplied, nor behind an activation
+    d["open"] = (need_x && need_w) || ((act != 0 || need_g) && (need_x || need_w || need_b));
     d["need_x"] = need_x;
     d["need_w"] = need_w;
     d["need_b"] = need_b;
@@ -248,7 +256,7 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const at::Tensor dy = grads[0];
-    once_differentiable(dy, "fp8_linear");
+    once_differentiable(dy, ctx->saved_data["open"].toBool(), "fp8_linear");
     const variable_list s = ctx->get_saved_variables();
     BelowAutograd below;
     auto& d = ctx->saved_data;

@@ -28,8 +28,8 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
+from ._autograd import differentiable_once
 from ._native import native, use_native
 from ._params import grad_sink
 from .linear import _ACTS, ACT_GELU, compute_dtype, gelu_grad_reference, gelu_reference
@@ -220,10 +220,12 @@ class _Fp8Linear(torch.autograd.Function):
         ctx.meta = (act, weight.dtype, weight.shape, gamma.dtype if gamma is not None else None,
                     bias.dtype if bias is not None else None)
         ctx.sinks = (grad_sink(weight), grad_sink(bias))
+        # y is linear in x, weight, bias and gamma alone, but not in two that are multiplied, nor behind an activation
+        ctx.open = (need_x and need_w) or ((act != 0 or need_g) and product)
         return y
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once("fp8_linear")
     def backward(ctx, dy):  # type: ignore[override]
         pre, g, bf, *flat = ctx.saved_tensors
         held = {k: Fp8Matrix(flat[2 * i], flat[2 * i + 1], cols, block)

@@ -20,8 +20,8 @@ backward pass leaves dq, dk and dv in one packed gradient.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
+from ._autograd import differentiable_once
 from ._native import native, use_native
 from ._params import grad_sink
 from .attention import _native_ok as _attention_native_ok
@@ -164,10 +164,11 @@ class _NativeNormRopeAttention(torch.autograd.Function):
         ctx.sinks = _Norms.sinks(qw, kw)
         ctx.w_dtypes = tuple(w.dtype if w is not None else None for w in (qw, kw))
         ctx.angles_meta = (angles.shape, angles.dtype) if angles is not None else None
+        ctx.open = True  # the softmax makes every gradient depend on every operand
         return o
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once("qk_norm_rope_attention")
     def backward(ctx, do):  # type: ignore[override]
         qkv, qk, o, lse, qw, kw, ang, pairs = ctx.saved_tensors
         b, n, _, h, d = qkv.shape

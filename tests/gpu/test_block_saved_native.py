@@ -162,3 +162,58 @@ def test_gamma_alone_needs_no_preactivation():
     for k, v in t.items():
         v.requires_grad_(k == "gamma")
     assert torch.equal(torch.autograd.grad(run(), t["gamma"], dy)[0], want)
+
+
+@pytest.mark.parametrize("second", [("x", "weight"), ("gamma", "bias"), ("gamma", "x"), ("gamma", "weight")])
+def test_second_derivative_of_a_linear_layer_is_refused_for_a_constant_gradient(second):
+    t, run = _linear()
+    for k, v in t.items():
+        v.requires_grad_(k in second)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(run().float().sum(), t[second[0]], create_graph=True)
+
+
+@pytest.mark.parametrize("leaf", ["x", "weight", "bias"])
+def test_second_derivative_behind_an_activation_is_refused(leaf):
+    t, run = _linear("gelu", gamma=False)
+    for k, v in t.items():
+        v.requires_grad_(k == leaf)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(run().float().sum(), t[leaf], create_graph=True)
+
+
+@pytest.mark.parametrize("wanted", ["x", "weight", "gamma", "bias"])
+def test_linear_layers_have_no_second_derivative_in_one_operand(wanted):
+    """The layer is linear in each operand alone: the gradient is a constant, and is returned as one."""
+    t, run = _linear()
+    for k, v in t.items():
+        v.requires_grad_(k == wanted)
+    want = torch.autograd.grad(run().float().sum(), t[wanted])[0]
+    got = torch.autograd.grad(run().float().sum(), t[wanted], create_graph=True)[0]
+    assert torch.equal(got, want) and not got.requires_grad
+
+
+@pytest.mark.parametrize("leaf", ["q", "k", "angles"])
+@pytest.mark.parametrize("entry", ["norm", "attention"])
+def test_second_derivative_of_head_norms_is_refused_for_a_constant_gradient(leaf, entry):
+    t = _heads()
+    packed = torch.stack([t["q"], t["k"], t["k"]], 2).detach().requires_grad_(leaf != "angles")
+    for k, v in t.items():
+        if k != "pairs":
+            v.requires_grad_(k == leaf)
+    if entry == "norm":
+        y = sum(o.float().sum() for o in qk_norm_rope(t["q"], t["k"], t["qw"], t["kw"], t["angles"], t["pairs"]))
+    else:
+        y = qk_norm_rope_attention(packed, t["qw"], t["kw"], t["angles"], t["pairs"], 0.125).float().sum()
+    wrt = t[leaf] if entry == "norm" or leaf == "angles" else packed
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, wrt, create_graph=True)
+
+
+def test_dropout_of_a_constant_gradient_needs_no_second_derivative():
+    from mia_train_b200.ops.dropout import dropout
+
+    x = torch.randn(40, 64, device=DEV, requires_grad=True)
+    rng = torch.tensor([3, 4], device=DEV)
+    got = torch.autograd.grad(dropout(x, 0.5, rng=rng).sum(), x, create_graph=True)[0]
+    assert torch.equal(got, torch.autograd.grad(dropout(x, 0.5, rng=rng).sum(), x)[0])

@@ -62,3 +62,23 @@ def test_gelu_without_a_product_gradient_keeps_no_preactivation(mode, monkeypatc
         for v in t.values():
             v.requires_grad_(True)
         assert torch.equal(g, torch.autograd.grad(run().float().sum(), t["gamma"])[0])
+
+
+@pytest.mark.parametrize("act,wanted", [(None, ("x", "weight")), (None, ("gamma", "bias")), (None, ("gamma", "x")),
+                                        ("gelu", ("x",)), ("gelu", ("weight",)), ("gelu", ("bias",))])
+def test_second_derivative_is_refused_for_a_constant_gradient(act, wanted):
+    t, run = _linear(act, gamma="gamma" in wanted)
+    for k, v in t.items():
+        v.requires_grad_(k in wanted)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(run().float().sum(), t[wanted[0]], create_graph=True)
+
+
+@pytest.mark.parametrize("wanted", ["x", "weight", "gamma", "bias"])
+def test_a_linear_layer_has_no_second_derivative_in_one_operand(wanted):
+    t, run = _linear()
+    for k, v in t.items():
+        v.requires_grad_(k == wanted)
+    want = torch.autograd.grad(run().float().sum(), t[wanted])[0]
+    got = torch.autograd.grad(run().float().sum(), t[wanted], create_graph=True)[0]
+    assert torch.equal(got, want) and not got.requires_grad
