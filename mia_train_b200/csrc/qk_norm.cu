@@ -349,9 +349,9 @@ __global__ void __launch_bounds__(32 * kQkWarps, 4) qk_norm_bwd_kernel(const QkN
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-        // zero past the last head: without an eps the root would be infinite there, and 0 r no zero
-        float r = rsqrtf(group_sum<LPR>(ss) * inv_d + p.eps);
-        if (h >= left) r = 0.f;
+        // past the last head all is zero: an eps of one keeps the root finite there, whatever the caller's (0 inf is no zero)
+        const float eps = h < left ? p.eps : 1.f;
+        const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + eps);
         qk_exchange<LPR>(gr[u], g, other, ex, cg, part, scattered, source);
         float dot = 0.f;
 #pragma unroll
