@@ -29,8 +29,12 @@
 // lanes fetched it), 16384 x 5120 x 1280 124 us, with GELU and its pre-activation 230 us.
 // Tried and slower: sums by packed f32x2 FMAs (1620 at 8192^3), 16 epilogue warps of 64 columns (1315), stores by
 // the lanes instead of TMA (16384 x 5120 x 1280: 155 us).
-// The scales are applied in fp32 outside the tensor core, so they may be any fp32 numbers, and no sum
-// longer than 128 products is left to the tensor core's own accumulation.
+// The scales are applied in fp32 outside the tensor core, so they may be any finite fp32 numbers, and no sum
+// longer than 128 products is left to the tensor core's own accumulation. A term is sum (sa sb) with a scale per block of
+// B and (sum sa) sb with one per row. Where the bracket may be past fp32's range though the term is not, the row is summed
+// in units of up to 2^40 (in place, in branches that other rows never take: 3 to 7 % of the time of the calls above for the
+// tests, against 10 to 50 % for longer arithmetic beside or inside the loop over K). Of the other end: products of scales
+// below 2^-149 count as zero, which leaves out less than 2^-125 a block (2^-111 with two e5m2 operands).
 //
 // All waits are bounded (see common.cuh); on a timeout the kernel records an error code, drains the
 // copies and MMAs it issued, frees its tensor memory and returns.
@@ -170,6 +174,13 @@ __device__ __forceinline__ void tc_mma_f8_block(uint32_t d_tmem, uint64_t a_desc
   if constexpr (CG == 2) MIA_MMA_F8_BLOCK("2");
   else MIA_MMA_F8_BLOCK("1");
 }
+
+// Larger units for the sums of rows whose scales would carry a term past fp32's range on the way to a product that lies
+// in it. 2^40 are enough: a sum is zero or at least 2^-32 (e5m2) in size, so that what is past the range in those
+// units is past it in the result. What such a row adds below 2^-149 units is lost.
+constexpr int kF8MaxUnits = 40;
+constexpr float kF8Up = 1099511627776.f, kF8Down = 1.f / kF8Up;  // 2^40
+constexpr float kF8LargeScale = 3.0948500982134507e26f;          // 2^88; a sum is at most 57344^2 128 < 2^39
 
 // 128 accumulators a thread (BN = 256) need more than the 168 registers that 384 threads can start with:
 // the four control warps hand theirs down. 128 * 40 + 256 * 232 = 384 * 168.
@@ -435,6 +446,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     constexpr int kChunks = kCols / kWidth;
     constexpr int kRowsT = SB_ROW ? 4 : 1;    // rows a thread holds: 8 i + lane / 4, or its lane
     const int row_t = SB_ROW ? lane / 4 : lane;
+    auto row_of = [](int j) { return SB_ROW ? (j >> 1 & 1) + 2 * (j >> 4 & 1) : 0; };  // of register j: which of kRowsT
     auto chunk_at = [](int c) { return SB_ROW ? (c / 2) * 32 + ((uint32_t)(c % 2 * 16) << 16) : c * 32; };  // TMEM offset
     constexpr int kLaneCols = kCols / 32;
     // One unit: the warps' halves are its two column ranges. Two units (a 256-wide tile of a pair): unit h
@@ -452,6 +464,20 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     uint64_t* const my_res = &res_bar[warp - kF8FirstEpi];
     uint32_t res_phase = 0;
     bool res_pending = false;
+    // The largest scales of a tile's blocks of B (kSb of them, see below), spread over the lanes.
+    constexpr int kSb = SB_ROW ? kLaneCols : HALVES;
+    float b_tile[kSb];
+    auto fetch_b_tile = [&](int index) {
+      if (index >= p.num_tiles) return;
+      const Unit v = work_unit(index);
+#pragma unroll
+      for (int i = 0; i < kSb; ++i) {
+        const float* const from = o.sb + v.kb0 * o.sb_ld + (min(v.n0 + n_col + 128 * i, p.N - 1) >> 7);
+        b_tile[i] = load_now(from + min(lane, v.num_k - 1) * o.sb_ld);
+        for (int kb = lane + 32; kb < v.num_k; kb += 32) b_tile[i] = fmaxf(fabsf(b_tile[i]), fabsf(load_now(from + kb * o.sb_ld)));
+      }
+    };
+    if (!SB_ROW) fetch_b_tile(worker);
     for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
       const Unit u = work_unit(tile);
       const int num_k = u.num_k;
@@ -464,7 +490,6 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       // Scales: this row's, and of B either one per block the warp's columns lie in (one, or two with HALVES
       // == 2) or, with a scale per row of B, those of columns n0 + column(32 i) + lane. Rows and columns past
       // the edge fetch the last one: their sums are never stored.
-      constexpr int kSb = SB_ROW ? kLaneCols : HALVES;
       const float* sa = o.sa + u.kb0 * o.sa_ld;
       int sa_at[kRowsT];
 #pragma unroll
@@ -486,6 +511,30 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           sb += o.sb_ld;
         }
       }
+      // The rows' units as powers of two: 1, or less where the sums are in larger ones. `large`: some row of the warp has
+      // larger ones.
+      float down[kRowsT];
+#pragma unroll
+      for (int i = 0; i < kRowsT; ++i) down[i] = 1.f;
+      bool large = false;
+      if (!SB_ROW) {
+        // The product of two scales can be past the range only if one of B is above 1 (weights beyond 448): then
+        // the rows' own products decide. B's scales of this tile came a tile ahead.
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSb; ++i) top = fmaxf(top, fabsf(b_tile[i]));
+        large = __any_sync(0xffffffffu, top >= 1.f);
+        if (large) {
+          int most = 0;  // of the sums of exponents: above those of every product
+          for (int kb = 0; kb < num_k; ++kb) {
+            auto exponent = [](float v) { return (int)(__float_as_uint(v) >> 23 & 255) - 126; };
+            const int ea = exponent(o.sa[(u.kb0 + kb) * o.sa_ld + sa_at[0]]);
+#pragma unroll
+            for (int i = 0; i < kSb; ++i) most = max(most, ea + exponent(o.sb[(u.kb0 + kb) * o.sb_ld + sb_at[i]]));
+          }
+          down[0] = __uint_as_float((uint32_t)(127 - min(max(most - 128, 0), kF8MaxUnits)) << 23);
+        }
+      }
       if (!FULL && p.residual != nullptr) {
         // this warp's part of the residual, into the staging rows its outputs will leave from; outside the K loop,
         // where the test alone cost the calls without a residual a tenth of their time
@@ -499,10 +548,34 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         __syncwarp();
         res_pending = true;
       }
+      // Whether a row's scale of the coming block is large enough to carry its product with a sum past the range.
+      auto large_rows = [&] {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRowsT; ++i) top = fmaxf(top, fabsf(sa_ahead[0][i]));
+        return top >= kF8LargeScale;
+      };
+      // The usual block with a scale per row of B: its unit is known to be full, and its row scales not to be large. One
+      // branch for both tests: a second one in this loop costs a tenth of the time.
+      bool usual = false;
       for (int kb = 0; kb < num_k; ++kb) {
-        if (!ready && !mbar_wait_warp(&tfull_bar[unit], unit_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
-          ok = false;
-          break;
+        if (SB_ROW ? !usual : !ready) {
+          if (!ready && !mbar_wait_warp(&tfull_bar[unit], unit_phase, abort_flag, p.err, kErrFp8EpilogueWait)) {
+            ok = false;
+            break;
+          }
+          if (SB_ROW) large = large || __any_sync(0xffffffffu, large_rows());
+          if (SB_ROW && large) {  // in place, so that the loop below keeps its registers
+#pragma unroll
+            for (int i = 0; i < kRowsT; ++i) {
+              const float f = fabsf(sa_ahead[0][i]) >= kF8LargeScale && down[i] == 1.f ? kF8Down : 1.f;
+              down[i] *= f;
+#pragma unroll
+              for (int j = 0; j < kCols; ++j)
+                if (row_of(j) == i) sum[j] *= f;
+              sa_ahead[0][i] *= down[i];
+            }
+          }
         }
         tc_fence_after();
         uint32_t r[2][kWidth];  // the next columns are on their way while these are added
@@ -521,8 +594,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         } else {
 #pragma unroll
           for (int i = 0; i < kSb; ++i) {
-            const float s = sa_ahead[0][0] * sb_ahead[0][i];
-            s1[i] = s > FLT_MAX ? FLT_MAX : s;  // two huge scales over a zero product stay zero; NaN stays NaN
+            const float s = sa_ahead[0][0] * (sb_ahead[0][i] * down[0]);
+            s1[i] = fabsf(s) > FLT_MAX ? copysignf(FLT_MAX, s) : s;  // a zero sum stays zero, and NaN NaN
           }
         }
 #pragma unroll
@@ -585,12 +658,24 @@ __global__ void __launch_bounds__(kF8Threads, 1)
               x[q] = fmaf(__uint_as_float(now[q]), s1[!SB_ROW && kSb == 2 ? c * kWidth / 64 : 0], x[q]);
           }
         }
-        ready = __shfl_sync(0xffffffffu, seen, 0) != 0;
-        __syncwarp();  // as in mbar_wait_warp
+        if (SB_ROW) {
+          const int news = __reduce_or_sync(0xffffffffu, seen | (large_rows() ? 2 : 0));
+          __syncwarp();  // as in mbar_wait_warp
+          ready = (news & 1) != 0;
+          usual = news == 1 && !large;
+        } else {
+          ready = __shfl_sync(0xffffffffu, seen, 0) != 0;
+          __syncwarp();  // as in mbar_wait_warp
+        }
         unit = next;
         unit_phase = next_phase;
       }
       if (!ok) break;
+      if (!SB_ROW) fetch_b_tile(tile + workers);
+      if (large) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) sum[j] *= 1.f / down[row_of(j)];
+      }
       if constexpr (!FULL) {
         // sum = op(sum, vec[n]) for a vector over the columns
         auto per_column = [&](const float* vec, auto op) {

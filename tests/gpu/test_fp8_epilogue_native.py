@@ -90,3 +90,81 @@ def test_weight_quantised_once_under_autocast_and_with_batches():
         assert torch.equal(y, fp8_linear(x, w, activation="gelu", residual=res))
     with pytest.raises(ValueError, match="no backward"):
         fp8_linear(x.requires_grad_(True), q)
+
+
+def _powers(exponents, cols=128):
+    return torch.tensor([2.0**e for e in exponents], device=DEV)[:, None].expand(-1, cols).contiguous()
+
+
+@pytest.mark.parametrize("block", [1, BLOCK])
+def test_row_scales_at_both_ends_of_the_range(block, tile):
+    """128 equal products of powers of two are exact whenever they are fp32 numbers, whatever their factors' sizes."""
+    rows = [120, 100, 60, 0, -60, -100, -120, -140]
+    a = quantize_fp8(_powers(rows))
+    for other in rows:
+        b = quantize_fp8(_powers([other] * 9 if block == BLOCK else [other, 0, -other if abs(other) < 127 else 0] * 3), block_rows=block)
+        want = a.dequantize().double() @ b.dequantize().double().t()
+        got = fp8_gemm(a, b, out_dtype=F32).double()
+        normal = (want >= 2.0**-126) & (want < 2.0**128)
+        assert torch.equal(got[normal], want[normal])
+        assert (got[want >= 2.0**128] == float("inf")).all()
+        # below the normal numbers: at most half a step of fp32's subnormals for each of the 128 products
+        assert ((got - want).abs()[want < 2.0**-126] <= 128 * 2.0**-150).all()
+    _no_errors()
+
+
+@pytest.mark.parametrize("block", [1, BLOCK])
+def test_small_sums_under_huge_scales(block, tile):
+    """Both blocks' largest values meet zeros; what is left is 2^-18 of a product of scales beyond fp32."""
+    a, b = torch.zeros(8, 256, device=DEV), torch.zeros(9, 256, device=DEV)
+    a[:, 0], a[:, 1] = 2.0**126, 2.0**109
+    b[:, 2], b[:, 1] = 2.0**30, 2.0**13
+    a[:, 128:], b[:, 128:] = 2.0**60, 2.0**50  # an ordinary block next to it
+    qa, qb = quantize_fp8(a), quantize_fp8(b, block_rows=block)
+    assert (qa.scale[0] == 2.0**118).all() and (qb.scale[0] == 2.0**22).all()
+    assert (fp8_gemm(qa, qb, out_dtype=F32) == 2.0**122 + 2.0**117).all()
+    _no_errors()
+
+
+@pytest.mark.parametrize("scale_a,scale_b", [(3e38, 1e-30), (1e-30, 3e38), (3e38, 2e-38), (1e-37, 1e30), (-2.5, 1e-3), (0.0, 3e38),
+                                              (3e38, 3e38), (1e-44, 1e38)])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+@pytest.mark.parametrize("block", [1, BLOCK])
+def test_any_fp32_scales(block, fmt, scale_a, scale_b, tile):
+    """Scales that a caller brings need not be powers of two, nor of one sign."""
+    torch.manual_seed(5)
+    one = quantize_fp8(torch.ones(140, 300, device=DEV), block_rows=block, dtype=fmt)
+    a0 = quantize_fp8(torch.randint(-3, 4, (130, 300), device=DEV).float())
+    a = Fp8Matrix(a0.data, torch.full_like(a0.scale, scale_a), 300)
+    b = Fp8Matrix(one.data, torch.full_like(one.scale, scale_b), 300, block)
+    sums = [(a0.data[:, c:min(c + 128, 300)].double()).sum(1, keepdim=True) * one.data[:, 0].double() for c in (0, 128, 256)]
+    fa, fb = (torch.tensor(v, dtype=F32).double().item() for v in (scale_a, scale_b))
+    terms = [s * fa * fb for s in sums]
+    want, size = sum(terms), sum(t.abs() for t in terms)
+    got = fp8_gemm(a, b, out_dtype=F32).double()
+    safe = size < 2.0**127
+    # two roundings of a term's scales, one of each of three sums
+    assert ((got - want).abs()[safe] <= 5 * 2.0**-24 * size[safe] + 2.0**-149).all()
+    big = torch.stack([t.abs() for t in terms]).amin(0) >= 2.0**128
+    assert not got[big].isfinite().any()
+    assert (got[size == 0] == 0).all()
+    _no_errors()
+
+
+@pytest.mark.parametrize("where", [0, 1, 2])
+@pytest.mark.parametrize("block", [1, BLOCK])
+def test_rows_next_to_a_huge_one_stay_exact(block, where, tile):
+    """Row 37 alone meets scales past the range, in one of three blocks; integers elsewhere are summed exactly."""
+    torch.manual_seed(6)
+    a, b = torch.randint(-4, 5, (300, 384), device=DEV).float(), torch.zeros(72, 384, device=DEV)
+    b[:] = torch.randint(-4, 5, (72, 384), device=DEV)
+    at = slice(128 * where, 128 * where + 128)
+    a[:, at], b[:, at] = 0, 0
+    a[37, 128 * where], a[37, 128 * where + 1] = 2.0**126, 2.0**109  # scale 2^118
+    b[:, 128 * where + 2], b[:, 128 * where + 1] = 2.0**30, 2.0**13  # scale 2^22
+    qa, qb = quantize_fp8(a), quantize_fp8(b, block_rows=block)
+    got = fp8_gemm(qa, qb, out_dtype=F32).double()
+    want = a.double() @ b.double().t()
+    want[37] = 2.0**122  # the integers are below half a step of it
+    assert torch.equal(got, want)
+    _no_errors()
