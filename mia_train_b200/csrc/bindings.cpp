@@ -94,7 +94,8 @@ void koleo_bwd(at::Tensor x, at::Tensor xn, at::Tensor nn, at::Tensor dist, doub
 at::Tensor axial_angles_fwd(at::Tensor coords, std::vector<at::Tensor> freqs);
 void axial_angles_bwd(at::Tensor dangles, at::Tensor coords, std::vector<at::Tensor> freqs,
                       std::vector<at::Tensor> dfreqs);
-at::Tensor dropout(const at::Tensor& x, const OptTensor& residual, int64_t dropped, const OptTensor& rng);
+at::Tensor dropout(const at::Tensor& x, const OptTensor& residual, int64_t dropped, const OptTensor& rng,
+                   int64_t rank_key);
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
                                                 const OptTensor& kw, const OptTensor& angles, const OptTensor& pairs,
                                                 double eps, const OptTensor& q_sink, const OptTensor& k_sink);

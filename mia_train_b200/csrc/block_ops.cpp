@@ -53,13 +53,13 @@ at::Tensor aligned(const at::Tensor& t) {
 
 struct DropoutNode : Function<DropoutNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& residual, int64_t dropped,
-                            const OptTensor& rng) {
+                            const OptTensor& rng, int64_t rank_key) {
     BelowAutograd below;
     const at::Tensor xc = x.contiguous();
     const OptTensor res = residual.has_value() ? OptTensor(residual->contiguous()) : OptTensor();
     at::Tensor used = at::empty({2}, x.options().dtype(at::kLong));
     at::Tensor y = at::empty_like(xc);
-    dropout_apply(xc, res, y, dropped, rng.has_value() ? OptTensor(rng->contiguous()) : OptTensor(), used);
+    dropout_launch(xc, res, y, dropped, rng.has_value() ? OptTensor(rng->contiguous()) : OptTensor(), used, rank_key);
     ctx->save_for_backward({used});
     ctx->saved_data["dropped"] = dropped;
     ctx->saved_data["need_x"] = x.requires_grad();
@@ -77,7 +77,7 @@ struct DropoutNode : Function<DropoutNode> {
       dx = at::empty_like(dyc);
       dropout_apply(dyc, {}, dx, ctx->saved_data["dropped"].toInt(), used, {});
     }
-    return {dx, ctx->saved_data["need_r"].toBool() ? dy : at::Tensor(), at::Tensor(), at::Tensor()};
+    return {dx, ctx->saved_data["need_r"].toBool() ? dy : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -303,8 +303,9 @@ struct Fp8LinearNode : Function<Fp8LinearNode> {
 
 }  // namespace
 
-at::Tensor dropout(const at::Tensor& x, const OptTensor& residual, int64_t dropped, const OptTensor& rng) {
-  return DropoutNode::apply(x, residual, dropped, rng);
+at::Tensor dropout(const at::Tensor& x, const OptTensor& residual, int64_t dropped, const OptTensor& rng,
+                   int64_t rank_key) {
+  return DropoutNode::apply(x, residual, dropped, rng, rank_key);
 }
 
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,

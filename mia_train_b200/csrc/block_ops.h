@@ -7,6 +7,8 @@ namespace mia {
 
 using OptTensor = c10::optional<at::Tensor>;
 
+void dropout_launch(at::Tensor x, OptTensor residual, at::Tensor y, int64_t dropped, OptTensor rng, OptTensor record,
+                    int64_t rank_key);
 void dropout_apply(at::Tensor x, OptTensor residual, at::Tensor y, int64_t dropped, OptTensor rng, OptTensor record);
 void qk_norm_fwd(at::Tensor q, at::Tensor k, OptTensor qw, OptTensor kw, OptTensor angles, at::Tensor pairs,
                  at::Tensor yq, at::Tensor yk, double eps);

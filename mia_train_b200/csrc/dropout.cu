@@ -33,6 +33,7 @@ struct DropRng {
   const int64_t* given;       // (seed, offset), or nullptr: take `state`
   int64_t* record;            // where the pair is written for the backward pass, or nullptr
   at::PhiloxCudaState state;  // PyTorch's generator; resolved on the device so that a captured graph draws anew
+  uint64_t rank_key;          // mixed into a drawn seed
 };
 
 __device__ __forceinline__ uint4 philox4x32_10(uint64_t group, uint64_t seed, uint64_t offset) {
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, c
     offset = (uint64_t)rng.given[1];
   } else {
     const auto so = at::cuda::philox::unpack(rng.state);
-    seed = std::get<0>(so);
+    seed = std::get<0>(so) ^ rng.rank_key;
     offset = std::get<1>(so);
   }
   if (rng.record != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -122,10 +123,10 @@ static void launch_dropout(const torch::Tensor& x, const c10::optional<torch::Te
 }
 
 // y = residual + dropout(x). `rng` holds (seed, offset); without it the pair is drawn from PyTorch's
-// CUDA generator of that device. `record` receives the pair that was used: the caller may advance
-// its own tensor before the backward pass.
-void dropout_apply(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor y, int64_t dropped,
-                   c10::optional<torch::Tensor> rng, c10::optional<torch::Tensor> record) {
+// CUDA generator of that device, the seed taken apart by `rank_key` (ranks seed their generators alike). `record` receives
+// the pair that was used: the caller may advance its own tensor before the backward pass.
+void dropout_launch(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor y, int64_t dropped,
+                    c10::optional<torch::Tensor> rng, c10::optional<torch::Tensor> record, int64_t rank_key) {
   TORCH_CHECK(x.is_cuda() && x.is_contiguous() && y.is_contiguous(), "dropout: contiguous CUDA tensors expected");
   TORCH_CHECK(y.device() == x.device() && y.scalar_type() == x.scalar_type() && y.numel() == x.numel(),
               "dropout: output must match the input");
@@ -149,6 +150,7 @@ void dropout_apply(torch::Tensor x, c10::optional<torch::Tensor> residual, torch
         c10::nullopt, at::cuda::detail::getDefaultCUDAGenerator(x.get_device()));
     std::lock_guard<std::mutex> lock(gen->mutex_);
     r.state = gen->philox_cuda_state(4);
+    r.rank_key = (uint64_t)rank_key;
   }
   if (record.has_value()) {
     check_pair(*record);
@@ -163,6 +165,11 @@ void dropout_apply(torch::Tensor x, c10::optional<torch::Tensor> residual, torch
   else if (x.scalar_type() == at::kHalf) launch_dropout<__half>(x, residual, y, (uint32_t)dropped, scale, r, stream);
   else if (x.scalar_type() == at::kFloat) launch_dropout<float>(x, residual, y, (uint32_t)dropped, scale, r, stream);
   else TORCH_CHECK(false, "dropout: bf16, fp16 or fp32 expected");
+}
+
+void dropout_apply(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor y, int64_t dropped,
+                   c10::optional<torch::Tensor> rng, c10::optional<torch::Tensor> record) {
+  dropout_launch(x, residual, y, dropped, rng, record, 0);
 }
 
 }  // namespace mia

@@ -39,6 +39,7 @@ from torch.utils.data import DataLoader, DistributedSampler
 from ..algorithms.base import BaseAlgorithm
 from ..data.base import BaseDataset
 from ..ops._native import raise_on_device_errors
+from ..ops.dropout import set_rank as set_dropout_rank
 from ..parallel.sequence_parallel import sync_partial_grads
 from ..parallel.parallel_dims import ParallelDims
 from ..parallel.parallelize import parallelize_algorithm, refresh_fsdp_grad_dtypes
@@ -131,6 +132,7 @@ class Trainer:
         self.scheduler = build_lr_scheduler(self.optimizer, config)
         self.checkpoints = CheckpointManager(self.algorithm, self.optimizer, self.output_dir / "checkpoints")
         dp_rank = self.dims.dp_rank(mesh) if mesh is not None else 0
+        set_dropout_rank(dp_rank)
         loader_args = {
             "batch_size": config.batch_size,
             "rank": dp_rank,

@@ -10,7 +10,8 @@ its strides.
 `rng` is an int64 tensor (seed, offset) on x's device, which makes the mask a function of the
 inputs; without it the pair is drawn from PyTorch's generator of that device, so `torch.manual_seed`
 reproduces it, activation checkpointing's saved generator state replays it, and every replay of a
-captured graph draws a new one. Calls that share an `rng` share their mask. CPU tensors run the
+captured graph draws a new one. `set_rank(r)` takes the drawn seeds of data-parallel ranks, which seed
+their generators alike, apart; the Trainer calls it. Calls that share an `rng` share their mask. CPU tensors run the
 same generator in PyTorch and give the same masks.
 """
 
@@ -59,8 +60,21 @@ def dropout_reference(
     return (y if residual is None else residual.to(acc) + y).to(x.dtype)
 
 
+_rank_key = 0
+
+
+def set_rank(rank: int) -> None:
+    """Masks that this process draws from here on are those of data-parallel rank `rank`; 0 is what one process draws.
+    An `rng` that a caller passes is taken as it is."""
+    global _rank_key
+    if rank < 0:
+        raise ValueError(f"rank must not be negative, got {rank}")
+    key = rank * 0x9E3779B97F4A7C15 % (1 << 64)  # odd: distinct for distinct ranks
+    _rank_key = key - (1 << 64) if key >> 63 else key
+
+
 def _draw(device: torch.device) -> torch.Tensor:
-    seed = torch.randint(-(1 << 63), (1 << 63) - 1, (1,), device=device)
+    seed = torch.randint(-(1 << 63), (1 << 63) - 1, (1,), device=device) ^ _rank_key
     return torch.cat([seed, torch.zeros_like(seed)])
 
 
@@ -110,5 +124,5 @@ def dropout(
     if dropped == 0:
         return x if residual is None else residual + x
     if x.dtype in _DTYPES and use_native(x):
-        return native().dropout(x, residual, dropped, rng)
+        return native().dropout(x, residual, dropped, rng, _rank_key)
     return _Dropout.apply(x, residual, dropped, rng)
