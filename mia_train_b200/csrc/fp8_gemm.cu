@@ -44,6 +44,7 @@
 
 #include <atomic>
 #include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 #include "block_ops.h"
@@ -66,6 +67,10 @@ struct Fp8Operands {
   const float* sb;
   int64_t sb_ld;
   int a_format, b_format;  // 0 = e4m3, 1 = e5m2
+  // A scale per row of B: scales of A from this power of two on may carry their product with a sum past the range.
+  // 128 products are below 2^25, 2^32 or 2^39 for none, one or two e5m2 operands.
+  int safe_exponent;
+  float safe_scale;
 };
 
 template <int CG, int BN, int STAGES>
@@ -176,11 +181,12 @@ __device__ __forceinline__ void tc_mma_f8_block(uint32_t d_tmem, uint64_t a_desc
 }
 
 // Larger units for the sums of rows whose scales would carry a term past fp32's range on the way to a product that lies
-// in it. 2^40 are enough: a sum is zero or at least 2^-32 (e5m2) in size, so that what is past the range in those
-// units is past it in the result. What such a row adds below 2^-149 units is lost.
-constexpr int kF8MaxUnits = 40;
-constexpr float kF8Up = 1099511627776.f, kF8Down = 1.f / kF8Up;  // 2^40
-constexpr float kF8LargeScale = 3.0948500982134507e26f;          // 2^88; a sum is at most 57344^2 128 < 2^39
+// in it: as large as that row needs, up to 2^40. More is not needed: a sum is zero or at least 2^-32 (e5m2) in size, so that
+// what is past the range in those units is past it in the result.
+constexpr int kF8HalfUnits = 20;
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// e with |v| < 2^e (infinities and NaN: 2^128)
+__device__ __forceinline__ int exponent_above(float v) { return min((int)(__float_as_uint(v) >> 23 & 255), 254) - 126; }
 
 // 128 accumulators a thread (BN = 256) need more than the 168 registers that 384 threads can start with:
 // the four control warps hand theirs down. 128 * 40 + 256 * 232 = 384 * 168.
@@ -511,8 +517,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           sb += o.sb_ld;
         }
       }
-      // The rows' units as powers of two: 1, or less where the sums are in larger ones. `large`: some row of the warp has
-      // larger ones.
+      // The rows' units. With a scale per row of B: 1 / down, above 1 only while a block with a large row scale is added
+      // (back in units of 1 a sum overflows where the result would). Else 1 / down^2 for the whole tile, half of it for
+      // either scale, so that no scale of the quantiser (2^-126 and more) is lost. Either way a row with such a block keeps
+      // nothing below 2^-109. `large`: some row of the warp has them.
       float down[kRowsT];
 #pragma unroll
       for (int i = 0; i < kRowsT; ++i) down[i] = 1.f;
@@ -525,14 +533,14 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int i = 0; i < kSb; ++i) top = fmaxf(top, fabsf(b_tile[i]));
         large = __any_sync(0xffffffffu, top >= 1.f);
         if (large) {
-          int most = 0;  // of the sums of exponents: above those of every product
+          int most = 128;  // above the exponents of every product
           for (int kb = 0; kb < num_k; ++kb) {
-            auto exponent = [](float v) { return (int)(__float_as_uint(v) >> 23 & 255) - 126; };
-            const int ea = exponent(o.sa[(u.kb0 + kb) * o.sa_ld + sa_at[0]]);
+            const int ea = exponent_above(o.sa[(u.kb0 + kb) * o.sa_ld + sa_at[0]]);
 #pragma unroll
-            for (int i = 0; i < kSb; ++i) most = max(most, ea + exponent(o.sb[(u.kb0 + kb) * o.sb_ld + sb_at[i]]));
+            for (int i = 0; i < kSb; ++i)
+              most = max(most, ea + exponent_above(o.sb[(u.kb0 + kb) * o.sb_ld + sb_at[i]]));
           }
-          down[0] = __uint_as_float((uint32_t)(127 - min(max(most - 128, 0), kF8MaxUnits)) << 23);
+          down[0] = power_of_two(-min((most - 127) / 2, kF8HalfUnits));
         }
       }
       if (!FULL && p.residual != nullptr) {
@@ -553,7 +561,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < kRowsT; ++i) top = fmaxf(top, fabsf(sa_ahead[0][i]));
-        return top >= kF8LargeScale;
+        return top >= o.safe_scale;
       };
       // The usual block with a scale per row of B: its unit is known to be full, and its row scales not to be large. One
       // branch for both tests: a second one in this loop costs a tenth of the time.
@@ -568,8 +576,9 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           if (SB_ROW && large) {  // in place, so that the loop below keeps its registers
 #pragma unroll
             for (int i = 0; i < kRowsT; ++i) {
-              const float f = fabsf(sa_ahead[0][i]) >= kF8LargeScale && down[i] == 1.f ? kF8Down : 1.f;
-              down[i] *= f;
+              const float unit = power_of_two(-max(exponent_above(sa_ahead[0][i]) - o.safe_exponent, 0));
+              const float f = unit / down[i];
+              down[i] = unit;
 #pragma unroll
               for (int j = 0; j < kCols; ++j)
                 if (row_of(j) == i) sum[j] *= f;
@@ -594,7 +603,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         } else {
 #pragma unroll
           for (int i = 0; i < kSb; ++i) {
-            const float s = sa_ahead[0][0] * (sb_ahead[0][i] * down[0]);
+            const float s = (sa_ahead[0][0] * down[0]) * (sb_ahead[0][i] * down[0]);
             s1[i] = fabsf(s) > FLT_MAX ? copysignf(FLT_MAX, s) : s;  // a zero sum stays zero, and NaN NaN
           }
         }
@@ -674,7 +683,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       if (!SB_ROW) fetch_b_tile(tile + workers);
       if (large) {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) sum[j] *= 1.f / down[row_of(j)];
+        for (int j = 0; j < kCols; ++j) sum[j] *= 1.f / (SB_ROW ? down[row_of(j)] : down[0] * down[0]);
       }
       if constexpr (!FULL) {
         // sum = op(sum, vec[n]) for a vector over the columns
@@ -954,6 +963,8 @@ void fp8_gemm(torch::Tensor a, torch::Tensor a_scale, bool a_block, torch::Tenso
   Fp8Operands o{};
   o.a_format = format(a);
   o.b_format = format(b);
+  o.safe_exponent = 102 - 7 * (o.a_format + o.b_format);
+  o.safe_scale = std::ldexp(1.f, o.safe_exponent);
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && d.dim() == 2 && a.stride(1) == 1 && b.stride(1) == 1 && d.is_contiguous(),
               "fp8_gemm: row-major 2-D operands expected");
   const int64_t M = a.size(0), N = b.size(0);

@@ -168,3 +168,18 @@ def test_rows_next_to_a_huge_one_stay_exact(block, where, tile):
     want[37] = 2.0**122  # the integers are below half a step of it
     assert torch.equal(got, want)
     _no_errors()
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+@pytest.mark.parametrize("block", [1, BLOCK])
+def test_tiny_blocks_of_a_row_with_huge_ones_count(block, fmt, first, tile):
+    """One block's scales multiply beyond fp32 over a zero sum; another's are at the ends of the range and give 32."""
+    a, b = torch.zeros(40, 256, device=DEV), torch.zeros(9, 256, device=DEV)
+    huge, tiny = (slice(0, 128), slice(128, 256)) if first else (slice(128, 256), slice(0, 128))
+    a[:, huge.start], b[:, huge.start + 1] = 2.0**126, 2.0**100
+    a[:, tiny], b[:, tiny] = 2.0**-120, 2.0**118
+    qa, qb = quantize_fp8(a, dtype=fmt), quantize_fp8(b, block_rows=block, dtype=fmt)
+    assert qa.scale.max() * qb.scale.max() == float("inf") and qa.scale.min() == 2.0**-126
+    assert (fp8_gemm(qa, qb, out_dtype=F32) == 32).all()
+    _no_errors()
