@@ -30,9 +30,20 @@ from torch.distributed._composable.replicate import replicate
 from torch.distributed.tensor.parallel import parallelize_module
 
 from ..algorithms.base import BaseAlgorithm
+from ..layers.common.blocks import TransformerBlock
+from ..layers.dinov3.block import SelfAttentionBlock
 from ..models.base import BaseModel
 from .parallel_dims import ParallelDims
 from .tensor_parallel import BlockTensorParallelPlan, apply_tensor_parallel
+
+
+def _drops_elements(block: nn.Module) -> bool:
+    """A transformer block of this framework with dropout; a model's own modules, outside the blocks, are its affair."""
+    if isinstance(block, TransformerBlock):
+        return block.dropout > 0.0
+    if isinstance(block, SelfAttentionBlock):
+        return block.attn.proj_drop.p > 0.0 or getattr(getattr(block.mlp, "drop", None), "p", 0.0) > 0.0
+    return False
 
 
 def _apply_tensor_parallel(model: nn.Module, mesh: DeviceMesh, dims: ParallelDims) -> None:
@@ -54,8 +65,7 @@ def _apply_tensor_parallel(model: nn.Module, mesh: DeviceMesh, dims: ParallelDim
             f"tensor parallelism (tp = {dims.tp}, tp_comm = {dims.tp_comm!r}): set [model] drop_path_rate = 0, "
             "use tp_comm = \"allreduce\", or train with data parallelism"
         )
-    dropped = [name for name, m in model.named_modules()
-               if getattr(m, "dropout", 0.0) or (isinstance(m, nn.Dropout) and m.p > 0.0)]
+    dropped = [name for name, m in model.named_modules() if _drops_elements(m)]
     if dropped:
         # every rank would have to draw the mask of the elements it holds
         raise ValueError(
