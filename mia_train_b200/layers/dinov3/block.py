@@ -60,7 +60,8 @@ class SelfAttentionBlock(nn.Module):
         self.norm1 = norm_layer(dim)
         self.attn: SelfAttention = attn_class(
             dim, num_heads=num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias, attn_drop=attn_drop,
-            proj_drop=drop, mask_k_bias=mask_k_bias, use_fa4=use_fa4, qk_norm=qk_norm, device=device,
+            proj_drop=drop, mask_k_bias=mask_k_bias, use_fa4=use_fa4, device=device,
+            **({"qk_norm": True} if qk_norm else {}),  # an attn_class need not know of it
         )
         self.ls1: nn.Module = LayerScale(dim, init_values=init_values, device=device) if init_values else nn.Identity()
         self.norm2 = norm_layer(dim)

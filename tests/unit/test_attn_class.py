@@ -1,0 +1,26 @@
+"""A block takes attention classes that were written before the query/key norm."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mia_train_b200.layers.dinov3.attention import SelfAttention
+from mia_train_b200.layers.dinov3.block import SelfAttentionBlock
+
+
+class Plain(SelfAttention):
+    def __init__(self, dim, num_heads=8, qkv_bias=False, proj_bias=True, attn_drop=0.0, proj_drop=0.0, mask_k_bias=False,
+                 use_fa4=False, device=None):
+        super().__init__(dim, num_heads, qkv_bias, proj_bias, attn_drop, proj_drop, mask_k_bias, use_fa4, device=device)
+
+
+def test_attention_class_without_qk_norm():
+    torch.manual_seed(0)
+    ours = SelfAttentionBlock(32, 2)
+    block = SelfAttentionBlock(32, 2, attn_class=Plain)
+    block.load_state_dict(ours.state_dict())
+    x = torch.randn(2, 5, 32)
+    assert torch.equal(block(x), ours(x))
+    with pytest.raises(TypeError, match="qk_norm"):
+        SelfAttentionBlock(32, 2, attn_class=Plain, qk_norm=True)
