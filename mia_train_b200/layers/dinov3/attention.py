@@ -86,8 +86,8 @@ class SelfAttention(nn.Module):
         proj_drop: float = 0.0,
         mask_k_bias: bool = False,
         use_fa4: bool = False,
-        qk_norm: bool = False,
         device=None,
+        qk_norm: bool = False,
     ) -> None:
         super().__init__()
         if use_fa4:

@@ -53,8 +53,8 @@ class SelfAttentionBlock(nn.Module):
         ffn_layer: Callable[..., Mlp | SwiGLUFFN] = Mlp,
         mask_k_bias: bool = False,
         use_fa4: bool = False,
-        qk_norm: bool = False,
         device=None,
+        qk_norm: bool = False,
     ) -> None:
         super().__init__()
         self.norm1 = norm_layer(dim)

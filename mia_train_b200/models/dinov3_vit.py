@@ -52,9 +52,9 @@ class DinoVisionTransformer(DinoVisionTransformer3D):
         use_fa4: bool = False,
         untie_cls_and_patch_norms: bool = False,
         untie_global_and_local_cls_norm: bool = False,
+        device: Any | None = None,
         qk_norm: bool = False,
         drop_rate: float = 0.0,
-        device: Any | None = None,
     ) -> None:
         super().__init__(
             img_size=img_size, patch_size=patch_size, in_chans=in_chans, pos_embed_rope_type="vanilla",

@@ -99,9 +99,9 @@ class DinoVisionTransformer3D(BaseModel):
         untie_global_and_local_cls_norm: bool = False,
         window_size: int = 0,
         global_every: int = 0,
+        device: Any | None = None,
         qk_norm: bool = False,
         drop_rate: float = 0.0,
-        device: Any | None = None,
     ) -> None:
         super().__init__()
         if norm_layer not in norm_layer_dict:

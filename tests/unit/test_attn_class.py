@@ -24,3 +24,17 @@ def test_attention_class_without_qk_norm():
     assert torch.equal(block(x), ours(x))
     with pytest.raises(TypeError, match="qk_norm"):
         SelfAttentionBlock(32, 2, attn_class=Plain, qk_norm=True)
+
+
+def test_new_options_come_after_every_former_argument():
+    """Calls with positional arguments mean what they meant."""
+    import inspect
+
+    from mia_train_b200.models.dinov3_vit import DinoVisionTransformer
+    from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D
+
+    for cls in (SelfAttention, SelfAttentionBlock, DinoVisionTransformer, DinoVisionTransformer3D):
+        names = list(inspect.signature(cls.__init__).parameters)
+        assert names.index("device") < names.index("qk_norm"), cls.__name__
+    attn = SelfAttention(32, 2, False, True, 0.0, 0.0, False, False, torch.device("cpu"))
+    assert attn.q_norm is None
