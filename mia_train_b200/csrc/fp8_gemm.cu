@@ -24,15 +24,16 @@
 //              shared memory so that four lanes hold 16 columns of one row.
 // What bounds it: the additions. 128 x 256 sums a K block and CTA are 256 FMA cycles of the SM at best, with a
 // scale per column twice that, against 512 cycles of MMA; with both emptied of arithmetic the same pipeline runs
-// at 2590 TFLOP/s. Measured (bf16 out): 8192^3 2010 TFLOP/s with scales per weight block, 1400 with a scale per
-// row of both; 16384 x 1280 x 5120 (M x N x K) 127 us (1690 TFLOP/s), with a residual 138 us (228 us when the
-// lanes fetched it), 16384 x 5120 x 1280 124 us, with GELU and its pre-activation 230 us.
+// at 2590 TFLOP/s. Measured (ten launches from a graph, bf16 out): 8192^3 2000 TFLOP/s with scales per weight block, 1330
+// with a scale per row of both; 16384 x 1280 x 5120 (M x N x K) 128 us (1680 TFLOP/s), with a residual 137 us (228 us when
+// the lanes fetched it), 16384 x 5120 x 1280 128 us, with GELU 230 us, with its pre-activation as well 246 us; 5120 x 1280 x
+// 16384 with row scales to fp32 192 us, added to a gradient 258 us.
 // Tried and slower: sums by packed f32x2 FMAs (1620 at 8192^3), 16 epilogue warps of 64 columns (1315), stores by
 // the lanes instead of TMA (16384 x 5120 x 1280: 155 us).
 // The scales are applied in fp32 outside the tensor core, so they may be any finite fp32 numbers, and no sum
 // longer than 128 products is left to the tensor core's own accumulation. A term is sum (sa sb) with a scale per block of
 // B and (sum sa) sb with one per row. Where the bracket may be past fp32's range though the term is not, the row is summed
-// in units of up to 2^40 (in place, in branches that other rows never take: 3 to 7 % of the time of the calls above for the
+// in units of up to 2^40 (in place, in branches that other rows never take: 2 to 5 % of the time of the calls above for the
 // tests, against 10 to 50 % for longer arithmetic beside or inside the loop over K). Of the other end: products of scales
 // below 2^-149 count as zero, which leaves out less than 2^-125 a block (2^-111 with two e5m2 operands).
 //
@@ -898,7 +899,7 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   const int tiles = p.num_m_tiles * p.num_n_tiles, num_k = (p.K + kF8K - 1) / kF8K, workers = sm_count(device) / CG;
   // Two halves of K where the last wave of whole tiles would leave many SMs idle (weight gradients: a long K and
   // few tiles). Both halves are added to a cleared fp32 output; a sum of two does not depend on their order. Measured
-  // at 5120 x 1280 x 16384 (100 tiles of 256 x 256 for 74 pairs): 217 -> 181 us.
+  // at 5120 x 1280 x 16384 (100 tiles of 256 x 256 for 74 pairs): 217 -> 187 us when it came, 192 us now.
   auto waves = [&](int units) { return (units + workers - 1) / workers; };
   p.splits = may_split && num_k >= 16 && 0.85 * 2 * waves(tiles) >= waves(2 * tiles) ? 2 : 1;
   p.k_blocks_per_split = (num_k + p.splits - 1) / p.splits;
@@ -922,8 +923,8 @@ static void launch_fp8(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
 // Tile shape: the share of the SMs' time that goes into real output (waves of tiles over the SMs, rows and
 // columns past the edge) counts for each shape, and a 256 x 256 tile runs about 1.4 times the rate of four
 // 128 x 128 ones. Measured, 256 against 128, bf16 out, scales per weight block: 16384 x 1280 x 5120 (M x N
-// x K) 125 / 205 us, 16384 x 5120 x 1280 122 / 143 us, 2048 x 4096 x 1024 16.5 / 18.6 us; with half of the
-// SMs idle 2048 x 1024 x 4096 22.7 / 16.5 us, 1029 x 640 x 1712 14.4 / 12.4 us.
+// x K) 128 / 217 us, 16384 x 5120 x 1280 129 / 156 us, 2048 x 4096 x 1024 16.6 / 19.2 us; with half of the
+// SMs idle 2048 x 1024 x 4096 21.0 / 15.4 us, 1029 x 640 x 1712 13.1 / 10.4 us.
 enum Fp8Tile : int { kTile128 = 0, kTile256 = 1 };
 
 // -1: by the rule below; otherwise every call takes this tile (`set_fp8_tile`, tests and measurements).

@@ -19,15 +19,16 @@
 // 256 / D' at a time (D' = D rounded up to a power of two, D' / 8 lanes a head), 16 bytes a lane. The grid
 // is as large as fits on the SMs at once; a warp loads several such steps together, the next ones (of the
 // next token as well) while it works on the last, and the next token's angles with them.
-// Partners: where every lane's eight channels are paired with eight channels of one other lane (rotation
-// by halves of a head of a power-of-two size), by shuffles; otherwise (axial chunks) through shared memory
+// Partners: where every lane's eight channels are paired with the same eight of one other lane (rotation by halves, where half
+// of a head is a multiple of eight), by shuffles; otherwise (axial chunks) through shared memory
 // at index c + c / 8, which spreads the stride of eight between lanes over all banks. Each element is read
-// once and written once: the kernels are bound by HBM.
+// once and written once.
 // Weight gradients: registers over a warp's tokens, one partial a CTA, summed in a fixed order by a
 // second kernel, so the result does not depend on the order in which CTAs run.
-// Measured, 4 x 4101 tokens of 16 query and 16 key heads of 64, bf16: forward 36 us (3.7 TB/s), backward 62 us
-// (3.3 TB/s). ncu: 0.6 instructions issued a cycle and scheduler, DRAM at a third: the instructions (19 a value
-// forward, 37 backward, a third of them the token's table and addresses) bound it before HBM does.
+// Measured, 4 x 4101 tokens of 16 query and 16 key heads of 64, bf16, ten launches from a graph: forward 34 us (4.0 TB/s),
+// backward 62 us (3.2 TB/s). ncu: 0.6 instructions issued a cycle and scheduler with 16 warps an SM, DRAM at a third: what
+// binds is the latency of the chain from a head's load over its sums to its store, with 19 instructions a value forward and
+// 37 backward, a third of them the token's table and addresses.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
