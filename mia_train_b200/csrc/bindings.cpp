@@ -106,6 +106,14 @@ at::Tensor fp8_linear_quantized(const at::Tensor& x, const at::Tensor& data, con
                                 int64_t K, const OptTensor& bias, const OptTensor& residual, const OptTensor& gamma,
                                 int64_t act, bool bf16);
 int64_t set_fp8_tile(int64_t tile);
+at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_bounds,
+                            const at::Tensor& k_bounds, double scale);
+std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                          const at::Tensor& freq, bool interleaved, double amplitude);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& x, int64_t k, double tau);
+at::Tensor top_logit_distillation(const at::Tensor& s, const at::Tensor& values, const at::Tensor& indices,
+                                  const OptTensor& teacher_lse, const OptTensor& weights, double tau,
+                                  double teacher_tau, double norm);
 }  // namespace mia
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -180,5 +188,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_linear", &mia::fp8_linear, "linear layer on 8-bit products as an autograd node");
   m.def("fp8_linear_quantized", &mia::fp8_linear_quantized, "8-bit linear layer on a weight quantised once");
   m.def("set_fp8_tile", &mia::set_fp8_tile, "-1: tile of the 8-bit GEMM by its rule; 0: 128 x 128, 1: 256 x 256; returns the previous");
+  m.def("packed_attention", &mia::packed_attention, "attention over packed sequences as an autograd node");
+  m.def("rotary", &mia::rotary, "rotation of q and k heads by their positions as an autograd node");
+  m.def("top_logits", &mia::top_logits, "k largest logits of every row, their indices and the log-sum-exp");
+  m.def("top_logit_distillation", &mia::top_logit_distillation, "divergence from a teacher's top logits as an autograd node");
   m.def("check_errors", &mia::read_and_clear_errors, "read and clear the device error word");
 }

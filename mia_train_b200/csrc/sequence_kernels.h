@@ -1,0 +1,90 @@
+// Launchers of the packed-attention, rotation and distillation kernels on plain pointers. They include no PyTorch header
+// (their nodes in sequence_ops.cpp check arguments, allocate, pick device and stream) and return the launch's status.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace mia {
+
+enum SequenceType : int { kSeqBf16 = 0, kSeqF16 = 1, kSeqF32 = 2, kSeqF64 = 3 };
+
+// Rows of heads: element (t, h, c) of a (T, H, D) tensor lies at t * row + h * head + c.
+struct HeadRows {
+  int64_t row, head;
+};
+
+struct PackedProblem {
+  const void *q, *k, *v;
+  HeadRows qs, ks, vs;
+  const int2* q_bounds;  // (queries): the keys [x, y) that a query sees; both ends never fall from one row to the next
+  const int2* k_bounds;  // (keys): the queries [x, y) that see a key; likewise
+  int Tq, Tk;            // rows of the sequences; rows behind them are not read
+  int Hq, Hk, group, D;
+  int lse_stride;        // columns of lse and delta: rows rounded up to 128
+  float scale;
+  SequenceType type;
+};
+
+// o (Tq.., Hq, D) contiguous; lse (Hq, lse_stride) fp32
+cudaError_t packed_fwd_rows(const PackedProblem& P, void* o, float* lse, cudaStream_t stream);
+// dout as strided rows; delta like lse (scratch); dq (.., Hq, D), dk and dv (.., Hk, D) contiguous
+cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
+                            float* delta, void* dq, void* dk, void* dv, cudaStream_t stream);
+
+struct TokenRows {
+  int64_t b, t, h;  // element strides of (B, T, H, D)
+};
+
+struct RotaryParams {
+  const void *q, *k;    // (B, T, H, D)
+  const void *xq, *xk;  // the forward pass's inputs, for the gradient of the frequencies
+  void *yq, *yk;
+  TokenRows qs, ks, xqs, xks, yqs, yks;
+  const void* pos;
+  int pos_type;   // 0: int64, 1: int32, 2: fp32, 3: fp64
+  int64_t pos_b;  // 0 where all rows of the batch share one row of positions
+  const void* freq;
+  int freq64;
+  int axes, P, D, T, Hq, Hk;
+  int64_t tokens;  // B * T
+  int group;       // tokens of a block at a time
+  float amplitude;
+  int inverse;
+  float* partial;  // (blocks, axes, P)
+};
+
+struct RotaryPlan {
+  bool vec;
+  int group;
+  unsigned grid;
+  size_t smem;
+};
+RotaryPlan rotary_plan(const RotaryParams& p, bool aligned, bool interleaved, bool learn);
+cudaError_t rotary_launch(RotaryParams p, const RotaryPlan& plan, SequenceType type, bool interleaved, float* dfreq,
+                          cudaStream_t stream);
+
+constexpr int kMaxTop = 256;     // top_logits
+constexpr int kMaxGiven = 1024;  // distillation
+
+cudaError_t top_logits_rows(const void* x, int64_t stride, int R, int V, int k, double tau, void* values,
+                            int64_t* indices, float* lse, SequenceType type, cudaStream_t stream);
+
+struct DistillParams {
+  const void* s;
+  int64_t s_row;
+  const void* values;  // (R, K)
+  const void* indices;
+  const float* lse;      // or null
+  const float* weights;  // or null
+  SequenceType type, value_type;
+  bool index64;
+  int R, V, K;
+  double tau, teacher_tau, norm;
+  double* stats;  // (R, 8)
+};
+cudaError_t distill_fwd(const DistillParams& p, double* row_loss, float* loss, cudaStream_t stream);
+cudaError_t distill_bwd(const DistillParams& p, const float* grad, void* ds, cudaStream_t stream);
+
+}  // namespace mia
