@@ -30,6 +30,7 @@ enum ErrorCode : int {
   kErrFp8MmaWait = 112,
   kErrFp8EpilogueWait = 113,
   kErrAttnWait = 201,
+  kErrPackedWait = 211,
   kErrCommWait = 301,
   kErrZeroReduceScatterWait = 401,
   kErrZeroNormWait = 402,

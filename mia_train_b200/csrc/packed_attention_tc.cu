@@ -1,0 +1,1105 @@
+// Packed-sequence attention on the 5th-generation tensor cores (formulas: packed_attention.cu), bf16 and fp16.
+//
+// Tiles are 128 consecutive rows of the packed array, wherever sequences begin and end: short sequences share a
+// tile and a tile's keys are one contiguous range, because the bounds of the rows never fall. A block of keys that
+// every row of the tile sees in full skips the mask. Heads of 8 .. 64 channels take 64-column tiles, up to 128 two of
+// them side by side; channels past the head are filled with zeros by the TMA unit and the products stop at the
+// next multiple of 16.
+//
+// All second products (P V, dS K, P^T dO, dS^T Q) take their first operand from tensor memory: the threads that
+// computed its row write it over the scores they read, half as many columns of 16-bit pairs, so that neither P nor
+// dS passes through shared memory.
+//
+// Masked entries are replaced before any maximum or product of this row, but the second products still multiply their
+// zeros with rows of other sequences. Where those hold an infinity or a NaN, the sum becomes NaN: an output row
+// that is not finite although its statistics are is computed again by the warp-per-row formulas, which read only what
+// the row sees.
+//
+// The backward pass is two kernels, one per owner of the sums (dQ by query tiles; dK and dV by key tiles): each
+// repeats S and dP, seven products instead of five, but no sum leaves its CTA, so there are no atomics, no fp32
+// buffers and the result has the same bits every time.
+//
+// Every wait is bounded (common.cuh); on expiry the kernel records kErrPackedWait, lets its copies and products land,
+// frees its tensor memory and returns.
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "packed_attention.h"
+
+namespace mia {
+namespace {
+
+constexpr int kRows = 128;  // rows of a tile, keys (or queries) of a block
+
+template <int DP>
+struct Tile {
+  static constexpr int kBytes = kRows * DP * 2;  // DP / 64 column groups of 128 rows x 128 bytes, swizzled
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  const bool ok = mbar_wait(bar, parity, abort_flag, err, kErrPackedWait);
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// 128 rows from `row` of head `h`; DP / 64 boxes
+template <int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int h) {
+#pragma unroll
+  for (int g = 0; g < DP / 64; ++g) tma_load_3d(dst + g * (kRows * 128), map, bar, g * 64, row, h);
+}
+
+// `bytes` (a multiple of 16, as both addresses) of global memory
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// exp2 of the multi-function unit: relative error 2^-22, far below the rounding of P; results under 2^-126 are 0.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// D(tmem) (+)= A(tmem, 16-bit pairs along K) * B(smem)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t idesc_of(int n, bool b_mn_major) {
+  const uint32_t bf16 = make_idesc_bf16(kRows, n, false, b_mn_major);
+  return std::is_same_v<T, __half> ? bf16 & ~((1u << 7) | (1u << 10)) : bf16;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+
+// Scores: d = A B^T over the head's channels, both tiles K-major.
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int D) {
+  for (int kk = 0; kk * 16 < D; ++kk) {
+    const uint32_t off = (kk >> 2) * (kRows * 128) + (kk & 3) * 32;
+    tc_mma_f16(d, make_sdesc_sw<128>(a + off, 16, 1024), make_sdesc_sw<128>(b + off, 16, 1024), idesc, kk > 0);
+  }
+}
+
+// Sums: d (+)= A B with A (128 x 128) in tensor memory, its second 64 columns of K at a + `second`, B the rows of a tile.
+__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t second, uint32_t b, uint32_t idesc,
+                                         bool accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    mma_ts(d, a + (kk >> 2) * second + (kk & 3) * 8, make_sdesc_sw<128>(b + kk * 2048, kRows * 128, 1024), idesc,
+           accumulate || kk > 0);
+}
+
+// 16 fp32 columns of this lane's row times `f`, as 16-bit values; returns NaN if any is not finite, else 0.
+template <typename T>
+__device__ __forceinline__ float store16(T* dst, const uint32_t (&v)[16], float f, bool first8, bool last8) {
+  float x[16], bad = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    x[e] = __uint_as_float(v[e]) * f;
+    bad = fmaf(x[e], 0.f, bad);
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if (g == 0 ? first8 : last8)
+      *reinterpret_cast<uint4*>(dst + 8 * g) =
+          make_uint4(pack2<T>(x[8 * g], x[8 * g + 1]), pack2<T>(x[8 * g + 2], x[8 * g + 3]),
+                     pack2<T>(x[8 * g + 4], x[8 * g + 5]), pack2<T>(x[8 * g + 6], x[8 * g + 7]));
+  return bad;
+}
+
+// ------------------------------------------------------------------------------------------- forward
+// A CTA owns NT tiles of 128 queries of one head. Warps 4 t .. 4 t + 3 hold tile t's rows, one thread per row: S from
+// tensor memory, running maximum and sum, P back over S. The accumulator O is rescaled in place, and only when a
+// block's maximum exceeds the reference maximum by more than 2^8 (P <= 2^8 until then). The last two warps load
+// (TMA) and issue the products. With two tiles one's softmax runs beside the other's products.
+//
+// Tensor memory: S (128 columns) and O (DP) per tile.
+template <int DP, int NT>
+struct FwdLayout {
+  static constexpr int kStages = DP == 64 && NT == 2 ? 3 : 2;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + NT * Tile<DP>::kBytes;
+  static constexpr int kV = kK + kStages * Tile<DP>::kBytes;
+  static constexpr int kBar = kV + kStages * Tile<DP>::kBytes;
+  static constexpr int kBytes = kBar + 256 + 1024;
+  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
+};
+
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
+    packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                         const __grid_constant__ CUtensorMap tmV, const PackedProblem P, T* __restrict__ o,
+                         float* __restrict__ lse, int* err) {
+  using L = FwdLayout<DP, NT>;
+  constexpr int S = L::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t *q_full = bar, *k_full = bar + 1, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+  uint64_t *s_full = v_empty + S, *p_full = s_full + NT, *o_full = p_full + NT, *drain = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int tiles = (P.Tq + NT * kRows - 1) / (NT * kRows);
+  const int h = blockIdx.x % P.Hq;
+  const int r0 = (tiles - 1 - (int)(blockIdx.x / P.Hq)) * NT * kRows;  // causal rows see the more keys the later they are
+  const int hk = h / P.group;
+
+  // key range of every tile, and of all
+  int begin[NT], end[NT];  // blocks
+  int from = 0, to = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    begin[t] = end[t] = 0;
+    const int a = r0 + t * kRows;
+    if (a >= P.Tq) continue;
+    const int lo = P.q_bounds[a].x, hi = P.q_bounds[min(a + kRows, P.Tq) - 1].y;
+    if (t == 0) from = to = lo;
+    if (hi <= lo) continue;
+    begin[t] = (lo - from) / kRows;
+    end[t] = (hi - from + kRows - 1) / kRows;
+    to = max(to, hi);
+  }
+  const int blocks = (to - from + kRows - 1) / kRows;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], kRows);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+  }
+  if (warp == NT * 4 + 1) {
+    tmem_alloc(tmem_slot, L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == NT * 4) {
+    if (lane == 0 && blocks > 0) {
+      // ---------------------------------------------------------------------------------- loads
+      int done = 0;
+      bool ok = true;
+      mbar_arrive_expect_tx(q_full, NT * Tile<DP>::kBytes);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) load_tile<DP>(smem + L::kQ + t * Tile<DP>::kBytes, &tmQ, q_full, r0 + t * kRows, h);
+      for (int j = 0; j < blocks; ++j) {
+        const int s = j % S;
+        const uint32_t free_parity = ((j / S) & 1) ^ 1;
+        if (!mbar_wait(&k_empty[s], free_parity, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[s], Tile<DP>::kBytes);
+        load_tile<DP>(smem + L::kK + s * Tile<DP>::kBytes, &tmK, &k_full[s], from + j * kRows, hk);
+        done = 2 * j + 1;
+        if (!mbar_wait(&v_empty[s], free_parity, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[s], Tile<DP>::kBytes);
+        load_tile<DP>(smem + L::kV + s * Tile<DP>::kBytes, &tmV, &v_full[s], from + j * kRows, hk);
+        done = 2 * j + 2;
+      }
+      if (!ok) {  // copies in flight land before shared memory is given back
+        mbar_wait(q_full, 0, nullptr, nullptr, 0);
+        for (int j = (done - 1) / 2; j >= 0 && j > (done - 1) / 2 - S - 1; --j) {
+          if (2 * j + 1 <= done) mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
+          if (2 * j + 2 <= done) mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
+        }
+      }
+    }
+  } else if (warp == NT * 4 + 1) {
+    if (lane == 0 && blocks > 0) {
+      // ------------------------------------------------------------------------------- products
+      const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_o = idesc_of<T>((P.D + 15) / 16 * 16, true);
+      const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+      bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrPackedWait);
+      for (int j = 0; j <= blocks && ok; ++j) {
+        if (j < blocks && !mbar_wait(&k_full[j % S], (j / S) & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (j > 0 && !mbar_wait(&v_full[(j - 1) % S], ((j - 1) / S) & 1, abort_flag, err, kErrPackedWait)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t t_s = tmem + t * kRows, t_o = tmem + NT * kRows + t * DP;
+          if (ok && j > begin[t] && j <= end[t]) {
+            const int it = j - 1 - begin[t];
+            if (!mbar_wait(&p_full[t], it & 1, abort_flag, err, kErrPackedWait)) {
+              ok = false;
+            } else {
+              tc_fence_after();
+              mma_sums(t_o, t_s, 32, v_addr + ((j - 1) % S) * Tile<DP>::kBytes, idesc_o, it > 0);
+            }
+          }
+          if (ok && j >= begin[t] && j < end[t]) {
+            tc_fence_after();
+            mma_scores(t_s, q_addr + t * Tile<DP>::kBytes, k_addr + (j % S) * Tile<DP>::kBytes, idesc_s, P.D);
+            tc_commit(&s_full[t]);
+          }
+        }
+        if (!ok) break;
+        if (j < blocks) tc_commit(&k_empty[j % S]);
+        if (j > 0) tc_commit(&v_empty[(j - 1) % S]);
+      }
+      if (ok) {
+        tc_commit(o_full);
+      } else {
+        tc_commit(drain);
+        mbar_wait(drain, 0, nullptr, nullptr, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------------------------ softmax
+    constexpr float kRescale = 8.f;
+    const int t = warp / 4, first = r0 + t * kRows;
+    const int r = (warp % 4) * 32 + lane, row = first + r;
+    const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t t_s = tmem + t * kRows + lane_off, t_o = tmem + NT * kRows + t * DP + lane_off;
+    const float scale_log2 = P.scale * kLog2e;
+    const int j0 = t == 0 ? begin[0] : begin[NT - 1], j1 = t == 0 ? end[0] : end[NT - 1];
+    const bool real = row < P.Tq;
+    const int2 mine = real ? P.q_bounds[row] : make_int2(0, 0);
+    int all_lo = 0, all_hi = 0;  // keys that every row of the tile sees
+    if (j1 > j0) {
+      all_lo = P.q_bounds[min(first + kRows, P.Tq) - 1].x;
+      all_hi = P.q_bounds[first].y;
+    }
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = j0; j < j1; ++j) {
+      if (!warp_wait(&s_full[t], (j - j0) & 1, abort_flag, err)) { ok = false; break; }
+      tc_fence_after();
+      const int kb = from + j * kRows;
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, v[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(v[c]);
+      if (kb < all_lo || kb + kRows > all_hi) {
+        const int a = mine.x - kb;
+        const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((uint32_t)(c * 32 + e - a) >= n) v[c][e] = 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][e]));
+      const float blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+      const bool move = blk > m + kRescale;  // of a first block with a key always
+      if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+        // s_full of this block follows every earlier product: O is at rest
+        const float alpha = move && m != -INFINITY ? exp2_approx(m - blk) : 1.f;
+#pragma unroll 1
+        for (int c = 0; c * 16 < P.D; ++c) {
+          uint32_t w[16];
+          tmem_ld_32x32b_x16(t_o + c * 16, w);
+          tmem_ld_wait_regs16(w);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+          tmem_st_32x32b_x16(t_o + c * 16, w);
+        }
+        l *= alpha;
+      }
+      if (move) m = blk;
+      const float ref = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e]), scale_log2, -ref));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e + 1]), scale_log2, -ref));
+          sum[c] += p0 + p1;
+          pk[e] = pack2<T>(p0, p1);
+        }
+        tmem_st_32x32b_x16(t_s + c * 16, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (ok && j1 > j0) ok = warp_wait(o_full, 0, abort_flag, err);
+    if (ok) {
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* dst = o + ((int64_t)(real ? row : 0) * P.Hq + h) * P.D;
+      float bad = 0.f;
+#pragma unroll 1
+      for (int c = 0; c * 16 < P.D; ++c) {
+        uint32_t w[16];
+        if (j1 > j0) {
+          tmem_ld_32x32b_x16(t_o + c * 16, w);
+          tmem_ld_wait_regs16(w);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = 0;
+        }
+        const bool both = real && c * 16 + 16 <= P.D;
+        const float b = store16<T>(dst + c * 16, w, inv, real, both);
+        bad += b;
+      }
+      if (real) lse[(int64_t)h * P.lse_stride + row] = l == 0.f ? INFINITY : m + log2f(l);
+      // rows that a masked neighbour's infinity or NaN may have reached
+      const bool partly = mine.x > from + j0 * kRows || mine.y < from + j1 * kRows;
+      uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad && l == l);
+      if (again != 0) {
+        __syncwarp();
+        float* scratch = reinterpret_cast<float*>(smem + L::kK) + warp * kRowScratch;  // every load has been consumed
+        while (again != 0) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int i = first + (warp % 4) * 32 + who;
+          const int2 b = P.q_bounds[i];
+          float acc[4], stat;
+          forward_row<T>((const T*)P.q + i * P.qs.row + h * P.qs.head, (const T*)P.k + hk * P.ks.head,
+                         (const T*)P.v + hk * P.vs.head, P.ks.row, P.vs.row, b.x, b.y, P.D, scale_log2, scratch, lane, acc,
+                         stat);
+          store_row<T>(o + ((int64_t)i * P.Hq + h) * P.D, acc, P.D, lane);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NT * 4 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+}
+
+// --------------------------------------------------------------------------------- backward: delta
+// delta_i = do_i . o_i. A CTA owns 128 rows of a head, 16 lanes a row. For fp16 also the largest norm of the
+// block's do rows: dS = p (dP - delta) is near |do| times a probability and would fall among fp16's subnormals, so
+// the backward kernels scale it by a power of two of that size.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restrict__ o, const T* __restrict__ dout,
+                                                              HeadRows ds, int Tq, int Hq, int D, int stride,
+                                                              float* __restrict__ delta, float* __restrict__ norms) {
+  __shared__ float top[16];
+  const int h = blockIdx.x % Hq, block = blockIdx.x / Hq;
+  const int lane = threadIdx.x % 16, slot = threadIdx.x / 16;
+  float most = 0.f;
+#pragma unroll 4
+  for (int u = 0; u < 8; ++u) {
+    const int i = block * kRows + u * 16 + slot;
+    float s = 0.f, n = 0.f;
+    if (i < Tq && lane * 8 < D) {
+      float a[8], b[8];
+      unpack8<T>(load_raw8<T>(o + ((int64_t)i * Hq + h) * D + lane * 8), a);
+      unpack8<T>(load_raw8<T>(dout + i * ds.row + h * ds.head + lane * 8), b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s = fmaf(a[e], b[e], s);
+        n = fmaf(b[e], b[e], n);
+      }
+    }
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, w);
+      n += __shfl_xor_sync(0xffffffffu, n, w);
+    }
+    if (lane == 0 && i < Tq) delta[(int64_t)h * stride + i] = s;
+    if (n <= 3e38f) most = fmaxf(most, n);
+  }
+  if constexpr (std::is_same_v<T, __half>) {
+    if (lane == 0) top[slot] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
+      norms[(int64_t)h * (stride / kRows) + block] = sqrtf(most);
+    }
+  }
+}
+
+// 2^-e for a largest norm of do near 2^e (fp16); dS is then at most 2^8 times the rows of v.
+__device__ __forceinline__ float ds_factor(float norm) {
+  if (!(norm > 0.f)) return 1.f;
+  return exp2f(-fminf(fmaxf(ceilf(log2f(norm)), -100.f), 100.f));
+}
+constexpr float kHalfShift = 8.f;  // fp16: P is kept times 2^8
+
+// ------------------------------------------------------------------------------------ backward: dQ
+// A CTA owns 128 queries of one head and goes through their keys. Eight warps: thread = query, half of a block's
+// keys each. S of the next block is computed before this block's softmax is done (two S buffers), dP as soon as the
+// last one has been read; dS goes back over S: keys 0 .. 63 of the block to the first 32 columns, the others to columns
+// 64 .. 95, which the same threads have read. Tensor memory: S twice, dP (128 columns each), dQ (DP).
+template <int DP>
+struct DqLayout {
+  static constexpr int kKStages = 3, kVStages = DP == 64 ? 3 : 2;
+  static constexpr int kQ = 0;
+  static constexpr int kDO = kQ + Tile<DP>::kBytes;
+  static constexpr int kK = kDO + Tile<DP>::kBytes;
+  static constexpr int kV = kK + kKStages * Tile<DP>::kBytes;
+  static constexpr int kBar = kV + kVStages * Tile<DP>::kBytes;
+  static constexpr int kBytes = kBar + 256 + 1024;
+};
+constexpr int kBwdThreads = 8 * 32 + 64;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                        const PackedProblem P, const T* __restrict__ dout, HeadRows dos, const float* __restrict__ lse,
+                        const float* __restrict__ delta, const float* __restrict__ norms, T* __restrict__ dq, int* err) {
+  using L = DqLayout<DP>;
+  constexpr int KS = L::kKStages, VS = L::kVStages;
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t *q_full = bar, *k_full = bar + 1, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
+  uint64_t *s_full = v_empty + VS, *dp_full = s_full + 2, *ds_full = dp_full + 1, *dq_full = ds_full + 1;
+  uint64_t* drain = dq_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int tiles = (P.Tq + kRows - 1) / kRows;
+  const int h = blockIdx.x % P.Hq;
+  const int r0 = (tiles - 1 - (int)(blockIdx.x / P.Hq)) * kRows;
+  const int hk = h / P.group;
+  const int from = P.q_bounds[r0].x, to = P.q_bounds[min(r0 + kRows, P.Tq) - 1].y;
+  const int blocks = to > from ? (to - from + kRows - 1) / kRows : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(dq_full, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+    prefetch_tensormap(&tmDO);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t c_dp = tmem + 256, c_dq = tmem + 384;
+
+  if (warp == 8) {
+    if (lane == 0 && blocks > 0) {
+      int nk = 0, nv = 0;
+      bool ok = true;
+      mbar_arrive_expect_tx(q_full, 2 * Tile<DP>::kBytes);
+      load_tile<DP>(smem + L::kQ, &tmQ, q_full, r0, h);
+      load_tile<DP>(smem + L::kDO, &tmDO, q_full, r0, h);
+      for (int j = 0; j < blocks; ++j) {
+        if (!mbar_wait(&k_empty[j % KS], ((j / KS) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[j % KS], Tile<DP>::kBytes);
+        load_tile<DP>(smem + L::kK + (j % KS) * Tile<DP>::kBytes, &tmK, &k_full[j % KS], from + j * kRows, hk);
+        ++nk;
+        if (!mbar_wait(&v_empty[j % VS], ((j / VS) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[j % VS], Tile<DP>::kBytes);
+        load_tile<DP>(smem + L::kV + (j % VS) * Tile<DP>::kBytes, &tmV, &v_full[j % VS], from + j * kRows, hk);
+        ++nv;
+      }
+      if (!ok) {
+        mbar_wait(q_full, 0, nullptr, nullptr, 0);
+        for (int j = nk - 1; j >= 0 && j >= nk - KS; --j) mbar_wait(&k_full[j % KS], (j / KS) & 1, nullptr, nullptr, 0);
+        for (int j = nv - 1; j >= 0 && j >= nv - VS; --j) mbar_wait(&v_full[j % VS], (j / VS) & 1, nullptr, nullptr, 0);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && blocks > 0) {
+      const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_g = idesc_of<T>((P.D + 15) / 16 * 16, true);
+      const uint32_t q_addr = smem_u32(smem + L::kQ), do_addr = smem_u32(smem + L::kDO);
+      const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+      auto scores = [&](int j) -> bool {
+        if (!mbar_wait(&k_full[j % KS], (j / KS) & 1, abort_flag, err, kErrPackedWait)) return false;
+        tc_fence_after();
+        mma_scores(tmem + (j & 1) * kRows, q_addr, k_addr + (j % KS) * Tile<DP>::kBytes, idesc_s, P.D);
+        tc_commit(&s_full[j & 1]);
+        return true;
+      };
+      auto d_probs = [&](int j) -> bool {
+        if (!mbar_wait(&v_full[j % VS], (j / VS) & 1, abort_flag, err, kErrPackedWait)) return false;
+        tc_fence_after();
+        mma_scores(c_dp, do_addr, v_addr + (j % VS) * Tile<DP>::kBytes, idesc_s, P.D);
+        tc_commit(&v_empty[j % VS]);
+        tc_commit(dp_full);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrPackedWait) && scores(0) && d_probs(0) &&
+                (blocks < 2 || scores(1));
+      for (int j = 0; j < blocks && ok; ++j) {
+        if (!mbar_wait(ds_full, j & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        tc_fence_after();
+        if (j + 1 < blocks && !d_probs(j + 1)) { ok = false; break; }
+        mma_sums(c_dq, tmem + (j & 1) * kRows, 64, k_addr + (j % KS) * Tile<DP>::kBytes, idesc_g, j > 0);
+        tc_commit(&k_empty[j % KS]);
+        if (j + 2 < blocks && !scores(j + 2)) { ok = false; break; }
+      }
+      if (ok) {
+        tc_commit(dq_full);
+      } else {
+        tc_commit(drain);
+        mbar_wait(drain, 0, nullptr, nullptr, 0);
+      }
+    }
+  } else {
+    const int half = warp / 4, r = (warp % 4) * 32 + lane, row = r0 + r;
+    const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const bool real = row < P.Tq;
+    const int2 mine = real ? P.q_bounds[row] : make_int2(0, 0);
+    const int all_lo = P.q_bounds[min(r0 + kRows, P.Tq) - 1].x, all_hi = P.q_bounds[r0].y;
+    const int64_t stat = (int64_t)h * P.lse_stride + (real ? row : r0);
+    const float lse_row = lse[stat], delta_row = delta[stat];
+    const float shift = kHalf ? lse_row - kHalfShift : lse_row;
+    const float factor = kHalf ? ds_factor(norms[(int64_t)h * (P.lse_stride / kRows) + r0 / kRows]) : 1.f;
+    const float scale_log2 = P.scale * kLog2e;
+    bool ok = true;
+    for (int j = 0; j < blocks; ++j) {
+      if (!warp_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, err)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t c_s = tmem + (j & 1) * kRows + half * 64 + lane_off;
+      const int kb = from + j * kRows;
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(c_s, v[0]);
+      tmem_ld_32x32b_x32(c_s + 32, v[1]);
+      tmem_ld_wait_regs(v[0]);
+      tmem_ld_wait_regs(v[1]);
+      const bool masked = kb < all_lo || kb + kRows > all_hi;
+      const int a = mine.x - kb - half * 64;
+      const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
+      float p[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) p[c][e] = exp2_approx(fmaf(__uint_as_float(v[c][e]), scale_log2, -shift));
+      if (!warp_wait(dp_full, j & 1, abort_flag, err)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(c_dp + half * 64 + c * 32 + lane_off, v[c]);
+      tmem_ld_wait_regs(v[0]);
+      tmem_ld_wait_regs(v[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float d = p[c][e] * (__uint_as_float(v[c][e]) - delta_row);
+          if constexpr (kHalf) d *= factor;
+          p[c][e] = d;
+        }
+        if (masked)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
+        tmem_st_32x32b_x16(c_s + c * 16, pk);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && blocks > 0) ok = warp_wait(dq_full, 0, abort_flag, err);
+    if (ok) {
+      tc_fence_after();
+      // fp16: the sums hold 2^8 factor dS
+      const float f = kHalf ? P.scale / (factor * 256.f) : P.scale;
+      T* dst = dq + ((int64_t)(real ? row : 0) * P.Hq + h) * P.D;
+      float bad = 0.f;
+#pragma unroll 1
+      for (int c = half; c * 16 < P.D; c += 2) {
+        uint32_t w[16];
+        if (blocks > 0) {
+          tmem_ld_32x32b_x16(c_dq + lane_off + c * 16, w);
+          tmem_ld_wait_regs16(w);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = 0;
+        }
+        bad += store16<T>(dst + c * 16, w, f, real, real && c * 16 + 16 <= P.D);
+      }
+      const bool partly = kHalf || mine.x > from || mine.y < from + blocks * kRows;
+      const float own = lse_row == INFINITY ? 0.f : fmaf(lse_row, 0.f, delta_row * 0.f);
+      uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad && own == own);
+      if (again != 0) {
+        __syncwarp();
+        float* scratch = reinterpret_cast<float*>(smem + L::kK) + warp * kRowScratch;
+        while (again != 0) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int i = r0 + (warp % 4) * 32 + who;
+          const int2 b = P.q_bounds[i];
+          const int64_t at = (int64_t)h * P.lse_stride + i;
+          float acc[4];
+          dq_row<T>((const T*)P.q + i * P.qs.row + h * P.qs.head, dout + i * dos.row + h * dos.head,
+                    (const T*)P.k + hk * P.ks.head, (const T*)P.v + hk * P.vs.head, P.ks.row, P.vs.row, b.x, b.y, P.D,
+                    P.scale, lse[at], delta[at], scratch, lane, acc);
+          // this warp's columns only: the other half's warp looks after its own
+          T* out = dq + ((int64_t)i * P.Hq + h) * P.D;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int c = lane + 32 * u;
+            if (c < P.D && ((c >> 4) & 1) == half) out[c] = from_f32<T>(acc[u]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ----------------------------------------------------------------------------- backward: dK and dV
+// A CTA owns 128 keys of one key head and goes through the queries that see them, for every query head of the
+// group. Eight warps: thread = key, half of a block's queries each. S^T = K Q^T -> P^T over S^T -> dV += P^T dO, then
+// dP^T = V dO^T -> dS^T over dP^T -> dK += dS^T Q; S^T of the next block is computed while dS^T of this one is formed
+// and the next dP^T while the next P^T is. Query blocks begin at multiples of 128, so that their statistics can be
+// copied with the tiles. Tensor memory: S^T, dP^T (128 columns each), dV, dK (DP each).
+template <int DP>
+struct DkvLayout {
+  static constexpr int kK = 0;
+  static constexpr int kV = kK + Tile<DP>::kBytes;
+  static constexpr int kQ = kV + Tile<DP>::kBytes;
+  static constexpr int kDO = kQ + 2 * Tile<DP>::kBytes;
+  static constexpr int kStat = kDO + 2 * Tile<DP>::kBytes;  // [2] lse, delta of 128 queries
+  static constexpr int kBar = kStat + 2 * 1024;
+  static constexpr int kBytes = kBar + 256 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                         const PackedProblem P, const T* __restrict__ dout, HeadRows dos, const float* __restrict__ lse,
+                         const float* __restrict__ delta, const float* __restrict__ norms, T* __restrict__ dk,
+                         T* __restrict__ dv, int* err) {
+  using L = DkvLayout<DP>;
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t *kv_full = bar, *q_full = bar + 1, *q_empty = q_full + 2, *s_full = q_empty + 2, *dp_full = s_full + 1;
+  uint64_t *p_full = dp_full + 1, *ds_full = p_full + 1, *g_full = ds_full + 1, *drain = g_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = blockIdx.x % P.Hk;
+  const int k0 = (int)(blockIdx.x / P.Hk) * kRows;  // causal keys are seen by the more queries the earlier they are
+  const int q_lo = P.k_bounds[k0].x, q_hi = P.k_bounds[min(k0 + kRows, P.Tk) - 1].y;
+  const int qb0 = q_lo / kRows, per_head = q_hi > q_lo ? (q_hi + kRows - 1) / kRows - qb0 : 0;
+  const int steps = per_head * P.group;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_full, 256);
+    mbar_init(ds_full, 256);
+    mbar_init(g_full, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+    prefetch_tensormap(&tmDO);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t c_s = tmem, c_dp = tmem + 128, c_dv = tmem + 256, c_dk = tmem + 256 + DP;
+
+  if (warp == 8) {
+    if (lane == 0 && steps > 0) {
+      int done = 0;
+      bool ok = true;
+      mbar_arrive_expect_tx(kv_full, 2 * Tile<DP>::kBytes);
+      load_tile<DP>(smem + L::kK, &tmK, kv_full, k0, g);
+      load_tile<DP>(smem + L::kV, &tmV, kv_full, k0, g);
+      for (int i = 0; i < steps; ++i) {
+        const int s = i & 1, h = g * P.group + i / per_head, q0 = (qb0 + i % per_head) * kRows;
+        if (!mbar_wait(&q_empty[s], ((i >> 1) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        mbar_arrive_expect_tx(&q_full[s], 2 * Tile<DP>::kBytes + 1024);
+        load_tile<DP>(smem + L::kQ + s * Tile<DP>::kBytes, &tmQ, &q_full[s], q0, h);
+        load_tile<DP>(smem + L::kDO + s * Tile<DP>::kBytes, &tmDO, &q_full[s], q0, h);
+        const int64_t at = (int64_t)h * P.lse_stride + q0;
+        bulk_load(smem + L::kStat + s * 1024, lse + at, 512, &q_full[s]);
+        bulk_load(smem + L::kStat + s * 1024 + 512, delta + at, 512, &q_full[s]);
+        ++done;
+      }
+      if (!ok) {
+        mbar_wait(kv_full, 0, nullptr, nullptr, 0);
+        for (int i = done - 1; i >= 0 && i >= done - 2; --i) mbar_wait(&q_full[i & 1], (i >> 1) & 1, nullptr, nullptr, 0);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && steps > 0) {
+      const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_g = idesc_of<T>((P.D + 15) / 16 * 16, true);
+      const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+      const uint32_t q_addr = smem_u32(smem + L::kQ), do_addr = smem_u32(smem + L::kDO);
+      auto scores = [&](int i) -> bool {
+        if (!mbar_wait(&q_full[i & 1], (i >> 1) & 1, abort_flag, err, kErrPackedWait)) return false;
+        tc_fence_after();
+        mma_scores(c_s, k_addr, q_addr + (i & 1) * Tile<DP>::kBytes, idesc_s, P.D);
+        tc_commit(s_full);
+        return true;
+      };
+      auto d_probs = [&](int i) {
+        mma_scores(c_dp, v_addr, do_addr + (i & 1) * Tile<DP>::kBytes, idesc_s, P.D);
+        tc_commit(dp_full);
+      };
+      bool ok = mbar_wait(kv_full, 0, abort_flag, err, kErrPackedWait) && scores(0);
+      if (ok) d_probs(0);
+      for (int i = 0; i < steps && ok; ++i) {
+        if (!mbar_wait(p_full, i & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        tc_fence_after();
+        mma_sums(c_dv, c_s, 64, do_addr + (i & 1) * Tile<DP>::kBytes, idesc_g, i > 0);
+        if (i + 1 < steps && !scores(i + 1)) { ok = false; break; }
+        if (!mbar_wait(ds_full, i & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        tc_fence_after();
+        mma_sums(c_dk, c_dp, 64, q_addr + (i & 1) * Tile<DP>::kBytes, idesc_g, i > 0);
+        tc_commit(&q_empty[i & 1]);
+        if (i + 1 < steps) d_probs(i + 1);
+      }
+      if (ok) {
+        tc_commit(g_full);
+      } else {
+        tc_commit(drain);
+        mbar_wait(drain, 0, nullptr, nullptr, 0);
+      }
+    }
+  } else {
+    const int half = warp / 4, r = (warp % 4) * 32 + lane, key = k0 + r;
+    const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const bool real = key < P.Tk;
+    const int2 mine = real ? P.k_bounds[key] : make_int2(0, 0);
+    const int all_lo = P.k_bounds[min(k0 + kRows, P.Tk) - 1].x, all_hi = P.k_bounds[k0].y;
+    const float scale_log2 = P.scale * kLog2e;
+    float factor = 1.f;
+    if constexpr (kHalf) {
+      float top = 0.f;
+      for (int i = 0; i < steps; ++i)
+        top = fmaxf(top, norms[(int64_t)(g * P.group + i / per_head) * (P.lse_stride / kRows) + qb0 + i % per_head]);
+      factor = ds_factor(top);
+    }
+    bool ok = true;
+    for (int i = 0; i < steps; ++i) {
+      const int q0 = (qb0 + i % per_head) * kRows;
+      if (!warp_wait(&q_full[i & 1], (i >> 1) & 1, abort_flag, err)) { ok = false; break; }
+      if (!warp_wait(s_full, i & 1, abort_flag, err)) { ok = false; break; }
+      tc_fence_after();
+      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i & 1) * 1024) + half * 16;
+      const float4* s_delta = s_lse + 32;
+      const bool masked = q0 < all_lo || q0 + kRows > all_hi;
+      const int a = mine.x - q0 - half * 64;
+      const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(c_s + half * 64 + lane_off, v[0]);
+      tmem_ld_32x32b_x32(c_s + half * 64 + 32 + lane_off, v[1]);
+      tmem_ld_wait_regs(v[0]);
+      tmem_ld_wait_regs(v[1]);
+      float p[2][32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 ls = s_lse[c * 8 + e];
+          const float sub[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            p[c][4 * e + u] = exp2_approx(fmaf(__uint_as_float(v[c][4 * e + u]), scale_log2,
+                                               kHalf ? kHalfShift - sub[u] : -sub[u]));
+        }
+        if (masked)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
+        tmem_st_32x32b_x16(c_s + half * 64 + c * 16 + lane_off, pk);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full);
+      if (!warp_wait(dp_full, i & 1, abort_flag, err)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(c_dp + half * 64 + c * 32 + lane_off, v[c]);
+      tmem_ld_wait_regs(v[0]);
+      tmem_ld_wait_regs(v[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 dl = s_delta[c * 8 + e];
+          const float sub[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float d = p[c][4 * e + u] * (__uint_as_float(v[c][4 * e + u]) - sub[u]);
+            if constexpr (kHalf) d *= factor;
+            p[c][4 * e + u] = d;
+          }
+        }
+        if (masked)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
+        tmem_st_32x32b_x16(c_dp + half * 64 + c * 16 + lane_off, pk);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && steps > 0) ok = warp_wait(g_full, 0, abort_flag, err);
+    if (ok) {
+      tc_fence_after();
+      const float fk = kHalf ? P.scale / (factor * 256.f) : P.scale, fv = kHalf ? 1.f / 256.f : 1.f;
+      const int64_t at = ((int64_t)(real ? key : 0) * P.Hk + g) * P.D;
+      float bad = 0.f;
+#pragma unroll 1
+      for (int c = half; c * 16 < P.D; c += 2) {
+        uint32_t w[16], u[16];
+        if (steps > 0) {
+          tmem_ld_32x32b_x16(c_dk + lane_off + c * 16, w);
+          tmem_ld_32x32b_x16(c_dv + lane_off + c * 16, u);
+          tmem_ld_wait_regs16(w);
+          tmem_ld_wait_regs16(u);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = u[e] = 0;
+        }
+        const bool both = real && c * 16 + 16 <= P.D;
+        bad += store16<T>(dk + at + c * 16, w, fk, real, both);
+        bad += store16<T>(dv + at + c * 16, u, fv, real, both);
+      }
+      const bool partly = kHalf || mine.x > qb0 * kRows || mine.y < (qb0 + per_head) * kRows;
+      uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad);
+      if (again != 0) {
+        __syncwarp();
+        float* scratch = reinterpret_cast<float*>(smem + L::kQ) + warp * kRowScratch;
+        while (again != 0) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int j = k0 + (warp % 4) * 32 + who;
+          const int2 b = P.k_bounds[j];
+          // a NaN among the statistics of its own queries makes the row NaN: nothing to mend
+          float own = 0.f;
+          for (int h = g * P.group; h < (g + 1) * P.group; ++h)
+            for (int i = b.x + lane; i < b.y; i += 32) {
+              const float s = lse[(int64_t)h * P.lse_stride + i];
+              if (s != s) own = s;
+            }
+          if (__any_sync(0xffffffffu, own != own)) continue;
+          float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int h = g * P.group; h < (g + 1) * P.group; ++h)
+            dkv_row<T>((const T*)P.k + j * P.ks.row + g * P.ks.head, (const T*)P.v + j * P.vs.row + g * P.vs.head,
+                       (const T*)P.q + h * P.qs.head, dout + h * dos.head, P.qs.row, dos.row, b.x, b.y, P.D, P.scale,
+                       lse + (int64_t)h * P.lse_stride, delta + (int64_t)h * P.lse_stride, scratch, lane, x, y);
+          const int64_t out = ((int64_t)j * P.Hk + g) * P.D;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int c = lane + 32 * u;
+            if (c < P.D && ((c >> 4) & 1) == half) {
+              dk[out + c] = from_f32<T>(x[u]);
+              dv[out + c] = from_f32<T>(y[u]);
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// --------------------------------------------------------------------------------------------- host
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t status = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found);
+    return status == cudaSuccess && found == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr)
+               : nullptr;
+  }();
+  return fn;
+}
+
+// Encoding a map needs a current context, which a thread (autograd's, say) has from its first call of the runtime on.
+cudaError_t context_current() {
+  int device = 0;
+  const cudaError_t status = cudaGetDevice(&device);
+  return status == cudaSuccess ? cudaSetDevice(device) : status;
+}
+
+// (D, rows, H) with boxes of 64 channels of 128 rows; rows past the last sequence and channels past the head read 0.
+bool map_rows(CUtensorMap* map, const void* base, HeadRows s, int rows, int H, int D, SequenceType type) {
+  if (encode_tiled() == nullptr) return false;
+  // a single row or head may come with any stride
+  const int64_t row = rows > 1 ? s.row : 8, head = H > 1 ? s.head : 8;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)H};
+  cuuint64_t strides[2] = {(cuuint64_t)(row * 2), (cuuint64_t)(head * 2)};
+  cuuint32_t box[3] = {64, kRows, 1}, step[3] = {1, 1, 1};
+  return encode_tiled()(map, type == kSeqBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K, typename... A>
+cudaError_t launch(K kernel, int64_t grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (status != cudaSuccess) return status;
+  kernel<<<(unsigned)grid, threads, smem, stream>>>(args...);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP>
+cudaError_t fwd(const PackedProblem& P, void* o, float* lse, int* err, cudaStream_t stream) {
+  CUtensorMap q, k, v;
+  const cudaError_t ready = context_current();
+  if (ready != cudaSuccess) return ready;
+  const int keys = P.Tk > 0 ? P.Tk : 1;  // without a key nothing is read
+  if (!map_rows(&q, P.q, P.qs, P.Tq, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, keys, P.Hk, P.D, P.type) ||
+      !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type))
+    return cudaErrorInvalidValue;
+  const int64_t pairs = (int64_t)((P.Tq + 2 * kRows - 1) / (2 * kRows)) * P.Hq;
+  // Two tiles a CTA share the loads of K and V; where that would leave SMs without work, one.
+  if (pairs >= 148)
+    return launch(packed_fwd_tc_kernel<T, DP, 2>, pairs, FwdLayout<DP, 2>::kThreads, FwdLayout<DP, 2>::kBytes, stream, q,
+                  k, v, P, (T*)o, lse, err);
+  return launch(packed_fwd_tc_kernel<T, DP, 1>, (int64_t)((P.Tq + kRows - 1) / kRows) * P.Hq, FwdLayout<DP, 1>::kThreads,
+                FwdLayout<DP, 1>::kBytes, stream, q, k, v, P, (T*)o, lse, err);
+}
+
+template <typename T, int DP>
+cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse, float* delta,
+                float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+  CUtensorMap q, k, v, g;
+  const cudaError_t ready = context_current();
+  if (ready != cudaSuccess) return ready;
+  const int keys = P.Tk > 0 ? P.Tk : 1, queries = P.Tq > 0 ? P.Tq : 1;
+  if (!map_rows(&q, P.q, P.qs, queries, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, keys, P.Hk, P.D, P.type) ||
+      !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type) || !map_rows(&g, dout, ds, queries, P.Hq, P.D, P.type))
+    return cudaErrorInvalidValue;
+  const int64_t q_tiles = (P.Tq + kRows - 1) / kRows, k_tiles = (P.Tk + kRows - 1) / kRows;
+  if (q_tiles > 0) {
+    packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>((const T*)o, (const T*)dout, ds, P.Tq, P.Hq,
+                                                                             P.D, P.lse_stride, delta, norms);
+    cudaError_t status = cudaGetLastError();
+    if (status != cudaSuccess) return status;
+    status = launch(packed_dq_tc_kernel<T, DP>, q_tiles * P.Hq, kBwdThreads, DqLayout<DP>::kBytes, stream, q, k, v, g, P,
+                    (const T*)dout, ds, lse, (const float*)delta, (const float*)norms, (T*)dq, err);
+    if (status != cudaSuccess) return status;
+  }
+  if (k_tiles == 0) return cudaSuccess;
+  return launch(packed_dkv_tc_kernel<T, DP>, k_tiles * P.Hk, kBwdThreads, DkvLayout<DP>::kBytes, stream, q, k, v, g, P,
+                (const T*)dout, ds, lse, (const float*)delta, (const float*)norms, (T*)dk, (T*)dv, err);
+}
+
+}  // namespace
+
+// A positive scale (the running maximum is taken before it), 16-bit values and up to 128 channels.
+bool packed_tc_ok(const PackedProblem& P) {
+  return (P.type == kSeqBf16 || P.type == kSeqF16) && P.scale > 0.f && P.D <= 128;
+}
+
+cudaError_t packed_fwd_tc(const PackedProblem& P, void* o, float* lse, int* err, cudaStream_t stream) {
+  if (P.type == kSeqBf16)
+    return P.D <= 64 ? fwd<__nv_bfloat16, 64>(P, o, lse, err, stream) : fwd<__nv_bfloat16, 128>(P, o, lse, err, stream);
+  return P.D <= 64 ? fwd<__half, 64>(P, o, lse, err, stream) : fwd<__half, 128>(P, o, lse, err, stream);
+}
+
+cudaError_t packed_bwd_tc(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
+                          float* delta, float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+  if (P.type == kSeqBf16)
+    return P.D <= 64 ? bwd<__nv_bfloat16, 64>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream)
+                     : bwd<__nv_bfloat16, 128>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream);
+  return P.D <= 64 ? bwd<__half, 64>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream)
+                   : bwd<__half, 128>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream);
+}
+
+}  // namespace mia

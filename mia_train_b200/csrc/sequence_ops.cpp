@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 
 #include "block_ops.h"
+#include "errors.h"
 #include "sequence_kernels.h"
 
 namespace mia {
@@ -99,7 +100,9 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     keep_for(q_bounds, stream);
     const PackedProblem P = problem(qc, kc, vc, q_bounds, k_bounds, scale);
     if (used > 0)
-      C10_CUDA_CHECK(packed_fwd_rows(P, o.data_ptr(), lse.data_ptr<float>(), stream));
+      C10_CUDA_CHECK(packed_tc_ok(P) ? packed_fwd_tc(P, o.data_ptr(), lse.data_ptr<float>(),
+                                                     error_word(q.get_device()), stream)
+                                     : packed_fwd_rows(P, o.data_ptr(), lse.data_ptr<float>(), stream));
     ctx->save_for_backward({qc, kc, vc, q_bounds, k_bounds, o, lse});
     ctx->saved_data["scale"] = scale;
     return o;
@@ -117,8 +120,15 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     keep_for(s[4], stream);
     const PackedProblem P = problem(s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble());
     const float* lse = s[6].data_ptr<float>();
-    C10_CUDA_CHECK(packed_bwd_rows(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
-                                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stream));
+    if (packed_tc_ok(P)) {
+      at::Tensor norms = at::empty({P.type == kSeqF16 ? s[6].numel() / 128 : 0}, s[6].options());
+      C10_CUDA_CHECK(packed_bwd_tc(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
+                                   norms.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   error_word(dout.get_device()), stream));
+    } else {
+      C10_CUDA_CHECK(packed_bwd_rows(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
+                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stream));
+    }
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };

@@ -95,6 +95,7 @@ ERROR_CODES = {
     112: "8-bit GEMM MMA issuer wait",
     113: "8-bit GEMM epilogue wait",
     201: "attention barrier wait",
+    211: "packed attention barrier wait",
     301: "collective flag wait",
     401: "sharded-optimizer reduce-scatter barrier",
     402: "sharded-optimizer gradient-norm exchange",
