@@ -38,8 +38,27 @@ struct Tile {
   static constexpr int kBytes = kRows * DP * 2;  // DP / 64 column groups of 128 rows x 128 bytes, swizzled
 };
 
+// mbar_wait that looks at the clock and at the abort flag on every 64th failed try only: reading %globaltimer takes
+// longer than most of these waits.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  uint64_t start = 0;
+#pragma unroll 1
+  for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+    if (n % 64 != 0) continue;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer_ns();
+    if (start == 0) start = now;
+    if (now - start > MIA_WAIT_LIMIT_NS) {
+      record_error(err, kErrPackedWait);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  const bool ok = mbar_wait(bar, parity, abort_flag, err, kErrPackedWait);
+  const bool ok = bounded_wait(bar, parity, abort_flag, err);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -98,21 +117,43 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-// Scores: d = A B^T over the head's channels, both tiles K-major.
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int D) {
-  for (int kk = 0; kk * 16 < D; ++kk) {
-    const uint32_t off = (kk >> 2) * (kRows * 128) + (kk & 3) * 32;
-    tc_mma_f16(d, make_sdesc_sw<128>(a + off, 16, 1024), make_sdesc_sw<128>(b + off, 16, 1024), idesc, kk > 0);
+// A launch of 12 warps with 168 registers a thread shares them out anew: the eight warps that hold rows of scores take
+// 216, the four of the loading and issuing group keep 72 (8 * 216 + 4 * 72 = 12 * 168).
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+
+// The issuing warp runs its loop as a whole, with one elected lane behind every product: what the products take then
+// stays in uniform registers. Issued from a branch of one thread they took 62 cycles each whatever their width
+// (128 x 64 x 16: 32 at the full rate), measured on 512 in a row.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+template <typename V>
+__device__ __forceinline__ V uniform(V x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Descriptor of a tile read along its rows' channels, and of one read along its rows; `tile_step` moves either by a tile.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return make_sdesc_sw<128>(addr, 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) { return make_sdesc_sw<128>(addr, kRows * 128, 1024); }
+template <int DP>
+__device__ __forceinline__ uint32_t tile_step(int n) { return (uint32_t)(n * (Tile<DP>::kBytes / 16)); }
+
+// Scores: d = A B^T over the head's channels.
+template <int DP>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int D) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const uint32_t off = (kk >> 2) * (kRows * 128 / 16) + (kk & 3) * 2;
+    if (kk == 0 || kk * 16 < D) tc_mma_f16(d, a + off, b + off, idesc, kk > 0);
   }
 }
 
-// Sums: d (+)= A B with A (128 x 128) in tensor memory, its second 64 columns of K at a + `second`, B the rows of a tile.
-__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t second, uint32_t b, uint32_t idesc,
-                                         bool accumulate) {
+// Sums: d (+)= A B with A (128 x 128) in 64 columns of tensor memory, B the rows of a tile.
+__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    mma_ts(d, a + (kk >> 2) * second + (kk & 3) * 8, make_sdesc_sw<128>(b + kk * 2048, kRows * 128, 1024), idesc,
-           accumulate || kk > 0);
+  for (int kk = 0; kk < 8; ++kk) mma_ts(d, a + kk * 8, b + kk * 128, idesc, accumulate || kk > 0);
 }
 
 // 16 fp32 columns of this lane's row times `f`, as 16-bit values; returns NaN if any is not finite, else 0.
@@ -137,9 +178,10 @@ __device__ __forceinline__ float store16(T* dst, const uint32_t (&v)[16], float 
 // A CTA owns NT tiles of 128 queries of one head. Warps 4 t .. 4 t + 3 hold tile t's rows, one thread per row: S from
 // tensor memory, running maximum and sum, P back over S. The accumulator O is rescaled in place, and only when a
 // block's maximum exceeds the reference maximum by more than 2^8 (P <= 2^8 until then). The last two warps load
-// (TMA) and issue the products. With two tiles one's softmax runs beside the other's products.
+// (TMA) and issue the products. With two tiles one's softmax runs beside the other's products; heads of up to 64
+// channels leave room for P next to S, so that the next S is computed as soon as this one has been read.
 //
-// Tensor memory: S (128 columns) and O (DP) per tile.
+// Tensor memory: S (128 columns), O (DP) and, for DP = 64, P (64) per tile.
 template <int DP, int NT>
 struct FwdLayout {
   static constexpr int kStages = DP == 64 && NT == 2 ? 3 : 2;
@@ -148,12 +190,14 @@ struct FwdLayout {
   static constexpr int kV = kK + kStages * Tile<DP>::kBytes;
   static constexpr int kBar = kV + kStages * Tile<DP>::kBytes;
   static constexpr int kBytes = kBar + 256 + 1024;
-  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr int kThreads = NT == 2 ? 384 : 192;
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
+  static constexpr bool kApart = DP == 64;  // P next to S instead of over it
+  static constexpr uint32_t kO = NT * kRows, kP = NT * (kRows + DP);
 };
 
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
     packed_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const PackedProblem P, T* __restrict__ o,
                          float* __restrict__ lse, int* err) {
@@ -163,11 +207,11 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t *q_full = bar, *k_full = bar + 1, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
-  uint64_t *s_full = v_empty + S, *p_full = s_full + NT, *o_full = p_full + NT, *drain = o_full + 1;
+  uint64_t *s_full = v_empty + S, *s_read = s_full + NT, *p_full = s_read + NT, *o_full = p_full + NT, *drain = o_full + NT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
   const int tiles = (P.Tq + NT * kRows - 1) / (NT * kRows);
   const int h = blockIdx.x % P.Hq;
   const int r0 = (tiles - 1 - (int)(blockIdx.x / P.Hq)) * NT * kRows;  // causal rows see the more keys the later they are
@@ -200,9 +244,10 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
     }
     for (int t = 0; t < NT; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&s_read[t], kRows);
       mbar_init(&p_full[t], kRows);
+      mbar_init(&o_full[t], 1);
     }
-    mbar_init(o_full, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -219,8 +264,9 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == NT * 4) {
-    if (lane == 0 && blocks > 0) {
+  if (warp >= NT * 4) {
+    if constexpr (NT == 2) fewer_registers();
+    if (warp == NT * 4 && lane == 0 && blocks > 0) {
       // ---------------------------------------------------------------------------------- loads
       int done = 0;
       bool ok = true;
@@ -230,11 +276,11 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
       for (int j = 0; j < blocks; ++j) {
         const int s = j % S;
         const uint32_t free_parity = ((j / S) & 1) ^ 1;
-        if (!mbar_wait(&k_empty[s], free_parity, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (!bounded_wait(&k_empty[s], free_parity, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&k_full[s], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kK + s * Tile<DP>::kBytes, &tmK, &k_full[s], from + j * kRows, hk);
         done = 2 * j + 1;
-        if (!mbar_wait(&v_empty[s], free_parity, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (!bounded_wait(&v_empty[s], free_parity, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&v_full[s], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kV + s * Tile<DP>::kBytes, &tmV, &v_full[s], from + j * kRows, hk);
         done = 2 * j + 2;
@@ -246,55 +292,74 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
           if (2 * j + 2 <= done) mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
         }
       }
-    }
-  } else if (warp == NT * 4 + 1) {
-    if (lane == 0 && blocks > 0) {
+    } else if (warp == NT * 4 + 1) {
       // ------------------------------------------------------------------------------- products
+      const bool one = elect_one();
       const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_o = idesc_of<T>((P.D + 15) / 16 * 16, true);
-      const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
-      bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrPackedWait);
-      for (int j = 0; j <= blocks && ok; ++j) {
-        if (j < blocks && !mbar_wait(&k_full[j % S], (j / S) & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
-        if (j > 0 && !mbar_wait(&v_full[(j - 1) % S], ((j - 1) / S) & 1, abort_flag, err, kErrPackedWait)) {
-          ok = false;
-          break;
-        }
+      const uint64_t q_desc = desc_k(uniform(smem_u32(smem + L::kQ))), k_desc = desc_k(uniform(smem_u32(smem + L::kK)));
+      const uint64_t v_desc = desc_mn(uniform(smem_u32(smem + L::kV)));
+      const uint32_t base = uniform(tmem);
+      const int n = uniform(blocks);
+      int b0[NT], b1[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint32_t t_s = tmem + t * kRows, t_o = tmem + NT * kRows + t * DP;
-          if (ok && j > begin[t] && j <= end[t]) {
-            const int it = j - 1 - begin[t];
-            if (!mbar_wait(&p_full[t], it & 1, abort_flag, err, kErrPackedWait)) {
-              ok = false;
-            } else {
-              tc_fence_after();
-              mma_sums(t_o, t_s, 32, v_addr + ((j - 1) % S) * Tile<DP>::kBytes, idesc_o, it > 0);
-            }
-          }
-          if (ok && j >= begin[t] && j < end[t]) {
-            tc_fence_after();
-            mma_scores(t_s, q_addr + t * Tile<DP>::kBytes, k_addr + (j % S) * Tile<DP>::kBytes, idesc_s, P.D);
-            tc_commit(&s_full[t]);
-          }
-        }
-        if (!ok) break;
-        if (j < blocks) tc_commit(&k_empty[j % S]);
-        if (j > 0) tc_commit(&v_empty[(j - 1) % S]);
+      for (int t = 0; t < NT; ++t) {
+        b0[t] = uniform(begin[t]);
+        b1[t] = uniform(end[t]);
       }
-      if (ok) {
-        tc_commit(o_full);
-      } else {
+      auto scores = [&](int t, int j) -> bool {
+        if (j < b0[t] || j >= b1[t]) return true;
+        const int it = j - b0[t];
+        if (L::kApart && it > 0 && !warp_wait(&s_read[t], (it - 1) & 1, abort_flag, err)) return false;
+        tc_fence_after();
+        if (one) {
+          mma_scores<DP>(base + t * kRows, q_desc + tile_step<DP>(t), k_desc + tile_step<DP>(j % S), idesc_s, P.D);
+          tc_commit(&s_full[t]);
+        }
+        return true;
+      };
+      auto sums = [&](int t, int j) -> bool {
+        if (j < b0[t] || j >= b1[t]) return true;
+        const int it = j - b0[t];
+        if (!warp_wait(&p_full[t], it & 1, abort_flag, err)) return false;
+        tc_fence_after();
+        if (one) {
+          mma_sums(base + L::kO + t * DP, L::kApart ? base + L::kP + t * 64 : base + t * kRows,
+                   v_desc + tile_step<DP>(j % S), idesc_o, it > 0);
+          tc_commit(&o_full[t]);
+        }
+        return true;
+      };
+      bool ok = n == 0 || warp_wait(q_full, 0, abort_flag, err);
+      for (int j = 0; j <= n && n > 0 && ok; ++j) {
+        if (j < n) ok = warp_wait(&k_full[j % S], (j / S) & 1, abort_flag, err);
+        if (ok && j > 0) ok = warp_wait(&v_full[(j - 1) % S], ((j - 1) / S) & 1, abort_flag, err);
+        if constexpr (L::kApart) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) ok = ok && (j == n || scores(t, j));
+          if (ok && j < n && one) tc_commit(&k_empty[j % S]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) ok = ok && (j == 0 || sums(t, j - 1));
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) ok = ok && (j == 0 || sums(t, j - 1)) && (j == n || scores(t, j));
+          if (ok && j < n && one) tc_commit(&k_empty[j % S]);
+        }
+        if (ok && j > 0 && one) tc_commit(&v_empty[(j - 1) % S]);
+      }
+      if (!ok && one) {
         tc_commit(drain);
         mbar_wait(drain, 0, nullptr, nullptr, 0);
       }
     }
   } else {
+    if constexpr (NT == 2) more_registers();
     // ------------------------------------------------------------------------------------ softmax
     constexpr float kRescale = 8.f;
     const int t = warp / 4, first = r0 + t * kRows;
     const int r = (warp % 4) * 32 + lane, row = first + r;
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
-    const uint32_t t_s = tmem + t * kRows + lane_off, t_o = tmem + NT * kRows + t * DP + lane_off;
+    const uint32_t t_s = tmem + t * kRows + lane_off, t_o = tmem + L::kO + t * DP + lane_off;
+    const uint32_t t_p = L::kApart ? tmem + L::kP + t * 64 + lane_off : t_s;
     const float scale_log2 = P.scale * kLog2e;
     const int j0 = t == 0 ? begin[0] : begin[NT - 1], j1 = t == 0 ? end[0] : end[NT - 1];
     const bool real = row < P.Tq;
@@ -315,6 +380,10 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
       for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, v[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(v[c]);
+      if constexpr (L::kApart) {
+        tc_fence_before();
+        mbar_arrive(&s_read[t]);
+      }
       if (kb < all_lo || kb + kRows > all_hi) {
         const int a = mine.x - kb;
         const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
@@ -332,7 +401,8 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
       const float blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
       const bool move = blk > m + kRescale;  // of a first block with a key always
       if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
-        // s_full of this block follows every earlier product: O is at rest
+        if (!warp_wait(&o_full[t], (j - j0 - 1) & 1, abort_flag, err)) { ok = false; break; }
+        tc_fence_after();
         const float alpha = move && m != -INFINITY ? exp2_approx(m - blk) : 1.f;
 #pragma unroll 1
         for (int c = 0; c * 16 < P.D; ++c) {
@@ -349,23 +419,26 @@ __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
       const float ref = m == -INFINITY ? 0.f : m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p0 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e]), scale_log2, -ref));
           const float p1 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e + 1]), scale_log2, -ref));
           sum[c] += p0 + p1;
-          pk[e] = pack2<T>(p0, p1);
+          v[c / 2][(c & 1) * 16 + e] = pack2<T>(p0, p1);
         }
-        tmem_st_32x32b_x16(t_s + c * 16, pk);
+      if (L::kApart && j > j0) {  // the place of P is free once the last P V is done
+        if (!warp_wait(&o_full[t], (j - j0 - 1) & 1, abort_flag, err)) { ok = false; break; }
+        tc_fence_after();
       }
+      tmem_st_32x32b_x32(t_p, v[0]);
+      tmem_st_32x32b_x32(t_p + 32, v[1]);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[t]);
     }
-    if (ok && j1 > j0) ok = warp_wait(o_full, 0, abort_flag, err);
+    if (ok && j1 > j0) ok = warp_wait(&o_full[t], (j1 - j0 - 1) & 1, abort_flag, err);
     if (ok) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -466,10 +539,10 @@ __device__ __forceinline__ float ds_factor(float norm) {
 constexpr float kHalfShift = 8.f;  // fp16: P is kept times 2^8
 
 // ------------------------------------------------------------------------------------ backward: dQ
-// A CTA owns 128 queries of one head and goes through their keys. Eight warps: thread = query, half of a block's
-// keys each. S of the next block is computed before this block's softmax is done (two S buffers), dP as soon as the
-// last one has been read; dS goes back over S: keys 0 .. 63 of the block to the first 32 columns, the others to columns
-// 64 .. 95, which the same threads have read. Tensor memory: S twice, dP (128 columns each), dQ (DP).
+// A CTA owns 128 queries of one head and goes through their keys. Two groups of four warps (thread = query) take the
+// blocks in turns, each with 128 columns of tensor memory of its own: S -> P in registers, dP over S, dS over dP (64
+// columns of 16-bit pairs, each written after what it covers has been read) -> dQ += dS K. While one group computes
+// exponentials the other one multiplies.
 template <int DP>
 struct DqLayout {
   static constexpr int kKStages = 3, kVStages = DP == 64 ? 3 : 2;
@@ -480,7 +553,7 @@ struct DqLayout {
   static constexpr int kBar = kV + kVStages * Tile<DP>::kBytes;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
-constexpr int kBwdThreads = 8 * 32 + 64;
+constexpr int kBwdThreads = 384;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -495,12 +568,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t *q_full = bar, *k_full = bar + 1, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
-  uint64_t *s_full = v_empty + VS, *dp_full = s_full + 2, *ds_full = dp_full + 1, *dq_full = ds_full + 1;
-  uint64_t* drain = dq_full + 1;
+  uint64_t *s_full = v_empty + VS, *s_read = s_full + 2, *dp_full = s_read + 2, *ds_full = dp_full + 2;
+  uint64_t *dq_full = ds_full + 2, *drain = dq_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
   const int tiles = (P.Tq + kRows - 1) / kRows;
   const int h = blockIdx.x % P.Hq;
   const int r0 = (tiles - 1 - (int)(blockIdx.x / P.Hq)) * kRows;
@@ -518,10 +591,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_read[s], 128);
+      mbar_init(&dp_full[s], 1);
+      mbar_init(&ds_full[s], 128);
+    }
     mbar_init(dq_full, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -539,21 +614,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t c_dp = tmem + 256, c_dq = tmem + 384;
+  const uint32_t c_dq = tmem + 256;
 
-  if (warp == 8) {
-    if (lane == 0 && blocks > 0) {
+  if (warp >= 8) {
+    fewer_registers();
+    if (warp == 8 && lane == 0 && blocks > 0) {
       int nk = 0, nv = 0;
       bool ok = true;
       mbar_arrive_expect_tx(q_full, 2 * Tile<DP>::kBytes);
       load_tile<DP>(smem + L::kQ, &tmQ, q_full, r0, h);
       load_tile<DP>(smem + L::kDO, &tmDO, q_full, r0, h);
       for (int j = 0; j < blocks; ++j) {
-        if (!mbar_wait(&k_empty[j % KS], ((j / KS) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (!bounded_wait(&k_empty[j % KS], ((j / KS) & 1) ^ 1, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&k_full[j % KS], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kK + (j % KS) * Tile<DP>::kBytes, &tmK, &k_full[j % KS], from + j * kRows, hk);
         ++nk;
-        if (!mbar_wait(&v_empty[j % VS], ((j / VS) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (!bounded_wait(&v_empty[j % VS], ((j / VS) & 1) ^ 1, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&v_full[j % VS], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kV + (j % VS) * Tile<DP>::kBytes, &tmV, &v_full[j % VS], from + j * kRows, hk);
         ++nv;
@@ -563,47 +639,63 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         for (int j = nk - 1; j >= 0 && j >= nk - KS; --j) mbar_wait(&k_full[j % KS], (j / KS) & 1, nullptr, nullptr, 0);
         for (int j = nv - 1; j >= 0 && j >= nv - VS; --j) mbar_wait(&v_full[j % VS], (j / VS) & 1, nullptr, nullptr, 0);
       }
-    }
-  } else if (warp == 9) {
-    if (lane == 0 && blocks > 0) {
+    } else if (warp == 9) {
+      const bool one = elect_one();
       const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_g = idesc_of<T>((P.D + 15) / 16 * 16, true);
-      const uint32_t q_addr = smem_u32(smem + L::kQ), do_addr = smem_u32(smem + L::kDO);
-      const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+      const uint64_t q_desc = desc_k(uniform(smem_u32(smem + L::kQ))), do_desc = desc_k(uniform(smem_u32(smem + L::kDO)));
+      const uint64_t k_desc = desc_k(uniform(smem_u32(smem + L::kK))), v_desc = desc_k(uniform(smem_u32(smem + L::kV)));
+      const uint64_t k_rows = desc_mn(uniform(smem_u32(smem + L::kK)));
+      const uint32_t base = uniform(tmem);
+      const int n = uniform(blocks);
       auto scores = [&](int j) -> bool {
-        if (!mbar_wait(&k_full[j % KS], (j / KS) & 1, abort_flag, err, kErrPackedWait)) return false;
+        if (!warp_wait(&k_full[j % KS], (j / KS) & 1, abort_flag, err)) return false;
         tc_fence_after();
-        mma_scores(tmem + (j & 1) * kRows, q_addr, k_addr + (j % KS) * Tile<DP>::kBytes, idesc_s, P.D);
-        tc_commit(&s_full[j & 1]);
+        if (one) {
+          mma_scores<DP>(base + (j & 1) * kRows, q_desc, k_desc + tile_step<DP>(j % KS), idesc_s, P.D);
+          tc_commit(&s_full[j & 1]);
+        }
         return true;
       };
       auto d_probs = [&](int j) -> bool {
-        if (!mbar_wait(&v_full[j % VS], (j / VS) & 1, abort_flag, err, kErrPackedWait)) return false;
+        if (!warp_wait(&v_full[j % VS], (j / VS) & 1, abort_flag, err)) return false;
+        if (!warp_wait(&s_read[j & 1], (j >> 1) & 1, abort_flag, err)) return false;
         tc_fence_after();
-        mma_scores(c_dp, do_addr, v_addr + (j % VS) * Tile<DP>::kBytes, idesc_s, P.D);
-        tc_commit(&v_empty[j % VS]);
-        tc_commit(dp_full);
+        if (one) {
+          mma_scores<DP>(base + (j & 1) * kRows, do_desc, v_desc + tile_step<DP>(j % VS), idesc_s, P.D);
+          tc_commit(&v_empty[j % VS]);
+          tc_commit(&dp_full[j & 1]);
+        }
         return true;
       };
-      bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrPackedWait) && scores(0) && d_probs(0) &&
-                (blocks < 2 || scores(1));
-      for (int j = 0; j < blocks && ok; ++j) {
-        if (!mbar_wait(ds_full, j & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+      auto sums = [&](int j) -> bool {
+        if (!warp_wait(&ds_full[j & 1], (j >> 1) & 1, abort_flag, err)) return false;
         tc_fence_after();
-        if (j + 1 < blocks && !d_probs(j + 1)) { ok = false; break; }
-        mma_sums(c_dq, tmem + (j & 1) * kRows, 64, k_addr + (j % KS) * Tile<DP>::kBytes, idesc_g, j > 0);
-        tc_commit(&k_empty[j % KS]);
-        if (j + 2 < blocks && !scores(j + 2)) { ok = false; break; }
+        if (one) {
+          mma_sums(base + 256, base + (j & 1) * kRows, k_rows + tile_step<DP>(j % KS), idesc_g, j > 0);
+          tc_commit(&k_empty[j % KS]);
+        }
+        return true;
+      };
+      bool ok = n == 0 || (warp_wait(q_full, 0, abort_flag, err) && scores(0) && (n < 2 || scores(1)));
+      for (int j = 0; j < n && ok; ++j) {
+        ok = d_probs(j);
+        if (ok && j > 0) ok = sums(j - 1) && (j + 1 >= n || scores(j + 1));
       }
-      if (ok) {
-        tc_commit(dq_full);
-      } else {
-        tc_commit(drain);
-        mbar_wait(drain, 0, nullptr, nullptr, 0);
+      ok = ok && (n == 0 || sums(n - 1));
+      if (one) {
+        if (ok) {
+          tc_commit(dq_full);
+        } else {
+          tc_commit(drain);
+          mbar_wait(drain, 0, nullptr, nullptr, 0);
+        }
       }
     }
   } else {
-    const int half = warp / 4, r = (warp % 4) * 32 + lane, row = r0 + r;
+    more_registers();
+    const int group = warp / 4, r = (warp % 4) * 32 + lane, row = r0 + r;
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t c_s = tmem + group * kRows + lane_off;
     const bool real = row < P.Tq;
     const int2 mine = real ? P.q_bounds[row] : make_int2(0, 0);
     const int all_lo = P.q_bounds[min(r0 + kRows, P.Tq) - 1].x, all_hi = P.q_bounds[r0].y;
@@ -613,50 +705,51 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const float factor = kHalf ? ds_factor(norms[(int64_t)h * (P.lse_stride / kRows) + r0 / kRows]) : 1.f;
     const float scale_log2 = P.scale * kLog2e;
     bool ok = true;
-    for (int j = 0; j < blocks; ++j) {
-      if (!warp_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, err)) { ok = false; break; }
+    for (int j = group; j < blocks; j += 2) {
+      const uint32_t parity = (j >> 1) & 1;
+      if (!warp_wait(&s_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t c_s = tmem + (j & 1) * kRows + half * 64 + lane_off;
+      uint32_t p[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(c_s + c * 32, p[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(p[c]);
+      tc_fence_before();
+      mbar_arrive(&s_read[group]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          p[c][e] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(p[c][e]), scale_log2, -shift)));
       const int kb = from + j * kRows;
-      uint32_t v[2][32];
-      tmem_ld_32x32b_x32(c_s, v[0]);
-      tmem_ld_32x32b_x32(c_s + 32, v[1]);
-      tmem_ld_wait_regs(v[0]);
-      tmem_ld_wait_regs(v[1]);
       const bool masked = kb < all_lo || kb + kRows > all_hi;
-      const int a = mine.x - kb - half * 64;
+      const int a = mine.x - kb;
       const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
-      float p[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) p[c][e] = exp2_approx(fmaf(__uint_as_float(v[c][e]), scale_log2, -shift));
-      if (!warp_wait(dp_full, j & 1, abort_flag, err)) { ok = false; break; }
+      if (!warp_wait(&dp_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(c_dp + half * 64 + c * 32 + lane_off, v[c]);
-      tmem_ld_wait_regs(v[0]);
-      tmem_ld_wait_regs(v[1]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(c_s + c * 32, v);
+        tmem_ld_wait_regs(v);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          float d = p[c][e] * (__uint_as_float(v[c][e]) - delta_row);
+          float d = __uint_as_float(p[c][e]) * (__uint_as_float(v[e]) - delta_row);
           if constexpr (kHalf) d *= factor;
-          p[c][e] = d;
+          v[e] = __float_as_uint(d);
         }
         if (masked)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+            if ((uint32_t)(c * 32 + e - a) >= n) v[e] = 0;
+        uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
         tmem_st_32x32b_x16(c_s + c * 16, pk);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(&ds_full[group]);
     }
     if (ok && blocks > 0) ok = warp_wait(dq_full, 0, abort_flag, err);
     if (ok) {
@@ -666,7 +759,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       T* dst = dq + ((int64_t)(real ? row : 0) * P.Hq + h) * P.D;
       float bad = 0.f;
 #pragma unroll 1
-      for (int c = half; c * 16 < P.D; c += 2) {
+      for (int c = group; c * 16 < P.D; c += 2) {
         uint32_t w[16];
         if (blocks > 0) {
           tmem_ld_32x32b_x16(c_dq + lane_off + c * 16, w);
@@ -693,12 +786,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           dq_row<T>((const T*)P.q + i * P.qs.row + h * P.qs.head, dout + i * dos.row + h * dos.head,
                     (const T*)P.k + hk * P.ks.head, (const T*)P.v + hk * P.vs.head, P.ks.row, P.vs.row, b.x, b.y, P.D,
                     P.scale, lse[at], delta[at], scratch, lane, acc);
-          // this warp's columns only: the other half's warp looks after its own
+          // this warp's columns only: the other group's warp looks after its own
           T* out = dq + ((int64_t)i * P.Hq + h) * P.D;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int c = lane + 32 * u;
-            if (c < P.D && ((c >> 4) & 1) == half) out[c] = from_f32<T>(acc[u]);
+            if (c < P.D && ((c >> 4) & 1) == group) out[c] = from_f32<T>(acc[u]);
           }
         }
       }
@@ -714,18 +807,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 // ----------------------------------------------------------------------------- backward: dK and dV
 // A CTA owns 128 keys of one key head and goes through the queries that see them, for every query head of the
-// group. Eight warps: thread = key, half of a block's queries each. S^T = K Q^T -> P^T over S^T -> dV += P^T dO, then
-// dP^T = V dO^T -> dS^T over dP^T -> dK += dS^T Q; S^T of the next block is computed while dS^T of this one is formed
-// and the next dP^T while the next P^T is. Query blocks begin at multiples of 128, so that their statistics can be
-// copied with the tiles. Tensor memory: S^T, dP^T (128 columns each), dV, dK (DP each).
+// group. Two groups of four warps (thread = key) take the query blocks in turns: S^T = K Q^T -> P^T over S^T -> dV +=
+// P^T dO, then dP^T = V dO^T -> dS^T over dP^T -> dK += dS^T Q; one group's exponentials run beside the other's dS.
+// Query blocks begin at multiples of 128, so that their statistics can be copied with the tiles. Tensor memory: S^T
+// (128 columns; for DP = 64 one per group), dP^T (128), dV, dK (DP each).
 template <int DP>
 struct DkvLayout {
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kScores = DP == 64 ? 2 : 1;  // S^T buffers: that many blocks ahead
   static constexpr int kK = 0;
   static constexpr int kV = kK + Tile<DP>::kBytes;
   static constexpr int kQ = kV + Tile<DP>::kBytes;
-  static constexpr int kDO = kQ + 2 * Tile<DP>::kBytes;
-  static constexpr int kStat = kDO + 2 * Tile<DP>::kBytes;  // [2] lse, delta of 128 queries
-  static constexpr int kBar = kStat + 2 * 1024;
+  static constexpr int kDO = kQ + kStages * Tile<DP>::kBytes;
+  static constexpr int kStat = kDO + kStages * Tile<DP>::kBytes;  // lse, delta of 128 queries, per stage
+  static constexpr int kBar = kStat + kStages * 1024;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
 
@@ -737,16 +832,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                          const float* __restrict__ delta, const float* __restrict__ norms, T* __restrict__ dk,
                          T* __restrict__ dv, int* err) {
   using L = DkvLayout<DP>;
+  constexpr int S = L::kStages, B = L::kScores;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t *kv_full = bar, *q_full = bar + 1, *q_empty = q_full + 2, *s_full = q_empty + 2, *dp_full = s_full + 1;
-  uint64_t *p_full = dp_full + 1, *ds_full = p_full + 1, *g_full = ds_full + 1, *drain = g_full + 1;
+  uint64_t *kv_full = bar, *q_full = bar + 1, *q_empty = q_full + S, *s_full = q_empty + S, *dp_full = s_full + 2;
+  uint64_t *p_full = dp_full + 2, *ds_full = p_full + 2, *g_full = ds_full + 2, *drain = g_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
   const int g = blockIdx.x % P.Hk;
   const int k0 = (int)(blockIdx.x / P.Hk) * kRows;  // causal keys are seen by the more queries the earlier they are
   const int q_lo = P.k_bounds[k0].x, q_hi = P.k_bounds[min(k0 + kRows, P.Tk) - 1].y;
@@ -755,14 +851,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < S; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(dp_full, 1);
-    mbar_init(p_full, 256);
-    mbar_init(ds_full, 256);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&dp_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&ds_full[s], 128);
+    }
     mbar_init(g_full, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -780,18 +878,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t c_s = tmem, c_dp = tmem + 128, c_dv = tmem + 256, c_dk = tmem + 256 + DP;
+  const uint32_t c_dp = tmem + B * kRows, c_dv = c_dp + kRows, c_dk = c_dv + DP;
 
-  if (warp == 8) {
-    if (lane == 0 && steps > 0) {
+  if (warp >= 8) {
+    fewer_registers();
+    if (warp == 8 && lane == 0 && steps > 0) {
       int done = 0;
       bool ok = true;
       mbar_arrive_expect_tx(kv_full, 2 * Tile<DP>::kBytes);
       load_tile<DP>(smem + L::kK, &tmK, kv_full, k0, g);
       load_tile<DP>(smem + L::kV, &tmV, kv_full, k0, g);
       for (int i = 0; i < steps; ++i) {
-        const int s = i & 1, h = g * P.group + i / per_head, q0 = (qb0 + i % per_head) * kRows;
-        if (!mbar_wait(&q_empty[s], ((i >> 1) & 1) ^ 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        const int s = i % S, h = g * P.group + i / per_head, q0 = (qb0 + i % per_head) * kRows;
+        if (!bounded_wait(&q_empty[s], ((i / S) & 1) ^ 1, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&q_full[s], 2 * Tile<DP>::kBytes + 1024);
         load_tile<DP>(smem + L::kQ + s * Tile<DP>::kBytes, &tmQ, &q_full[s], q0, h);
         load_tile<DP>(smem + L::kDO + s * Tile<DP>::kBytes, &tmDO, &q_full[s], q0, h);
@@ -802,48 +901,62 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) {
         mbar_wait(kv_full, 0, nullptr, nullptr, 0);
-        for (int i = done - 1; i >= 0 && i >= done - 2; --i) mbar_wait(&q_full[i & 1], (i >> 1) & 1, nullptr, nullptr, 0);
+        for (int i = done - 1; i >= 0 && i >= done - S; --i) mbar_wait(&q_full[i % S], (i / S) & 1, nullptr, nullptr, 0);
       }
-    }
-  } else if (warp == 9) {
-    if (lane == 0 && steps > 0) {
+    } else if (warp == 9) {
+      const bool one = elect_one();
       const uint32_t idesc_s = idesc_of<T>(kRows, false), idesc_g = idesc_of<T>((P.D + 15) / 16 * 16, true);
-      const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
-      const uint32_t q_addr = smem_u32(smem + L::kQ), do_addr = smem_u32(smem + L::kDO);
+      const uint64_t k_desc = desc_k(uniform(smem_u32(smem + L::kK))), v_desc = desc_k(uniform(smem_u32(smem + L::kV)));
+      const uint64_t q_desc = desc_k(uniform(smem_u32(smem + L::kQ))), do_desc = desc_k(uniform(smem_u32(smem + L::kDO)));
+      const uint64_t q_rows = desc_mn(uniform(smem_u32(smem + L::kQ))), do_rows = desc_mn(uniform(smem_u32(smem + L::kDO)));
+      const uint32_t base = uniform(tmem), u_dp = base + B * kRows, u_dv = u_dp + kRows, u_dk = u_dv + DP;
+      const int n = uniform(steps);
       auto scores = [&](int i) -> bool {
-        if (!mbar_wait(&q_full[i & 1], (i >> 1) & 1, abort_flag, err, kErrPackedWait)) return false;
+        if (!warp_wait(&q_full[i % S], (i / S) & 1, abort_flag, err)) return false;
         tc_fence_after();
-        mma_scores(c_s, k_addr, q_addr + (i & 1) * Tile<DP>::kBytes, idesc_s, P.D);
-        tc_commit(s_full);
+        if (one) {
+          mma_scores<DP>(base + (i % B) * kRows, k_desc, q_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          tc_commit(&s_full[i & 1]);
+        }
         return true;
       };
-      auto d_probs = [&](int i) {
-        mma_scores(c_dp, v_addr, do_addr + (i & 1) * Tile<DP>::kBytes, idesc_s, P.D);
-        tc_commit(dp_full);
+      auto d_probs = [&](int i) {  // its tiles have been waited for by its scores
+        if (one) {
+          mma_scores<DP>(u_dp, v_desc, do_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          tc_commit(&dp_full[i & 1]);
+        }
       };
-      bool ok = mbar_wait(kv_full, 0, abort_flag, err, kErrPackedWait) && scores(0);
-      if (ok) d_probs(0);
-      for (int i = 0; i < steps && ok; ++i) {
-        if (!mbar_wait(p_full, i & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+      bool ok = n == 0 || (warp_wait(kv_full, 0, abort_flag, err) && scores(0));
+      if (ok && n > 0) d_probs(0);
+      if (ok && B > 1 && n > 1) ok = scores(1);
+      for (int i = 0; i < n && ok; ++i) {
+        ok = warp_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, err);
+        if (!ok) break;
         tc_fence_after();
-        mma_sums(c_dv, c_s, 64, do_addr + (i & 1) * Tile<DP>::kBytes, idesc_g, i > 0);
-        if (i + 1 < steps && !scores(i + 1)) { ok = false; break; }
-        if (!mbar_wait(ds_full, i & 1, abort_flag, err, kErrPackedWait)) { ok = false; break; }
+        if (one) mma_sums(u_dv, base + (i % B) * kRows, do_rows + tile_step<DP>(i % S), idesc_g, i > 0);
+        ok = (i + B >= n || scores(i + B)) && warp_wait(&ds_full[i & 1], (i >> 1) & 1, abort_flag, err);
+        if (!ok) break;
         tc_fence_after();
-        mma_sums(c_dk, c_dp, 64, q_addr + (i & 1) * Tile<DP>::kBytes, idesc_g, i > 0);
-        tc_commit(&q_empty[i & 1]);
-        if (i + 1 < steps) d_probs(i + 1);
+        if (one) {
+          mma_sums(u_dk, u_dp, q_rows + tile_step<DP>(i % S), idesc_g, i > 0);
+          tc_commit(&q_empty[i % S]);
+        }
+        if (i + 1 < n) d_probs(i + 1);
       }
-      if (ok) {
-        tc_commit(g_full);
-      } else {
-        tc_commit(drain);
-        mbar_wait(drain, 0, nullptr, nullptr, 0);
+      if (one) {
+        if (ok) {
+          tc_commit(g_full);
+        } else {
+          tc_commit(drain);
+          mbar_wait(drain, 0, nullptr, nullptr, 0);
+        }
       }
     }
   } else {
-    const int half = warp / 4, r = (warp % 4) * 32 + lane, key = k0 + r;
+    more_registers();
+    const int group = warp / 4, r = (warp % 4) * 32 + lane, key = k0 + r;
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t t_s = tmem + (group % B) * kRows + lane_off, t_dp = c_dp + lane_off;
     const bool real = key < P.Tk;
     const int2 mine = real ? P.k_bounds[key] : make_int2(0, 0);
     const int all_lo = P.k_bounds[min(k0 + kRows, P.Tk) - 1].x, all_hi = P.k_bounds[k0].y;
@@ -856,76 +969,75 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       factor = ds_factor(top);
     }
     bool ok = true;
-    for (int i = 0; i < steps; ++i) {
+    for (int i = group; i < steps; i += 2) {
+      const uint32_t parity = (i >> 1) & 1;
       const int q0 = (qb0 + i % per_head) * kRows;
-      if (!warp_wait(&q_full[i & 1], (i >> 1) & 1, abort_flag, err)) { ok = false; break; }
-      if (!warp_wait(s_full, i & 1, abort_flag, err)) { ok = false; break; }
+      if (!warp_wait(&q_full[i % S], (i / S) & 1, abort_flag, err)) { ok = false; break; }
+      if (!warp_wait(&s_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
-      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i & 1) * 1024) + half * 16;
+      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i % S) * 1024);
       const float4* s_delta = s_lse + 32;
       const bool masked = q0 < all_lo || q0 + kRows > all_hi;
-      const int a = mine.x - q0 - half * 64;
+      const int a = mine.x - q0;
       const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
-      uint32_t v[2][32];
-      tmem_ld_32x32b_x32(c_s + half * 64 + lane_off, v[0]);
-      tmem_ld_32x32b_x32(c_s + half * 64 + 32 + lane_off, v[1]);
-      tmem_ld_wait_regs(v[0]);
-      tmem_ld_wait_regs(v[1]);
-      float p[2][32];
+      uint32_t p[4][32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, p[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(p[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 ls = s_lse[c * 8 + e];
           const float sub[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            p[c][4 * e + u] = exp2_approx(fmaf(__uint_as_float(v[c][4 * e + u]), scale_log2,
-                                               kHalf ? kHalfShift - sub[u] : -sub[u]));
+            p[c][4 * e + u] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(p[c][4 * e + u]), scale_log2,
+                                                               kHalf ? kHalfShift - sub[u] : -sub[u])));
         }
         if (masked)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0;
         uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
-        tmem_st_32x32b_x16(c_s + half * 64 + c * 16 + lane_off, pk);
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
+        tmem_st_32x32b_x16(t_s + c * 16, pk);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(p_full);
-      if (!warp_wait(dp_full, i & 1, abort_flag, err)) { ok = false; break; }
+      mbar_arrive(&p_full[group]);
+      if (!warp_wait(&dp_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(c_dp + half * 64 + c * 32 + lane_off, v[c]);
-      tmem_ld_wait_regs(v[0]);
-      tmem_ld_wait_regs(v[1]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t_dp + c * 32, v);
+        tmem_ld_wait_regs(v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 dl = s_delta[c * 8 + e];
           const float sub[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            float d = p[c][4 * e + u] * (__uint_as_float(v[c][4 * e + u]) - sub[u]);
+            float d = __uint_as_float(p[c][4 * e + u]) * (__uint_as_float(v[4 * e + u]) - sub[u]);
             if constexpr (kHalf) d *= factor;
-            p[c][4 * e + u] = d;
+            v[4 * e + u] = __float_as_uint(d);
           }
         }
         if (masked)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0.f;
+            if ((uint32_t)(c * 32 + e - a) >= n) v[e] = 0;
         uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(p[c][2 * e], p[c][2 * e + 1]);
-        tmem_st_32x32b_x16(c_dp + half * 64 + c * 16 + lane_off, pk);
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+        tmem_st_32x32b_x16(t_dp + c * 16, pk);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(&ds_full[group]);
     }
     if (ok && steps > 0) ok = warp_wait(g_full, 0, abort_flag, err);
     if (ok) {
@@ -934,7 +1046,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int64_t at = ((int64_t)(real ? key : 0) * P.Hk + g) * P.D;
       float bad = 0.f;
 #pragma unroll 1
-      for (int c = half; c * 16 < P.D; c += 2) {
+      for (int c = group; c * 16 < P.D; c += 2) {
         uint32_t w[16], u[16];
         if (steps > 0) {
           tmem_ld_32x32b_x16(c_dk + lane_off + c * 16, w);
@@ -976,7 +1088,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int c = lane + 32 * u;
-            if (c < P.D && ((c >> 4) & 1) == half) {
+            if (c < P.D && ((c >> 4) & 1) == group) {
               dk[out + c] = from_f32<T>(x[u]);
               dv[out + c] = from_f32<T>(y[u]);
             }
