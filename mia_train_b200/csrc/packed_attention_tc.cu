@@ -333,19 +333,23 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
       for (int j = 0; j <= n && n > 0 && ok; ++j) {
         if (j < n) ok = warp_wait(&k_full[j % S], (j / S) & 1, abort_flag, err);
         if (ok && j > 0) ok = warp_wait(&v_full[(j - 1) % S], ((j - 1) / S) & 1, abort_flag, err);
-        if constexpr (L::kApart) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) ok = ok && (j == n || scores(t, j));
+        if constexpr (L::kApart && NT == 2) {
+          // the second tile's sums wait for the first tile's next scores: the tiles' softmax fall into turns
+          ok = ok && (j == n || scores(0, j)) && (j < 2 || sums(1, j - 2));
+          if (ok && j > 1 && one) tc_commit(&v_empty[(j - 2) % S]);
+          ok = ok && (j == n || scores(1, j)) && (j == 0 || sums(0, j - 1));
           if (ok && j < n && one) tc_commit(&k_empty[j % S]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) ok = ok && (j == 0 || sums(t, j - 1));
         } else {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) ok = ok && (j == 0 || sums(t, j - 1)) && (j == n || scores(t, j));
+          for (int t = 0; t < NT; ++t) {
+            if (L::kApart) ok = ok && (j == n || scores(t, j)) && (j == 0 || sums(t, j - 1));
+            else ok = ok && (j == 0 || sums(t, j - 1)) && (j == n || scores(t, j));
+          }
           if (ok && j < n && one) tc_commit(&k_empty[j % S]);
+          if (ok && j > 0 && one) tc_commit(&v_empty[(j - 1) % S]);
         }
-        if (ok && j > 0 && one) tc_commit(&v_empty[(j - 1) % S]);
       }
+      if constexpr (L::kApart && NT == 2) ok = ok && (n == 0 || sums(1, n - 1));
       if (!ok && one) {
         tc_commit(drain);
         mbar_wait(drain, 0, nullptr, nullptr, 0);
@@ -540,12 +544,12 @@ constexpr float kHalfShift = 8.f;  // fp16: P is kept times 2^8
 
 // ------------------------------------------------------------------------------------ backward: dQ
 // A CTA owns 128 queries of one head and goes through their keys. Two groups of four warps (thread = query) take the
-// blocks in turns, each with 128 columns of tensor memory of its own: S -> P in registers, dP over S, dS over dP (64
-// columns of 16-bit pairs, each written after what it covers has been read) -> dQ += dS K. While one group computes
-// exponentials the other one multiplies.
+// blocks in turns. A block has 128 of three times 128 columns of tensor memory: S -> P in registers, dP over S, dS over
+// dP (64 columns of 16-bit pairs, each written after what it covers has been read) -> dQ += dS K. While one group
+// computes exponentials the other one multiplies, and the third place takes the scores of the block after.
 template <int DP>
 struct DqLayout {
-  static constexpr int kKStages = 3, kVStages = DP == 64 ? 3 : 2;
+  static constexpr int kKStages = 4, kVStages = DP == 64 ? 3 : 1;
   static constexpr int kQ = 0;
   static constexpr int kDO = kQ + Tile<DP>::kBytes;
   static constexpr int kK = kDO + Tile<DP>::kBytes;
@@ -614,7 +618,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t c_dq = tmem + 256;
+  const uint32_t c_dq = tmem + 3 * kRows;
 
   if (warp >= 8) {
     fewer_registers();
@@ -651,7 +655,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!warp_wait(&k_full[j % KS], (j / KS) & 1, abort_flag, err)) return false;
         tc_fence_after();
         if (one) {
-          mma_scores<DP>(base + (j & 1) * kRows, q_desc, k_desc + tile_step<DP>(j % KS), idesc_s, P.D);
+          mma_scores<DP>(base + (j % 3) * kRows, q_desc, k_desc + tile_step<DP>(j % KS), idesc_s, P.D);
           tc_commit(&s_full[j & 1]);
         }
         return true;
@@ -661,7 +665,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!warp_wait(&s_read[j & 1], (j >> 1) & 1, abort_flag, err)) return false;
         tc_fence_after();
         if (one) {
-          mma_scores<DP>(base + (j & 1) * kRows, do_desc, v_desc + tile_step<DP>(j % VS), idesc_s, P.D);
+          mma_scores<DP>(base + (j % 3) * kRows, do_desc, v_desc + tile_step<DP>(j % VS), idesc_s, P.D);
           tc_commit(&v_empty[j % VS]);
           tc_commit(&dp_full[j & 1]);
         }
@@ -671,15 +675,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!warp_wait(&ds_full[j & 1], (j >> 1) & 1, abort_flag, err)) return false;
         tc_fence_after();
         if (one) {
-          mma_sums(base + 256, base + (j & 1) * kRows, k_rows + tile_step<DP>(j % KS), idesc_g, j > 0);
+          mma_sums(base + 3 * kRows, base + (j % 3) * kRows, k_rows + tile_step<DP>(j % KS), idesc_g, j > 0);
           tc_commit(&k_empty[j % KS]);
         }
         return true;
       };
       bool ok = n == 0 || (warp_wait(q_full, 0, abort_flag, err) && scores(0) && (n < 2 || scores(1)));
       for (int j = 0; j < n && ok; ++j) {
-        ok = d_probs(j);
-        if (ok && j > 0) ok = sums(j - 1) && (j + 1 >= n || scores(j + 1));
+        ok = d_probs(j) && (j == 0 || sums(j - 1)) && (j + 2 >= n || scores(j + 2));
       }
       ok = ok && (n == 0 || sums(n - 1));
       if (one) {
@@ -695,7 +698,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     more_registers();
     const int group = warp / 4, r = (warp % 4) * 32 + lane, row = r0 + r;
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
-    const uint32_t c_s = tmem + group * kRows + lane_off;
     const bool real = row < P.Tq;
     const int2 mine = real ? P.q_bounds[row] : make_int2(0, 0);
     const int all_lo = P.q_bounds[min(r0 + kRows, P.Tq) - 1].x, all_hi = P.q_bounds[r0].y;
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const float scale_log2 = P.scale * kLog2e;
     bool ok = true;
     for (int j = group; j < blocks; j += 2) {
-      const uint32_t parity = (j >> 1) & 1;
+      const uint32_t parity = (j >> 1) & 1, c_s = tmem + (j % 3) * kRows + lane_off;
       if (!warp_wait(&s_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
       uint32_t p[4][32];
@@ -727,24 +729,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
       if (!warp_wait(&dp_full[group], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
+      uint32_t v[2][32];  // the next 32 columns are on their way while these are worked on
+      tmem_ld_32x32b_x32(c_s, v[0]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(c_s + c * 32, v);
-        tmem_ld_wait_regs(v);
+        uint32_t(&x)[32] = v[c & 1];
+        tmem_ld_wait_regs(x);
+        if (c < 3) tmem_ld_32x32b_x32(c_s + (c + 1) * 32, v[(c + 1) & 1]);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          float d = __uint_as_float(p[c][e]) * (__uint_as_float(v[e]) - delta_row);
+          float d = __uint_as_float(p[c][e]) * (__uint_as_float(x[e]) - delta_row);
           if constexpr (kHalf) d *= factor;
-          v[e] = __float_as_uint(d);
+          p[c][e] = __float_as_uint(d);
         }
         if (masked)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((uint32_t)(c * 32 + e - a) >= n) v[e] = 0;
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0;
         uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
         tmem_st_32x32b_x16(c_s + c * 16, pk);
       }
       tmem_st_wait();
@@ -807,14 +811,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 // ----------------------------------------------------------------------------- backward: dK and dV
 // A CTA owns 128 keys of one key head and goes through the queries that see them, for every query head of the
-// group. Two groups of four warps (thread = key) take the query blocks in turns: S^T = K Q^T -> P^T over S^T -> dV +=
-// P^T dO, then dP^T = V dO^T -> dS^T over dP^T -> dK += dS^T Q; one group's exponentials run beside the other's dS.
-// Query blocks begin at multiples of 128, so that their statistics can be copied with the tiles. Tensor memory: S^T
-// (128 columns; for DP = 64 one per group), dP^T (128), dV, dK (DP each).
+// group: S^T = K Q^T -> P^T -> dV += P^T dO, dP^T = V dO^T over S^T as soon as that has been read -> dS^T -> dK += dS^T Q;
+// thread = key. Query blocks begin at multiples of 128, so that their statistics can be copied with the tiles.
+//
+// DP = 64: two groups of four warps take the blocks in turns, one's exponentials beside the other's dS. Tensor memory
+// per group: S^T, then dP^T, then dS^T (128 columns) and P^T (64); dV and dK (64 each).
+// DP = 128: dV and dK leave room for one S^T / dP^T (128), P^T and dS^T (64 each): all eight warps share a block, half
+// of its queries each, and the products are the bound (2048 cycles a block against 1024 of exponentials).
 template <int DP>
 struct DkvLayout {
-  static constexpr int kStages = DP == 64 ? 3 : 2;
-  static constexpr int kScores = DP == 64 ? 2 : 1;  // S^T buffers: that many blocks ahead
+  static constexpr bool kTurns = DP == 64;
+  static constexpr int kStages = kTurns ? 4 : 2;
+  static constexpr uint32_t kX = 0, kXStep = kTurns ? 192 : 0, kP = 128, kDS = kTurns ? 0 : 192;  // columns
+  static constexpr uint32_t kDV = kTurns ? 384 : 256, kDK = kDV + DP;
   static constexpr int kK = 0;
   static constexpr int kV = kK + Tile<DP>::kBytes;
   static constexpr int kQ = kV + Tile<DP>::kBytes;
@@ -832,13 +841,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                          const float* __restrict__ delta, const float* __restrict__ norms, T* __restrict__ dk,
                          T* __restrict__ dv, int* err) {
   using L = DkvLayout<DP>;
-  constexpr int S = L::kStages, B = L::kScores;
+  constexpr int S = L::kStages;
+  constexpr bool kTurns = L::kTurns;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t *kv_full = bar, *q_full = bar + 1, *q_empty = q_full + S, *s_full = q_empty + S, *dp_full = s_full + 2;
-  uint64_t *p_full = dp_full + 2, *ds_full = p_full + 2, *g_full = ds_full + 2, *drain = g_full + 1;
+  // two of each, in turns; without turns only the first is used
+  uint64_t *kv_full = bar, *q_full = bar + 1, *q_empty = q_full + S, *s_full = q_empty + S, *s_read = s_full + 2;
+  uint64_t *dp_full = s_read + 2, *dp_read = dp_full + 2, *p_full = dp_read + 2, *ds_full = p_full + 2;
+  uint64_t *g_full = ds_full + 2, *drain = g_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -856,10 +868,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&q_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
+      constexpr int kArrive = kTurns ? 128 : 256;
       mbar_init(&s_full[s], 1);
+      mbar_init(&s_read[s], kArrive);
       mbar_init(&dp_full[s], 1);
-      mbar_init(&p_full[s], 128);
-      mbar_init(&ds_full[s], 128);
+      mbar_init(&dp_read[s], kArrive);
+      mbar_init(&p_full[s], kArrive);
+      mbar_init(&ds_full[s], kArrive);
     }
     mbar_init(g_full, 1);
     mbar_init(drain, 1);
@@ -878,7 +893,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t c_dp = tmem + B * kRows, c_dv = c_dp + kRows, c_dk = c_dv + DP;
 
   if (warp >= 8) {
     fewer_registers();
@@ -909,39 +923,56 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint64_t k_desc = desc_k(uniform(smem_u32(smem + L::kK))), v_desc = desc_k(uniform(smem_u32(smem + L::kV)));
       const uint64_t q_desc = desc_k(uniform(smem_u32(smem + L::kQ))), do_desc = desc_k(uniform(smem_u32(smem + L::kDO)));
       const uint64_t q_rows = desc_mn(uniform(smem_u32(smem + L::kQ))), do_rows = desc_mn(uniform(smem_u32(smem + L::kDO)));
-      const uint32_t base = uniform(tmem), u_dp = base + B * kRows, u_dv = u_dp + kRows, u_dk = u_dv + DP;
+      const uint32_t base = uniform(tmem);
       const int n = uniform(steps);
+      auto turn = [&](int i) { return kTurns ? i & 1 : 0; };
+      auto phase = [&](int i) -> uint32_t { return kTurns ? (i >> 1) & 1 : i & 1; };
       auto scores = [&](int i) -> bool {
         if (!warp_wait(&q_full[i % S], (i / S) & 1, abort_flag, err)) return false;
         tc_fence_after();
         if (one) {
-          mma_scores<DP>(base + (i % B) * kRows, k_desc, q_desc + tile_step<DP>(i % S), idesc_s, P.D);
-          tc_commit(&s_full[i & 1]);
+          mma_scores<DP>(base + turn(i) * L::kXStep, k_desc, q_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          tc_commit(&s_full[turn(i)]);
         }
         return true;
       };
-      auto d_probs = [&](int i) {  // its tiles have been waited for by its scores
+      auto d_probs = [&](int i) -> bool {
+        if (!warp_wait(&s_read[turn(i)], phase(i), abort_flag, err)) return false;
+        tc_fence_after();
         if (one) {
-          mma_scores<DP>(u_dp, v_desc, do_desc + tile_step<DP>(i % S), idesc_s, P.D);
-          tc_commit(&dp_full[i & 1]);
+          mma_scores<DP>(base + turn(i) * L::kXStep, v_desc, do_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          tc_commit(&dp_full[turn(i)]);
         }
+        return true;
       };
-      bool ok = n == 0 || (warp_wait(kv_full, 0, abort_flag, err) && scores(0));
-      if (ok && n > 0) d_probs(0);
-      if (ok && B > 1 && n > 1) ok = scores(1);
-      for (int i = 0; i < n && ok; ++i) {
-        ok = warp_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, err);
-        if (!ok) break;
+      auto sums_v = [&](int i) -> bool {
+        if (!warp_wait(&p_full[turn(i)], phase(i), abort_flag, err)) return false;
         tc_fence_after();
-        if (one) mma_sums(u_dv, base + (i % B) * kRows, do_rows + tile_step<DP>(i % S), idesc_g, i > 0);
-        ok = (i + B >= n || scores(i + B)) && warp_wait(&ds_full[i & 1], (i >> 1) & 1, abort_flag, err);
-        if (!ok) break;
+        if (one)
+          mma_sums(base + L::kDV, base + turn(i) * L::kXStep + L::kP, do_rows + tile_step<DP>(i % S), idesc_g, i > 0);
+        return true;
+      };
+      auto sums_k = [&](int i) -> bool {
+        if (!warp_wait(&ds_full[turn(i)], phase(i), abort_flag, err)) return false;
         tc_fence_after();
         if (one) {
-          mma_sums(u_dk, u_dp, q_rows + tile_step<DP>(i % S), idesc_g, i > 0);
+          mma_sums(base + L::kDK, base + turn(i) * L::kXStep + L::kDS, q_rows + tile_step<DP>(i % S), idesc_g, i > 0);
           tc_commit(&q_empty[i % S]);
         }
-        if (i + 1 < n) d_probs(i + 1);
+        return true;
+      };
+      bool ok = n == 0 || (warp_wait(kv_full, 0, abort_flag, err) && scores(0));
+      if constexpr (kTurns) {
+        ok = ok && (n < 2 || scores(1));
+        for (int i = 0; i < n && ok; ++i)
+          ok = d_probs(i) && (i == 0 || (sums_k(i - 1) && (i + 1 >= n || scores(i + 1)))) && sums_v(i);
+        ok = ok && (n == 0 || sums_k(n - 1));
+      } else {
+        for (int i = 0; i < n && ok; ++i) {
+          ok = d_probs(i) && sums_v(i);
+          if (ok && i + 1 < n) ok = warp_wait(dp_read, i & 1, abort_flag, err) && scores(i + 1);
+          ok = ok && sums_k(i);
+        }
       }
       if (one) {
         if (ok) {
@@ -956,7 +987,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     more_registers();
     const int group = warp / 4, r = (warp % 4) * 32 + lane, key = k0 + r;
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
-    const uint32_t t_s = tmem + (group % B) * kRows + lane_off, t_dp = c_dp + lane_off;
+    // a group's own block, or a half of the common block's queries
+    constexpr int C = kTurns ? 4 : 2;
+    const int bi = kTurns ? group : 0, off = kTurns ? 0 : group * 64;
+    const uint32_t t_x = tmem + bi * L::kXStep + off + lane_off;
+    const uint32_t t_p = tmem + bi * L::kXStep + L::kP + off / 2 + lane_off;
+    const uint32_t t_ds = tmem + bi * L::kXStep + L::kDS + off / 2 + lane_off;
     const bool real = key < P.Tk;
     const int2 mine = real ? P.k_bounds[key] : make_int2(0, 0);
     const int all_lo = P.k_bounds[min(k0 + kRows, P.Tk) - 1].x, all_hi = P.k_bounds[k0].y;
@@ -969,24 +1005,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       factor = ds_factor(top);
     }
     bool ok = true;
-    for (int i = group; i < steps; i += 2) {
-      const uint32_t parity = (i >> 1) & 1;
-      const int q0 = (qb0 + i % per_head) * kRows;
+    for (int i = kTurns ? group : 0; i < steps; i += kTurns ? 2 : 1) {
+      const uint32_t parity = kTurns ? (i >> 1) & 1 : i & 1;
+      const int q0 = (qb0 + i % per_head) * kRows + off;
       if (!warp_wait(&q_full[i % S], (i / S) & 1, abort_flag, err)) { ok = false; break; }
-      if (!warp_wait(&s_full[group], parity, abort_flag, err)) { ok = false; break; }
+      if (!warp_wait(&s_full[bi], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
-      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i % S) * 1024);
+      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i % S) * 1024) + off / 4;
       const float4* s_delta = s_lse + 32;
-      const bool masked = q0 < all_lo || q0 + kRows > all_hi;
+      const bool masked = q0 < all_lo || q0 + C * 32 > all_hi;
       const int a = mine.x - q0;
       const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
-      uint32_t p[4][32];
+      uint32_t p[C][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, p[c]);
+      for (int c = 0; c < C; ++c) tmem_ld_32x32b_x32(t_x + c * 32, p[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(p[c]);
+      for (int c = 0; c < C; ++c) tmem_ld_wait_regs(p[c]);
+      tc_fence_before();
+      mbar_arrive(&s_read[bi]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < C; ++c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 ls = s_lse[c * 8 + e];
@@ -1003,41 +1041,52 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
-        tmem_st_32x32b_x16(t_s + c * 16, pk);
+        tmem_st_32x32b_x16(t_p + c * 16, pk);  // the last P^T there has been multiplied: this S^T came after it
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[group]);
-      if (!warp_wait(&dp_full[group], parity, abort_flag, err)) { ok = false; break; }
+      mbar_arrive(&p_full[bi]);
+      if (!warp_wait(&dp_full[bi], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(t_x, v[0]);
+      if constexpr (!kTurns) {
+        tmem_ld_32x32b_x32(t_x + 32, v[1]);
+        tmem_ld_wait_regs(v[0]);
+        tmem_ld_wait_regs(v[1]);
+        tc_fence_before();
+        mbar_arrive(&dp_read[bi]);
+      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t_dp + c * 32, v);
-        tmem_ld_wait_regs(v);
+      for (int c = 0; c < C; ++c) {
+        uint32_t(&x)[32] = v[c & 1];
+        if constexpr (kTurns) {  // the next 32 columns are on their way while these are worked on
+          tmem_ld_wait_regs(x);
+          if (c + 1 < C) tmem_ld_32x32b_x32(t_x + (c + 1) * 32, v[(c + 1) & 1]);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 dl = s_delta[c * 8 + e];
           const float sub[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            float d = __uint_as_float(p[c][4 * e + u]) * (__uint_as_float(v[4 * e + u]) - sub[u]);
+            float d = __uint_as_float(p[c][4 * e + u]) * (__uint_as_float(x[4 * e + u]) - sub[u]);
             if constexpr (kHalf) d *= factor;
-            v[4 * e + u] = __float_as_uint(d);
+            p[c][4 * e + u] = __float_as_uint(d);
           }
         }
         if (masked)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((uint32_t)(c * 32 + e - a) >= n) v[e] = 0;
+            if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0;
         uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-        tmem_st_32x32b_x16(t_dp + c * 16, pk);
+        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
+        tmem_st_32x32b_x16(t_ds + c * 16, pk);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&ds_full[group]);
+      mbar_arrive(&ds_full[bi]);
     }
     if (ok && steps > 0) ok = warp_wait(g_full, 0, abort_flag, err);
     if (ok) {
@@ -1049,8 +1098,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int c = group; c * 16 < P.D; c += 2) {
         uint32_t w[16], u[16];
         if (steps > 0) {
-          tmem_ld_32x32b_x16(c_dk + lane_off + c * 16, w);
-          tmem_ld_32x32b_x16(c_dv + lane_off + c * 16, u);
+          tmem_ld_32x32b_x16(tmem + L::kDK + lane_off + c * 16, w);
+          tmem_ld_32x32b_x16(tmem + L::kDV + lane_off + c * 16, u);
           tmem_ld_wait_regs16(w);
           tmem_ld_wait_regs16(u);
         } else {
