@@ -92,6 +92,58 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Two fp32 values in one 64-bit register, for the instructions that work on both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// max of three; NaN if any is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of both on the FMA pipe, for finite x: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the
+// low bits of the sum), 2^f by a polynomial of degree 4 fitted here to the least relative error on [-1/2, 1/2] (2.6e-6,
+// iteratively reweighted least squares on 40001 points), n added to the exponent. x below -126 counts as -126.
+__device__ __forceinline__ void exp2_fma(f32x2 x, float& p0, float& p1) {
+  float a, b;
+  split(x, a, b);
+  x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 magic = pair_of(12582912.f, 12582912.f);
+  const f32x2 t = add2(x, magic);
+  const f32x2 f = add2(x, mul2(add2(t, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f)));
+  f32x2 y = fma2(f, pair_of(0.00957005936652422f, 0.00957005936652422f), pair_of(0.055917758494615555f, 0.055917758494615555f));
+  y = fma2(y, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, pair_of(0.6931218504905701f, 0.6931218504905701f));
+  y = fma2(y, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  split(t, t0, t1);
+  split(y, p0, p1);
+  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
 // D(tmem) (+)= A(tmem, 16-bit pairs along K) * B(smem)
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -388,7 +440,8 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
         tc_fence_before();
         mbar_arrive(&s_read[t]);
       }
-      if (kb < all_lo || kb + kRows > all_hi) {
+      const bool masked = kb < all_lo || kb + kRows > all_hi;
+      if (masked) {
         const int a = mine.x - kb;
         const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
 #pragma unroll
@@ -397,12 +450,19 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
           for (int e = 0; e < 32; ++e)
             if ((uint32_t)(c * 32 + e - a) >= n) v[c][e] = 0xff800000u;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[4];
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = max3_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), __uint_as_float(v[c][2]));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][e]));
-      const float blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+        for (int e = 3; e < 31; e += 2) mx[c] = max3_nan(mx[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+      }
+      mx[0] = max3_nan(mx[0], mx[1], __uint_as_float(v[0][31]));
+      mx[2] = max3_nan(mx[2], mx[3], __uint_as_float(v[1][31]));
+      mx[0] = max3_nan(mx[0], __uint_as_float(v[2][31]), __uint_as_float(v[3][31]));
+      const float blk = fmaxf(mx[0], mx[2]) * scale_log2;
+      // a score of infinity or NaN that this row sees makes it NaN (fmaxf may drop one of two NaN, so both are asked)
+      if (!(mx[0] < INFINITY) || !(mx[2] < INFINITY)) m = NAN;
       const bool move = blk > m + kRescale;  // of a first block with a key always
       if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
         if (!warp_wait(&o_full[t], (j - j0 - 1) & 1, abort_flag, err)) { ok = false; break; }
@@ -421,23 +481,39 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
       }
       if (move) m = blk;
       const float ref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      // Where nothing is masked a quarter of the exponentials go to the FMA pipe: the multi-function unit takes 8 cycles
+      // for a warp's 32 and is the bound of this loop.
+      const f32x2 scale2 = pair_of(scale_log2, scale_log2), ref2 = pair_of(-ref, -ref);
+      f32x2 sum[2] = {0, 0};
+      auto exponentials = [&](auto mixed) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e]), scale_log2, -ref));
-          const float p1 = exp2_approx(fmaf(__uint_as_float(v[c][2 * e + 1]), scale_log2, -ref));
-          sum[c] += p0 + p1;
-          v[c / 2][(c & 1) * 16 + e] = pack2<T>(p0, p1);
-        }
+          for (int e = 0; e < 16; ++e) {
+            const f32x2 x = fma2(pair_of(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, ref2);
+            float p0, p1;
+            if (decltype(mixed)::value && e % 4 == 3) {
+              exp2_fma(x, p0, p1);
+            } else {
+              split(x, p0, p1);
+              p0 = exp2_approx(p0);
+              p1 = exp2_approx(p1);
+            }
+            sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
+            v[c / 2][(c & 1) * 16 + e] = pack2<T>(p0, p1);
+          }
+      };
+      if (masked) exponentials(std::false_type{});
+      else exponentials(std::true_type{});
+      float sum0, sum1;
+      split(add2(sum[0], sum[1]), sum0, sum1);
       if (L::kApart && j > j0) {  // the place of P is free once the last P V is done
         if (!warp_wait(&o_full[t], (j - j0 - 1) & 1, abort_flag, err)) { ok = false; break; }
         tc_fence_after();
       }
       tmem_st_32x32b_x32(t_p, v[0]);
       tmem_st_32x32b_x32(t_p + 32, v[1]);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += sum0 + sum1;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[t]);
@@ -706,6 +782,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const float shift = kHalf ? lse_row - kHalfShift : lse_row;
     const float factor = kHalf ? ds_factor(norms[(int64_t)h * (P.lse_stride / kRows) + r0 / kRows]) : 1.f;
     const float scale_log2 = P.scale * kLog2e;
+    const f32x2 scale2 = pair_of(scale_log2, scale_log2), shift2 = pair_of(-shift, -shift);
+    const f32x2 delta2 = pair_of(-delta_row, -delta_row), factor2 = pair_of(factor, factor);
     bool ok = true;
     for (int j = group; j < blocks; j += 2) {
       const uint32_t parity = (j >> 1) & 1, c_s = tmem + (j % 3) * kRows + lane_off;
@@ -721,8 +799,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          p[c][e] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(p[c][e]), scale_log2, -shift)));
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          split(fma2(pair_of(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1])), scale2, shift2), x0, x1);
+          p[c][2 * e] = __float_as_uint(exp2_approx(x0));
+          p[c][2 * e + 1] = __float_as_uint(exp2_approx(x1));
+        }
       const int kb = from + j * kRows;
       const bool masked = kb < all_lo || kb + kRows > all_hi;
       const int a = mine.x - kb;
@@ -737,10 +819,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld_wait_regs(x);
         if (c < 3) tmem_ld_32x32b_x32(c_s + (c + 1) * 32, v[(c + 1) & 1]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float d = __uint_as_float(p[c][e]) * (__uint_as_float(x[e]) - delta_row);
-          if constexpr (kHalf) d *= factor;
-          p[c][e] = __float_as_uint(d);
+        for (int e = 0; e < 16; ++e) {
+          f32x2 d = mul2(pair_of(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1])),
+                         add2(pair_of(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), delta2));
+          if constexpr (kHalf) d = mul2(d, factor2);
+          float d0, d1;
+          split(d, d0, d1);
+          p[c][2 * e] = __float_as_uint(d0);
+          p[c][2 * e + 1] = __float_as_uint(d1);
         }
         if (masked)
 #pragma unroll
@@ -1004,6 +1090,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         top = fmaxf(top, norms[(int64_t)(g * P.group + i / per_head) * (P.lse_stride / kRows) + qb0 + i % per_head]);
       factor = ds_factor(top);
     }
+    const f32x2 scale2 = pair_of(scale_log2, scale_log2), factor2 = pair_of(factor, factor);
     bool ok = true;
     for (int i = kTurns ? group : 0; i < steps; i += kTurns ? 2 : 1) {
       const uint32_t parity = kTurns ? (i >> 1) & 1 : i & 1;
@@ -1023,25 +1110,34 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int c = 0; c < C; ++c) tmem_ld_wait_regs(p[c]);
       tc_fence_before();
       mbar_arrive(&s_read[bi]);
+      // all exponentials before the first store: the stores keep loads and arithmetic from moving across them
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 ls = s_lse[c * 8 + e];
-          const float sub[4] = {ls.x, ls.y, ls.z, ls.w};
+          float x[4];
+          split(fma2(pair_of(__uint_as_float(p[c][4 * e]), __uint_as_float(p[c][4 * e + 1])), scale2,
+                     pair_of(kHalf ? kHalfShift - ls.x : -ls.x, kHalf ? kHalfShift - ls.y : -ls.y)), x[0], x[1]);
+          split(fma2(pair_of(__uint_as_float(p[c][4 * e + 2]), __uint_as_float(p[c][4 * e + 3])), scale2,
+                     pair_of(kHalf ? kHalfShift - ls.z : -ls.z, kHalf ? kHalfShift - ls.w : -ls.w)), x[2], x[3]);
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            p[c][4 * e + u] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(p[c][4 * e + u]), scale_log2,
-                                                               kHalf ? kHalfShift - sub[u] : -sub[u])));
+          for (int u = 0; u < 4; ++u) p[c][4 * e + u] = __float_as_uint(exp2_approx(x[u]));
         }
-        if (masked)
+      if (masked)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if ((uint32_t)(c * 32 + e - a) >= n) p[c][e] = 0;
-        uint32_t pk[16];
+      // the last P^T there has been multiplied: this S^T came after it
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
-        tmem_st_32x32b_x16(t_p + c * 16, pk);  // the last P^T there has been multiplied: this S^T came after it
+      for (int c = 0; c < C; c += 2) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          pk[e] = pack2<T>(__uint_as_float(p[c + e / 16][2 * e % 32]), __uint_as_float(p[c + e / 16][2 * e % 32 + 1]));
+        tmem_st_32x32b_x32(t_p + c * 16, pk);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -1060,19 +1156,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         uint32_t(&x)[32] = v[c & 1];
+        float4 dl[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dl[e] = s_delta[c * 8 + e];
         if constexpr (kTurns) {  // the next 32 columns are on their way while these are worked on
           tmem_ld_wait_regs(x);
           if (c + 1 < C) tmem_ld_32x32b_x32(t_x + (c + 1) * 32, v[(c + 1) & 1]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float4 dl = s_delta[c * 8 + e];
-          const float sub[4] = {dl.x, dl.y, dl.z, dl.w};
+          f32x2 d[2] = {add2(pair_of(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])), pair_of(-dl[e].x, -dl[e].y)),
+                        add2(pair_of(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])), pair_of(-dl[e].z, -dl[e].w))};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            float d = __uint_as_float(p[c][4 * e + u]) * (__uint_as_float(x[4 * e + u]) - sub[u]);
-            if constexpr (kHalf) d *= factor;
-            p[c][4 * e + u] = __float_as_uint(d);
+          for (int u = 0; u < 2; ++u) {
+            d[u] = mul2(d[u], pair_of(__uint_as_float(p[c][4 * e + 2 * u]), __uint_as_float(p[c][4 * e + 2 * u + 1])));
+            if constexpr (kHalf) d[u] = mul2(d[u], factor2);
+            float d0, d1;
+            split(d[u], d0, d1);
+            p[c][4 * e + 2 * u] = __float_as_uint(d0);
+            p[c][4 * e + 2 * u + 1] = __float_as_uint(d1);
           }
         }
         if (masked)
