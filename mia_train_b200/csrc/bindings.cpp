@@ -107,7 +107,8 @@ at::Tensor fp8_linear_quantized(const at::Tensor& x, const at::Tensor& data, con
                                 int64_t act, bool bf16);
 int64_t set_fp8_tile(int64_t tile);
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_bounds,
-                            const at::Tensor& k_bounds, double scale);
+                            const at::Tensor& k_bounds, double scale, const OptTensor& items, const OptTensor& pieces,
+                            int64_t max_queries, int64_t tile_pairs, int64_t pairs);
 std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                           const at::Tensor& freq, bool interleaved, double amplitude);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& x, int64_t k, double tau);

@@ -6,7 +6,8 @@
 //
 // q (Tq, Hq, D), k and v (Tk, Hk, D); a key head serves Hq / Hk query heads, whose contributions to dk and dv add up.
 // The mask is a pair of bounds per query (and, for dk and dv, per key), made once for a batch's lengths; rows that
-// see nothing give zeros. This file holds the kernels with a warp per row, which run every head size and type.
+// see nothing give zeros. This file holds the kernels with a warp per row, which run every head size and type, and the
+// forward kernel for few queries over many keys.
 #include <type_traits>
 
 #include "packed_attention.h"
@@ -87,6 +88,175 @@ __global__ void __launch_bounds__(kWarps * 32) packed_dkv_rows_kernel(PackedProb
   store_row<T>(dv + at * P.D, c, P.D, lane);
 }
 
+// ------------------------------------------------------------------------- few queries, many keys
+// A tile of 128 queries computes 128 rows of scores for every key that one of them sees. Where a sequence has few
+// queries (a pooling query over all tokens of a volume, the next token behind a long context) almost all of that is
+// masked, and there are fewer tiles than SMs. Here a CTA takes up to R rows (queries and heads that share a key head)
+// of one sequence and a piece of its keys, and the pieces' sums are joined by a second kernel. It is bound by reading
+// K and V: LP lanes hold a row's channels, eight each, and a warp has eight 16-byte loads of K and of V a lane under way.
+// 16 sequences of 1029 .. 4101 keys, one query, 16 heads of 64 fp16: 805 us by tiles, 47 us here (39 us at 5.6 TB/s and 7 us for joining).
+constexpr int kFewThreads = 128;
+
+template <typename T, int LP, int R>
+__global__ void __launch_bounds__(kFewThreads) packed_few_kernel(PackedProblem P, PackedFew few, T* __restrict__ o,
+                                                                 float* __restrict__ lse) {
+  constexpr int KP = 32 / LP, U = 8, W = U * KP;  // keys of a load, loads, keys of a warp at a time
+  __shared__ float red[4][R][LP * 8 + 2];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = lane % LP, g = lane / LP;
+  const int4 item = few.items[blockIdx.x];  // first query, queries, keys [z, w)
+  const int hk = blockIdx.y, r0 = blockIdx.z * R, rows = item.y * P.group;
+  if (r0 >= rows) return;
+  const bool in = c * 8 < P.D;
+  float q[R][8], acc[R][8], m[R], l[R];
+  int lo[R], hi[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = min(r0 + r, rows - 1), i = item.x + row / P.group, h = hk * P.group + row % P.group;
+    Raw8<T> raw = {};
+    if (in) raw = load_raw8<T>((const T*)P.q + i * P.qs.row + h * P.qs.head + c * 8);
+    unpack8<T>(raw, q[r]);
+    const int2 b = P.q_bounds[i];
+    lo[r] = b.x;
+    hi[r] = b.y;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[r][e] *= P.scale * kLog2e;
+      acc[r][e] = 0.f;
+    }
+  }
+  const T *kp = (const T*)P.k + hk * P.ks.head + c * 8, *vp = (const T*)P.v + hk * P.vs.head + c * 8;
+  for (int kb = item.z + warp * W; kb < item.w; kb += 4 * W) {
+    Raw8<T> kr[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = kb + u * KP + g;
+      kr[u] = vr[u] = {};
+      if (in && key < item.w) {
+        kr[u] = load_raw8<T>(kp + key * P.ks.row);
+        vr[u] = load_raw8<T>(vp + key * P.vs.row);
+      }
+    }
+    float s[R][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[8];
+      unpack8<T>(kr[u], x);
+      const int key = kb + u * KP + g;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d = fmaf(q[r][e], x[e], d);
+#pragma unroll
+        for (int w = 1; w < LP; w *= 2) d += __shfl_xor_sync(0xffffffffu, d, w);
+        s[r][u] = key >= lo[r] && key < min(hi[r], item.w) ? d : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = s[r][0];
+#pragma unroll
+      for (int u = 1; u < U; ++u) top = fmaxf(top, s[r][u]);
+#pragma unroll
+      for (int w = LP; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float m_new = fmaxf(m[r], top), ref = m_new == -INFINITY ? 0.f : m_new, fade = exp2f(m[r] - ref);
+      m[r] = m_new;
+      l[r] *= fade;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][e] *= fade;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[r][u] = exp2f(s[r][u] - ref);
+        l[r] += s[r][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[8];
+      unpack8<T>(vr[u], x);
+      const int key = kb + u * KP + g;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (key >= lo[r] && key < hi[r])  // what a row does not see is not multiplied either
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(s[r][u], x[e], acc[r][e]);
+    }
+  }
+  // a warp's keys lie in KP groups of lanes, the CTA's in four warps
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int w = LP; w < 32; w *= 2) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], w);
+    }
+    if (g == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[warp][r][c * 8 + e] = acc[r][e];
+      if (c == 0) {
+        red[warp][r][LP * 8] = m[r];
+        red[warp][r][LP * 8 + 1] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  for (int at = threadIdx.x; at < R * LP * 8; at += kFewThreads) {
+    const int r = at / (LP * 8), ch = at % (LP * 8), row = r0 + r;
+    if (row >= rows || ch >= P.D) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, red[w][r][LP * 8]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, value = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(red[w][r][LP * 8] - ref);
+      sum += f * red[w][r][LP * 8 + 1];
+      value += f * red[w][r][ch];
+    }
+    if (few.partial == nullptr) {
+      const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
+      o[((int64_t)i * P.Hq + h) * P.D + ch] = from_f32<T>(sum == 0.f ? 0.f : value / sum);
+      if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
+    } else {
+      float* part = few.partial + (((int64_t)blockIdx.x * P.Hk + hk) * few.rows + row) * (P.D + 2);
+      part[ch] = value;
+      if (ch == 0) {
+        part[P.D] = top;
+        part[P.D + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the pieces of a sequence's keys in their order, a CTA per row and key head.
+template <typename T>
+__global__ void __launch_bounds__(128) packed_few_join_kernel(PackedProblem P, PackedFew few, T* __restrict__ o,
+                                                              float* __restrict__ lse) {
+  const int2 seq = few.pieces[blockIdx.x];  // first item, items
+  if (seq.y == 0) return;
+  const int4 item = few.items[seq.x];
+  const int hk = blockIdx.y, row = blockIdx.z, ch = threadIdx.x;
+  if (row >= item.y * P.group) return;
+  const int64_t step = (int64_t)P.Hk * few.rows * (P.D + 2);
+  const float* part = few.partial + ((int64_t)seq.x * P.Hk + hk) * few.rows * (P.D + 2) + (int64_t)row * (P.D + 2);
+  float top = -INFINITY;
+  for (int n = 0; n < seq.y; ++n) top = fmaxf(top, part[n * step + P.D]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, value = 0.f;
+  for (int n = 0; n < seq.y; ++n) {
+    const float f = exp2f(part[n * step + P.D] - ref);
+    sum += f * part[n * step + P.D + 1];
+    if (ch < P.D) value += f * part[n * step + ch];
+  }
+  const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
+  if (ch < P.D) o[((int64_t)i * P.Hq + h) * P.D + ch] = from_f32<T>(sum == 0.f ? 0.f : value / sum);
+  if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
+}
+
 unsigned grid_of(int64_t items, int per) { return (unsigned)((items + per - 1) / per); }
 
 template <typename F>
@@ -102,6 +272,21 @@ cudaError_t packed_fwd_rows(const PackedProblem& P, void* o, float* lse, cudaStr
   by_type(P.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     packed_fwd_rows_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, kWarps), kWarps * 32, 0, stream>>>(P, (T*)o, lse);
+  });
+  return cudaGetLastError();
+}
+
+cudaError_t packed_fwd_few(const PackedProblem& P, const PackedFew& few, void* o, float* lse, cudaStream_t stream) {
+  const bool wide = P.D > 64, several = few.rows > 1;
+  by_type(P.type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    auto go = [&](auto kernel, int r) {
+      kernel<<<dim3(few.count, P.Hk, (few.rows + r - 1) / r), kFewThreads, 0, stream>>>(P, few, (T*)o, lse);
+    };
+    if (wide) several ? go(packed_few_kernel<T, 16, 4>, 4) : go(packed_few_kernel<T, 16, 1>, 1);
+    else several ? go(packed_few_kernel<T, 8, 4>, 4) : go(packed_few_kernel<T, 8, 1>, 1);
+    if (few.partial != nullptr)
+      packed_few_join_kernel<T><<<dim3(few.sequences, P.Hk, few.rows), 128, 0, stream>>>(P, few, (T*)o, lse);
   });
   return cudaGetLastError();
 }

@@ -29,6 +29,15 @@ struct PackedProblem {
 
 // o (Tq.., Hq, D) contiguous; lse (Hq, lse_stride) fp32
 cudaError_t packed_fwd_rows(const PackedProblem& P, void* o, float* lse, cudaStream_t stream);
+// Few queries over many keys: pieces of a sequence's keys with all of its queries.
+struct PackedFew {
+  const int4* items;   // (count): first query, queries, keys [z, w)
+  const int2* pieces;  // (sequences): first item, items
+  int count, sequences;
+  int rows;        // most queries of a sequence times the heads that share a key head
+  float* partial;  // (count, Hk, rows, D + 2) fp32, or null where every sequence is one item
+};
+cudaError_t packed_fwd_few(const PackedProblem& P, const PackedFew& few, void* o, float* lse, cudaStream_t stream);
 // dout as strided rows; delta like lse (scratch); dq (.., Hq, D), dk and dv (.., Hk, D) contiguous
 cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
                             float* delta, void* dq, void* dk, void* dv, cudaStream_t stream);

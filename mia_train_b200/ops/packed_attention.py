@@ -25,6 +25,8 @@ import torch
 from ._native import native, use_native
 
 MAX_HEAD_DIM = 128
+MAX_FEW = 64  # queries of a sequence that the kernel for few queries takes
+PIECE = 512  # keys of a sequence that it takes at a time
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -84,6 +86,26 @@ class PackedSequences:
             q_lo = q_lo + np.clip(j - np.repeat(lk - lq, lk), 0, np.repeat(lq, lk))
         self.q_bounds = self._table(k_lo, k_hi)
         self.k_bounds = self._table(q_lo, q_hi)
+        self.max_queries = int(lq.max(initial=0))
+        self.pairs = int((k_hi - k_lo).sum())
+        # scores that 128-row tiles compute: every tile all keys from its first row's first to its last row's last
+        tiles = k_hi[np.minimum(np.arange(127, self.num_queries + 127, 128), self.num_queries - 1)] - k_lo[::128]
+        self.tile_pairs = int((-(-np.maximum(tiles, 0) // 128)).sum()) * 128 * 128
+        self.items = self.pieces = None
+        if self.tile_pairs > 16 * self.pairs and self.max_queries <= MAX_FEW:
+            self._make_items(q0, lq, k0, lk)
+
+    def _make_items(self, q0: np.ndarray, lq: np.ndarray, k0: np.ndarray, lk: np.ndarray) -> None:
+        """Pieces of at most `PIECE` keys of every sequence that has queries."""
+        some = lq > 0
+        q0, lq, k0, lk = q0[some], lq[some], k0[some], lk[some]
+        count = np.maximum(-(-lk // PIECE), 1)
+        first = np.cumsum(count) - count
+        seq = np.repeat(np.arange(len(lq)), count)
+        lo = k0[seq] + (np.arange(len(seq)) - first[seq]) * PIECE
+        hi = np.minimum(lo + PIECE, (k0 + lk)[seq])
+        self.items = torch.from_numpy(np.stack([q0[seq], lq[seq], lo, hi], 1).astype(np.int32)).to(self.device)
+        self.pieces = self._table(first, count)
 
     def _table(self, lo: np.ndarray, hi: np.ndarray) -> torch.Tensor:
         # a copy from pageable memory: it is there when the call returns, for any stream
@@ -149,5 +171,6 @@ def packed_attention(
                              f"{MAX_HEAD_DIM} channels, got {q.dtype} heads of {d}")
         if q.shape[1] > 65535:
             raise ValueError(f"at most 65535 query heads, got {q.shape[1]}")
-        return native().packed_attention(q, k, v, sequences.q_bounds, sequences.k_bounds, scale)
+        return native().packed_attention(q, k, v, sequences.q_bounds, sequences.k_bounds, scale, sequences.items,
+                                         sequences.pieces, sequences.max_queries, sequences.tile_pairs, sequences.pairs)
     return packed_attention_reference(q, k, v, sequences, scale)

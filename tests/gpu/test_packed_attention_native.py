@@ -325,3 +325,31 @@ def test_refusals():
     ):
         with pytest.raises(ValueError):
             bad()
+
+
+FEW = [([1] * 6, [700, 3, 0, 1500, 513, 512]), ([1, 2, 0, 3], [5000, 900, 40, 2100]), ([5], [9000]), ([1] * 40, [300] * 40)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("lq,lk", FEW, ids=str)
+def test_few_queries_over_many_keys(lq, lk, dtype, causal):
+    assert PackedSequences(lq, lk, causal=causal, device=DEV).items is not None
+    _compare(lq, lk, 2, 2, 64, dtype, causal, pad=2)
+
+
+@pytest.mark.parametrize("hq,hk", [(8, 1), (6, 2), (3, 3)])
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 128])
+def test_few_queries_of_grouped_heads(hq, hk, d):
+    _compare([1, 3, 1], [2000, 1800, 4000], hq, hk, d, BF16, True)
+
+
+def test_few_queries_do_not_see_what_is_masked():
+    lq, lk = [2, 2], [1500, 1400]
+    q, k, v, do = _inputs(lq, lk, 2, 1, 64, BF16, pad=4)
+    seq = PackedSequences(lq, lk, causal=True, device=DEV)
+    clean = packed_attention(q, k, v, seq)
+    k[1499], v[1499] = math.nan, math.nan  # the first sequence's last key: its last query alone sees it
+    k[2900:], v[2900:] = math.inf, math.nan
+    got = packed_attention(q, k, v, seq)
+    assert got[1].isnan().all() and torch.equal(got[0], clean[0]) and torch.equal(got[2:], clean[2:])
