@@ -51,7 +51,20 @@ __device__ __forceinline__ void for_row(const T* row, int V, F&& f) {
     float one = to_f32(row[threadIdx.x]);
     f((int)threadIdx.x, one);
   }
-  for (int i = threadIdx.x; i < vecs; i += kThreads) {
+  constexpr int kAtOnce = 4;  // loads of a thread under way before the first is worked on
+  int i = threadIdx.x;
+  for (; i + (kAtOnce - 1) * kThreads < vecs; i += kAtOnce * kThreads) {
+    Raw8<T> raw[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) raw[u] = load_raw8<T>(row + ahead + (i + u * kThreads) * 8);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      float v[8];
+      unpack8<T>(raw[u], v);
+      f(ahead + (i + u * kThreads) * 8, v);
+    }
+  }
+  for (; i < vecs; i += kThreads) {
     float v[8];
     unpack8<T>(load_raw8<T>(row + ahead + i * 8), v);
     f(ahead + i * 8, v);
@@ -61,6 +74,16 @@ __device__ __forceinline__ void for_row(const T* row, int V, F&& f) {
     float one = to_f32(row[at]);
     f(at, one);
   }
+}
+
+// The largest of eight; NaN if any is.
+__device__ __forceinline__ float max8_nan(const float (&v)[8]) {
+  float r, q;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(q) : "f"(v[3]), "f"(v[4]), "f"(v[5]));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(r), "f"(v[6]), "f"(v[7]));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(q));
+  return r;
 }
 
 // Running maximum m (of raw logits) and sum l of exp((s - m) / tau).
@@ -73,10 +96,8 @@ struct Soft {
     }
     l += s == -INFINITY ? 0.f : ex2((s - m) * c);
   }
-  __device__ __forceinline__ void add8(const float (&v)[8], float c) {
-    float top = v[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, v[e]);
+  // `top` is the largest of the eight, or NaN
+  __device__ __forceinline__ void add8(const float (&v)[8], float top, float c) {
     if (top > m) {
       l *= m == -INFINITY ? 0.f : ex2((m - top) * c);
       m = top;
@@ -140,6 +161,13 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The number with a key (for a key that none has, one near it that is not above it); -inf for keys below all.
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if (key <= 0x007fffffu) return -INFINITY;
+  if (key >= 0xff800000u) return INFINITY;
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 __device__ int block_count(int mine, int* scratch /* kWarpsPer */) {
   const int w = __reduce_add_sync(0xffffffffu, mine);
   __syncthreads();
@@ -182,12 +210,11 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
       if (v != v) soft.l = v;
       best[0] = max(best[0], key_of(v));
     } else {
-      soft.add8(v, c);
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, key_of(v[e]));
-      if (turn) best[1] = max(best[1], top);
-      else best[0] = max(best[0], top);
+      const float top = max8_nan(v);
+      soft.add8(v, top, c);
+      const uint32_t key = key_of(top);
+      if (turn) best[1] = max(best[1], key);
+      else best[0] = max(best[0], key);
       turn ^= 1;
     }
   });
@@ -197,7 +224,16 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
     lse[blockIdx.x] = nan ? NAN : soft.m == INFINITY ? INFINITY : soft.l == 0.f ? -INFINITY : fmaf(soft.m, inv_tau, logf(soft.l));
 
   // A row shorter than the groups leaves some of them empty, and then the bound may be 0: every element is taken.
-  const uint32_t bound = kth_key(k, [&](uint32_t t) { return block_count((best[0] >= t) + (best[1] >= t), counts); });
+  // Any bound that at least k groups reach will do; the search ends where not many more do.
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = bound | (1u << bit);
+    const int n = __syncthreads_count(best[0] >= t) + __syncthreads_count(best[1] >= t);
+    if (n < k) continue;
+    bound = t;
+    if (n <= k + k / 4 + 4) break;
+  }
+  const float floor_of = value_of(bound);
   auto collect = [&](int at, float v, uint32_t least) {
     const uint32_t key = key_of(v);
     if (key >= least) {
@@ -205,17 +241,17 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
       if (n < kCandidates) list[n] = (uint64_t)key << 32 | (0xffffffffu - (uint32_t)at);
     }
   };
-  auto scan = [&](uint32_t least) {
+  auto scan = [&](uint32_t least, float least_value) {
     for_row<T>(row, V, [&](int at, auto& v) {
       if constexpr (std::is_same_v<std::decay_t<decltype(v)>, float>) {
         collect(at, v, least);
-      } else {
+      } else if (!(max8_nan(v) < least_value)) {  // one of them may reach the bound, or is NaN
 #pragma unroll
         for (int e = 0; e < 8; ++e) collect(at + e, v[e], least);
       }
     });
   };
-  scan(bound);
+  scan(bound, floor_of);
   __syncthreads();
   int n = n_list;
   if (n > kCandidates) {
@@ -233,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
     __syncthreads();
     if (threadIdx.x == 0) n_list = 0;
     __syncthreads();
-    if (exact != 0xffffffffu) scan(exact + 1);
+    if (exact != 0xffffffffu) scan(exact + 1, value_of(exact));
     __syncthreads();
     n = n_list;  // less than k
     int found = 0;
@@ -330,7 +366,7 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillParams p, 
           for (int e = 0; e < 8; ++e)
             if (bits >> e & 1) v[e] = -INFINITY;
       }
-      gen.add8(v, c);
+      gen.add8(v, max8_nan(v), c);
     }
   });
   block_join(gen, c, red);

@@ -75,6 +75,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) sum[a][e] = 0.f;
 
+  constexpr int kAtOnce = sizeof(T) == 4 || (kLearn && !kInter) ? 2 : 4;
+  const int step_t = slots / H, step_h = slots % H;
   const int64_t groups = (p.tokens + p.group - 1) / p.group;
   for (int64_t gi = blockIdx.x; gi < groups; gi += gridDim.x) {
     const int64_t first = gi * p.group;
@@ -83,82 +85,122 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     for (int i = threadIdx.x; i < n * p.P; i += kThreads) table[i] = turn(p, first + i / p.P, i % p.P);
     __syncthreads();
     if (slot >= slots) continue;
-#pragma unroll 2
-    for (int at = slot; at < n * H; at += slots) {
-      const int tk = at / H, h = at % H;
-      const int64_t token = first + tk, b = token / p.T, t = token % p.T;
-      const bool is_q = h < p.Hq;
-      const int hh = is_q ? h : h - p.Hq;
-      const TokenRows rs = is_q ? p.qs : p.ks, ws = is_q ? p.yqs : p.yks;
-      const T* src = (const T*)(is_q ? p.q : p.k) + b * rs.b + t * rs.t + hh * rs.h;
-      T* dst = (T*)(is_q ? p.yq : p.yk) + b * ws.b + t * ws.t + hh * ws.h;
-      if (!rotates) {
-        if constexpr (kVec) {
-          const Raw8<T> raw = load_raw8<T>(src + c1);
+    int tk = slot / H, h = slot % H;
+    for (int at = slot; at < n * H; at += kAtOnce * slots) {
+      // the loads of kAtOnce heads are under way before the first is worked on
+      constexpr int kVecs = !kVec ? 1 : kInter ? 1 : 2;
+      Raw8<T> raw[kAtOnce][kVecs];
+      Raw8<T> kept[kLearn ? kAtOnce : 1][kVecs];
+      T one[kAtOnce][2], own[kLearn ? kAtOnce : 1][2];
+      int token_of[kAtOnce];
+      T* dst[kAtOnce];
 #pragma unroll
-          for (int u = 0; u < (int)(sizeof(raw.u) / 16); ++u) reinterpret_cast<uint4*>(dst + c1)[u] = raw.u[u];
-        } else {
-          dst[c1] = src[c1];
+      for (int u = 0; u < kAtOnce; ++u) {
+        dst[u] = nullptr;
+        if (at + u * slots < n * H) {
+          const int64_t token = first + tk, b = token / p.T, t = token - b * p.T;
+          const bool is_q = h < p.Hq;
+          const int hh = is_q ? h : h - p.Hq;
+          const TokenRows rs = is_q ? p.qs : p.ks, ws = is_q ? p.yqs : p.yks;
+          const T* src = (const T*)(is_q ? p.q : p.k) + b * rs.b + t * rs.t + hh * rs.h;
+          dst[u] = (T*)(is_q ? p.yq : p.yk) + b * ws.b + t * ws.t + hh * ws.h;
+          token_of[u] = tk;
+          if constexpr (kVec) {
+            raw[u][0] = load_raw8<T>(src + c1);
+            if (!kInter && rotates) raw[u][kVecs - 1] = load_raw8<T>(src + c2);
+          } else {
+            one[u][0] = src[c1];
+            if (rotates) one[u][1] = src[c2];
+          }
+          if constexpr (kLearn) {
+            const TokenRows xs = is_q ? p.xqs : p.xks;
+            const T* x = (const T*)(is_q ? p.xq : p.xk) + b * xs.b + t * xs.t + hh * xs.h;
+            if (rotates) {
+              if constexpr (kVec) {
+                kept[u][0] = load_raw8<T>(x + c1);
+                if (!kInter) kept[u][kVecs - 1] = load_raw8<T>(x + c2);
+              } else {
+                own[u][0] = x[c1];
+                own[u][1] = x[c2];
+              }
+            }
+          }
         }
-        continue;
+        tk += step_t;
+        h += step_h;
+        if (h >= H) {
+          h -= H;
+          ++tk;
+        }
       }
-      float x1[kPairs], x2[kPairs];
-      auto pairs_of = [&](const T* row) {
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (dst[u] == nullptr) break;
+        if (!rotates) {
+          if constexpr (kVec) {
+#pragma unroll
+            for (int w = 0; w < (int)(sizeof(Raw8<T>) / 16); ++w) reinterpret_cast<uint4*>(dst[u] + c1)[w] = raw[u][0].u[w];
+          } else {
+            dst[u][c1] = one[u][0];
+          }
+          continue;
+        }
+        float x1[kPairs], x2[kPairs];
+        auto pairs_of = [&](const Raw8<T>(&r)[kVecs], const T(&single)[2]) {
+          if constexpr (!kVec) {
+            x1[0] = to_f32(single[0]);
+            x2[0] = to_f32(single[1]);
+          } else if constexpr (kInter) {
+            float x[8];
+            unpack8<T>(r[0], x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x1[e] = x[2 * e];
+              x2[e] = x[2 * e + 1];
+            }
+          } else {
+            unpack8<T>(r[0], x1);
+            unpack8<T>(r[kVecs - 1], x2);
+          }
+        };
+        pairs_of(raw[u], one[u]);
+        const float2* cs = table + token_of[u] * p.P + v * kPairs;
+        float y1[kPairs], y2[kPairs];
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          const float2 r = cs[e];
+          y1[e] = x1[e] * r.x - x2[e] * r.y;
+          y2[e] = x2[e] * r.x + x1[e] * r.y;
+        }
         if constexpr (!kVec) {
-          x1[0] = to_f32(row[c1]);
-          x2[0] = to_f32(row[c2]);
+          dst[u][c1] = from_f32<T>(y1[0]);
+          dst[u][c2] = from_f32<T>(y2[0]);
         } else if constexpr (kInter) {
-          float x[8];
-          unpack8<T>(load_raw8<T>(row + c1), x);
+          float y[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x1[e] = x[2 * e];
-            x2[e] = x[2 * e + 1];
+            y[2 * e] = y1[e];
+            y[2 * e + 1] = y2[e];
           }
+          store8<T>(dst[u] + c1, y);
         } else {
-          const Raw8<T> a = load_raw8<T>(row + c1), c = load_raw8<T>(row + c2);
-          unpack8<T>(a, x1);
-          unpack8<T>(c, x2);
+          store8<T>(dst[u] + c1, y1);
+          store8<T>(dst[u] + c2, y2);
         }
-      };
-      pairs_of(src);
-      const float2* cs = table + tk * p.P + v * kPairs;
-      float y1[kPairs], y2[kPairs];
+        if constexpr (kLearn) {
+          // Here x is dy and y its gradient dx = R(-angle) dy: dy2 y1 - dy1 y2 of the forward pass's outputs is the
+          // same turned back by the angle, dx2 x1 - dx1 x2 with its inputs.
+          pairs_of(kept[u], own[u]);
+          const int64_t row = position_row(p, first + token_of[u]) * p.axes;
 #pragma unroll
-      for (int e = 0; e < kPairs; ++e) {
-        const float2 r = cs[e];
-        y1[e] = x1[e] * r.x - x2[e] * r.y;
-        y2[e] = x2[e] * r.x + x1[e] * r.y;
-      }
-      if constexpr (!kVec) {
-        dst[c1] = from_f32<T>(y1[0]);
-        dst[c2] = from_f32<T>(y2[0]);
-      } else if constexpr (kInter) {
-        float y[8];
+          for (int e = 0; e < kPairs; ++e) x1[e] = y2[e] * x1[e] - y1[e] * x2[e];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] = y1[e];
-          y[2 * e + 1] = y2[e];
-        }
-        store8<T>(dst + c1, y);
-      } else {
-        store8<T>(dst + c1, y1);
-        store8<T>(dst + c2, y2);
-      }
-      if constexpr (kLearn) {
-        // Here x is dy and y its gradient dx = R(-angle) dy: dy2 y1 - dy1 y2 of the forward pass's outputs is the
-        // same turned back by the angle, dx2 x1 - dx1 x2 with its inputs.
-        const TokenRows xs = is_q ? p.xqs : p.xks;
-        pairs_of((const T*)(is_q ? p.xq : p.xk) + b * xs.b + t * xs.t + hh * xs.h);
-        const int64_t row = position_row(p, token) * p.axes;
+          for (int a = 0; a < kMaxAxes; ++a) {
+            if (a >= p.axes) break;
+            const float at_a = (float)position_of(p, row + a);
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) x1[e] = y2[e] * x1[e] - y1[e] * x2[e];
-#pragma unroll
-        for (int a = 0; a < kMaxAxes; ++a) {
-          if (a >= p.axes) break;
-          const float at_a = (float)position_of(p, row + a);
-#pragma unroll
-          for (int e = 0; e < kPairs; ++e) sum[a][e] = fmaf(at_a, x1[e], sum[a][e]);
+            for (int e = 0; e < kPairs; ++e) sum[a][e] = fmaf(at_a, x1[e], sum[a][e]);
+          }
         }
       }
     }
@@ -211,10 +253,10 @@ RotaryPlan rotary_plan(const RotaryParams& p, bool aligned, bool interleaved, bo
   const int pairs = plan.vec ? (interleaved ? 4 : 8) : 1, w = plan.vec ? 8 : 1;
   const int items = p.P / pairs + (p.D - 2 * p.P) / w;
   const int slots = kThreads / items;
-  // Tokens of a block at a time: enough for some eight items a thread, few enough that every SM has two blocks, and at
+  // Tokens of a block at a time: enough for some sixteen items a thread, few enough that every SM has two blocks, and at
   // most 32 KB of tables.
   const int64_t per_token = (int64_t)items * (p.Hq + p.Hk);
-  int64_t group = std::max<int64_t>(1, 8 * kThreads / per_token);
+  int64_t group = std::max<int64_t>(1, 16 * kThreads / per_token);
   group = std::min<int64_t>(group, std::max<int64_t>(1, p.tokens / (2 * 148)));
   group = std::min<int64_t>(group, std::max(1, 4096 / std::max(p.P, 1)));
   plan.group = (int)group;
