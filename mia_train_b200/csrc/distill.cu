@@ -190,7 +190,7 @@ __device__ uint32_t kth_key(int k, F&& count) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restrict__ x, int64_t stride, int V, int k,
+__global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __restrict__ x, int64_t stride, int V, int k,
                                                               float inv_tau, T* __restrict__ values,
                                                               int64_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ uint64_t list[kCandidates];
@@ -321,7 +321,7 @@ __device__ __forceinline__ int index_at(const DistillParams& p, int64_t i) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillParams p, double* __restrict__ row_loss) {
+__global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams p, double* __restrict__ row_loss) {
   extern __shared__ uint32_t given[];  // a bit per class, where there is a rest
   __shared__ double sums[4 * kWarpsPer];
   __shared__ float red[2 * kWarpsPer];

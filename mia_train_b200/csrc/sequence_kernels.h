@@ -64,7 +64,7 @@ struct RotaryParams {
   int freq64;
   int axes, P, D, T, Hq, Hk;
   int64_t tokens;  // B * T
-  int group;       // tokens of a block at a time
+  int heads;       // of a block
   float amplitude;
   int inverse;
   float* partial;  // (blocks, axes, P)
@@ -72,8 +72,8 @@ struct RotaryParams {
 
 struct RotaryPlan {
   bool vec;
-  int group;
-  unsigned grid;
+  int heads;              // of a block
+  unsigned grid, chunks;  // blocks over tokens, over heads
   size_t smem;
 };
 RotaryPlan rotary_plan(const RotaryParams& p, bool aligned, bool interleaved, bool learn);

@@ -223,7 +223,7 @@ void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& position
   const RotaryPlan plan = rotary_plan(p, aligned, interleaved, learn);
   at::Tensor partial;
   if (learn) {
-    partial = at::empty({(int64_t)plan.grid, p.axes, p.P}, q.options().dtype(at::kFloat));
+    partial = at::empty({(int64_t)plan.grid * plan.chunks, p.axes, p.P}, q.options().dtype(at::kFloat));
     p.partial = partial.data_ptr<float>();
   }
   C10_CUDA_CHECK(rotary_launch(p, plan, type_of(q), interleaved, learn ? dfreq->data_ptr<float>() : nullptr, stream));
