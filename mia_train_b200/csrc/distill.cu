@@ -2,7 +2,7 @@
 //
 // Top logits of a row: the k largest, largest first, equal ones by the lower index, and logsumexp(x / tau). A NaN
 // counts as larger than every number. One block owns a row. Pass 1 reads it once: running maximum and sum of the
-// log-sum-exp, and the largest value of each of 1024 interleaved groups. The k-th largest of those group maxima is a
+// log-sum-exp, and the largest value of each of 512 (or 1024) interleaved groups. The k-th largest of those group maxima is a
 // value that at least k elements reach, and few more do (65536 normal values and k = 64: about 66). Pass 2 finds the
 // row in L2 and collects what reaches it; every candidate then counts how many come before it. A row in which too
 // many elements are equal takes the exact k-th value by bisection over the bits instead, and its ties in order of
@@ -30,8 +30,12 @@
 namespace mia {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarpsPer = kThreads / 32;
+// Threads of a row's block: 256, six blocks an SM, so that one row's barriers lie behind another's loads; for long rows
+// that are fewer than two for every SM 512, for the row's own time (16 rows of 65536 fp32: 18 -> 14 us; 1024 threads
+// wait longer for each other: 15 us, and 11 instead of 5 us for 4 rows of 1000).
+constexpr int kMany = 256, kFew = 512;
+int threads_for(int rows, int classes) { return rows < 2 * 148 && classes >= 16384 ? kFew : kMany; }
+
 constexpr int kCandidates = 2048;
 constexpr float kLog2eF = 1.4426950408889634f;
 
@@ -42,7 +46,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Calls f(index, values) for the row's elements, eight aligned ones at a time, and f(index, value) for those at both ends.
-template <typename T, typename F>
+template <int NT, typename T, typename F>
 __device__ __forceinline__ void for_row(const T* row, int V, F&& f) {
   constexpr int kAlign = 16 / sizeof(T);
   const int ahead = min(V, (int)((kAlign - (reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kAlign) % kAlign));
@@ -53,18 +57,18 @@ __device__ __forceinline__ void for_row(const T* row, int V, F&& f) {
   }
   constexpr int kAtOnce = 4;  // loads of a thread under way before the first is worked on
   int i = threadIdx.x;
-  for (; i + (kAtOnce - 1) * kThreads < vecs; i += kAtOnce * kThreads) {
+  for (; i + (kAtOnce - 1) * NT < vecs; i += kAtOnce * NT) {
     Raw8<T> raw[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) raw[u] = load_raw8<T>(row + ahead + (i + u * kThreads) * 8);
+    for (int u = 0; u < kAtOnce; ++u) raw[u] = load_raw8<T>(row + ahead + (i + u * NT) * 8);
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       float v[8];
       unpack8<T>(raw[u], v);
-      f(ahead + (i + u * kThreads) * 8, v);
+      f(ahead + (i + u * NT) * 8, v);
     }
   }
-  for (; i < vecs; i += kThreads) {
+  for (; i < vecs; i += NT) {
     float v[8];
     unpack8<T>(load_raw8<T>(row + ahead + i * 8), v);
     f(ahead + i * 8, v);
@@ -118,7 +122,8 @@ struct Soft {
   }
 };
 
-__device__ void block_join(Soft& a, float c, float* scratch /* 2 * kWarpsPer */) {
+template <int NT>
+__device__ void block_join(Soft& a, float c, float* scratch /* 2 * NT / 32 */) {
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, a.m, w), l2 = __shfl_xor_sync(0xffffffffu, a.l, w);
@@ -127,15 +132,15 @@ __device__ void block_join(Soft& a, float c, float* scratch /* 2 * kWarpsPer */)
   __syncthreads();
   if (threadIdx.x % 32 == 0) {
     scratch[threadIdx.x / 32] = a.m;
-    scratch[kWarpsPer + threadIdx.x / 32] = a.l;
+    scratch[(NT / 32) + threadIdx.x / 32] = a.l;
   }
   __syncthreads();
   a = Soft();
-  for (int w = 0; w < kWarpsPer; ++w) a.join(scratch[w], scratch[kWarpsPer + w], c);
+  for (int w = 0; w < (NT / 32); ++w) a.join(scratch[w], scratch[(NT / 32) + w], c);
 }
 
-template <int N>
-__device__ void block_sum(double (&v)[N], double* scratch /* N * kWarpsPer */) {
+template <int NT, int N>
+__device__ void block_sum(double (&v)[N], double* scratch /* N * NT / 32 */) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -143,12 +148,12 @@ __device__ void block_sum(double (&v)[N], double* scratch /* N * kWarpsPer */) {
   __syncthreads();
   if (threadIdx.x % 32 == 0)
 #pragma unroll
-    for (int n = 0; n < N; ++n) scratch[n * kWarpsPer + threadIdx.x / 32] = v[n];
+    for (int n = 0; n < N; ++n) scratch[n * (NT / 32) + threadIdx.x / 32] = v[n];
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     v[n] = 0.0;
-    for (int w = 0; w < kWarpsPer; ++w) v[n] += scratch[n * kWarpsPer + w];
+    for (int w = 0; w < (NT / 32); ++w) v[n] += scratch[n * (NT / 32) + w];
   }
 }
 
@@ -168,13 +173,14 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-__device__ int block_count(int mine, int* scratch /* kWarpsPer */) {
+template <int NT>
+__device__ int block_count(int mine, int* scratch /* NT / 32 */) {
   const int w = __reduce_add_sync(0xffffffffu, mine);
   __syncthreads();
   if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = w;
   __syncthreads();
   int n = 0;
-  for (int i = 0; i < kWarpsPer; ++i) n += scratch[i];
+  for (int i = 0; i < (NT / 32); ++i) n += scratch[i];
   return n;
 }
 
@@ -189,13 +195,13 @@ __device__ uint32_t kth_key(int k, F&& count) {
   return t;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __restrict__ x, int64_t stride, int V, int k,
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) top_logits_kernel(const T* __restrict__ x, int64_t stride, int V, int k,
                                                               float inv_tau, T* __restrict__ values,
                                                               int64_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ uint64_t list[kCandidates];
-  __shared__ float red[2 * kWarpsPer];
-  __shared__ int counts[kWarpsPer];
+  __shared__ float red[2 * (NT / 32)];
+  __shared__ int counts[(NT / 32)];
   __shared__ int n_list;
   const T* row = x + (int64_t)blockIdx.x * stride;
   const float c = inv_tau * kLog2eF;
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
   Soft soft;
   uint32_t best[2] = {0, 0};  // the two groups of this thread; 0 is below the key of every number
   int turn = 0;
-  for_row<T>(row, V, [&](int, auto& v) {
+  for_row<NT, T>(row, V, [&](int, auto& v) {
     if constexpr (std::is_same_v<std::decay_t<decltype(v)>, float>) {
       soft.add(v, c);
       if (v != v) soft.l = v;
@@ -218,8 +224,8 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
       turn ^= 1;
     }
   });
-  block_join(soft, c, red);
-  const bool nan = block_count(best[0] == 0xffffffffu || best[1] == 0xffffffffu, counts) > 0;
+  block_join<NT>(soft, c, red);
+  const bool nan = block_count<NT>(best[0] == 0xffffffffu || best[1] == 0xffffffffu, counts) > 0;
   if (threadIdx.x == 0)
     lse[blockIdx.x] = nan ? NAN : soft.m == INFINITY ? INFINITY : soft.l == 0.f ? -INFINITY : fmaf(soft.m, inv_tau, logf(soft.l));
 
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
     }
   };
   auto scan = [&](uint32_t least, float least_value) {
-    for_row<T>(row, V, [&](int at, auto& v) {
+    for_row<NT, T>(row, V, [&](int at, auto& v) {
       if constexpr (std::is_same_v<std::decay_t<decltype(v)>, float>) {
         collect(at, v, least);
       } else if (!(max8_nan(v) < least_value)) {  // one of them may reach the bound, or is NaN
@@ -258,13 +264,13 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
     // too many: the exact k-th key, everything above it, and of its equals the first in order
     const uint32_t exact = kth_key(k, [&](uint32_t t) {
       int mine = 0;
-      for_row<T>(row, V, [&](int, auto& v) {
+      for_row<NT, T>(row, V, [&](int, auto& v) {
         if constexpr (std::is_same_v<std::decay_t<decltype(v)>, float>) mine += key_of(v) >= t;
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e) mine += key_of(v[e]) >= t;
       });
-      return block_count(mine, counts);
+      return block_count<NT>(mine, counts);
     });
     __syncthreads();
     if (threadIdx.x == 0) n_list = 0;
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
     __syncthreads();
     n = n_list;  // less than k
     int found = 0;
-    for (int base = 0; base < V && n + found < k; base += kThreads) {
+    for (int base = 0; base < V && n + found < k; base += NT) {
       const int at = base + (int)threadIdx.x;
       const bool equal = at < V && key_of(to_f32(row[at])) == exact;
       const uint32_t votes = __ballot_sync(0xffffffffu, equal);
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
       if (threadIdx.x % 32 == 0) counts[threadIdx.x / 32] = __popc(votes);
       __syncthreads();
       int before = found + __popc(votes & ((1u << (threadIdx.x % 32)) - 1)), all = 0;
-      for (int w = 0; w < kWarpsPer; ++w) {
+      for (int w = 0; w < (NT / 32); ++w) {
         if (w < (int)threadIdx.x / 32) before += counts[w];
         all += counts[w];
       }
@@ -291,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __rest
     n = k;
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t me = list[i];
     int before = 0;
     for (int j = 0; j < n; ++j) before += list[j] > me;
@@ -320,11 +326,11 @@ __device__ __forceinline__ int index_at(const DistillParams& p, int64_t i) {
   return at >= 0 && at < p.V ? (int)at : -1;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams p, double* __restrict__ row_loss) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) distill_fwd_kernel(DistillParams p, double* __restrict__ row_loss) {
   extern __shared__ uint32_t given[];  // a bit per class, where there is a rest
-  __shared__ double sums[4 * kWarpsPer];
-  __shared__ float red[2 * kWarpsPer];
+  __shared__ double sums[4 * (NT / 32)];
+  __shared__ float red[2 * (NT / 32)];
   const int r = blockIdx.x;
   const double w = p.weights != nullptr ? (double)p.weights[r] : 1.0;
   if (w == 0.0) {
@@ -339,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams 
   Soft gen, top;
   double distinct = 0.0;
   if (tail) {
-    for (int i = threadIdx.x; i < (p.V + 31) / 32; i += kThreads) given[i] = 0;
+    for (int i = threadIdx.x; i < (p.V + 31) / 32; i += NT) given[i] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < p.K; j += kThreads) {
+    for (int j = threadIdx.x; j < p.K; j += NT) {
       const int at = index_at(p, first + j);
       if (at < 0) continue;
       if (atomicOr(&given[at / 32], 1u << (at % 32)) >> (at % 32) & 1) continue;
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams 
     }
     __syncthreads();
   }
-  for_row<T>(row, p.V, [&](int at, auto& v) {
+  for_row<NT, T>(row, p.V, [&](int at, auto& v) {
     if constexpr (std::is_same_v<std::decay_t<decltype(v)>, float>) {
       if (tail && given[at / 32] >> (at % 32) & 1) return;
       gen.add(v, c);
@@ -369,31 +375,31 @@ __global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams 
       gen.add8(v, max8_nan(v), c);
     }
   });
-  block_join(gen, c, red);
+  block_join<NT>(gen, c, red);
   Soft all = gen;
   if (tail) {
-    block_join(top, c, red);
+    block_join<NT>(top, c, red);
     all.join(top.m, top.l, c);
   }
   // the teacher's side: log-sum-exp of the given values, unless that of all of them came along
   double lse_t = tail ? (double)p.lse[r] : 0.0;
   if (!tail) {
     float m = -INFINITY;
-    for (int j = threadIdx.x; j < p.K; j += kThreads)
+    for (int j = threadIdx.x; j < p.K; j += NT)
       if (index_at(p, first + j) >= 0) m = fmaxf(m, (float)value_at(p, first + j));
     Soft mm;
     mm.m = m;
-    block_join(mm, 0.f, red);
+    block_join<NT>(mm, 0.f, red);
     const double ref = mm.m == -INFINITY ? 0.0 : (double)mm.m * inv_tau_t;
     double sum[1] = {0.0};
-    for (int j = threadIdx.x; j < p.K; j += kThreads)
+    for (int j = threadIdx.x; j < p.K; j += NT)
       if (index_at(p, first + j) >= 0) sum[0] += exp(value_at(p, first + j) * inv_tau_t - ref);
-    block_sum<1>(sum, sums);
+    block_sum<NT, 1>(sum, sums);
     lse_t = sum[0] == 0.0 ? INFINITY : ref + log(sum[0]);  // nothing given: every share is 0
   }
   const double log_all = log((double)all.l);
   double acc[3] = {0.0, 0.0, distinct};  // loss, mass, classes
-  for (int j = threadIdx.x; j < p.K; j += kThreads) {
+  for (int j = threadIdx.x; j < p.K; j += NT) {
     const int at = index_at(p, first + j);
     if (at < 0) continue;
     const double log_p = value_at(p, first + j) * inv_tau_t - lse_t, share = exp(log_p);
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams 
     if (share != 0.0) acc[0] += share * (log_p - log_q);
     acc[1] += share;
   }
-  block_sum<3>(acc, sums);
+  block_sum<NT, 3>(acc, sums);
   if (threadIdx.x != 0) return;
   double loss = acc[0], mass = acc[1], coef = mass;
   if (tail) {
@@ -423,17 +429,18 @@ __global__ void __launch_bounds__(kThreads, 3) distill_fwd_kernel(DistillParams 
 }
 
 // sum of the rows' losses in order, over norm
-__global__ void __launch_bounds__(kThreads) distill_sum_kernel(const double* __restrict__ rows, int R, double norm,
+template <int NT>
+__global__ void __launch_bounds__(NT) distill_sum_kernel(const double* __restrict__ rows, int R, double norm,
                                                                float* __restrict__ out) {
-  __shared__ double sums[kWarpsPer];
+  __shared__ double sums[(NT / 32)];
   double s[1] = {0.0};
-  for (int i = threadIdx.x; i < R; i += kThreads) s[0] += rows[i];
-  block_sum<1>(s, sums);
+  for (int i = threadIdx.x; i < R; i += NT) s[0] += rows[i];
+  block_sum<NT, 1>(s, sums);
   if (threadIdx.x == 0) *out = (float)(s[0] / norm);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_bwd_kernel(DistillParams p, const float* __restrict__ grad,
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const float* __restrict__ grad,
                                                                T* __restrict__ ds) {
   __shared__ int at_of[kMaxGiven];
   __shared__ float share_of[kMaxGiven];
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(DistillParams p, 
   const double w = p.weights != nullptr ? (double)p.weights[r] : 1.0;
   const int vec_ahead = min(p.V, (int)((8 - (reinterpret_cast<uintptr_t>(out) / sizeof(T)) % 8) % 8));
   if (w == 0.0) {
-    for (int i = threadIdx.x; i < p.V; i += kThreads) out[i] = from_f32<T>(0.f);
+    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(0.f);
     return;
   }
   const T* row = (const T*)p.s + r * p.s_row;
@@ -455,14 +462,14 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(DistillParams p, 
   const float ref = m == -INFINITY ? 0.f : m;
   // a rest of no mass at all has no gradient
   const float coef = st[kGenL] == 0.0 ? 0.f : (float)(scale * st[kGenCoef] / st[kGenL]);
-  for (int j = threadIdx.x; j < p.K; j += kThreads) {
+  for (int j = threadIdx.x; j < p.K; j += NT) {
     at_of[j] = index_at(p, first + j);
     share_of[j] = at_of[j] < 0 ? 0.f : (float)exp(value_at(p, first + j) * inv_tau_t - st[kLseT]);
   }
   const bool same = (reinterpret_cast<uintptr_t>(row) / sizeof(T)) % 8 == (reinterpret_cast<uintptr_t>(out) / sizeof(T)) % 8;
   if (same) {
     const int vecs = (p.V - vec_ahead) / 8;
-    for (int i = threadIdx.x; i < vecs; i += kThreads) {
+    for (int i = threadIdx.x; i < vecs; i += NT) {
       float v[8];
       unpack8<T>(load_raw8<T>(row + vec_ahead + i * 8), v);
 #pragma unroll
@@ -470,16 +477,16 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(DistillParams p, 
       store8<T>(out + vec_ahead + i * 8, v);
     }
     const int end = vec_ahead + vecs * 8;
-    for (int i = threadIdx.x; i < vec_ahead + (p.V - end); i += kThreads) {
+    for (int i = threadIdx.x; i < vec_ahead + (p.V - end); i += NT) {
       const int at = i < vec_ahead ? i : end + i - vec_ahead;
       out[at] = from_f32<T>(ex2((to_f32(row[at]) - ref) * c) * coef);
     }
   } else {
-    for (int i = threadIdx.x; i < p.V; i += kThreads) out[i] = from_f32<T>(ex2((to_f32(row[i]) - ref) * c) * coef);
+    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(ex2((to_f32(row[i]) - ref) * c) * coef);
   }
   __syncthreads();  // the given classes replace what the pass wrote in their places
   const double inv_l = 1.0 / st[kAllL], all_m = st[kAllM], mass = st[kMass];
-  for (int j = threadIdx.x; j < p.K; j += kThreads) {
+  for (int j = threadIdx.x; j < p.K; j += NT) {
     const int at = at_of[j];
     if (at < 0) continue;
     bool again = false;
@@ -508,8 +515,11 @@ cudaError_t top_logits_rows(const void* x, int64_t stride, int R, int V, int k, 
                             int64_t* indices, float* lse, SequenceType type, cudaStream_t stream) {
   by_type(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    top_logits_kernel<T><<<R, kThreads, 0, stream>>>((const T*)x, stride, V, k, (float)(1.0 / tau), (T*)values, indices,
-                                                    lse);
+    auto go = [&](auto kernel, int threads) {
+      kernel<<<R, threads, 0, stream>>>((const T*)x, stride, V, k, (float)(1.0 / tau), (T*)values, indices, lse);
+    };
+    if (threads_for(R, V) == kMany) go(top_logits_kernel<T, kMany>, kMany);
+    else go(top_logits_kernel<T, kFew>, kFew);
   });
   return cudaGetLastError();
 }
@@ -520,20 +530,25 @@ cudaError_t distill_fwd(const DistillParams& p, double* row_loss, float* loss, c
     const size_t smem = p.lse != nullptr ? (size_t)(p.V + 31) / 32 * 4 : 0;
     by_type(p.type, [&](auto* tag) {
       using T = std::remove_pointer_t<decltype(tag)>;
-      if (smem > 32 * 1024)
-        status = cudaFuncSetAttribute(distill_fwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (status == cudaSuccess) distill_fwd_kernel<T><<<p.R, kThreads, smem, stream>>>(p, row_loss);
+      auto go = [&](auto kernel, int threads) {
+        if (smem > 32 * 1024)
+          status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (status == cudaSuccess) kernel<<<p.R, threads, smem, stream>>>(p, row_loss);
+      };
+      if (threads_for(p.R, p.V) == kMany) go(distill_fwd_kernel<T, kMany>, kMany);
+      else go(distill_fwd_kernel<T, kFew>, kFew);
     });
   }
   if (status != cudaSuccess) return status;
-  distill_sum_kernel<<<1, kThreads, 0, stream>>>(row_loss, p.R, p.norm, loss);
+  distill_sum_kernel<kMany><<<1, kMany, 0, stream>>>(row_loss, p.R, p.norm, loss);
   return cudaGetLastError();
 }
 
 cudaError_t distill_bwd(const DistillParams& p, const float* grad, void* ds, cudaStream_t stream) {
   by_type(p.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    distill_bwd_kernel<T><<<p.R, kThreads, 0, stream>>>(p, grad, (T*)ds);
+    if (threads_for(p.R, p.V) == kMany) distill_bwd_kernel<T, kMany><<<p.R, kMany, 0, stream>>>(p, grad, (T*)ds);
+    else distill_bwd_kernel<T, kFew><<<p.R, kFew, 0, stream>>>(p, grad, (T*)ds);
   });
   return cudaGetLastError();
 }
