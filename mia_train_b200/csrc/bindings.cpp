@@ -110,7 +110,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
                             const at::Tensor& k_bounds, double scale, const OptTensor& items, const OptTensor& pieces,
                             int64_t max_queries, int64_t tile_pairs, int64_t pairs);
 std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
-                                          const at::Tensor& freq, bool interleaved, double amplitude);
+                                          const OptTensor& freq, bool interleaved, double amplitude);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& x, int64_t k, double tau);
 at::Tensor top_logit_distillation(const at::Tensor& s, const at::Tensor& values, const at::Tensor& indices,
                                   const OptTensor& teacher_lse, const OptTensor& weights, double tau,

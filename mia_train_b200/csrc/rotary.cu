@@ -3,7 +3,7 @@
 //   angle[t, p] = sum_a position[t, a] F[a, p]
 //   y1 = amplitude (x1 cos - x2 sin),  y2 = amplitude (x2 cos + x1 sin)   for every pair (x1, x2) of the head
 //
-// with the pairs (p, p + P) ("half") or (2 p, 2 p + 1) ("interleaved") of the first 2 P channels; the others are
+// (or the angles themselves are given), with the pairs (p, p + P) ("half") or (2 p, 2 p + 1) ("interleaved") of the first 2 P channels; the others are
 // copied. The gradient of x is the rotation of dy by the negative angles, that of the table
 // dF[a, p] = sum_t position[t, a] sum_heads (dy2 y1 - dy1 y2).
 //
@@ -57,7 +57,12 @@ __device__ __forceinline__ uint2 frequency(const RotaryParams& p, int i) {
 // (cos, sin) of the token's angle of pair i, times the amplitude; `at` is the token's row of positions
 __device__ __forceinline__ float2 turn(const RotaryParams& p, const uint2* table, int64_t at, int i) {
   float half;  // in half turns
-  if (p.pos_type <= 1) {
+  if (p.freq == nullptr) {
+    const float x = ((const float*)p.pos)[at + i];
+    const float hi = 0.15915493667125702f, lo = 6.4206382432985265e-09f;  // 1 / (2 pi) as two fp32
+    const float w = x * hi, whole = w - rintf(w) + fmaf(x, lo, fmaf(x, hi, -w));
+    half = 2.f * (whole - rintf(whole));
+  } else if (p.pos_type <= 1) {
     uint64_t u = 0;
     for (int a = 0; a < p.axes; ++a) {
       const uint2 f = table[a * p.P + i];
@@ -120,12 +125,14 @@ __global__ void __launch_bounds__(kThreads, kLearn ? 2 : 3) rotary_kernel(const 
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) sum[a][e] = 0.f;
 
-  for (int i = threadIdx.x; i < p.axes * p.P; i += kThreads) table[i] = frequency(p, i);
-  __syncthreads();
+  if (p.freq != nullptr) {
+    for (int i = threadIdx.x; i < p.axes * p.P; i += kThreads) table[i] = frequency(p, i);
+    __syncthreads();
+  }
   for (int64_t token = (int64_t)blockIdx.x * slots + slot; slot < slots && token < p.tokens;
        token += (int64_t)gridDim.x * slots) {
     const int64_t b = token / p.T, t = token - b * p.T;
-    const int64_t at = position_row(p, token) * p.axes;
+    const int64_t at = position_row(p, token) * (p.freq == nullptr ? p.P : p.axes);
     float2 cs[kPairs];
     float g[kPairs];
 #pragma unroll

@@ -60,7 +60,7 @@ struct RotaryParams {
   const void* pos;
   int pos_type;   // 0: int64, 1: int32, 2: fp32, 3: fp64
   int64_t pos_b;  // 0 where all rows of the batch share one row of positions
-  const void* freq;
+  const void* freq;  // (axes, P), or null: then pos holds the angles (.., P) in fp32
   int freq64;
   int axes, P, D, T, Hq, Hk;
   int64_t tokens;  // B * T

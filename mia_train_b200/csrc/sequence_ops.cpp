@@ -179,7 +179,7 @@ bool in_vectors(const at::Tensor& x) {
 
 // q, k (B, T, H, D) -> yq, yk; `inverse` turns back. With xq and xk (the forward pass's inputs, where q and k are
 // gradients) also dfreq (axes, P) fp32. k may have no heads.
-void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const at::Tensor& freq,
+void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const OptTensor& freq,
             bool interleaved, double amplitude, bool inverse, const at::Tensor& yq, const at::Tensor& yk,
             const OptTensor& xq, const OptTensor& xk, const OptTensor& dfreq) {
   const bool learn = dfreq.has_value();
@@ -200,10 +200,11 @@ void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& position
   const at::ScalarType pt = positions.scalar_type();
   p.pos_type = pt == at::kLong ? 0 : pt == at::kInt ? 1 : pt == at::kFloat ? 2 : 3;
   p.pos_b = positions.size(0) == 1 ? 0 : 1;
-  p.freq = freq.data_ptr();
-  p.freq64 = freq.scalar_type() == at::kDouble;
-  p.axes = (int)freq.size(0);
-  p.P = (int)freq.size(1);
+  p.freq = freq.has_value() ? freq->data_ptr() : nullptr;
+  p.freq64 = freq.has_value() && freq->scalar_type() == at::kDouble;
+  p.axes = freq.has_value() ? (int)freq->size(0) : 1;
+  p.P = (int)positions.size(2);
+  if (freq.has_value()) p.P = (int)freq->size(1);
   p.D = (int)q.size(3);
   p.T = (int)q.size(1);
   p.Hq = (int)q.size(2);
@@ -230,17 +231,18 @@ void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& position
 }
 
 struct RotaryNode : Function<RotaryNode> {
-  // q, k (B, T, H, D); positions (1 or B, T, axes); freq (axes, P)
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
-                               const at::Tensor& positions, const at::Tensor& freq, bool interleaved, double amplitude) {
+  // q, k (B, T, H, D); positions (1 or B, T, axes) and freq (axes, P), or angles (1 or B, T, P) alone
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                               const OptTensor& freq, bool interleaved, double amplitude) {
     BelowAutograd below;
     const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
-    const at::Tensor qc = heads(q), kc = heads(k), pos = positions.contiguous(), f = freq.contiguous();
+    const at::Tensor qc = heads(q), kc = heads(k), pos = positions.contiguous();
+    const OptTensor f = freq.has_value() ? OptTensor(freq->contiguous()) : OptTensor();
     at::Tensor out = at::empty({B, T, Hq + Hk, D}, q.options());
     at::Tensor yq = out.narrow(2, 0, Hq), yk = out.narrow(2, Hq, Hk);
     rotate(qc, kc, pos, f, interleaved, amplitude, false, yq, yk, {}, {}, {});
-    const bool learn = freq.requires_grad();
-    ctx->save_for_backward({pos, f, learn ? qc : at::Tensor(), learn ? kc : at::Tensor()});
+    const bool learn = freq.has_value() && freq->requires_grad();
+    ctx->save_for_backward({pos, value(f), learn ? qc : at::Tensor(), learn ? kc : at::Tensor()});
     auto& d = ctx->saved_data;
     d["interleaved"] = interleaved;
     d["amplitude"] = amplitude;
@@ -270,7 +272,7 @@ struct RotaryNode : Function<RotaryNode> {
       xk = s[3];
       df = at::empty(s[1].sizes(), one.options().dtype(at::kFloat));
     }
-    rotate(gq, gk, s[0], s[1], d["interleaved"].toBool(), d["amplitude"].toDouble(), true, dq, dk, xq, xk, df);
+    rotate(gq, gk, s[0], opt(s[1]), d["interleaved"].toBool(), d["amplitude"].toDouble(), true, dq, dk, xq, xk, df);
     at::Tensor dfreq;
     if (df.has_value()) dfreq = df->to(s[1].scalar_type());
     return {dq, dk, at::Tensor(), dfreq, at::Tensor(), at::Tensor()};
@@ -349,7 +351,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
 }
 
 std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
-                                          const at::Tensor& freq, bool interleaved, double amplitude) {
+                                          const OptTensor& freq, bool interleaved, double amplitude) {
   variable_list out = RotaryNode::apply(q, k, positions, freq, interleaved, amplitude);
   return {out[0], out[1]};
 }

@@ -11,6 +11,10 @@ attention core the native fused RoPE+attention kernel; the rotation pairs channe
 i.e. `rope_rotate_half`. `use_fa4` is accepted for config compatibility; FlashAttention-4 is not
 part of this framework, so requesting it is an error.
 
+With `packed_crops` set, `forward_list` runs the attention of all crops in one call on their tokens laid end to
+end (`ops.packed_attention`), instead of one call per crop size; fp32 on CUDA, angles that are learned and head
+sizes that the packed kernel does not take keep the crop-wise calls.
+
 `qk_norm` adds an RMS norm over every query and key head (`q_norm`, `k_norm`), applied with the rotation in
 one kernel. `proj_drop` > 0 drops elements of the projected output in training, fused with the residual add.
 """
@@ -18,6 +22,7 @@ one kernel. `proj_drop` > 0 drops elements of the projected output in training, 
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 from collections.abc import Iterator
 from typing import Any
@@ -29,7 +34,9 @@ import torch.nn.functional as F
 from ...ops._native import reference_math
 from ...ops.attention import rope_attention
 from ...ops.dropout import dropout
-from ...ops.qk_norm import qk_norm_rope_attention
+from ...ops.packed_attention import MAX_HEAD_DIM, PackedSequences, packed_attention
+from ...ops.qk_norm import qk_norm_rope, qk_norm_rope_attention
+from ...ops.rotary import rotary
 from ...parallel.tensor_parallel import rope_to_tp
 from ..common.attention import flash4_status, head_norms
 from ..common.batched_tokens import cat_keep_shapes, uncat_with_shapes
@@ -75,7 +82,15 @@ def half_pairs(head_dim: int, device: torch.device) -> torch.Tensor:
     return torch.stack([idx, idx + half], dim=1).to(device)
 
 
+@functools.lru_cache(maxsize=64)
+def _crop_sequences(shapes: tuple[tuple[int, int], ...], device: torch.device) -> PackedSequences:
+    """The sequences of crops of `shapes` (samples, tokens), which a run meets again in every step."""
+    return PackedSequences([n for b, n in shapes for _ in range(b)], device=device)
+
+
 class SelfAttention(nn.Module):
+    packed_crops = False
+
     def __init__(
         self,
         dim: int,
@@ -156,12 +171,55 @@ class SelfAttention(nn.Module):
         out = self.compute_attention(self._qkv(x), attn_bias=attn_bias, rope=rope)
         return self.project(out, residual=residual, gamma=gamma)
 
+    # -- crops packed end to end --------------------------------------------------------------
+    def _packs(self, qkv: torch.Tensor, rope_list) -> bool:
+        if not self.packed_crops or len(rope_list) < 2:
+            return False
+        if qkv.is_cuda and (qkv.dtype not in (torch.bfloat16, torch.float16) or self.head_dim % 8
+                            or self.head_dim > MAX_HEAD_DIM):
+            return False
+        given = [isinstance(r, RopeTables) for r in rope_list]
+        if not all(given):
+            return all(r is None for r in rope_list)
+        return not any(r.angles.requires_grad for r in rope_list)
+
+    def _packed_angles(self, shapes: tuple[tuple[int, int], ...], rope_list) -> torch.Tensor:
+        """(sum of tokens, P) angles: 0 for prefix tokens, the same for every sample of a crop."""
+        kept = rope_list[0].packed
+        if shapes not in kept:
+            rows = []
+            for (b, n), rope in zip(shapes, rope_list, strict=True):
+                one = F.pad(rope.angles.float(), (0, 0, n - rope.angles.shape[-2], 0))
+                rows.append(one.expand(b, *one.shape).reshape(b * n, -1))
+            kept[shapes] = torch.cat(rows)
+        return kept[shapes]
+
+    def _attend_packed(self, qkv: torch.Tensor, shapes: tuple[tuple[int, int], ...], rope_list) -> torch.Tensor:
+        """(tokens, 3 C) projections of all crops -> (tokens, C)."""
+        c = qkv.shape[-1] // 3
+        q, k, v = qkv.reshape(qkv.shape[0], 3, self.num_heads, c // self.num_heads).unbind(1)
+        angles = self._packed_angles(shapes, rope_list) if rope_list[0] is not None else None
+        if self.q_norm is not None:
+            qw, kw, eps = head_norms(self)
+            pairs = self._pairs_on(qkv.device) if angles is not None else None
+            q, k = (x.squeeze(0) for x in qk_norm_rope(q[None], k[None], qw, kw, angles[None] if angles is not None else None,
+                                                       pairs, eps))
+        elif angles is not None:
+            q, k = rotary(q, k, angles, None)
+        return packed_attention(q, k, v, _crop_sequences(shapes, qkv.device), self.scale).reshape(-1, c)
+
     def forward_list(self, x_list, attn_bias=None, rope_list=None, residual_list=None, gamma=None) -> list[torch.Tensor]:
         assert len(x_list) == len(rope_list)
         flat, shapes, counts = cat_keep_shapes(x_list)
-        qkv_list = uncat_with_shapes(self._qkv(flat), shapes, counts)
-        outs = [self.compute_attention(q, attn_bias=attn_bias, rope=r) for q, r in zip(qkv_list, rope_list, strict=True)]
-        flat, shapes, counts = cat_keep_shapes(outs)
+        qkv = self._qkv(flat)
+        if attn_bias is None and self._packs(qkv, rope_list):
+            flat = self._attend_packed(qkv, tuple((s[0], s[1]) for s in shapes), rope_list)
+            shapes = [torch.Size((*s[:-1], flat.shape[-1])) for s in shapes]
+        else:
+            qkv_list = uncat_with_shapes(qkv, shapes, counts)
+            outs = [self.compute_attention(q, attn_bias=attn_bias, rope=r)
+                    for q, r in zip(qkv_list, rope_list, strict=True)]
+            flat, shapes, counts = cat_keep_shapes(outs)
         res = None
         if residual_list is not None:
             res, _, _ = cat_keep_shapes(residual_list)

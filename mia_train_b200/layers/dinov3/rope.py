@@ -30,11 +30,14 @@ class RopeTables:
     Not a tuple on purpose: FSDP rebuilds tuple forward arguments element by element (and may cast
     them), which would lose the angles; an object of this class passes through untouched."""
 
-    __slots__ = ("angles", "_pair")
+    __slots__ = ("angles", "_pair", "packed")
 
     def __init__(self, angles: torch.Tensor) -> None:
         self.angles = angles
         self._pair: tuple[torch.Tensor, torch.Tensor] | None = None
+        # angles of every token of a list of crops, by the crops' shapes: made by the first block that packs
+        # them and used by the others of this forward pass (the tables themselves are made anew in each)
+        self.packed: dict[tuple, torch.Tensor] = {}
 
     def _tables(self) -> tuple[torch.Tensor, torch.Tensor]:
         if self._pair is None:

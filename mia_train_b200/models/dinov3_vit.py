@@ -55,6 +55,7 @@ class DinoVisionTransformer(DinoVisionTransformer3D):
         device: Any | None = None,
         qk_norm: bool = False,
         drop_rate: float = 0.0,
+        packed_crops: bool = False,
     ) -> None:
         super().__init__(
             img_size=img_size, patch_size=patch_size, in_chans=in_chans, pos_embed_rope_type="vanilla",
@@ -69,7 +70,7 @@ class DinoVisionTransformer(DinoVisionTransformer3D):
             ffn_layer=ffn_layer, ffn_bias=ffn_bias, proj_bias=proj_bias, n_storage_tokens=n_storage_tokens,
             mask_k_bias=mask_k_bias, use_fa4=use_fa4, untie_cls_and_patch_norms=untie_cls_and_patch_norms,
             untie_global_and_local_cls_norm=untie_global_and_local_cls_norm, qk_norm=qk_norm, drop_rate=drop_rate,
-            device=device,
+            packed_crops=packed_crops, device=device,
         )
 
     def _make_patch_embed(self, img_size, patch_size, in_chans, embed_dim) -> nn.Module:

@@ -16,6 +16,8 @@ Differences:
   patch grid, with the class and register tokens visible to every window and attending globally;
   every `global_every`-th block attends globally. `window_size = 0` (the default) is the
   reference's all-global model.
+* New: `packed_crops` attends to crops of all sizes in one call (`ops.packed_attention`) where a list of crops runs
+  through the blocks together; the sequence-parallel modes, which take crop by crop, are as without it.
 * New: `tensor_parallel_plan()` -- colwise qkv / fc1 / w1 / w2 and rowwise proj / fc2 / w3, so
   `[parallelism].tp > 1` works on this model.
 """
@@ -102,6 +104,7 @@ class DinoVisionTransformer3D(BaseModel):
         device: Any | None = None,
         qk_norm: bool = False,
         drop_rate: float = 0.0,
+        packed_crops: bool = False,
     ) -> None:
         super().__init__()
         if norm_layer not in norm_layer_dict:
@@ -148,6 +151,8 @@ class DinoVisionTransformer3D(BaseModel):
             )
             for _ in range(depth)
         )
+        for blk in self.blocks:
+            blk.attn.packed_crops = packed_crops
         self.chunked_blocks = False
         self.norm = norm_cls(embed_dim)
         self.untie_cls_and_patch_norms = untie_cls_and_patch_norms

@@ -8,9 +8,10 @@
 
 with the pairs (p, p + P) for `layout="half"` and (2 p, 2 p + 1) for `"interleaved"`; the other channels are copied.
 `positions` are integers or floats, one per token, (T) or (B, T), with `frequencies` (P), or one coordinate per axis,
-(T, A) or (B, T, A), with `frequencies` (A, P) and A <= 4. The angles are formed and reduced to a turn in 64 bits, so
-that far positions lose nothing; the rest is fp32, rounded once. q and k may be strided views of a packed projection;
-the outputs share one contiguous buffer. `k` may be None. Gradients go to q, k and the frequencies, not to positions.
+(T, A) or (B, T, A), with `frequencies` (A, P) and A <= 4. Without frequencies `positions` holds the angles themselves,
+fp32 (T, P) or (B, T, P). Angles are reduced to a turn with at least 48 bits, of integer positions with 53, so that
+those of far positions are as good as of near ones; the rest is fp32, rounded once. q and k may be strided views of a packed projection;
+the outputs share one contiguous buffer. `k` may be None. Gradients go to q, k and the frequencies, not to positions or angles.
 
 `rotary_frequencies(rotary_dim, base, scaling=...)` gives the frequencies base^(-p / P) in fp64 and the amplitude:
 
@@ -95,7 +96,7 @@ def rotary(
     q: torch.Tensor,
     k: torch.Tensor | None,
     positions: torch.Tensor,
-    frequencies: torch.Tensor,
+    frequencies: torch.Tensor | None,
     *,
     layout: str = "half",
     amplitude: float = 1.0,
@@ -113,19 +114,25 @@ def rotary(
                          f"{q.device} and {k.dtype} {tuple(k.shape)} on {k.device}")
     batched = q.dim() == 4
     b, t, hq, d = q.shape if batched else (1, *q.shape)
-    if frequencies.dim() not in (1, 2) or frequencies.dtype not in (torch.float32, torch.float64):
+    if frequencies is None:
+        if positions.dim() not in (2, 3) or positions.dtype != torch.float32:
+            raise ValueError(f"angles must be fp32 (T, P) or (B, T, P), got {positions.dtype} {tuple(positions.shape)}")
+        multi, table, axes, p = True, None, positions.shape[-1], positions.shape[-1]
+    elif frequencies.dim() not in (1, 2) or frequencies.dtype not in (torch.float32, torch.float64):
         raise ValueError(f"frequencies must be fp32 or fp64 (P) or (A, P), got {frequencies.dtype} {tuple(frequencies.shape)}")
-    multi = frequencies.dim() == 2
-    table = frequencies if multi else frequencies.unsqueeze(0)
-    axes, p = table.shape
-    if not 1 <= axes <= MAX_AXES or 2 * p > d:
+    else:
+        multi = frequencies.dim() == 2
+        table = frequencies if multi else frequencies.unsqueeze(0)
+        axes, p = table.shape
+    if 2 * p > d or (table is not None and not 1 <= axes <= MAX_AXES):
         raise ValueError(f"{axes} axes and {p} pairs: at most {MAX_AXES} axes and {d // 2} pairs of a head of {d}")
     where = positions if multi else positions.unsqueeze(-1)
     if positions.dtype not in _POSITIONS or tuple(where.shape) not in {(t, axes), (1, t, axes), (b, t, axes)}:
         raise ValueError(f"positions must be int32, int64, fp32 or fp64 for {t} tokens of {b} rows and {axes} axes, got "
                          f"{positions.dtype} {tuple(positions.shape)}")
-    if positions.device != q.device or frequencies.device != q.device:
-        raise ValueError(f"q is on {q.device}, positions on {positions.device}, frequencies on {frequencies.device}")
+    if positions.device != q.device or (table is not None and table.device != q.device):
+        raise ValueError(f"q is on {q.device}, positions on {positions.device}, frequencies on "
+                         f"{table.device if table is not None else None}")
     if positions.requires_grad:
         raise ValueError("rotary gives no gradient for positions")
     if where.dim() == 2:
@@ -137,7 +144,7 @@ def rotary(
         if not batched:
             yq, yk = yq.squeeze(0), yk.squeeze(0)
         return yq, (None if k is None else yk)
-    angles = (where.double().unsqueeze(-1) * table.double()).sum(-2)
+    angles = where.double() if table is None else (where.double().unsqueeze(-1) * table.double()).sum(-2)
     if not batched:
         angles = angles.squeeze(0)
     return (_rotate_reference(q, angles, layout, amplitude),

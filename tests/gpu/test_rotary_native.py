@@ -159,3 +159,19 @@ def test_changed_operands_and_second_derivatives_are_refused():
         torch.autograd.grad(y, leaf, dq, create_graph=True)
     y, _ = rotary(leaf, None, positions, freq)  # linear in q: a constant gradient is returned
     torch.autograd.grad(y, leaf, dq, create_graph=True)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("far", [1.0, 300.0, 1e5])
+def test_given_angles(far, dtype, layout):
+    """Angles in radians, reduced from their fp32 value: 2^-48 of it is lost."""
+    q, k, _, _, dq, dk = _case(2, 40, 3, 1, 64, 16, 1, dtype)
+    angles = far * torch.randn(1, 40, 16, device=DEV)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k)]
+    y = rotary(*leaves, angles, None, layout=layout)
+    grads = torch.autograd.grad(y, leaves, (dq, dk))
+    eye = torch.eye(16, device=DEV)
+    for got, x, turned in ((y[0], q, angles), (y[1], k, angles), (grads[0], dq, -angles), (grads[1], dk, -angles)):
+        want = _turn(x.double(), turned, eye, layout, 1.0)
+        _within(got, want, 16 * U * 2 * x.double().abs().amax(-1, keepdim=True), dtype)

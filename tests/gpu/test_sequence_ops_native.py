@@ -1,0 +1,71 @@
+"""Rotation, packed attention and distillation together, as a step on crops of several sizes runs them, on the GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover - collected on CPU, skipped there
+    pytest.skip("needs CUDA", allow_module_level=True)
+
+from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D  # noqa: E402
+from mia_train_b200.ops._native import reference_math  # noqa: E402
+from mia_train_b200.ops.distill import top_logit_distillation, top_logits  # noqa: E402
+from mia_train_b200.ops.packed_attention import PackedSequences, packed_attention  # noqa: E402
+from mia_train_b200.ops.rotary import rotary, rotary_frequencies  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+
+
+@pytest.mark.parametrize("kw", [{}, {"qk_norm": True}], ids=str)
+def test_model_with_packed_crops(kw):
+    """bf16 crops of two sizes through two blocks, packed and crop by crop, both against the fp32 model: the two ways round
+    the same quantities (P, the attention's output, dS) to bf16, each time by 2^-9 at most."""
+    kw = dict(img_size=32, patch_size=8, in_chans=1, embed_dim=128, depth=2, num_heads=2, n_storage_tokens=4, **kw)
+    torch.manual_seed(0)
+    plain = DinoVisionTransformer3D(**kw).to(DEV)
+    packed = DinoVisionTransformer3D(packed_crops=True, **kw).to(DEV)
+    packed.load_state_dict(plain.state_dict())
+    crops = [torch.randn(2, 1, 32, 32, 32, device=DEV), torch.randn(6, 1, 16, 16, 16, device=DEV)]
+    outs = []
+    for model, half in ((plain, False), (plain, True), (packed, True)):
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=half):
+            out = model.forward_features(crops, [None, None])
+            # not a function of the norm's mean square, which is 1 whatever the weights
+            loss = sum(o["x_norm_patchtokens"].float().sin().mean() for o in out)
+        # one weight of every kind behind and before the attention
+        some = [model.blocks[0].attn.qkv.weight, model.blocks[0].attn.proj.weight, model.blocks[1].attn.qkv.weight]
+        outs.append([o["x_norm_patchtokens"].detach().float() for o in out] + list(torch.autograd.grad(loss, some)))
+    for i, (exact, a, b) in enumerate(zip(*outs, strict=True)):
+        off = [(x - exact).norm() for x in (a, b)]
+        assert off[1] <= 2 * off[0] + 2.0**-9 * exact.norm(), (i, off, exact.norm())
+
+
+def test_distilling_a_small_encoder_from_stored_logits():
+    """One step: tokens of three sequences rotated, attended to and projected to classes, against a teacher's top
+    logits. The native step against the same operators as PyTorch math in fp32 on the same values."""
+    torch.manual_seed(0)
+    lengths, hq, hk, d, v = [33, 70, 1], 4, 2, 32, 5000
+    t = sum(lengths)
+    x = torch.randn(t, 64, device=DEV)
+    wq = (torch.randn(64, (hq + 2 * hk) * d, device=DEV) / 8).requires_grad_(True)
+    wo = (torch.randn(hq * d, v, device=DEV) / hq / d**0.5).requires_grad_(True)
+    freq, amplitude = rotary_frequencies(d // 2, scaling="yarn", factor=4.0, original_length=64, device=DEV)
+    positions = torch.cat([torch.arange(n, device=DEV) for n in lengths])
+    values, indices, lse = top_logits(torch.randn(t, v, device=DEV), 32)
+
+    def step():
+        h = (x @ wq).view(t, hq + 2 * hk, d)
+        q, k = rotary(h[:, :hq], h[:, hq:hq + hk], positions, freq, layout="interleaved", amplitude=amplitude)
+        o = packed_attention(q, k, h[:, hq + hk:], PackedSequences(lengths, causal=True, device=DEV))
+        loss = top_logit_distillation(o.reshape(t, -1) @ wo, values, indices, teacher_lse=lse, tau=0.5)
+        return loss.detach(), *torch.autograd.grad(loss, (wq, wo))
+
+    got = step()
+    with reference_math():
+        want = step()
+    for a, b in zip(got, want, strict=True):
+        # fp32 throughout: sums of at most 5000 terms, errors of 2^-24 a term growing like their root, few steps deep
+        assert (a - b).norm() <= 2.0**-16 * b.norm()

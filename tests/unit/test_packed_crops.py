@@ -1,0 +1,89 @@
+"""`packed_crops`: all crops of a step in one attention call, on the CPU and in 64 bits (in 32 the first norms, which divide
+by the 0.02 of the initial class token, alone leave some gradients with three digits)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mia_train_b200.models.dinov3_vit import DinoVisionTransformer
+from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D
+
+KW = dict(patch_size=8, in_chans=1, embed_dim=48, depth=2, num_heads=2, n_storage_tokens=2, pos_embed_rope_dtype="fp32")
+
+
+def _pair(cls=DinoVisionTransformer3D, **kw):
+    torch.manual_seed(0)
+    plain = cls(img_size=16, **KW, **kw)
+    packed = cls(img_size=16, packed_crops=True, **KW, **kw)
+    packed.load_state_dict(plain.state_dict())
+    return plain.double(), packed.double()
+
+
+def _same(a, b):
+    """The crop-wise call rotates q and k in 32 bits: sine, cosine, two products and a sum, 4 half steps of 2^-24 of each,
+    which move the scores (below 1 here) and with them the outputs by at most 2^-21 a block; a gradient has twice that
+    from forward and backward pass, in both of the two blocks."""
+    assert (a - b).abs().max() <= 2.0**-19 * a.abs().max()
+
+
+def _crops(rank=3):
+    torch.manual_seed(1)
+    return [torch.randn(2, 1, *(16,) * rank).double(), torch.randn(5, 1, *(8,) * rank).double()]
+
+
+def _features(model, crops, masks=None):
+    out = model.forward_features(crops, masks or [None, None])
+    loss = sum((o["x_norm_patchtokens"].sin().sum() + o["x_norm_clstoken"].square().sum()) for o in out)
+    grads = torch.autograd.grad(loss, [p for p in model.parameters() if p.requires_grad], allow_unused=True)
+    return [o[k] for o in out for k in ("x_norm_patchtokens", "x_norm_clstoken")], grads
+
+
+@pytest.mark.parametrize("kw", [{}, {"qk_norm": True}, {"mask_k_bias": True, "layerscale_init": 0.1},
+                                {"pos_embed_rope_type": "superposition"}], ids=str)
+def test_packed_crops_give_what_separate_calls_give(kw):
+    plain, packed = _pair(**kw)
+    if "mask_k_bias" in kw:
+        for m in (plain, packed):
+            for blk in m.blocks:
+                blk.attn.qkv.bias_mask.fill_(1.0)
+    masks = [torch.tensor([[True, False, True] + [False] * 5] * 2), None]
+    for want, got in zip(*(_features(m, _crops(), masks) for m in (plain, packed)), strict=True):
+        for a, b in zip(want, got, strict=True):
+            assert (a is None) == (b is None)
+            if a is not None:
+                _same(a, b)
+
+
+def test_packed_crops_of_the_2d_model_and_one_crop_size():
+    plain, packed = _pair(DinoVisionTransformer)
+    for want, got in zip(_features(plain, _crops(2))[0], _features(packed, _crops(2))[0], strict=True):
+        _same(want, got)
+    x = _crops(2)[0]
+    assert torch.equal(plain(x), packed(x))  # nothing to pack
+
+
+def test_packed_crops_with_stochastic_depth():
+    plain, packed = _pair(drop_path_rate=0.4)
+    out = []
+    for m in (plain, packed):
+        m.train()
+        torch.manual_seed(3)  # the blocks draw the same samples
+        out.append(_features(m, _crops())[0])
+    for a, b in zip(*out, strict=True):
+        _same(a, b)
+
+
+def test_the_packed_path_runs(monkeypatch):
+    from mia_train_b200.layers.dinov3 import attention as module
+
+    calls = []
+    real = module.packed_attention
+    monkeypatch.setattr(module, "packed_attention", lambda *a: calls.append(a[0].shape) or real(*a))
+    _, packed = _pair()
+    packed.forward_features(_crops(), [None, None])
+    assert calls == [(2 * 11 + 5 * 4, 2, 24)] * 2  # 8 + 3 and 1 + 3 tokens, two blocks
+    learned = _pair(pos_embed_rope_type="superposition")[1]
+    calls.clear()
+    learned.forward_features(_crops(), [None, None])
+    assert not calls or not learned.rope_embed.depth_scale.requires_grad

@@ -214,3 +214,16 @@ def test_distillation_refusals():
                 lambda: top_logit_distillation(s, values.repeat(1, 600), indices.repeat(1, 600))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_rotation_by_given_angles():
+    torch.manual_seed(0)
+    q, k, angles = torch.randn(2, 5, 3, 8), torch.randn(2, 5, 1, 8), 30 * torch.randn(5, 4)
+    pair = torch.arange(4)
+    pairs = torch.stack([pair, pair + 4], 1)
+    for got, x in zip(rotary(q, k, angles, None), (q, k), strict=True):
+        assert torch.allclose(got, rotate_pairs_reference(x, angles, pairs), atol=1e-5)
+    for bad in (lambda: rotary(q, k, angles.double(), None), lambda: rotary(q, k, angles[0], None),
+                lambda: rotary(q, k, torch.randn(5, 5), None), lambda: rotary(q, k, angles.requires_grad_(True), None)):
+        with pytest.raises(ValueError):
+            bad()
