@@ -189,6 +189,11 @@ __device__ __forceinline__ V uniform(V x) { return __shfl_sync(0xffffffffu, x, 0
 // Descriptor of a tile read along its rows' channels, and of one read along its rows; `tile_step` moves either by a tile.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return make_sdesc_sw<128>(addr, 16, 1024); }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) { return make_sdesc_sw<128>(addr, kRows * 128, 1024); }
+// 128 rows of 16 bytes one after the other, without swizzle; the second 8 of 16 channels `second` bytes behind.
+__device__ __forceinline__ uint64_t desc_columns(uint32_t addr, uint32_t second) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((second >> 4) & 0x3FFFu) << 16 | (uint64_t)(128 >> 4) << 32 |
+         (uint64_t)1 << 46;
+}
 template <int DP>
 __device__ __forceinline__ uint32_t tile_step(int n) { return (uint32_t)(n * (Tile<DP>::kBytes / 16)); }
 
@@ -227,16 +232,17 @@ __device__ __forceinline__ float store16(T* dst, const uint32_t (&v)[16], float 
 }
 
 // ------------------------------------------------------------------------------------------- forward
-// A CTA owns NT tiles of 128 queries of one head. Warps 4 t .. 4 t + 3 hold tile t's rows, one thread per row: S from
+// A CTA owns NT tiles of 128 queries of one head (two for wide heads). Warps 4 t .. 4 t + 3 hold tile t's rows, one thread per row: S from
 // tensor memory, running maximum and sum, P back over S. The accumulator O is rescaled in place, and only when a
 // block's maximum exceeds the reference maximum by more than 2^8 (P <= 2^8 until then). The last two warps load
-// (TMA) and issue the products. With two tiles one's softmax runs beside the other's products; heads of up to 64
-// channels leave room for P next to S, so that the next S is computed as soon as this one has been read.
+// (TMA) and issue the products. With two tiles, or two CTAs on an SM, one's softmax runs beside the other's products; heads
+// of up to 64 channels leave room for P next to S, so that the next S is computed as soon as this one has been read.
 //
 // Tensor memory: S (128 columns), O (DP) and, for DP = 64, P (64) per tile.
 template <int DP, int NT>
 struct FwdLayout {
-  static constexpr int kStages = DP == 64 && NT == 2 ? 3 : 2;
+  static_assert(DP == 128 || NT == 1, "two tiles of 64 channels leave no room for P");
+  static constexpr int kStages = 2;
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + NT * Tile<DP>::kBytes;
   static constexpr int kV = kK + kStages * Tile<DP>::kBytes;
@@ -385,23 +391,14 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
       for (int j = 0; j <= n && n > 0 && ok; ++j) {
         if (j < n) ok = warp_wait(&k_full[j % S], (j / S) & 1, abort_flag, err);
         if (ok && j > 0) ok = warp_wait(&v_full[(j - 1) % S], ((j - 1) / S) & 1, abort_flag, err);
-        if constexpr (L::kApart && NT == 2) {
-          // the second tile's sums wait for the first tile's next scores: the tiles' softmax fall into turns
-          ok = ok && (j == n || scores(0, j)) && (j < 2 || sums(1, j - 2));
-          if (ok && j > 1 && one) tc_commit(&v_empty[(j - 2) % S]);
-          ok = ok && (j == n || scores(1, j)) && (j == 0 || sums(0, j - 1));
-          if (ok && j < n && one) tc_commit(&k_empty[j % S]);
-        } else {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (L::kApart) ok = ok && (j == n || scores(t, j)) && (j == 0 || sums(t, j - 1));
-            else ok = ok && (j == 0 || sums(t, j - 1)) && (j == n || scores(t, j));
-          }
-          if (ok && j < n && one) tc_commit(&k_empty[j % S]);
-          if (ok && j > 0 && one) tc_commit(&v_empty[(j - 1) % S]);
+        for (int t = 0; t < NT; ++t) {
+          if (L::kApart) ok = ok && (j == n || scores(t, j)) && (j == 0 || sums(t, j - 1));
+          else ok = ok && (j == 0 || sums(t, j - 1)) && (j == n || scores(t, j));
         }
+        if (ok && j < n && one) tc_commit(&k_empty[j % S]);
+        if (ok && j > 0 && one) tc_commit(&v_empty[(j - 1) % S]);
       }
-      if constexpr (L::kApart && NT == 2) ok = ok && (n == 0 || sums(1, n - 1));
       if (!ok && one) {
         tc_commit(drain);
         mbar_wait(drain, 0, nullptr, nullptr, 0);
@@ -571,13 +568,35 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
 // delta_i = do_i . o_i. A CTA owns 128 rows of a head, 16 lanes a row. For fp16 also the largest norm of the
 // block's do rows: dS = p (dP - delta) is near |do| times a probability and would fall among fp16's subnormals, so
 // the backward kernels scale it by a power of two of that size.
+//
+// The kernel for dK and dV has its queries along the columns; a statistic per column read from shared memory by every
+// thread would take 4 cycles of its port for each 4 columns and warp, as long as the exponentials, and in the way of the
+// products' operands. It is subtracted by the tensor core instead: as 8 more channels, -lse / (scale log2 e) and -delta
+// as sums of 16-bit values (each what the ones before leave: 24 bits after three bf16, 33 after three fp16, and beyond
+// fp16's range up to eight times its largest), times ones.
+template <typename T>
+__device__ __forceinline__ uint4 as_channels(float x) {
+  constexpr float kMost = std::is_same_v<T, __half> ? 65504.f : 3.3895314e38f;
+  float v[8];
+  const bool finite = fabsf(x) < INFINITY;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = finite ? to_f32(from_f32<T>(fminf(fmaxf(x, -kMost), kMost))) : e == 0 ? x : 0.f;
+    x -= finite ? v[e] : 0.f;
+  }
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restrict__ o, const T* __restrict__ dout,
                                                               HeadRows ds, int Tq, int Hq, int D, int stride,
-                                                              float* __restrict__ delta, float* __restrict__ norms) {
+                                                              const float* __restrict__ lse, float inv_scale_log2,
+                                                              float* __restrict__ delta, uint4* __restrict__ channels,
+                                                              float* __restrict__ norms) {
   __shared__ float top[16];
   const int h = blockIdx.x % Hq, block = blockIdx.x / Hq;
   const int lane = threadIdx.x % 16, slot = threadIdx.x / 16;
+  const int64_t rows = (int64_t)Hq * stride;
   float most = 0.f;
 #pragma unroll 4
   for (int u = 0; u < 8; ++u) {
@@ -598,7 +617,11 @@ __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restric
       s += __shfl_xor_sync(0xffffffffu, s, w);
       n += __shfl_xor_sync(0xffffffffu, n, w);
     }
-    if (lane == 0 && i < Tq) delta[(int64_t)h * stride + i] = s;
+    if (i < Tq && lane < 2) {
+      const int64_t at = (int64_t)h * stride + i;
+      if (lane == 0) delta[at] = s;
+      channels[lane * rows + at] = as_channels<T>(lane == 0 ? -lse[at] * inv_scale_log2 : -s);
+    }
     if (n <= 3e38f) most = fmaxf(most, n);
   }
   if constexpr (std::is_same_v<T, __half>) {
@@ -898,7 +921,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // ----------------------------------------------------------------------------- backward: dK and dV
 // A CTA owns 128 keys of one key head and goes through the queries that see them, for every query head of the
 // group: S^T = K Q^T -> P^T -> dV += P^T dO, dP^T = V dO^T over S^T as soon as that has been read -> dS^T -> dK += dS^T Q;
-// thread = key. Query blocks begin at multiples of 128, so that their statistics can be copied with the tiles.
+// thread = key; lse and delta of the queries are 8 more channels of both products (packed_delta_tc_kernel). Query blocks
+// begin at multiples of 128.
 //
 // DP = 64: two groups of four warps take the blocks in turns, one's exponentials beside the other's dS. Tensor memory
 // per group: S^T, then dP^T, then dS^T (128 columns) and P^T (64); dV and dK (64 each).
@@ -914,8 +938,10 @@ struct DkvLayout {
   static constexpr int kV = kK + Tile<DP>::kBytes;
   static constexpr int kQ = kV + Tile<DP>::kBytes;
   static constexpr int kDO = kQ + kStages * Tile<DP>::kBytes;
-  static constexpr int kStat = kDO + kStages * Tile<DP>::kBytes;  // lse, delta of 128 queries, per stage
-  static constexpr int kBar = kStat + kStages * 1024;
+  static constexpr int kStat = kDO + kStages * Tile<DP>::kBytes;  // channels of lse and delta (2 KB each), per stage
+  static constexpr int kOnes = kStat + kStages * 4096;            // 128 rows of 8 ones
+  static constexpr int kZeros = kOnes + 2048;                     // and of 8 zeros, the other half of a step of 16
+  static constexpr int kBar = kZeros + 2048;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
 
@@ -924,8 +950,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                          const PackedProblem P, const T* __restrict__ dout, HeadRows dos, const float* __restrict__ lse,
-                         const float* __restrict__ delta, const float* __restrict__ norms, T* __restrict__ dk,
-                         T* __restrict__ dv, int* err) {
+                         const float* __restrict__ delta, const uint4* __restrict__ channels,
+                         const float* __restrict__ norms, T* __restrict__ dk, T* __restrict__ dv, int* err) {
   using L = DkvLayout<DP>;
   constexpr int S = L::kStages;
   constexpr bool kTurns = L::kTurns;
@@ -975,6 +1001,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  {
+    const uint32_t one2 = pack2<T>(1.f, 1.f);
+    if (threadIdx.x < 128) reinterpret_cast<uint4*>(smem + L::kOnes)[threadIdx.x] = make_uint4(one2, one2, one2, one2);
+    else if (threadIdx.x < 256) reinterpret_cast<uint4*>(smem + L::kZeros)[threadIdx.x - 128] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -991,12 +1023,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int i = 0; i < steps; ++i) {
         const int s = i % S, h = g * P.group + i / per_head, q0 = (qb0 + i % per_head) * kRows;
         if (!bounded_wait(&q_empty[s], ((i / S) & 1) ^ 1, abort_flag, err)) { ok = false; break; }
-        mbar_arrive_expect_tx(&q_full[s], 2 * Tile<DP>::kBytes + 1024);
+        mbar_arrive_expect_tx(&q_full[s], 2 * Tile<DP>::kBytes + 4096);
         load_tile<DP>(smem + L::kQ + s * Tile<DP>::kBytes, &tmQ, &q_full[s], q0, h);
         load_tile<DP>(smem + L::kDO + s * Tile<DP>::kBytes, &tmDO, &q_full[s], q0, h);
         const int64_t at = (int64_t)h * P.lse_stride + q0;
-        bulk_load(smem + L::kStat + s * 1024, lse + at, 512, &q_full[s]);
-        bulk_load(smem + L::kStat + s * 1024 + 512, delta + at, 512, &q_full[s]);
+        bulk_load(smem + L::kStat + s * 4096, channels + at, 2048, &q_full[s]);
+        bulk_load(smem + L::kStat + s * 4096 + 2048, channels + (int64_t)P.Hq * P.lse_stride + at, 2048, &q_full[s]);
         ++done;
       }
       if (!ok) {
@@ -1011,6 +1043,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint64_t q_rows = desc_mn(uniform(smem_u32(smem + L::kQ))), do_rows = desc_mn(uniform(smem_u32(smem + L::kDO)));
       const uint32_t base = uniform(tmem);
       const int n = uniform(steps);
+      const uint32_t stat_addr = uniform(smem_u32(smem + L::kStat)), ones_addr = uniform(smem_u32(smem + L::kOnes));
+      const uint32_t zeros_addr = ones_addr + (L::kZeros - L::kOnes);
+      const uint64_t ones_desc = desc_columns(ones_addr, zeros_addr - ones_addr);
+      // one more step of 16: the statistics' 8 channels and 8 zeros, times ones (and zeros)
+      auto subtract = [&](uint32_t d, int i, int which) {
+        const uint32_t from = stat_addr + (i % S) * 4096 + which * 2048;
+        tc_mma_f16(d, ones_desc, desc_columns(from, zeros_addr - from), idesc_s, 1);
+      };
       auto turn = [&](int i) { return kTurns ? i & 1 : 0; };
       auto phase = [&](int i) -> uint32_t { return kTurns ? (i >> 1) & 1 : i & 1; };
       auto scores = [&](int i) -> bool {
@@ -1018,6 +1058,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         if (one) {
           mma_scores<DP>(base + turn(i) * L::kXStep, k_desc, q_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          subtract(base + turn(i) * L::kXStep, i, 0);
           tc_commit(&s_full[turn(i)]);
         }
         return true;
@@ -1027,6 +1068,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         if (one) {
           mma_scores<DP>(base + turn(i) * L::kXStep, v_desc, do_desc + tile_step<DP>(i % S), idesc_s, P.D);
+          subtract(base + turn(i) * L::kXStep, i, 1);
           tc_commit(&dp_full[turn(i)]);
         }
         return true;
@@ -1090,16 +1132,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         top = fmaxf(top, norms[(int64_t)(g * P.group + i / per_head) * (P.lse_stride / kRows) + qb0 + i % per_head]);
       factor = ds_factor(top);
     }
-    const f32x2 scale2 = pair_of(scale_log2, scale_log2), factor2 = pair_of(factor, factor);
+    const float shift = kHalf ? kHalfShift : 0.f;
+    const f32x2 scale2 = pair_of(scale_log2, scale_log2), shift2 = pair_of(shift, shift), factor2 = pair_of(factor, factor);
     bool ok = true;
     for (int i = kTurns ? group : 0; i < steps; i += kTurns ? 2 : 1) {
       const uint32_t parity = kTurns ? (i >> 1) & 1 : i & 1;
       const int q0 = (qb0 + i % per_head) * kRows + off;
-      if (!warp_wait(&q_full[i % S], (i / S) & 1, abort_flag, err)) { ok = false; break; }
       if (!warp_wait(&s_full[bi], parity, abort_flag, err)) { ok = false; break; }
       tc_fence_after();
-      const float4* s_lse = reinterpret_cast<const float4*>(smem + L::kStat + (i % S) * 1024) + off / 4;
-      const float4* s_delta = s_lse + 32;
       const bool masked = q0 < all_lo || q0 + C * 32 > all_hi;
       const int a = mine.x - q0;
       const uint32_t n = (uint32_t)max(mine.y - mine.x, 0);
@@ -1114,15 +1154,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 ls = s_lse[c * 8 + e];
-          float x[4];
-          split(fma2(pair_of(__uint_as_float(p[c][4 * e]), __uint_as_float(p[c][4 * e + 1])), scale2,
-                     pair_of(kHalf ? kHalfShift - ls.x : -ls.x, kHalf ? kHalfShift - ls.y : -ls.y)), x[0], x[1]);
-          split(fma2(pair_of(__uint_as_float(p[c][4 * e + 2]), __uint_as_float(p[c][4 * e + 3])), scale2,
-                     pair_of(kHalf ? kHalfShift - ls.z : -ls.z, kHalf ? kHalfShift - ls.w : -ls.w)), x[2], x[3]);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) p[c][4 * e + u] = __float_as_uint(exp2_approx(x[u]));
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          split(fma2(pair_of(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1])), scale2, shift2), x0, x1);
+          p[c][2 * e] = __float_as_uint(exp2_approx(x0));
+          p[c][2 * e + 1] = __float_as_uint(exp2_approx(x1));
         }
       if (masked)
 #pragma unroll
@@ -1156,26 +1192,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         uint32_t(&x)[32] = v[c & 1];
-        float4 dl[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dl[e] = s_delta[c * 8 + e];
         if constexpr (kTurns) {  // the next 32 columns are on their way while these are worked on
           tmem_ld_wait_regs(x);
           if (c + 1 < C) tmem_ld_32x32b_x32(t_x + (c + 1) * 32, v[(c + 1) & 1]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f32x2 d[2] = {add2(pair_of(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])), pair_of(-dl[e].x, -dl[e].y)),
-                        add2(pair_of(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])), pair_of(-dl[e].z, -dl[e].w))};
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            d[u] = mul2(d[u], pair_of(__uint_as_float(p[c][4 * e + 2 * u]), __uint_as_float(p[c][4 * e + 2 * u + 1])));
-            if constexpr (kHalf) d[u] = mul2(d[u], factor2);
-            float d0, d1;
-            split(d[u], d0, d1);
-            p[c][4 * e + 2 * u] = __float_as_uint(d0);
-            p[c][4 * e + 2 * u + 1] = __float_as_uint(d1);
-          }
+        for (int e = 0; e < 16; ++e) {
+          f32x2 d = mul2(pair_of(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1])),
+                         pair_of(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])));
+          if constexpr (kHalf) d = mul2(d, factor2);
+          float d0, d1;
+          split(d, d0, d1);
+          p[c][2 * e] = __float_as_uint(d0);
+          p[c][2 * e + 1] = __float_as_uint(d1);
         }
         if (masked)
 #pragma unroll
@@ -1310,8 +1339,10 @@ cudaError_t fwd(const PackedProblem& P, void* o, float* lse, int* err, cudaStrea
       !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type))
     return cudaErrorInvalidValue;
   const int64_t pairs = (int64_t)((P.Tq + 2 * kRows - 1) / (2 * kRows)) * P.Hq;
-  // Two tiles a CTA share the loads of K and V; where that would leave SMs without work, one.
-  if (pairs >= 148)
+  // Heads of up to 64 channels: a tile a CTA and two CTAs an SM, whose softmax fall into turns by themselves (4 x 4101
+  // tokens, 16 heads of 64: 437 us against 492 with two tiles in one CTA, which run in step). Wider heads have room for
+  // one CTA, with two tiles that share the loads of K and V unless that would leave SMs without work.
+  if constexpr (DP == 128) if (pairs >= 148)
     return launch(packed_fwd_tc_kernel<T, DP, 2>, pairs, FwdLayout<DP, 2>::kThreads, FwdLayout<DP, 2>::kBytes, stream, q,
                   k, v, P, (T*)o, lse, err);
   return launch(packed_fwd_tc_kernel<T, DP, 1>, (int64_t)((P.Tq + kRows - 1) / kRows) * P.Hq, FwdLayout<DP, 1>::kThreads,
@@ -1320,7 +1351,7 @@ cudaError_t fwd(const PackedProblem& P, void* o, float* lse, int* err, cudaStrea
 
 template <typename T, int DP>
 cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse, float* delta,
-                float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+                void* channels, float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
   CUtensorMap q, k, v, g;
   const cudaError_t ready = context_current();
   if (ready != cudaSuccess) return ready;
@@ -1330,8 +1361,9 @@ cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRow
     return cudaErrorInvalidValue;
   const int64_t q_tiles = (P.Tq + kRows - 1) / kRows, k_tiles = (P.Tk + kRows - 1) / kRows;
   if (q_tiles > 0) {
-    packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>((const T*)o, (const T*)dout, ds, P.Tq, P.Hq,
-                                                                             P.D, P.lse_stride, delta, norms);
+    packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>(
+        (const T*)o, (const T*)dout, ds, P.Tq, P.Hq, P.D, P.lse_stride, lse, 1.f / (P.scale * kLog2e), delta,
+        (uint4*)channels, norms);
     cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return status;
     status = launch(packed_dq_tc_kernel<T, DP>, q_tiles * P.Hq, kBwdThreads, DqLayout<DP>::kBytes, stream, q, k, v, g, P,
@@ -1340,7 +1372,7 @@ cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRow
   }
   if (k_tiles == 0) return cudaSuccess;
   return launch(packed_dkv_tc_kernel<T, DP>, k_tiles * P.Hk, kBwdThreads, DkvLayout<DP>::kBytes, stream, q, k, v, g, P,
-                (const T*)dout, ds, lse, (const float*)delta, (const float*)norms, (T*)dk, (T*)dv, err);
+                (const T*)dout, ds, lse, (const float*)delta, (const uint4*)channels, (const float*)norms, (T*)dk, (T*)dv, err);
 }
 
 }  // namespace
@@ -1357,12 +1389,13 @@ cudaError_t packed_fwd_tc(const PackedProblem& P, void* o, float* lse, int* err,
 }
 
 cudaError_t packed_bwd_tc(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
-                          float* delta, float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+                          float* delta, void* channels, float* norms, void* dq, void* dk, void* dv, int* err,
+                          cudaStream_t stream) {
   if (P.type == kSeqBf16)
-    return P.D <= 64 ? bwd<__nv_bfloat16, 64>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream)
-                     : bwd<__nv_bfloat16, 128>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream);
-  return P.D <= 64 ? bwd<__half, 64>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream)
-                   : bwd<__half, 128>(P, o, dout, ds, lse, delta, norms, dq, dk, dv, err, stream);
+    return P.D <= 64 ? bwd<__nv_bfloat16, 64>(P, o, dout, ds, lse, delta, channels, norms, dq, dk, dv, err, stream)
+                     : bwd<__nv_bfloat16, 128>(P, o, dout, ds, lse, delta, channels, norms, dq, dk, dv, err, stream);
+  return P.D <= 64 ? bwd<__half, 64>(P, o, dout, ds, lse, delta, channels, norms, dq, dk, dv, err, stream)
+                   : bwd<__half, 128>(P, o, dout, ds, lse, delta, channels, norms, dq, dk, dv, err, stream);
 }
 
 }  // namespace mia

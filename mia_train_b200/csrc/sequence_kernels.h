@@ -42,11 +42,13 @@ cudaError_t packed_fwd_few(const PackedProblem& P, const PackedFew& few, void* o
 cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
                             float* delta, void* dq, void* dk, void* dv, cudaStream_t stream);
 
-// The tensor-core kernels, where packed_tc_ok: same arguments; norms (Hq, lse_stride / 128) fp32 is scratch for fp16.
+// The tensor-core kernels, where packed_tc_ok: same arguments; channels (2, Hq, lse_stride, 8) of the inputs' type is
+// scratch, and for fp16 norms (Hq, lse_stride / 128) fp32.
 bool packed_tc_ok(const PackedProblem& P);
 cudaError_t packed_fwd_tc(const PackedProblem& P, void* o, float* lse, int* err, cudaStream_t stream);
 cudaError_t packed_bwd_tc(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
-                          float* delta, float* norms, void* dq, void* dk, void* dv, int* err, cudaStream_t stream);
+                          float* delta, void* channels, float* norms, void* dq, void* dk, void* dv, int* err,
+                          cudaStream_t stream);
 
 struct TokenRows {
   int64_t b, t, h;  // element strides of (B, T, H, D)

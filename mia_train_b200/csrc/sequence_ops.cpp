@@ -155,8 +155,9 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     const float* lse = s[6].data_ptr<float>();
     if (packed_tc_ok(P)) {
       at::Tensor norms = at::empty({P.type == kSeqF16 ? s[6].numel() / 128 : 0}, s[6].options());
+      at::Tensor channels = at::empty({2 * s[6].numel() * 8}, s[0].options());
       C10_CUDA_CHECK(packed_bwd_tc(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
-                                   norms.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   channels.data_ptr(), norms.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                    error_word(dout.get_device()), stream));
     } else {
       C10_CUDA_CHECK(packed_bwd_rows(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
