@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "pair_math.cuh"
 #include "sequence_kernels.h"
 #include "vec8.cuh"
 
@@ -109,10 +110,17 @@ struct Soft {
     // with m = -inf (all of them, or NaN next to them) the differences would be NaN: 0 stands in for m, the terms of
     // -inf are 0 and those of NaN stay NaN
     const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
+    const f32x2 ref2 = pair_of(-ref, -ref), c2 = pair_of(c, c);
+    f32x2 sum = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += ex2((v[e] - ref) * c);
-    l += s;
+    for (int e = 0; e < 8; e += 2) {
+      float a, b;
+      split(mul2(add2(pair_of(v[e], v[e + 1]), ref2), c2), a, b);
+      sum = add2(sum, pair_of(ex2(a), ex2(b)));
+    }
+    float a, b;
+    split(sum, a, b);
+    l += a + b;
   }
   __device__ __forceinline__ void join(float m2, float l2, float c) {
     const float top = fmaxf(m, m2);
@@ -472,8 +480,13 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
     for (int i = threadIdx.x; i < vecs; i += NT) {
       float v[8];
       unpack8<T>(load_raw8<T>(row + vec_ahead + i * 8), v);
+      const f32x2 ref2 = pair_of(-ref, -ref), c2 = pair_of(c, c), coef2 = pair_of(coef, coef);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = ex2((v[e] - ref) * c) * coef;
+      for (int e = 0; e < 8; e += 2) {
+        float a, b;
+        split(mul2(add2(pair_of(v[e], v[e + 1]), ref2), c2), a, b);
+        split(mul2(pair_of(ex2(a), ex2(b)), coef2), v[e], v[e + 1]);
+      }
       store8<T>(out + vec_ahead + i * 8, v);
     }
     const int end = vec_ahead + vecs * 8;
