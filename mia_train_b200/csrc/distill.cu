@@ -38,7 +38,6 @@ constexpr int kMany = 256, kFew = 512;
 int threads_for(int rows, int classes) { return rows < 2 * 148 && classes >= 16384 ? kFew : kMany; }
 
 constexpr int kCandidates = 2048;
-constexpr float kLog2eF = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -91,47 +90,63 @@ __device__ __forceinline__ float max8_nan(const float (&v)[8]) {
   return r;
 }
 
+// log2(e) / tau as two fp32: with one, every exponent would be off by the same 2^-25 of it, which a small divergence (a
+// difference of far larger terms) shows.
+struct Rate {
+  float hi, lo;
+  __device__ __forceinline__ explicit Rate(double inv_tau) {
+    const double c = inv_tau * 1.4426950408889634074;
+    hi = __double2float_rd(c);
+    if ((double)hi == c && c > 0.0) hi = __uint_as_float(__float_as_uint(hi) - 1);
+    lo = (float)(c - (double)hi);  // positive, so that -inf stays -inf
+  }
+  __device__ __forceinline__ float operator()(float d) const { return fmaf(d, lo, d * hi); }
+  __device__ __forceinline__ f32x2 operator()(f32x2 d) const {
+    return fma2(d, pair_of(lo, lo), mul2(d, pair_of(hi, hi)));
+  }
+};
+
 // Running maximum m (of raw logits) and sum l of exp((s - m) / tau).
 struct Soft {
   float m = -INFINITY, l = 0.f;
-  __device__ __forceinline__ void add(float s, float c) {
+  __device__ __forceinline__ void add(float s, Rate c) {
     if (s > m) {
-      l *= m == -INFINITY ? 0.f : ex2((m - s) * c);
+      l *= m == -INFINITY ? 0.f : ex2(c(m - s));
       m = s;
     }
-    l += s == -INFINITY ? 0.f : ex2((s - m) * c);
+    l += s == -INFINITY ? 0.f : ex2(c(s - m));
   }
   // `top` is the largest of the eight, or NaN
-  __device__ __forceinline__ void add8(const float (&v)[8], float top, float c) {
+  __device__ __forceinline__ void add8(const float (&v)[8], float top, Rate c) {
     if (top > m) {
-      l *= m == -INFINITY ? 0.f : ex2((m - top) * c);
+      l *= m == -INFINITY ? 0.f : ex2(c(m - top));
       m = top;
     }
     // with m = -inf (all of them, or NaN next to them) the differences would be NaN: 0 stands in for m, the terms of
     // -inf are 0 and those of NaN stay NaN
     const float ref = m == -INFINITY ? 0.f : m;
-    const f32x2 ref2 = pair_of(-ref, -ref), c2 = pair_of(c, c);
+    const f32x2 ref2 = pair_of(-ref, -ref);
     f32x2 sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       float a, b;
-      split(mul2(add2(pair_of(v[e], v[e + 1]), ref2), c2), a, b);
+      split(c(add2(pair_of(v[e], v[e + 1]), ref2)), a, b);
       sum = add2(sum, pair_of(ex2(a), ex2(b)));
     }
     float a, b;
     split(sum, a, b);
     l += a + b;
   }
-  __device__ __forceinline__ void join(float m2, float l2, float c) {
+  __device__ __forceinline__ void join(float m2, float l2, Rate c) {
     const float top = fmaxf(m, m2);
     const float ref = top == -INFINITY ? 0.f : top;
-    l = l * ex2((m - ref) * c) + l2 * ex2((m2 - ref) * c);
+    l = l * ex2(c(m - ref)) + l2 * ex2(c(m2 - ref));
     m = top;
   }
 };
 
 template <int NT>
-__device__ void block_join(Soft& a, float c, float* scratch /* 2 * NT / 32 */) {
+__device__ void block_join(Soft& a, Rate c, float* scratch /* 2 * NT / 32 */) {
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, a.m, w), l2 = __shfl_xor_sync(0xffffffffu, a.l, w);
@@ -205,14 +220,14 @@ __device__ uint32_t kth_key(int k, F&& count) {
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) top_logits_kernel(const T* __restrict__ x, int64_t stride, int V, int k,
-                                                              float inv_tau, T* __restrict__ values,
+                                                              double inv_tau, T* __restrict__ values,
                                                               int64_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ uint64_t list[kCandidates];
   __shared__ float red[2 * (NT / 32)];
   __shared__ int counts[(NT / 32)];
   __shared__ int n_list;
   const T* row = x + (int64_t)blockIdx.x * stride;
-  const float c = inv_tau * kLog2eF;
+  const Rate c(inv_tau);
   if (threadIdx.x == 0) n_list = 0;
 
   Soft soft;
@@ -235,7 +250,7 @@ __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) top_logits_kernel(con
   block_join<NT>(soft, c, red);
   const bool nan = block_count<NT>(best[0] == 0xffffffffu || best[1] == 0xffffffffu, counts) > 0;
   if (threadIdx.x == 0)
-    lse[blockIdx.x] = nan ? NAN : soft.m == INFINITY ? INFINITY : soft.l == 0.f ? -INFINITY : fmaf(soft.m, inv_tau, logf(soft.l));
+    lse[blockIdx.x] = nan ? NAN : soft.m == INFINITY ? INFINITY : soft.l == 0.f ? -INFINITY : (float)(soft.m * inv_tau + log((double)soft.l));
 
   // A row shorter than the groups leaves some of them empty, and then the bound may be 0: every element is taken.
   // Any bound that at least k groups reach will do; the search ends where not many more do.
@@ -348,7 +363,7 @@ __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) distill_fwd_kernel(Di
   const T* row = (const T*)p.s + r * p.s_row;
   const int64_t first = (int64_t)r * p.K;
   const double inv_tau = 1.0 / p.tau, inv_tau_t = 1.0 / p.teacher_tau;
-  const float c = (float)inv_tau * kLog2eF;
+  const Rate c(inv_tau);
   const bool tail = p.lse != nullptr;
   Soft gen, top;
   double distinct = 0.0;
@@ -397,7 +412,7 @@ __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) distill_fwd_kernel(Di
       if (index_at(p, first + j) >= 0) m = fmaxf(m, (float)value_at(p, first + j));
     Soft mm;
     mm.m = m;
-    block_join<NT>(mm, 0.f, red);
+    block_join<NT>(mm, Rate(0.0), red);
     const double ref = mm.m == -INFINITY ? 0.0 : (double)mm.m * inv_tau_t;
     double sum[1] = {0.0};
     for (int j = threadIdx.x; j < p.K; j += NT)
@@ -464,7 +479,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
   const int64_t first = (int64_t)r * p.K;
   const double* st = p.stats + (int64_t)r * kStats;
   const double inv_tau = 1.0 / p.tau, inv_tau_t = 1.0 / p.teacher_tau;
-  const float c = (float)inv_tau * kLog2eF;
+  const Rate c(inv_tau);
   const double scale = (double)*grad * w / p.norm * inv_tau;
   const float m = (float)st[kGenM];
   const float ref = m == -INFINITY ? 0.f : m;
@@ -480,11 +495,11 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
     for (int i = threadIdx.x; i < vecs; i += NT) {
       float v[8];
       unpack8<T>(load_raw8<T>(row + vec_ahead + i * 8), v);
-      const f32x2 ref2 = pair_of(-ref, -ref), c2 = pair_of(c, c), coef2 = pair_of(coef, coef);
+      const f32x2 ref2 = pair_of(-ref, -ref), coef2 = pair_of(coef, coef);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float a, b;
-        split(mul2(add2(pair_of(v[e], v[e + 1]), ref2), c2), a, b);
+        split(c(add2(pair_of(v[e], v[e + 1]), ref2)), a, b);
         split(mul2(pair_of(ex2(a), ex2(b)), coef2), v[e], v[e + 1]);
       }
       store8<T>(out + vec_ahead + i * 8, v);
@@ -492,10 +507,10 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
     const int end = vec_ahead + vecs * 8;
     for (int i = threadIdx.x; i < vec_ahead + (p.V - end); i += NT) {
       const int at = i < vec_ahead ? i : end + i - vec_ahead;
-      out[at] = from_f32<T>(ex2((to_f32(row[at]) - ref) * c) * coef);
+      out[at] = from_f32<T>(ex2(c(to_f32(row[at]) - ref)) * coef);
     }
   } else {
-    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(ex2((to_f32(row[i]) - ref) * c) * coef);
+    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(ex2(c(to_f32(row[i]) - ref)) * coef);
   }
   __syncthreads();  // the given classes replace what the pass wrote in their places
   const double inv_l = 1.0 / st[kAllL], all_m = st[kAllM], mass = st[kMass];
@@ -529,7 +544,7 @@ cudaError_t top_logits_rows(const void* x, int64_t stride, int R, int V, int k, 
   by_type(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     auto go = [&](auto kernel, int threads) {
-      kernel<<<R, threads, 0, stream>>>((const T*)x, stride, V, k, (float)(1.0 / tau), (T*)values, indices, lse);
+      kernel<<<R, threads, 0, stream>>>((const T*)x, stride, V, k, 1.0 / tau, (T*)values, indices, lse);
     };
     if (threads_for(R, V) == kMany) go(top_logits_kernel<T, kMany>, kMany);
     else go(top_logits_kernel<T, kFew>, kFew);

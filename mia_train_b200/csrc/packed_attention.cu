@@ -8,6 +8,7 @@
 // The mask is a pair of bounds per query (and, for dk and dv, per key), made once for a batch's lengths; rows that
 // see nothing give zeros. This file holds the kernels with a warp per row, which run every head size and type, and the
 // forward kernel for few queries over many keys.
+#include <algorithm>
 #include <type_traits>
 
 #include "packed_attention.h"
@@ -30,13 +31,14 @@ __global__ void __launch_bounds__(kWarps * 32) packed_fwd_rows_kernel(PackedProb
   forward_row<T>((const T*)P.q + i * P.qs.row + h * P.qs.head, (const T*)P.k + g * P.ks.head,
                  (const T*)P.v + g * P.vs.head, P.ks.row, P.vs.row, b.x, b.y, P.D, P.scale * kLog2e, scratch[warp], lane,
                  acc, stat);
-  store_row<T>(o + at * P.D, acc, P.D, lane);
+  store_row_low<T>(o + at * P.D, P.o_low != nullptr ? (T*)P.o_low + at * P.D : nullptr, acc, P.D, lane);
   if (lane == 0) lse[(int64_t)h * P.lse_stride + i] = stat;
 }
 
 // delta_i = do_i . o_i, a warp per row
 template <typename T>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const T* __restrict__ o, const T* __restrict__ dout, HeadRows ds,
+__global__ void __launch_bounds__(256) packed_delta_kernel(const T* __restrict__ o, const T* __restrict__ low,
+                                                           const T* __restrict__ dout, HeadRows ds,
                                                     int Tq, int Hq, int D, int stride, float* __restrict__ delta) {
   const int lane = threadIdx.x % 32;
   const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
@@ -44,7 +46,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const T* __restrict__
   const int i = (int)(at / Hq), h = (int)(at % Hq);
   const T *a = o + at * D, *b = dout + i * ds.row + h * ds.head;
   float s = 0.f;
-  for (int c = lane; c < D; c += 32) s = fmaf(to_f32(a[c]), to_f32(b[c]), s);
+  for (int c = lane; c < D; c += 32)
+    s = fmaf(low != nullptr ? to_f32(a[c]) + to_f32(low[at * D + c]) : to_f32(a[c]), to_f32(b[c]), s);
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
   if (lane == 0) delta[(int64_t)h * stride + i] = s;
@@ -96,6 +99,13 @@ __global__ void __launch_bounds__(kWarps * 32) packed_dkv_rows_kernel(PackedProb
 // K and V: LP lanes hold a row's channels, eight each, and a warp has eight 16-byte loads of K and of V a lane under way.
 // 16 sequences of 1029 .. 4101 keys, one query, 16 heads of 64 fp16: 805 us by tiles, 47 us here (39 us at 5.6 TB/s and 7 us for joining).
 constexpr int kFewThreads = 128;
+
+template <typename T>
+__device__ __forceinline__ void store_low(T* o, T* low, int64_t at, float x) {
+  const T y = from_f32<T>(x);
+  o[at] = y;
+  if (low != nullptr) low[at] = from_f32<T>(x - to_f32(y));
+}
 
 template <typename T, int LP, int R>
 __global__ void __launch_bounds__(kFewThreads) packed_few_kernel(PackedProblem P, PackedFew few, T* __restrict__ o,
@@ -219,7 +229,7 @@ __global__ void __launch_bounds__(kFewThreads) packed_few_kernel(PackedProblem P
     }
     if (few.partial == nullptr) {
       const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
-      o[((int64_t)i * P.Hq + h) * P.D + ch] = from_f32<T>(sum == 0.f ? 0.f : value / sum);
+      store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, sum == 0.f ? 0.f : value / sum);
       if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
     } else {
       float* part = few.partial + (((int64_t)blockIdx.x * P.Hk + hk) * few.rows + row) * (P.D + 2);
@@ -253,11 +263,12 @@ __global__ void __launch_bounds__(128) packed_few_join_kernel(PackedProblem P, P
     if (ch < P.D) value += f * part[n * step + ch];
   }
   const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
-  if (ch < P.D) o[((int64_t)i * P.Hq + h) * P.D + ch] = from_f32<T>(sum == 0.f ? 0.f : value / sum);
+  if (ch < P.D) store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, sum == 0.f ? 0.f : value / sum);
   if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
-unsigned grid_of(int64_t items, int per) { return (unsigned)((items + per - 1) / per); }
+int64_t blocks_of(int64_t items, int per) { return (items + per - 1) / per; }
+unsigned grid_of(int64_t items, int per) { return (unsigned)blocks_of(items, per); }
 
 template <typename F>
 void by_type(SequenceType type, F&& f) {
@@ -269,6 +280,7 @@ void by_type(SequenceType type, F&& f) {
 }  // namespace
 
 cudaError_t packed_fwd_rows(const PackedProblem& P, void* o, float* lse, cudaStream_t stream) {
+  if (blocks_of((int64_t)P.Tq * P.Hq, kWarps) > 0x7fffffff) return cudaErrorInvalidConfiguration;
   by_type(P.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     packed_fwd_rows_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, kWarps), kWarps * 32, 0, stream>>>(P, (T*)o, lse);
@@ -293,12 +305,13 @@ cudaError_t packed_fwd_few(const PackedProblem& P, const PackedFew& few, void* o
 
 cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,
                             float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  if (blocks_of((int64_t)std::max(P.Tq, P.Tk) * P.Hq, kWarps) > 0x7fffffff) return cudaErrorInvalidConfiguration;
   by_type(P.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const T* go = (const T*)dout;
     if (P.Tq > 0) {
-      packed_delta_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, 8), 256, 0, stream>>>((const T*)o, go, ds, P.Tq, P.Hq, P.D,
-                                                                                  P.lse_stride, delta);
+      packed_delta_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, 8), 256, 0, stream>>>(
+          (const T*)o, (const T*)P.o_low, go, ds, P.Tq, P.Hq, P.D, P.lse_stride, delta);
       packed_dq_rows_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, kWarps), kWarps * 32, 0, stream>>>(P, go, ds, lse, delta,
                                                                                                  (T*)dq);
     }

@@ -134,6 +134,18 @@ __device__ void dkv_row(const T* k, const T* v, const T* q, const T* dout, int64
   __syncwarp();
 }
 
+// store_row, and in `low` (which may be null) what rounding took away
+template <typename T>
+__device__ __forceinline__ void store_row_low(T* dst, T* low, const float (&x)[4], int D, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < D) {
+      const T y = from_f32<T>(x[i]);
+      dst[lane + 32 * i] = y;
+      if (low != nullptr) low[lane + 32 * i] = from_f32<T>(x[i] - to_f32(y));
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void store_row(T* dst, const float (&x)[4], int D, int lane) {
 #pragma unroll

@@ -208,6 +208,18 @@ __device__ __forceinline__ float store16(T* dst, const uint32_t (&v)[16], float 
   return bad;
 }
 
+// The same of x, which is finite where it is wanted, less what 16 bits keep of it.
+template <typename T>
+__device__ __forceinline__ void store16_low(T* dst, const uint32_t (&v)[16], float f, bool first8, bool last8) {
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float x = __uint_as_float(v[e]) * f;
+    w[e] = __float_as_uint(x - to_f32(from_f32<T>(x)));
+  }
+  store16<T>(dst, w, 1.f, first8, last8);
+}
+
 // ------------------------------------------------------------------------------------------- forward
 // A CTA owns NT tiles of 128 queries of one head (two for wide heads). Warps 4 t .. 4 t + 3 hold tile t's rows, one thread per row: S from
 // tensor memory, running maximum and sum, P back over S. The accumulator O is rescaled in place, and only when a
@@ -509,8 +521,8 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
           for (int e = 0; e < 16; ++e) w[e] = 0;
         }
         const bool both = real && c * 16 + 16 <= P.D;
-        const float b = store16<T>(dst + c * 16, w, inv, real, both);
-        bad += b;
+        bad += store16<T>(dst + c * 16, w, inv, real, both);
+        if (P.o_low != nullptr) store16_low<T>((T*)P.o_low + (dst - o) + c * 16, w, inv, real, both);
       }
       if (real) lse[(int64_t)h * P.lse_stride + row] = l == 0.f ? INFINITY : m + log2f(l);
       // rows that a masked neighbour's infinity or NaN may have reached
@@ -528,7 +540,8 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
           forward_row<T>((const T*)P.q + i * P.qs.row + h * P.qs.head, (const T*)P.k + hk * P.ks.head,
                          (const T*)P.v + hk * P.vs.head, P.ks.row, P.vs.row, b.x, b.y, P.D, scale_log2, scratch, lane, acc,
                          stat);
-          store_row<T>(o + ((int64_t)i * P.Hq + h) * P.D, acc, P.D, lane);
+          const int64_t out = ((int64_t)i * P.Hq + h) * P.D;
+          store_row_low<T>(o + out, P.o_low != nullptr ? (T*)P.o_low + out : nullptr, acc, P.D, lane);
         }
       }
     }
@@ -542,18 +555,27 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
 }
 
 // --------------------------------------------------------------------------------- backward: delta
-// delta_i = do_i . o_i. A CTA owns 128 rows of a head, 16 lanes a row. For fp16 also the largest norm of the
+// delta_i = do_i . o_i, with o as it was before rounding: where a row has few keys, dP - delta is a small difference. A CTA
+// owns 128 rows of a head, 16 lanes a row. For fp16 also the largest norm of the
 // block's do rows: dS = p (dP - delta) is near |do| times a probability and would fall among fp16's subnormals, so
 // the backward kernels scale it by a power of two of that size.
 //
 // The kernel for dK and dV has its queries along the columns; a statistic per column read from shared memory by every
 // thread would take 4 cycles of its port for each 4 columns and warp, as long as the exponentials, and in the way of the
 // products' operands. It is subtracted by the tensor core instead: as 8 more channels, -lse / (scale log2 e) and -delta
-// as sums of 16-bit values (each what the ones before leave: 24 bits after three bf16, 33 after three fp16, and beyond
-// fp16's range up to eight times its largest), times ones.
+// as sums of 16-bit values (each what the ones before leave: 24 bits after three bf16, 33 after three fp16) times ones;
+// for fp16 times 64, with which they reach 3.3e7. What is beyond becomes NaN, and the rows that it reaches are computed
+// again without tensor cores.
+template <typename T>
+__host__ __device__ constexpr float channel_unit() {
+  return std::is_same_v<T, __half> ? 64.f : 1.f;
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 as_channels(float x) {
   constexpr float kMost = std::is_same_v<T, __half> ? 65504.f : 3.3895314e38f;
+  x *= 1.f / channel_unit<T>();
+  if (std::is_same_v<T, __half> && fabsf(x) > 8.f * kMost && fabsf(x) < INFINITY) x = NAN;
   float v[8];
   const bool finite = fabsf(x) < INFINITY;
 #pragma unroll
@@ -565,7 +587,8 @@ __device__ __forceinline__ uint4 as_channels(float x) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restrict__ o, const T* __restrict__ dout,
+__global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restrict__ o, const T* __restrict__ low,
+                                                              const T* __restrict__ dout,
                                                               HeadRows ds, int Tq, int Hq, int D, int stride,
                                                               const float* __restrict__ lse, float inv_scale_log2,
                                                               float* __restrict__ delta, uint4* __restrict__ channels,
@@ -583,6 +606,12 @@ __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restric
       float a[8], b[8];
       unpack8<T>(load_raw8<T>(o + ((int64_t)i * Hq + h) * D + lane * 8), a);
       unpack8<T>(load_raw8<T>(dout + i * ds.row + h * ds.head + lane * 8), b);
+      if (low != nullptr) {
+        float c[8];
+        unpack8<T>(load_raw8<T>(low + ((int64_t)i * Hq + h) * D + lane * 8), c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] += c[e];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s = fmaf(a[e], b[e], s);
@@ -916,7 +945,7 @@ struct DkvLayout {
   static constexpr int kQ = kV + Tile<DP>::kBytes;
   static constexpr int kDO = kQ + kStages * Tile<DP>::kBytes;
   static constexpr int kStat = kDO + kStages * Tile<DP>::kBytes;  // channels of lse and delta (2 KB each), per stage
-  static constexpr int kOnes = kStat + kStages * 4096;            // 128 rows of 8 ones
+  static constexpr int kOnes = kStat + kStages * 4096;            // 128 rows of 8 times the channels' unit
   static constexpr int kZeros = kOnes + 2048;                     // and of 8 zeros, the other half of a step of 16
   static constexpr int kBar = kZeros + 2048;
   static constexpr int kBytes = kBar + 256 + 1024;
@@ -979,7 +1008,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_relinquish();
   }
   {
-    const uint32_t one2 = pack2<T>(1.f, 1.f);
+    const uint32_t one2 = pack2<T>(channel_unit<T>(), channel_unit<T>());
     if (threadIdx.x < 128) reinterpret_cast<uint4*>(smem + L::kOnes)[threadIdx.x] = make_uint4(one2, one2, one2, one2);
     else if (threadIdx.x < 256) reinterpret_cast<uint4*>(smem + L::kZeros)[threadIdx.x - 128] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
@@ -1336,10 +1365,11 @@ cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRow
   if (!map_rows(&q, P.q, P.qs, queries, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, keys, P.Hk, P.D, P.type) ||
       !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type) || !map_rows(&g, dout, ds, queries, P.Hq, P.D, P.type))
     return cudaErrorInvalidValue;
-  const int64_t q_tiles = (P.Tq + kRows - 1) / kRows, k_tiles = (P.Tk + kRows - 1) / kRows;
+  const int64_t q_tiles = ((int64_t)P.Tq + kRows - 1) / kRows, k_tiles = ((int64_t)P.Tk + kRows - 1) / kRows;
+  if (q_tiles * P.Hq > 0x7fffffff) return cudaErrorInvalidConfiguration;
   if (q_tiles > 0) {
     packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>(
-        (const T*)o, (const T*)dout, ds, P.Tq, P.Hq, P.D, P.lse_stride, lse, 1.f / (P.scale * kLog2e), delta,
+        (const T*)o, (const T*)P.o_low, (const T*)dout, ds, P.Tq, P.Hq, P.D, P.lse_stride, lse, 1.f / (P.scale * kLog2e), delta,
         (uint4*)channels, norms);
     cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return status;
@@ -1354,9 +1384,10 @@ cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRow
 
 }  // namespace
 
-// A positive scale (the running maximum is taken before it), 16-bit values and up to 128 channels.
+// A positive scale (the running maximum is taken before it) that the statistics can be divided by, 16-bit values and up
+// to 128 channels.
 bool packed_tc_ok(const PackedProblem& P) {
-  return (P.type == kSeqBf16 || P.type == kSeqF16) && P.scale > 0.f && P.D <= 128;
+  return (P.type == kSeqBf16 || P.type == kSeqF16) && P.scale > 1e-12f && P.D <= 128;
 }
 
 cudaError_t packed_fwd_tc(const PackedProblem& P, void* o, float* lse, int* err, cudaStream_t stream) {

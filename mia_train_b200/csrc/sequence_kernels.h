@@ -25,6 +25,7 @@ struct PackedProblem {
   int lse_stride;        // columns of lse and delta: rows rounded up to 128
   float scale;
   SequenceType type;
+  void* o_low;  // like o, or null: what rounding took from o, written forward and added to o again for delta
 };
 
 // o (Tq.., Hq, D) contiguous; lse (Hq, lse_stride) fp32

@@ -74,6 +74,7 @@ PackedProblem problem(const at::Tensor& q, const at::Tensor& k, const at::Tensor
   P.lse_stride = (P.Tq + 127) / 128 * 128;
   P.scale = (float)scale;
   P.type = type_of(q);
+  P.o_low = nullptr;
   return P;
 }
 
@@ -107,7 +108,7 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const at::Tensor& q_bounds, const at::Tensor& k_bounds, double scale,
                             const OptTensor& items, const OptTensor& pieces, int64_t max_queries, int64_t tile_pairs,
-                            int64_t pairs) {
+                            int64_t pairs, bool grad) {
     BelowAutograd below;
     const at::Tensor qc = heads(q), kc = heads(k), vc = heads(v);
     const int64_t used = q_bounds.size(0);
@@ -116,8 +117,15 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     const c10::cuda::CUDAGuard guard(q.device());
     const auto stream = at::cuda::getCurrentCUDAStream();
     keep_for(q_bounds, stream);
-    const PackedProblem P = problem(qc, kc, vc, q_bounds, k_bounds, scale);
-    if (used > 0 && items.has_value() && few_is_faster(P, max_queries, tile_pairs, pairs)) {
+    PackedProblem P = problem(qc, kc, vc, q_bounds, k_bounds, scale);
+    at::Tensor low;
+    if (grad && P.type != kSeqF32) low = at::empty(o.sizes(), o.options());
+    P.o_low = low.defined() ? low.data_ptr() : nullptr;
+    if (P.Tk == 0) {  // nobody sees anything
+      o.zero_();
+      lse.fill_(INFINITY);
+      if (low.defined()) low.zero_();
+    } else if (used > 0 && items.has_value() && few_is_faster(P, max_queries, tile_pairs, pairs)) {
       PackedFew few;
       few.items = reinterpret_cast<const int4*>(items->data_ptr<int>());
       few.pieces = reinterpret_cast<const int2*>(pieces->data_ptr<int>());
@@ -136,7 +144,7 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
                                                      error_word(q.get_device()), stream)
                                      : packed_fwd_rows(P, o.data_ptr(), lse.data_ptr<float>(), stream));
     }
-    ctx->save_for_backward({qc, kc, vc, q_bounds, k_bounds, o, lse});
+    ctx->save_for_backward({qc, kc, vc, q_bounds, k_bounds, o, lse, low});
     ctx->saved_data["scale"] = scale;
     return o;
   }
@@ -151,9 +159,12 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     const auto stream = at::cuda::getCurrentCUDAStream();
     keep_for(s[3], stream);
     keep_for(s[4], stream);
-    const PackedProblem P = problem(s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble());
+    PackedProblem P = problem(s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble());
+    P.o_low = s[7].defined() ? s[7].data_ptr() : nullptr;
     const float* lse = s[6].data_ptr<float>();
-    if (packed_tc_ok(P)) {
+    if (P.Tq == 0 || P.Tk == 0) {
+      for (at::Tensor* x : {&dq, &dk, &dv}) x->zero_();
+    } else if (packed_tc_ok(P)) {
       at::Tensor norms = at::empty({P.type == kSeqF16 ? s[6].numel() / 128 : 0}, s[6].options());
       at::Tensor channels = at::empty({2 * s[6].numel() * 8}, s[0].options());
       C10_CUDA_CHECK(packed_bwd_tc(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
@@ -164,7 +175,7 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
                                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stream));
     }
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+            at::Tensor(), at::Tensor()};
   }
 };
 
@@ -214,7 +225,7 @@ void rotate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& position
   p.amplitude = (float)amplitude;
   p.inverse = inverse;
   p.partial = nullptr;
-  if (p.tokens == 0 || p.Hq + p.Hk == 0) {
+  if (p.tokens == 0 || p.Hq + p.Hk == 0 || p.D == 0) {
     if (learn) dfreq->zero_();
     return;
   }
@@ -348,7 +359,9 @@ struct DistillNode : Function<DistillNode> {
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_bounds,
                             const at::Tensor& k_bounds, double scale, const OptTensor& items, const OptTensor& pieces,
                             int64_t max_queries, int64_t tile_pairs, int64_t pairs) {
-  return PackedAttentionNode::apply(q, k, v, q_bounds, k_bounds, scale, items, pieces, max_queries, tile_pairs, pairs);
+  return PackedAttentionNode::apply(q, k, v, q_bounds, k_bounds, scale, items, pieces, max_queries, tile_pairs, pairs,
+                                    at::GradMode::is_enabled() &&
+                                        (q.requires_grad() || k.requires_grad() || v.requires_grad()));
 }
 
 std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,

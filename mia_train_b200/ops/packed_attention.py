@@ -9,7 +9,8 @@ the gradients, and so do rows behind the last sequence, which are not read.
 
 On CUDA in bf16 and fp16 with D % 8 == 0 and D <= 128 this is the native kernel, in fp32 a native kernel without
 tensor cores; statistics and sums are held in fp32. The probabilities and their gradients are rounded to the inputs'
-type on their way into the second matrix products. Sums have a fixed order: the same inputs give the same bits. What a
+type on their way into the second matrix products; what rounding takes from the output is kept for the backward pass (a
+second tensor of its size). Sums have a fixed order: the same inputs give the same bits. What a
 sequence holds reaches no other sequence's results, not even an infinity or NaN. On the CPU it is PyTorch math,
 sequence by sequence.
 """
@@ -25,7 +26,7 @@ import torch
 from ._native import native, use_native
 
 MAX_HEAD_DIM = 128
-MAX_FEW = 64  # queries of a sequence that the kernel for few queries takes
+MAX_FEW = 16  # queries of a sequence that the kernel for few queries takes
 PIECE = 512  # keys of a sequence that it takes at a time
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 

@@ -353,3 +353,36 @@ def test_few_queries_do_not_see_what_is_masked():
     k[2900:], v[2900:] = math.inf, math.nan
     got = packed_attention(q, k, v, seq)
     assert got[1].isnan().all() and torch.equal(got[0], clean[0]) and torch.equal(got[2:], clean[2:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lq,lk", [([3, 2], [0, 0]), ([0, 0], [4, 1]), ([], []), ([0], [0])], ids=str)
+def test_tensors_without_rows(lq, lk, dtype):
+    q, k, v, do = _inputs(lq, list(lk), 2, 1, 32, dtype)
+    for x, like in zip(_run(q, k, v, do, PackedSequences(lq, lk, device=DEV)), (q, q, k, v), strict=True):
+        assert x.shape == like.shape and (x == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("scale", [1e-13, 1e-8, 1e-4])
+def test_tiny_scales(scale, dtype):
+    """The row statistics divided by the scale pass the range of the values that the tensor core subtracts."""
+    lengths = [200, 60]
+    _compare(lengths, lengths, 2, 1, 64, dtype, False, scale=scale)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("size", [40.0, 400.0])
+def test_half_precision_scores_beyond_its_range(size, sign):
+    """Every score the same and far from 0: q . k is 1e5 and 1e7, P is uniform and its gradients are not 0."""
+    lengths = [150]
+    q, k, v, do = _inputs(lengths, lengths, 1, 1, 64, F16)
+    q, k = torch.full_like(q, size), torch.full_like(k, sign * size)
+    got = _run(q, k, v, do, PackedSequences(lengths, device=DEV))
+    want = do.double().mean(0, keepdim=True).expand_as(do)  # dv = P^T do with P = 1 / 150
+    # the scores are whole numbers below 2^24 and equal: P is off by the statistics' rounding, 2^-24 of 1.4e6 in units
+    # of log2 at most, then by half a step of fp16 in P and dv; 150 products of that
+    rel = 2.0**-24 * size * size * 64 * 0.125 * 1.45 * 2
+    bound = (rel + 2.0**-10) * do.double().abs().mean(0, keepdim=True) + 2.0**-11 * want.abs() + 2.0**-24
+    assert ((got[3].double() - want).abs() <= bound).all()
+    assert ((got[0].double() - v.double().mean(0, keepdim=True)).abs() <= (2.0**-10) * v.double().abs().mean(0, keepdim=True) * 2 + 2.0**-10).all()

@@ -175,3 +175,8 @@ def test_given_angles(far, dtype, layout):
     for got, x, turned in ((y[0], q, angles), (y[1], k, angles), (grads[0], dq, -angles), (grads[1], dk, -angles)):
         want = _turn(x.double(), turned, eye, layout, 1.0)
         _within(got, want, 16 * U * 2 * x.double().abs().amax(-1, keepdim=True), dtype)
+
+
+def test_heads_without_channels():
+    q = torch.zeros(2, 3, 2, 0, device=DEV, dtype=BF16)
+    assert rotary(q, q, torch.arange(3, device=DEV), torch.zeros(0, device=DEV))[0].shape == q.shape
