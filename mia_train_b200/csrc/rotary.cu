@@ -3,8 +3,8 @@
 //   angle[t, p] = sum_a position[t, a] F[a, p]
 //   y1 = amplitude (x1 cos - x2 sin),  y2 = amplitude (x2 cos + x1 sin)   for every pair (x1, x2) of the head
 //
-// (or the angles themselves are given), with the pairs (p, p + P) ("half") or (2 p, 2 p + 1) ("interleaved") of the first 2 P channels; the others are
-// copied. The gradient of x is the rotation of dy by the negative angles, that of the table
+// (or the angles themselves are given), with the pairs (p, p + P) ("half") or (2 p, 2 p + 1) ("interleaved") of the
+// first 2 P channels; the others are copied. The gradient of x is the rotation of dy by the negative angles, that of the table
 // dF[a, p] = sum_t position[t, a] sum_heads (dy2 y1 - dy1 y2).
 //
 // Angles, in turns (1 is 2 pi), where whole turns fall away for nothing: an integer position times the frequency as a
