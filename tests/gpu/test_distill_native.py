@@ -297,3 +297,21 @@ def test_second_derivatives_and_refusals():
     ):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_offsets_beyond_32_bits():
+    """The last of more than 2^31 logits give the same bits as in a tensor of their own (of 300 rows: fewer are summed by
+    more threads, in another order)."""
+    s = torch.zeros(33000, 65536, device=DEV, dtype=BF16)
+    s[-3:] = _logits(3, 65536, BF16)
+    near = s[-300:].clone()
+    for got, want in zip(top_logits(s, 5), top_logits(near, 5), strict=True):
+        assert torch.equal(got[-300:], want)
+    values, indices, _ = top_logits(s, 4)
+    w = torch.zeros(33000, device=DEV)
+    w[-3:] = 1.0
+    leaves = [s.requires_grad_(True), near.requires_grad_(True)]
+    losses = [top_logit_distillation(x, values[-len(x):], indices[-len(x):], weights=w[-len(x):], norm=3.0) for x in leaves]
+    assert torch.equal(*losses)
+    grads = [torch.autograd.grad(loss, x)[0] for loss, x in zip(losses, leaves, strict=True)]
+    assert torch.equal(grads[0][-300:], grads[1]) and not grads[0][:300].any() and grads[1][-3:].any()

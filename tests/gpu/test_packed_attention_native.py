@@ -386,3 +386,21 @@ def test_half_precision_scores_beyond_its_range(size, sign):
     bound = (rel + 2.0**-10) * do.double().abs().mean(0, keepdim=True) + 2.0**-11 * want.abs() + 2.0**-24
     assert ((got[3].double() - want).abs() <= bound).all()
     assert ((got[0].double() - v.double().mean(0, keepdim=True)).abs() <= (2.0**-10) * v.double().abs().mean(0, keepdim=True) * 2 + 2.0**-10).all()
+
+
+@pytest.mark.parametrize("last", [1, 200])
+def test_offsets_beyond_32_bits(last):
+    """Keys whose elements lie past 2^31 in a wide buffer give what they give at its start (tiles and few queries)."""
+    wide = torch.zeros(270000, 8192, device=DEV, dtype=BF16)
+    torch.manual_seed(0)
+    small = torch.randn(last + 300, 8192, device=DEV).to(BF16)
+    wide[-(last + 300):] = small
+    first = wide.shape[0] - small.shape[0]
+    views = [wide[:, 64 * i:64 * (i + 2)].view(-1, 2, 64) for i in (10, 40)]
+    q = torch.randn(1 + last, 2, 64, device=DEV).to(BF16)
+    do = torch.randn(1 + last, 2, 64, device=DEV).to(BF16)
+    got = _run(q, *views, do, PackedSequences([1, last], [first, last + 300], device=DEV))
+    near = [small[:, 64 * i:64 * (i + 2)].view(-1, 2, 64) for i in (10, 40)]
+    want, bound = _expected(q[1:], *near, do[1:], [last], [last + 300], False, 0.125, BF16)
+    for x, y, b in zip((got[0][1:], got[1][1:], got[2][first:], got[3][first:]), want, bound, strict=True):
+        assert ((x.double() - y).abs() <= b).all()
