@@ -404,3 +404,24 @@ def test_offsets_beyond_32_bits(last):
     want, bound = _expected(q[1:], *near, do[1:], [last], [last + 300], False, 0.125, BF16)
     for x, y, b in zip((got[0][1:], got[1][1:], got[2][first:], got[3][first:]), want, bound, strict=True):
         assert ((x.double() - y).abs() <= b).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_computed_again_leave_the_other_tile_of_their_block_alone(dtype, causal):
+    """Wide heads in enough tiles for two a block: a NaN and an infinity in V make neighbours' rows of one tile be computed
+    again while the other tile still goes through its keys. The clean sequences stay within the bounds."""
+    # 10 pairs of tiles of 16 heads; sequences end inside of tiles, and the second tile of a pair sees other and more keys
+    lengths = [100, 60, 900, 40, 1300, 130]
+    q, k, v, do = _inputs(lengths, lengths, 16, 4, 128, dtype)
+    want, bound = _expected(q, k, v, do, lengths, lengths, causal, 128**-0.5, dtype)
+    clean = torch.ones(sum(lengths), dtype=torch.bool, device=DEV)
+    for at, bad in ((1, math.nan), (3, math.inf)):  # whole sequences: causal or not, no clean row sees them
+        first = sum(lengths[:at])
+        v[first:first + lengths[at], :, 7] = bad
+        clean[first:first + lengths[at]] = False
+    o = packed_attention(q, k, v, PackedSequences(lengths, causal=causal, device=DEV))
+    raise_on_device_errors(DEV)
+    err = (o.double() - want[0]).abs()
+    assert torch.isfinite(o[clean]).all() and (err <= bound[0])[clean].all()
+    assert not torch.isfinite(o[~clean][..., 7]).any()
