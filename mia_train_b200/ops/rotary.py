@@ -18,7 +18,9 @@ the outputs share one contiguous buffer. `k` may be None. Gradients go to q, k a
 * "linear": positions are divided by `factor`.
 * "ntk": the base grows so that the last pair's frequency is divided by `factor` and the first pair's kept.
 * "yarn": pairs that turn more than `beta_fast` times over `original_length` are kept, those that turn less than
-  `beta_slow` times are divided by `factor`, with a linear ramp between; the amplitude is 0.1 ln(factor) + 1.
+  `beta_slow` times are divided by `factor`, with a linear ramp over the pairs between, whose ends are whole pairs (below
+  and above) within 0 .. rotary_dim - 1; the upper end may lie past the last pair, which then is not divided in full. The
+  amplitude is 0.1 ln(factor) + 1.
 """
 
 from __future__ import annotations
@@ -71,7 +73,7 @@ def rotary_frequencies(
                              f"{original_length}, {beta_slow} and {beta_fast}")
         # a pair turns original_length * freq / (2 pi) times: solved for the pair's number
         low, high = (p * math.log(original_length / (turns * 2 * math.pi)) / math.log(base) for turns in (beta_fast, beta_slow))
-        low, high = max(math.floor(low), 0), min(math.ceil(high), p - 1)
+        low, high = max(math.floor(low), 0), min(math.ceil(high), rotary_dim - 1)
         ramp = ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq * (1 - ramp) + freq / factor * ramp
         amplitude = 0.1 * math.log(factor) + 1.0

@@ -227,3 +227,31 @@ def test_rotation_by_given_angles():
                 lambda: rotary(q, k, torch.randn(5, 5), None), lambda: rotary(q, k, angles.requires_grad_(True), None)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("dim,base,length", [(64, 100.0, 4096), (128, 10000.0, 131072), (64, 100.0, 200), (128, 10000.0, 4096),
+                                             (6, 10000.0, 131072), (32, 10000.0, 20)])
+def test_yarn_divides_only_pairs_that_turn_seldom(dim, base, length):
+    """A pair's share of the division by the number of its turns, pair by pair. Where the ramp ends past the last pair (a small
+    base, a long trained length) the last pairs turn often and are not divided in full."""
+    factor, fast, slow = 8.0, 32.0, 1.0
+    plain, _ = rotary_frequencies(dim, base)
+    yarn, _ = rotary_frequencies(dim, base, scaling="yarn", factor=factor, original_length=length)
+
+    def pair_of(turns):  # the pair that turns so often, not a whole number
+        return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), dim - 1)
+    for n, (a, b) in enumerate(zip(plain.tolist(), yarn.tolist(), strict=True)):
+        share = min(max((n - low) / (high - low), 0.0), 1.0)  # of the division
+        assert b == pytest.approx(a * (1 - share) + a / factor * share, rel=1e-12)
+        if length * a / (2 * math.pi) >= fast:
+            assert share <= 1 / (high - low)  # the lower end is a whole pair
+
+
+def test_yarn_values_known_in_advance():
+    """By hand: base 100, 64 channels, length 4096: the ramp is from pair 20 to 46, the last pair (31) 11 / 26 along it."""
+    plain, _ = rotary_frequencies(64, 100.0)
+    yarn, _ = rotary_frequencies(64, 100.0, scaling="yarn", factor=8.0, original_length=4096)
+    assert (yarn[31] / plain[31]).item() == pytest.approx(1 - 11 / 26 * 7 / 8, rel=1e-12)
+    assert torch.equal(yarn[:21], plain[:21])
