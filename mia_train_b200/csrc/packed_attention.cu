@@ -229,8 +229,9 @@ __global__ void __launch_bounds__(kFewThreads) packed_few_kernel(PackedProblem P
     }
     if (few.partial == nullptr) {
       const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
-      store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, sum == 0.f ? 0.f : value / sum);
-      if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
+      const int2 b = P.q_bounds[i];
+      store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, row_value(b.y > b.x, value, sum));
+      if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = row_lse(b.y > b.x, top, sum);
     } else {
       float* part = few.partial + (((int64_t)blockIdx.x * P.Hk + hk) * few.rows + row) * (P.D + 2);
       part[ch] = value;
@@ -263,8 +264,9 @@ __global__ void __launch_bounds__(128) packed_few_join_kernel(PackedProblem P, P
     if (ch < P.D) value += f * part[n * step + ch];
   }
   const int i = item.x + row / P.group, h = hk * P.group + row % P.group;
-  if (ch < P.D) store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, sum == 0.f ? 0.f : value / sum);
-  if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = sum == 0.f ? INFINITY : top + log2f(sum);
+  const int2 b = P.q_bounds[i];
+  if (ch < P.D) store_low<T>(o, (T*)P.o_low, ((int64_t)i * P.Hq + h) * P.D + ch, row_value(b.y > b.x, value, sum));
+  if (ch == 0) lse[(int64_t)h * P.lse_stride + i] = row_lse(b.y > b.x, top, sum);
 }
 
 int64_t blocks_of(int64_t items, int per) { return (items + per - 1) / per; }

@@ -32,8 +32,17 @@ __device__ __forceinline__ float dot_row(const float* a, const T* b, int D) {
   return s;
 }
 
+// What a row's sums give, and its lse. A sum of weights of 0 is a row that sees no key (zeros, and an lse of +inf, with
+// which every later exp2(s - lse) is 0) or one whose scores are all -inf (NaN, as 0 / 0).
+__device__ __forceinline__ float row_value(bool sees, float value, float sum) {
+  return sum != 0.f ? value / sum : sees ? NAN : 0.f;
+}
+__device__ __forceinline__ float row_lse(bool sees, float m, float sum) {
+  return sum != 0.f ? m + log2f(sum) : sees ? NAN : INFINITY;
+}
+
 // o_i = sum_j p_ij v_j with p the softmax of scale q_i . k_j, by running maximum and sum. lse is m + log2(l) in units
-// of log2, +inf where no key has any weight (then every later exp2(s - lse) is 0).
+// of log2.
 template <typename T>
 __device__ void forward_row(const T* q, const T* k, const T* v, int64_t k_row, int64_t v_row, int lo, int hi, int D,
                             float scale_log2, float* scratch, int lane, float (&o)[4], float& lse) {
@@ -67,10 +76,10 @@ __device__ void forward_row(const T* q, const T* k, const T* v, int64_t k_row, i
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = row_value(hi > lo, 1.f, l);
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] *= inv;
-  lse = l == 0.f ? INFINITY : m + log2f(l);
+  lse = row_lse(hi > lo, m, l);
   __syncwarp();
 }
 

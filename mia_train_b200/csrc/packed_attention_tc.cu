@@ -508,9 +508,12 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
       mbar_arrive(&p_full[t]);
     }
     if (ok && j1 > j0) ok = warp_wait(&o_full[t], (j1 - j0 - 1) & 1, abort_flag, err);
+    const bool sees = mine.y > mine.x;
+    // Every score that the row sees is -inf: the exponentials of the FMA pipe, which end at 2^-126, are not 0 then.
+    if (m == -INFINITY) l = 0.f;
     if (ok) {
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = row_value(sees, 1.f, l);
       T* dst = o + ((int64_t)(real ? row : 0) * P.Hq + h) * P.D;
       float bad = 0.f;
 #pragma unroll 1
@@ -527,10 +530,10 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
         bad += store16<T>(dst + c * 16, w, inv, real, both);
         if (P.o_low != nullptr) store16_low<T>((T*)P.o_low + (dst - o) + c * 16, w, inv, real, both);
       }
-      if (real) lse[(int64_t)h * P.lse_stride + row] = l == 0.f ? INFINITY : m + log2f(l);
+      if (real) lse[(int64_t)h * P.lse_stride + row] = row_lse(sees, m, l);
       // rows that a masked neighbour's infinity or NaN may have reached
       const bool partly = mine.x > from + j0 * kRows || mine.y < from + j1 * kRows;
-      uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad && l == l);
+      uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad && inv == inv);
       if (again != 0) {
         __syncwarp();
         float* scratch = reinterpret_cast<float*>(smem + L::kScratch) + warp * kRowScratch;

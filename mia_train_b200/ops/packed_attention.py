@@ -5,7 +5,7 @@ used by every layer. `packed_attention(q, k, v, sequences, scale)` takes q (Tq, 
 divisor of Hq (query head h reads key head h // (Hq // Hk)), and returns (Tq, Hq, D): every query attends to the
 keys of its own sequence. With `causal`, the last query of a sequence sees its last key, the one before it one key
 less: query i of Lq sees the keys j <= i + Lk - Lq of Lk. A query that sees no key gives zeros and takes no part in
-the gradients, and so do rows behind the last sequence, which are not read.
+the gradients, and so do rows behind the last sequence, which are not read. A query whose scores are all -inf is 0 / 0: NaN.
 
 On CUDA in bf16 and fp16 with D % 8 == 0 and D <= 128 this is the native kernel, in fp32 a native kernel without
 tensor cores; statistics and sums are held in fp32. The probabilities and their gradients are rounded to the inputs'

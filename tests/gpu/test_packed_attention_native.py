@@ -425,3 +425,27 @@ def test_rows_computed_again_leave_the_other_tile_of_their_block_alone(dtype, ca
     err = (o.double() - want[0]).abs()
     assert torch.isfinite(o[clean]).all() and (err <= bound[0])[clean].all()
     assert not torch.isfinite(o[~clean][..., 7]).any()
+
+
+BLIND = [([256], None, 2, 1, 64), ([130, 300], None, 2, 2, 64), ([130, 300], None, 2, 1, 128), ([900, 1300, 300], None, 16, 16, 128),
+         ([1, 2, 3], [600, 700, 40], 2, 1, 64), ([2, 1], [300, 200], 3, 1, 32)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("lq,lk,hq,hk,d", BLIND, ids=str)
+def test_a_query_whose_scores_are_all_minus_infinity_gives_nan(lq, lk, hq, hk, d, dtype, causal):
+    """0 / 0 in every kernel, in blocks with and without a mask; what does not see the query is not touched."""
+    lk = lq if lk is None else lk
+    q, k, v, do = _inputs(lq, list(lk), hq, hk, d, dtype)
+    k[..., 0] = k[..., 0].abs() + 0.25
+    bad = lq[0] - 1  # the first sequence's last query sees all of its keys, causal or not
+    want, bound = _expected(q, k, v, do, lq, lk, causal, d**-0.5, dtype)
+    q[bad, :, 0] = -math.inf
+    got = _run(q, k, v, do, PackedSequences(lq, lk, causal=causal, device=DEV))
+    raise_on_device_errors(DEV)
+    assert got[0][bad].isnan().all() and got[1][bad].isnan().all()
+    assert got[2][:lk[0]].isnan().all() and got[3][:lk[0]].isnan().all()
+    rows = torch.arange(sum(lq), device=DEV) != bad
+    for x, y, b, keep in zip(got, want, bound, (rows, rows, slice(lk[0], None), slice(lk[0], None)), strict=True):
+        assert ((x.double() - y).abs() <= b)[keep].all()

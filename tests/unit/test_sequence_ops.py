@@ -255,3 +255,10 @@ def test_yarn_values_known_in_advance():
     yarn, _ = rotary_frequencies(64, 100.0, scaling="yarn", factor=8.0, original_length=4096)
     assert (yarn[31] / plain[31]).item() == pytest.approx(1 - 11 / 26 * 7 / 8, rel=1e-12)
     assert torch.equal(yarn[:21], plain[:21])
+
+
+def test_a_query_whose_scores_are_all_minus_infinity_gives_nan():
+    q, k = torch.randn(5, 2, 8), torch.rand(5, 1, 8) + 0.1
+    q[1, :, 0] = -math.inf
+    out = packed_attention(q, k, k, PackedSequences([2, 3], device="cpu"))
+    assert out[1].isnan().all() and out[[0, 2, 3, 4]].isfinite().all()
