@@ -562,9 +562,10 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
 
 // --------------------------------------------------------------------------------- backward: delta
 // delta_i = do_i . o_i, with o as it was before rounding: where a row has few keys, dP - delta is a small difference. A CTA
-// owns 128 rows of a head, 16 lanes a row. For fp16 also the largest norm of the
-// block's do rows: dS = p (dP - delta) is near |do| times a probability and would fall among fp16's subnormals, so
-// the backward kernels scale it by a power of two of that size.
+// owns 128 rows of a head, 16 lanes a row. For fp16 also the norm of every do row and the block's largest: dS = p (dP - delta)
+// is near |do| times a probability and would fall among fp16's subnormals, so the backward kernels scale it by a power of two
+// of that size: that of the query's own row for dQ, for dK that of the largest among the queries that see the key, so that no
+// other sequence's gradients set the step that this one's are rounded to.
 //
 // The kernel for dK and dV has its queries along the columns; a statistic per column read from shared memory by every
 // thread would take 4 cycles of its port for each 4 columns and warp, as long as the exponentials, and in the way of the
@@ -633,6 +634,7 @@ __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restric
       const int64_t at = (int64_t)h * stride + i;
       if (lane == 0) delta[at] = s;
       channels[lane * rows + at] = as_channels<T>(lane == 0 ? -lse[at] * inv_scale_log2 : -s);
+      if (std::is_same_v<T, __half> && lane == 0) norms[at] = n <= 3e38f ? sqrtf(n) : 0.f;
     }
     if (n <= 3e38f) most = fmaxf(most, n);
   }
@@ -641,17 +643,49 @@ __global__ void __launch_bounds__(256) packed_delta_tc_kernel(const T* __restric
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
-      norms[(int64_t)h * (stride / kRows) + block] = sqrtf(most);
+      norms[rows + (int64_t)h * (stride / kRows) + block] = sqrtf(most);
     }
   }
 }
 
-// 2^-e for a largest norm of do near 2^e (fp16); dS is then at most 2^8 times the rows of v.
+// 2^-e for a (largest) norm of do near 2^e (fp16); dS is then at most 2^8 times the rows of v.
 __device__ __forceinline__ float ds_factor(float norm) {
   if (!(norm > 0.f)) return 1.f;
   return exp2f(-fminf(fmaxf(ceilf(log2f(norm)), -100.f), 100.f));
 }
 constexpr float kHalfShift = 8.f;  // fp16: P is kept times 2^8
+
+// The largest norm of the do rows in [mine.x, mine.y) of `heads` heads from `first`; 0 for none. A whole warp calls it, its
+// lanes with the bounds of consecutive keys: lanes whose queries end together (a sequence's keys) share all but the first of
+// them, and whole blocks of 128 queries have theirs in `blocks`.
+__device__ __forceinline__ float largest_norm(const float* norms, const float* blocks, int stride, int first, int heads,
+                                              int2 mine, int lane) {
+  float top = 0.f;
+  uint32_t left = __ballot_sync(0xffffffffu, mine.y > mine.x);
+  while (left != 0) {
+    const int leader = __ffs(left) - 1, end = __shfl_sync(0xffffffffu, mine.y, leader);
+    const bool member = mine.y > mine.x && mine.y == end;
+    const uint32_t members = __ballot_sync(0xffffffffu, member);
+    left &= ~members;
+    const int begin = __shfl_sync(0xffffffffu, mine.x, leader);
+    const int common = __shfl_sync(0xffffffffu, mine.x, 31 - __clz(members));  // the bounds never fall
+    const int b0 = (common + kRows - 1) / kRows, b1 = end / kRows;             // whole blocks
+    const int head_end = b0 < b1 ? b0 * kRows : end, tail = b0 < b1 ? b1 * kRows : end;
+    for (int h = first; h < first + heads; ++h) {
+      const float *row = norms + (int64_t)h * stride, *block = blocks + (int64_t)h * (stride / kRows);
+      float m = 0.f;
+      for (int i = common + lane; i < head_end; i += 32) m = fmaxf(m, row[i]);
+      for (int b = b0 + lane; b < b1; b += 32) m = fmaxf(m, block[b]);
+      for (int i = tail + lane; i < end; i += 32) m = fmaxf(m, row[i]);
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+      if (member) top = fmaxf(top, m);
+      for (int i = begin; i < common; ++i)
+        if (member && i >= mine.x) top = fmaxf(top, row[i]);
+    }
+  }
+  return top;
+}
 
 // ------------------------------------------------------------------------------------ backward: dQ
 // A CTA owns 128 queries of one head and goes through their keys. Two groups of four warps (thread = query) take the
@@ -815,7 +849,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int64_t stat = (int64_t)h * P.lse_stride + (real ? row : r0);
     const float lse_row = lse[stat], delta_row = delta[stat];
     const float shift = kHalf ? lse_row - kHalfShift : lse_row;
-    const float factor = kHalf ? ds_factor(norms[(int64_t)h * (P.lse_stride / kRows) + r0 / kRows]) : 1.f;
+    const float factor = kHalf ? ds_factor(norms[stat]) : 1.f;
     const float scale_log2 = P.scale * kLog2e;
     const f32x2 scale2 = pair_of(scale_log2, scale_log2), shift2 = pair_of(-shift, -shift);
     const f32x2 delta2 = pair_of(-delta_row, -delta_row), factor2 = pair_of(factor, factor);
@@ -1138,12 +1172,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int all_lo = P.k_bounds[min(k0 + kRows, P.Tk) - 1].x, all_hi = P.k_bounds[k0].y;
     const float scale_log2 = P.scale * kLog2e;
     float factor = 1.f;
-    if constexpr (kHalf) {
-      float top = 0.f;
-      for (int i = 0; i < steps; ++i)
-        top = fmaxf(top, norms[(int64_t)(g * P.group + i / per_head) * (P.lse_stride / kRows) + qb0 + i % per_head]);
-      factor = ds_factor(top);
-    }
+    if constexpr (kHalf)
+      factor = ds_factor(largest_norm(norms, norms + (int64_t)P.Hq * P.lse_stride, P.lse_stride, g * P.group, P.group, mine, lane));
     const float shift = kHalf ? kHalfShift : 0.f;
     const f32x2 scale2 = pair_of(scale_log2, scale_log2), shift2 = pair_of(shift, shift), factor2 = pair_of(factor, factor);
     bool ok = true;

@@ -44,7 +44,7 @@ cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* d
                             float* delta, void* dq, void* dk, void* dv, cudaStream_t stream);
 
 // The tensor-core kernels, where packed_tc_ok: same arguments; channels (2, Hq, lse_stride, 8) of the inputs' type is
-// scratch, and for fp16 norms (Hq, lse_stride / 128) fp32.
+// scratch, and for fp16 norms, (Hq, lse_stride) fp32 and behind them (Hq, lse_stride / 128).
 bool packed_tc_ok(const PackedProblem& P);
 cudaError_t packed_fwd_tc(const PackedProblem& P, void* o, float* lse, int* err, cudaStream_t stream);
 cudaError_t packed_bwd_tc(const PackedProblem& P, const void* o, const void* dout, HeadRows ds, const float* lse,

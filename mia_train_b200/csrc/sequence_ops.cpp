@@ -165,7 +165,7 @@ struct PackedAttentionNode : Function<PackedAttentionNode> {
     if (P.Tq == 0 || P.Tk == 0) {
       for (at::Tensor* x : {&dq, &dk, &dv}) x->zero_();
     } else if (packed_tc_ok(P)) {
-      at::Tensor norms = at::empty({P.type == kSeqF16 ? s[6].numel() / 128 : 0}, s[6].options());
+      at::Tensor norms = at::empty({P.type == kSeqF16 ? s[6].numel() / 128 * 129 : 0}, s[6].options());
       at::Tensor channels = at::empty({2 * s[6].numel() * 8}, s[0].options());
       C10_CUDA_CHECK(packed_bwd_tc(P, s[5].data_ptr(), dout.data_ptr(), rows_of(dout), lse, delta.data_ptr<float>(),
                                    channels.data_ptr(), norms.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

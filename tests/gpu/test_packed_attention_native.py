@@ -449,3 +449,40 @@ def test_a_query_whose_scores_are_all_minus_infinity_gives_nan(lq, lk, hq, hk, d
     rows = torch.arange(sum(lq), device=DEV) != bad
     for x, y, b, keep in zip(got, want, bound, (rows, rows, slice(lk[0], None), slice(lk[0], None)), strict=True):
         assert ((x.double() - y).abs() <= b)[keep].all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hq,hk,d", [([60, 60], 1, 1, 64), ([130, 1, 40, 300], 4, 2, 64), ([100, 700, 90], 2, 1, 128),
+                                             ([0, 520, 3, 0, 257], 3, 3, 32)], ids=str)
+def test_gradients_do_not_depend_on_other_sequences_gradients(lengths, hq, hk, d, dtype, causal):
+    """The first non-empty sequence's incoming gradients are 2^-9, the others' 2^4 (fp16 has 2^-24 to 2^15): its own results
+    are within the bounds of its own size, and the same bits whatever the others' are."""
+    q, k, v, do = _inputs(lengths, lengths, hq, hk, d, dtype)
+    seq = PackedSequences(lengths, causal=causal, device=DEV)
+    own = slice(0, next(n for n in lengths if n))
+    do[own] *= 2.0**-9
+    first = _run(q, k, v, do, seq)
+    do[own.stop:] *= 16
+    got = _run(q, k, v, do, seq)
+    raise_on_device_errors(DEV)
+    want, bound = _expected(*(x[own] for x in (q, k, v, do)), [own.stop], [own.stop], causal, d**-0.5, dtype)
+    for x, y, z, b in zip(got, first, want, bound, strict=True):
+        assert torch.equal(x[own], y[own])
+        assert ((x[own].double() - z).abs() <= b).all()
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 1)])
+def test_half_precision_gradients_of_late_queries(hq, hk):
+    """Causal, do falls from 2^4 at the first queries to 2^-10 at the last: keys that only small gradients reach keep them."""
+    n = 600
+    q, k, v, do = _inputs([n], [n], hq, hk, 64, F16)
+    do *= torch.exp2(torch.linspace(4, -10, n, device=DEV))[:, None, None].half()
+    seq = PackedSequences([n], causal=True, device=DEV)
+    got = _run(q, k, v, do, seq)
+    # with gradients of the last 200 queries alone, the bounds of whose size hold for the last 200 keys
+    late = do.clone()
+    late[:400] = 0
+    want, bound = _expected(q, k, v, late, [n], [n], True, 0.125, F16)
+    for x, y, b in zip(got[1:], want[1:], bound[1:], strict=True):
+        assert ((x.double() - y).abs() <= b)[400:].all()
