@@ -53,9 +53,11 @@ class PackedSequences:
     """Lengths of sequences laid end to end, and with them which query sees which key.
 
     `lengths` are the query rows of every sequence, `key_lengths` its key rows (the same where None). Built on the
-    host: lengths on a CUDA device are read back first. The tables go to `device` before the constructor returns.
+    host: lengths on a CUDA device are read back first. The tables go to `device` before the constructor returns. Made in
+    inference mode, a plan serves training too.
     """
 
+    @torch.inference_mode(False)
     def __init__(
         self,
         lengths: Sequence[int] | torch.Tensor,

@@ -69,3 +69,17 @@ def test_distilling_a_small_encoder_from_stored_logits():
     for a, b in zip(got, want, strict=True):
         # fp32 throughout: sums of at most 5000 terms, errors of 2^-24 a term growing like their root, few steps deep
         assert (a - b).norm() <= 2.0**-16 * b.norm()
+
+
+def test_packed_crops_train_after_an_evaluation_in_inference_mode():
+    kw = dict(img_size=32, patch_size=8, in_chans=1, embed_dim=128, depth=2, num_heads=2, n_storage_tokens=4)
+    torch.manual_seed(0)
+    model = DinoVisionTransformer3D(packed_crops=True, **kw).to(DEV)
+    crops = [torch.randn(2, 1, 32, 32, 32, device=DEV), torch.randn(6, 1, 16, 16, 16, device=DEV)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with torch.inference_mode():
+            want = model.forward_features(crops, [None, None])
+        out = model.forward_features(crops, [None, None])
+        sum(o["x_norm_patchtokens"].float().sin().mean() for o in out).backward()
+    assert all(torch.equal(a["x_prenorm"], b["x_prenorm"]) for a, b in zip(want, out, strict=True))
+    assert model.blocks[0].attn.qkv.weight.grad.isfinite().all()

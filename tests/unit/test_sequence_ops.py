@@ -262,3 +262,11 @@ def test_a_query_whose_scores_are_all_minus_infinity_gives_nan():
     q[1, :, 0] = -math.inf
     out = packed_attention(q, k, k, PackedSequences([2, 3], device="cpu"))
     assert out[1].isnan().all() and out[[0, 2, 3, 4]].isfinite().all()
+
+
+def test_plans_made_in_inference_mode_serve_training():
+    """Autograd does not save tensors that were made in inference mode."""
+    with torch.inference_mode():
+        own = PackedSequences([5, 0, 3], [700, 2, 9], device="cpu")
+    assert own.items is not None
+    assert not any(t.is_inference() for t in (own.q_bounds, own.k_bounds, own.items, own.pieces))
