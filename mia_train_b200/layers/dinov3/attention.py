@@ -22,8 +22,8 @@ one kernel. `proj_drop` > 0 drops elements of the projected output in training, 
 from __future__ import annotations
 
 import contextlib
-import functools
 import math
+from collections import OrderedDict
 from collections.abc import Iterator
 from typing import Any
 
@@ -34,7 +34,7 @@ import torch.nn.functional as F
 from ...ops._native import reference_math
 from ...ops.attention import rope_attention
 from ...ops.dropout import dropout
-from ...ops.packed_attention import MAX_HEAD_DIM, PackedSequences, packed_attention
+from ...ops.packed_attention import MAX_HEAD_DIM, PackedSequences, capturing, packed_attention
 from ...ops.qk_norm import qk_norm_rope, qk_norm_rope_attention
 from ...ops.rotary import rotary
 from ...parallel.tensor_parallel import rope_to_tp
@@ -82,10 +82,29 @@ def half_pairs(head_dim: int, device: torch.device) -> torch.Tensor:
     return torch.stack([idx, idx + half], dim=1).to(device)
 
 
-@functools.lru_cache(maxsize=64)
-def _crop_sequences(shapes: tuple[tuple[int, int], ...], device: torch.device) -> PackedSequences:
-    """The sequences of crops of `shapes` (samples, tokens), which a run meets again in every step."""
-    return PackedSequences([n for b, n in shapes for _ in range(b)], device=device)
+class CropPlans:
+    """The `PackedSequences` of the crop shapes that a model meets step after step: the last `most` of them, and for good
+    those that a captured step reads, whose replays find the tables by their addresses."""
+
+    def __init__(self, most: int = 64) -> None:
+        self.most = most
+        self._recent: OrderedDict[tuple, PackedSequences] = OrderedDict()
+        self._captured: dict[tuple, PackedSequences] = {}
+
+    def __call__(self, shapes: tuple[tuple[int, int], ...], device: torch.device) -> PackedSequences:
+        """The sequences of crops of `shapes` (samples, tokens)."""
+        key = (shapes, device)
+        if key in self._captured:
+            return self._captured[key]
+        if key not in self._recent:
+            self._recent[key] = PackedSequences([n for b, n in shapes for _ in range(b)], device=device)
+            if len(self._recent) > self.most:
+                self._recent.popitem(last=False)
+        self._recent.move_to_end(key)
+        if capturing(device):
+            self._captured[key] = self._recent.pop(key)
+            return self._captured[key]
+        return self._recent[key]
 
 
 class SelfAttention(nn.Module):
@@ -119,6 +138,7 @@ class SelfAttention(nn.Module):
         self.q_norm = RMSNorm(self.head_dim).to(device) if qk_norm else None
         self.k_norm = RMSNorm(self.head_dim).to(device) if qk_norm else None
         self._pairs: torch.Tensor | None = None
+        self.crop_plans = CropPlans()  # a model gives its blocks one in common
 
     # -- projections ----------------------------------------------------------------------
     def _qkv(self, x: torch.Tensor) -> torch.Tensor:
@@ -206,7 +226,7 @@ class SelfAttention(nn.Module):
                                                        pairs, eps))
         elif angles is not None:
             q, k = rotary(q, k, angles, None)
-        return packed_attention(q, k, v, _crop_sequences(shapes, qkv.device), self.scale).reshape(-1, c)
+        return packed_attention(q, k, v, self.crop_plans(shapes, qkv.device), self.scale).reshape(-1, c)
 
     def forward_list(self, x_list, attn_bias=None, rope_list=None, residual_list=None, gamma=None) -> list[torch.Tensor]:
         assert len(x_list) == len(rope_list)

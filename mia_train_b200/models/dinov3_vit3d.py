@@ -31,6 +31,7 @@ from typing import Any, Literal
 import torch
 import torch.nn as nn
 
+from ..layers.dinov3.attention import CropPlans
 from ..layers.dinov3.block import SelfAttentionBlock, _norm
 from ..layers.dinov3.config import dtype_dict, ffn_layer_dict, init_weights_vit, norm_layer_dict
 from ..layers.dinov3.ffn import SwiGLUFFN
@@ -151,8 +152,10 @@ class DinoVisionTransformer3D(BaseModel):
             )
             for _ in range(depth)
         )
+        plans = CropPlans()
         for blk in self.blocks:
             blk.attn.packed_crops = packed_crops
+            blk.attn.crop_plans = plans
         self.chunked_blocks = False
         self.norm = norm_cls(embed_dim)
         self.untie_cls_and_patch_norms = untie_cls_and_patch_norms

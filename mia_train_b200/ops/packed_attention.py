@@ -49,12 +49,21 @@ def _host_lengths(lengths: Sequence[int] | torch.Tensor, name: str) -> np.ndarra
     return out
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether what this thread launches on `device` now goes into a CUDA graph."""
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class PackedSequences:
     """Lengths of sequences laid end to end, and with them which query sees which key.
 
     `lengths` are the query rows of every sequence, `key_lengths` its key rows (the same where None). Built on the
-    host: lengths on a CUDA device are read back first. The tables go to `device` before the constructor returns. Made in
-    inference mode, a plan serves training too.
+    host: lengths on a CUDA device are read back first. The tables go to `device` before the constructor returns, which
+    waits for that: it cannot be called while a graph is captured. A graph that was captured with a plan reads its tables in
+    every replay, so the plan has to stay as long as the graph. Made in inference mode, a plan serves training too.
     """
 
     @torch.inference_mode(False)
@@ -77,6 +86,8 @@ class PackedSequences:
         self.device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        if capturing(self.device):
+            raise RuntimeError("PackedSequences are copied from the host: make them before a graph is captured")
         q0, k0 = np.concatenate([[0], np.cumsum(lq)[:-1]]), np.concatenate([[0], np.cumsum(lk)[:-1]])
         if len(lq) == 0:
             q0 = k0 = lq

@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover - collected on CPU, skipped there
     pytest.skip("needs CUDA", allow_module_level=True)
 
+from mia_train_b200.layers.dinov3.attention import SelfAttention  # noqa: E402
 from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D  # noqa: E402
 from mia_train_b200.ops._native import reference_math  # noqa: E402
 from mia_train_b200.ops.distill import top_logit_distillation, top_logits  # noqa: E402
@@ -83,3 +84,27 @@ def test_packed_crops_train_after_an_evaluation_in_inference_mode():
         sum(o["x_norm_patchtokens"].float().sin().mean() for o in out).backward()
     assert all(torch.equal(a["x_prenorm"], b["x_prenorm"]) for a, b in zip(want, out, strict=True))
     assert model.blocks[0].attn.qkv.weight.grad.isfinite().all()
+
+
+def test_a_captured_block_keeps_its_plan():
+    """Replayed after more crop shapes than a model keeps plans for, with the memory that theirs may have left written to."""
+    torch.manual_seed(0)
+    attn = SelfAttention(128, num_heads=2).to(DEV, torch.bfloat16)
+    attn.packed_crops = True
+    crops = [torch.randn(2, 200, 128, device=DEV, dtype=torch.bfloat16), torch.randn(3, 90, 128, device=DEV, dtype=torch.bfloat16)]
+    with torch.no_grad():
+        want = attn.forward_list(crops, rope_list=[None, None])
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            got = attn.forward_list(crops, rope_list=[None, None])
+            with pytest.raises(RuntimeError, match="before a graph is captured"):
+                attn.forward_list([x[:, :7] for x in crops], rope_list=[None, None])
+        for n in range(1, 81):
+            attn.forward_list([crops[0][:, :n], crops[1][:, :n]], rope_list=[None, None])
+        junk = [torch.zeros(n, device=DEV, dtype=torch.int32) for n in (512, 1024, 1340, 2048) for _ in range(200)]
+        for x in got:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+    assert len(junk) == 800 and all(torch.equal(a, b) for a, b in zip(got, want, strict=True))

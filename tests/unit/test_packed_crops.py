@@ -3,11 +3,14 @@ by the 0.02 of the initial class token, alone leave some gradients with three di
 
 from __future__ import annotations
 
+from copy import deepcopy
+
 import pytest
 import torch
 
 from mia_train_b200.models.dinov3_vit import DinoVisionTransformer
 from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D
+from mia_train_b200.ops.packed_attention import PackedSequences
 
 KW = dict(patch_size=8, in_chans=1, embed_dim=48, depth=2, num_heads=2, n_storage_tokens=2, pos_embed_rope_dtype="fp32")
 
@@ -87,3 +90,45 @@ def test_the_packed_path_runs(monkeypatch):
     calls.clear()
     learned.forward_features(_crops(), [None, None])
     assert not calls or not learned.rope_embed.depth_scale.requires_grad
+
+
+def test_blocks_share_their_plans():
+    model = DinoVisionTransformer3D(img_size=16, packed_crops=True, **KW)
+    model.forward_features([x.float() for x in _crops()], [None, None])
+    shapes = ((2, 11), (5, 4))
+    plan = model.blocks[0].attn.crop_plans(shapes, torch.device("cpu"))
+    assert plan is model.blocks[1].attn.crop_plans(shapes, torch.device("cpu")) and len(model.blocks[0].attn.crop_plans._recent) == 1
+
+
+def test_plans_stay_as_long_as_a_captured_step_may_read_them(monkeypatch):
+    from mia_train_b200.layers.dinov3 import attention as module
+
+    cpu, plans = torch.device("cpu"), module.CropPlans(most=3)
+    first = plans(((2, 5),), cpu)
+    assert plans(((2, 5),), cpu) is first
+    monkeypatch.setattr(module, "capturing", lambda device: True)
+    assert plans(((2, 5),), cpu) is first
+    monkeypatch.setattr(module, "capturing", lambda device: False)
+    others = [plans(((1, n),), cpu) for n in range(1, 9)]
+    assert plans(((2, 5),), cpu) is first and plans(((1, 8),), cpu) is others[-1]
+    assert plans(((1, 1),), cpu) is not others[0]  # the others go, the longest unused first
+    assert plans._recent.keys() == {(((1, n),), cpu) for n in (1, 7, 8)}
+
+
+def test_plans_are_not_made_while_a_graph_is_captured(monkeypatch):
+    from mia_train_b200.ops import packed_attention as module
+
+    monkeypatch.setattr(module, "capturing", lambda device: True)
+    with pytest.raises(RuntimeError, match="before a graph is captured"):
+        PackedSequences([3], device="cpu")
+
+
+def test_a_copied_model_has_plans_of_its_own():
+    model = DinoVisionTransformer3D(img_size=16, packed_crops=True, **KW)
+    model.forward_features([x.float() for x in _crops()], [None, None])
+    copy = deepcopy(model)
+    mine, its = model.blocks[0].attn.crop_plans, copy.blocks[0].attn.crop_plans
+    assert its is not mine and its is copy.blocks[1].attn.crop_plans and its._recent.keys() == mine._recent.keys()
+    for a, b in zip(model.forward_features([x.float() for x in _crops()], [None, None]),
+                    copy.forward_features([x.float() for x in _crops()], [None, None]), strict=True):
+        assert torch.equal(a["x_prenorm"], b["x_prenorm"])
