@@ -76,6 +76,7 @@ class LinearKMaskedBias(nn.Linear):
         return F.linear(input, self.weight, self.masked_bias())
 
 
+@torch.inference_mode(False)  # blocks keep them, and autograd does not save what was made in inference mode
 def half_pairs(head_dim: int, device: torch.device) -> torch.Tensor:
     half = head_dim // 2
     idx = torch.arange(half, dtype=torch.int32)

@@ -108,3 +108,18 @@ def test_a_captured_block_keeps_its_plan():
         graph.replay()
         torch.cuda.synchronize()
     assert len(junk) == 800 and all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("packed", [False, True])
+def test_blocks_train_after_an_evaluation_in_inference_mode(packed, qk_norm):
+    """The channel pairs that blocks keep are saved for backward."""
+    model = DinoVisionTransformer3D(img_size=32, patch_size=8, in_chans=1, embed_dim=128, depth=1, num_heads=2, qk_norm=qk_norm,
+                                    packed_crops=packed).to(DEV)
+    crops = [torch.randn(2, 1, 32, 32, 32, device=DEV), torch.randn(6, 1, 16, 16, 16, device=DEV)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with torch.inference_mode():
+            model.forward_features(crops, [None, None])
+        out = model.forward_features(crops, [None, None])
+        sum(o["x_norm_patchtokens"].float().sin().mean() for o in out).backward()
+    assert model.blocks[0].attn.qkv.weight.grad.isfinite().all()

@@ -132,3 +132,10 @@ def test_a_copied_model_has_plans_of_its_own():
     for a, b in zip(model.forward_features([x.float() for x in _crops()], [None, None]),
                     copy.forward_features([x.float() for x in _crops()], [None, None]), strict=True):
         assert torch.equal(a["x_prenorm"], b["x_prenorm"])
+
+
+def test_channel_pairs_made_in_inference_mode_serve_training():
+    model = DinoVisionTransformer3D(img_size=16, **KW)
+    with torch.inference_mode():
+        model.forward_features([x.float() for x in _crops()], [None, None])
+    assert not model.blocks[0].attn._pairs.is_inference()
