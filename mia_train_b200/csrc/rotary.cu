@@ -42,12 +42,16 @@ __device__ __forceinline__ int64_t position_row(const RotaryParams& p, int64_t t
   return p.pos_b == 0 ? token % p.T : token;
 }
 
-// Frequency i in turns: a fraction of 2^64, or (high, low) fp32, as the positions are integers or not.
+// Frequency i in turns: a fraction of 2^64, or (high, low) fp32, as the positions are integers or not. A fraction of all
+// ones says that the frequency is not finite; none that is comes to that (64-bit floats below 1 end at 1 - 2^-53, and f - floor(f)
+// rounds to 1 itself for f just below 0, which is 0 of the next turn).
+constexpr uint64_t kNotFinite = ~uint64_t(0);
 __device__ __forceinline__ uint2 frequency(const RotaryParams& p, int i) {
   double f = p.freq64 ? ((const double*)p.freq)[i] : (double)((const float*)p.freq)[i];
   f *= 0.15915494309189533577;  // 1 / (2 pi)
   if (p.pos_type <= 1) {
-    const uint64_t u = (uint64_t)((f - floor(f)) * 18446744073709551616.0);  // 2^64; the fraction is below 1
+    const double part = f - floor(f);
+    const uint64_t u = !isfinite(f) ? kNotFinite : part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;  // 2^64
     return make_uint2((uint32_t)u, (uint32_t)(u >> 32));
   }
   const float hi = (float)f, lo = (float)(f - (double)hi);
@@ -64,12 +68,14 @@ __device__ __forceinline__ float2 turn(const RotaryParams& p, const uint2* table
     half = 2.f * (whole - rintf(whole));
   } else if (p.pos_type <= 1) {
     uint64_t u = 0;
+    bool finite = true;
     for (int a = 0; a < p.axes; ++a) {
       const uint2 f = table[a * p.P + i];
+      finite = finite && (f.x & f.y) != (uint32_t)kNotFinite;
       const int64_t x = p.pos_type == 0 ? ((const int64_t*)p.pos)[at + a] : (int64_t)((const int*)p.pos)[at + a];
       u += (uint64_t)x * ((uint64_t)f.y << 32 | f.x);
     }
-    half = (float)(int)((u + 0x80000000u) >> 32) * 4.6566128730773926e-10f;  // 2^-31
+    half = finite ? (float)(int)((u + 0x80000000u) >> 32) * 4.6566128730773926e-10f : NAN;  // 2^-31
   } else {
     float whole = 0.f, rest = 0.f;
     for (int a = 0; a < p.axes; ++a) {

@@ -180,3 +180,46 @@ def test_given_angles(far, dtype, layout):
 def test_heads_without_channels():
     q = torch.zeros(2, 3, 2, 0, device=DEV, dtype=BF16)
     assert rotary(q, q, torch.arange(3, device=DEV), torch.zeros(0, device=DEV))[0].shape == q.shape
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("table", [torch.float32, torch.float64])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, torch.float32, torch.float64])
+def test_frequencies_that_are_not_finite_give_nan(kind, table, layout):
+    """In their own pairs, at every position (0 too), in outputs and in gradients."""
+    q, k, positions, freq, dq, dk = _case(1, 40, 2, 1, 64, 32, 1, F32)
+    positions[0, 7] = 0
+    bad = {3: torch.nan, 9: torch.inf, 30: -torch.inf}
+    freq = freq.to(table)
+    for at, x in bad.items():
+        freq[0, at] = x
+    leaves = [q.detach().requires_grad_(True), k.detach().requires_grad_(True), freq[0].detach().requires_grad_(True)]
+    y = rotary(*leaves[:2], positions.squeeze(-1).to(kind), leaves[2], layout=layout)
+    grads = torch.autograd.grad(y, leaves, (dq, dk))
+    pair = torch.zeros(32, dtype=torch.bool, device=DEV)
+    pair[list(bad)] = True
+    channel = pair.repeat(2) if layout == "half" else pair.repeat_interleave(2)
+    for x in (*y, *grads[:2]):
+        assert x[..., channel].isnan().all() and x[..., ~channel].isfinite().all()
+    assert torch.equal(grads[2].isnan(), pair)
+
+
+@pytest.mark.parametrize("f", [-1e-20, -2.0**-60, 1e300, -3.25, 6.283185307179586])
+def test_frequencies_at_the_ends_of_a_turn(f):
+    q, k, positions, freq, dq, dk = _case(1, 40, 2, 1, 64, 32, 1, F32)
+    freq = torch.full((1, 32), f, device=DEV, dtype=torch.float64)
+    if abs(f) < 100:
+        _compare(q, k, positions, freq, dq, dk, "half", 1.0, False)
+    else:  # far beyond what 64 bits resolve: any angle, but a rotation
+        y, _ = rotary(q, k, positions.squeeze(-1), freq[0])
+        assert torch.allclose(y[..., :32] ** 2 + y[..., 32:] ** 2, q[..., :32] ** 2 + q[..., 32:] ** 2, rtol=1e-5)
+
+
+@pytest.mark.parametrize("far", [1.0, 1e5])
+def test_angles_that_are_not_finite_give_nan(far):
+    q = torch.randn(1, 5, 1, 8, device=DEV)
+    angles = far * torch.randn(5, 4, device=DEV)
+    angles[2, 1], angles[3, 2] = torch.nan, torch.inf
+    y, _ = rotary(q, None, angles, None)
+    bad = ~angles.isfinite().repeat(1, 2)
+    assert torch.equal(y[0, :, 0].isnan(), bad)
