@@ -343,6 +343,10 @@ __device__ __forceinline__ double value_at(const DistillParams& p, int64_t i) {
   return ((const double*)p.values)[i];
 }
 
+__device__ __forceinline__ double number_at(const void* x, bool wide, int i) {
+  return wide ? ((const double*)x)[i] : (double)((const float*)x)[i];
+}
+
 // The class of entry i, -1 where it names none.
 __device__ __forceinline__ int index_at(const DistillParams& p, int64_t i) {
   const int64_t at = p.index64 ? ((const int64_t*)p.indices)[i] : (int64_t)((const int*)p.indices)[i];
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) distill_fwd_kernel(Di
   __shared__ double sums[4 * (NT / 32)];
   __shared__ float red[2 * (NT / 32)];
   const int r = blockIdx.x;
-  const double w = p.weights != nullptr ? (double)p.weights[r] : 1.0;
+  const double w = p.weights != nullptr ? number_at(p.weights, p.weights64, r) : 1.0;
   if (w == 0.0) {
     if (threadIdx.x == 0) row_loss[r] = 0.0;
     return;
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(NT, NT == kMany ? 6 : 1) distill_fwd_kernel(Di
     all.join(top.m, top.l, c);
   }
   // the teacher's side: log-sum-exp of the given values, unless that of all of them came along
-  double lse_t = tail ? (double)p.lse[r] : 0.0;
+  double lse_t = tail ? number_at(p.lse, p.lse64, r) : 0.0;
   if (!tail) {
     float m = -INFINITY;
     for (int j = threadIdx.x; j < p.K; j += NT)
@@ -466,10 +470,10 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const float* __restrict__ grad,
                                                                T* __restrict__ ds) {
   __shared__ int at_of[kMaxGiven];
-  __shared__ float share_of[kMaxGiven];
+  __shared__ float share_of[kMaxGiven];  // off by 2^-25 of it: the student's probability beside it has the 2^-22 of exp2 in its sum
   const int r = p.R - 1 - blockIdx.x;  // the rows that the forward pass read last may still be in L2
   T* out = ds + (int64_t)r * p.V;
-  const double w = p.weights != nullptr ? (double)p.weights[r] : 1.0;
+  const double w = p.weights != nullptr ? number_at(p.weights, p.weights64, r) : 1.0;
   const int vec_ahead = min(p.V, (int)((8 - (reinterpret_cast<uintptr_t>(out) / sizeof(T)) % 8) % 8));
   if (w == 0.0) {
     for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(0.f);

@@ -94,10 +94,10 @@ struct DistillParams {
   int64_t s_row;
   const void* values;  // (R, K)
   const void* indices;
-  const float* lse;      // or null
-  const float* weights;  // or null
+  const void* lse;      // (R), or null
+  const void* weights;  // (R), or null
   SequenceType type, value_type;
-  bool index64;
+  bool index64, lse64, weights64;  // int64 indices; fp64 instead of fp32
   int R, V, K;
   double tau, teacher_tau, norm;
   double* stats;  // (R, 8)

@@ -301,8 +301,10 @@ DistillParams distill_params(const at::Tensor& s, const at::Tensor& values, cons
   p.s_row = s.stride(0);
   p.values = values.data_ptr();
   p.indices = indices.data_ptr();
-  p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
-  p.weights = weights.has_value() ? weights->data_ptr<float>() : nullptr;
+  p.lse = lse.has_value() ? lse->data_ptr() : nullptr;
+  p.weights = weights.has_value() ? weights->data_ptr() : nullptr;
+  p.lse64 = lse.has_value() && lse->scalar_type() == at::kDouble;
+  p.weights64 = weights.has_value() && weights->scalar_type() == at::kDouble;
   p.type = type_of(s);
   p.value_type = type_of(values);
   p.index64 = indices.scalar_type() == at::kLong;
@@ -316,6 +318,12 @@ DistillParams distill_params(const at::Tensor& s, const at::Tensor& values, cons
   return p;
 }
 
+// A number per row in fp32, or in fp64 if it came so: the rest of 1 is a difference of what the lse gives.
+OptTensor row_numbers(const OptTensor& x) {
+  if (!x.has_value()) return x;
+  return x->scalar_type() == at::kDouble ? x->contiguous() : x->to(at::kFloat).contiguous();
+}
+
 struct DistillNode : Function<DistillNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& student, const at::Tensor& values,
                             const at::Tensor& indices, const OptTensor& teacher_lse, const OptTensor& weights, double tau,
@@ -323,8 +331,7 @@ struct DistillNode : Function<DistillNode> {
     BelowAutograd below;
     const at::Tensor s = student.stride(1) == 1 || student.size(1) <= 1 ? student : student.contiguous();
     const at::Tensor t = values.contiguous(), at_ = indices.contiguous();
-    const OptTensor lse = teacher_lse.has_value() ? OptTensor(teacher_lse->to(at::kFloat).contiguous()) : OptTensor();
-    const OptTensor w = weights.has_value() ? OptTensor(weights->to(at::kFloat).contiguous()) : OptTensor();
+    const OptTensor lse = row_numbers(teacher_lse), w = row_numbers(weights);
     at::Tensor stats = at::empty({s.size(0), 8}, s.options().dtype(at::kDouble));
     at::Tensor loss = at::empty({}, s.options().dtype(at::kFloat));
     at::Tensor rows = at::empty({s.size(0)}, stats.options());

@@ -315,3 +315,32 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(*losses)
     grads = [torch.autograd.grad(loss, x)[0] for loss, x in zip(losses, leaves, strict=True)]
     assert torch.equal(grads[0][-300:], grads[1]) and not grads[0][:300].any() and grads[1][-3:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("weights", [None, F32, torch.float64])
+def test_a_rest_of_the_teacher_far_below_one(dtype, weights):
+    """The shares given sum to 1 - 3e-8 and the student is as sure: with teacher_lse in fp64 the others' gradient, which is
+    all rest, has the bound's digits. (In fp32 an lse near 30 is off by 1e-6, thirty times the rest.)"""
+    v = 3000
+    s = torch.zeros(3, v, device=DEV)
+    s[:, 0] = 40.0
+    teacher = _logits(3, v, F32).double()
+    teacher[:, 0] = 26.0
+    values, indices = teacher.topk(2, dim=1)
+    lse = torch.logsumexp(teacher, 1)
+    assert ((1 - (values - lse[:, None]).exp().sum(1)) < 1e-7).all()
+    w = torch.tensor([1.0, 0.0, 0.3], device=DEV, dtype=weights) if weights else None
+    _, grad = _check_distill(s.to(dtype), values, indices, 1.0, 1.0, lse, w)
+    if dtype != F16:  # the others' share of the rest: its bound says something
+        assert (grad[0, 1:] < 0).any()
+
+
+@pytest.mark.parametrize("kind", [BF16, F16, F32, torch.float64])
+def test_distill_types_of_lse_and_weights(kind):
+    s = _logits(3, 500, BF16)
+    values, indices = s.float().topk(5, dim=1)
+    lse, w = torch.logsumexp(s.double(), 1).to(kind) + 0.125, torch.tensor([0.5, 0.0, 2.0], device=DEV, dtype=kind)
+    _check_distill(s, values, indices, 1.0, 1.0, lse, w)
+    both = torch.stack([lse, w], 1)  # strided
+    _check_distill(s, values, indices, 1.0, 1.0, both[:, 0], both[:, 1])
