@@ -334,6 +334,7 @@ cudaError_t rotary_launch(RotaryParams p, const RotaryPlan& plan, SequenceType t
                                                : run((float*)nullptr);
   if (status != cudaSuccess || dfreq == nullptr) return status;
   const int per = p.axes * p.P;
+  if (per == 0) return cudaSuccess;  // no pairs: the table has no element
   rotary_sum_kernel<<<(per + 3) / 4, 128, 0, stream>>>(p.partial, (int)(plan.grid * plan.chunks), per, dfreq);
   return cudaGetLastError();
 }

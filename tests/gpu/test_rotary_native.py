@@ -223,3 +223,11 @@ def test_angles_that_are_not_finite_give_nan(far):
     y, _ = rotary(q, None, angles, None)
     bad = ~angles.isfinite().repeat(1, 2)
     assert torch.equal(y[0, :, 0].isnan(), bad)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("axes", [1, 3])
+@pytest.mark.parametrize("d", [64, 33])
+def test_a_learned_table_without_pairs(d, axes, layout):
+    """Nothing turns: the heads are copied, and the table's gradient has no element."""
+    _compare(*_case(2, 13, 3, 2, d, 0, axes, BF16), layout, 1.0, True)
