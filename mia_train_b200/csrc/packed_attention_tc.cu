@@ -78,6 +78,22 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   for (int g = 0; g < DP / 64; ++g) tma_load_3d(dst + g * (kRows * 128), map, bar, g * 64, row, h);
 }
 
+// Of `issued` loads that go through `stages` stages in turns, the first that may still be in flight; the ones before it have
+// been consumed, or their stages would not have been loaded again. A loader that gives up waits for [this, issued) before
+// shared memory is given back; the barrier of an earlier load has moved on to a later phase, for which a wait would run out.
+constexpr __host__ __device__ int first_in_flight(int issued, int stages) { return issued > stages ? issued - stages : 0; }
+
+constexpr bool waits_for_last_phases(int stages) {
+  for (int issued = 0; issued <= 5 * stages; ++issued)
+    for (int i = 0; i < issued; ++i) {
+      bool last = true;  // phase of its stage
+      for (int later = i + 1; later < issued; ++later) last = last && later % stages != i % stages;
+      if (last != (i >= first_in_flight(issued, stages))) return false;
+    }
+  return true;
+}
+static_assert(waits_for_last_phases(1) && waits_for_last_phases(2) && waits_for_last_phases(3) && waits_for_last_phases(4));
+
 // `bytes` (a multiple of 16, as both addresses) of global memory
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -318,7 +334,7 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
     if constexpr (NT == 2) fewer_registers();
     if (warp == NT * 4 && lane == 0 && blocks > 0) {
       // ---------------------------------------------------------------------------------- loads
-      int done = 0;
+      int nk = 0, nv = 0;
       bool ok = true;
       mbar_arrive_expect_tx(q_full, NT * Tile<DP>::kBytes);
 #pragma unroll
@@ -329,18 +345,16 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
         if (!bounded_wait(&k_empty[s], free_parity, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&k_full[s], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kK + s * Tile<DP>::kBytes, &tmK, &k_full[s], from + j * kRows, hk);
-        done = 2 * j + 1;
+        ++nk;
         if (!bounded_wait(&v_empty[s], free_parity, abort_flag, err)) { ok = false; break; }
         mbar_arrive_expect_tx(&v_full[s], Tile<DP>::kBytes);
         load_tile<DP>(smem + L::kV + s * Tile<DP>::kBytes, &tmV, &v_full[s], from + j * kRows, hk);
-        done = 2 * j + 2;
+        ++nv;
       }
       if (!ok) {  // copies in flight land before shared memory is given back
         mbar_wait(q_full, 0, nullptr, nullptr, 0);
-        for (int j = (done - 1) / 2; j >= 0 && j > (done - 1) / 2 - S - 1; --j) {
-          if (2 * j + 1 <= done) mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
-          if (2 * j + 2 <= done) mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
-        }
+        for (int j = first_in_flight(nk, S); j < nk; ++j) mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
+        for (int j = first_in_flight(nv, S); j < nv; ++j) mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, nullptr, 0);
       }
     } else if (warp == NT * 4 + 1) {
       // ------------------------------------------------------------------------------- products
@@ -785,8 +799,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) {
         mbar_wait(q_full, 0, nullptr, nullptr, 0);
-        for (int j = nk - 1; j >= 0 && j >= nk - KS; --j) mbar_wait(&k_full[j % KS], (j / KS) & 1, nullptr, nullptr, 0);
-        for (int j = nv - 1; j >= 0 && j >= nv - VS; --j) mbar_wait(&v_full[j % VS], (j / VS) & 1, nullptr, nullptr, 0);
+        for (int j = first_in_flight(nk, KS); j < nk; ++j) mbar_wait(&k_full[j % KS], (j / KS) & 1, nullptr, nullptr, 0);
+        for (int j = first_in_flight(nv, VS); j < nv; ++j) mbar_wait(&v_full[j % VS], (j / VS) & 1, nullptr, nullptr, 0);
       }
     } else if (warp == 9) {
       const bool one = elect_one();
@@ -1079,7 +1093,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) {
         mbar_wait(kv_full, 0, nullptr, nullptr, 0);
-        for (int i = done - 1; i >= 0 && i >= done - S; --i) mbar_wait(&q_full[i % S], (i / S) & 1, nullptr, nullptr, 0);
+        for (int i = first_in_flight(done, S); i < done; ++i) mbar_wait(&q_full[i % S], (i / S) & 1, nullptr, nullptr, 0);
       }
     } else if (warp == 9) {
       const bool one = elect_one();
