@@ -42,7 +42,7 @@ from ..common.attention import flash4_status, head_norms
 from ..common.batched_tokens import cat_keep_shapes, uncat_with_shapes
 from ..common.lora import apply_linear
 from ..common.rms_norm import RMSNorm
-from .rope import RopeTables
+from .rope import CropRopes, RopeTables, angles_end_to_end
 
 
 @contextlib.contextmanager
@@ -202,24 +202,16 @@ class SelfAttention(nn.Module):
         given = [isinstance(r, RopeTables) for r in rope_list]
         if not all(given):
             return all(r is None for r in rope_list)
-        return not any(r.angles.requires_grad for r in rope_list)
-
-    def _packed_angles(self, shapes: tuple[tuple[int, int], ...], rope_list) -> torch.Tensor:
-        """(sum of tokens, P) angles: 0 for prefix tokens, the same for every sample of a crop."""
-        kept = rope_list[0].packed
-        if shapes not in kept:
-            rows = []
-            for (b, n), rope in zip(shapes, rope_list, strict=True):
-                one = F.pad(rope.angles.float(), (0, 0, n - rope.angles.shape[-2], 0))
-                rows.append(one.expand(b, *one.shape).reshape(b * n, -1))
-            kept[shapes] = torch.cat(rows)
-        return kept[shapes]
+        return not any(r.angles.requires_grad or r.angles.dim() != 2 for r in rope_list)
 
     def _attend_packed(self, qkv: torch.Tensor, shapes: tuple[tuple[int, int], ...], rope_list) -> torch.Tensor:
         """(tokens, 3 C) projections of all crops -> (tokens, C)."""
         c = qkv.shape[-1] // 3
         q, k, v = qkv.reshape(qkv.shape[0], 3, self.num_heads, c // self.num_heads).unbind(1)
-        angles = self._packed_angles(shapes, rope_list) if rope_list[0] is not None else None
+        angles = None
+        if rope_list[0] is not None:
+            kept = isinstance(rope_list, CropRopes)
+            angles = rope_list.end_to_end(shapes) if kept else angles_end_to_end(rope_list, shapes)
         if self.q_norm is not None:
             qw, kw, eps = head_norms(self)
             pairs = self._pairs_on(qkv.device) if angles is not None else None

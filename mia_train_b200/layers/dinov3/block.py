@@ -23,7 +23,7 @@ from ..common.layer_scale import LayerScale
 from ..common.rms_norm import RMSNorm
 from .attention import SelfAttention
 from .ffn import Mlp, SwiGLUFFN
-from .rope import RopeTables
+from .rope import CropRopes, RopeTables
 
 
 def _norm(module: nn.Module, x: torch.Tensor) -> torch.Tensor:
@@ -99,7 +99,9 @@ class SelfAttentionBlock(nn.Module):
         scales = [b / s for b, s in zip(sizes, subsets, strict=True)]
         idx1 = [torch.randperm(b, device=x.device)[:s] for x, b, s in zip(x_list, sizes, subsets, strict=True)]
         sub1 = [x[i] for x, i in zip(x_list, idx1, strict=True)]
-        ropes = [self._maybe_index_rope(r, i) for r, i in zip(rope_list, idx1, strict=True)] if rope_list else rope_list
+        ropes = rope_list
+        if not isinstance(rope_list, CropRopes):  # those hold nothing per sample
+            ropes = [self._maybe_index_rope(r, i) for r, i in zip(rope_list, idx1, strict=True)] if rope_list else rope_list
         flat, shapes, counts = cat_keep_shapes(sub1)
         res1 = self.attn.forward_list(uncat_with_shapes(_norm(self.norm1, flat), shapes, counts), rope_list=ropes)
         x_attn = [

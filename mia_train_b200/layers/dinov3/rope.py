@@ -13,6 +13,7 @@ native attention consumes the angles directly as channel pairs (i, i + D_head / 
 from __future__ import annotations
 
 import math
+from collections.abc import Iterable, Sequence
 from typing import Literal
 
 import torch
@@ -30,14 +31,11 @@ class RopeTables:
     Not a tuple on purpose: FSDP rebuilds tuple forward arguments element by element (and may cast
     them), which would lose the angles; an object of this class passes through untouched."""
 
-    __slots__ = ("angles", "_pair", "packed")
+    __slots__ = ("angles", "_pair")
 
     def __init__(self, angles: torch.Tensor) -> None:
         self.angles = angles
         self._pair: tuple[torch.Tensor, torch.Tensor] | None = None
-        # angles of every token of a list of crops, by the crops' shapes: made by the first block that packs
-        # them and used by the others of this forward pass (the tables themselves are made anew in each)
-        self.packed: dict[tuple, torch.Tensor] = {}
 
     def _tables(self) -> tuple[torch.Tensor, torch.Tensor]:
         if self._pair is None:
@@ -53,6 +51,30 @@ class RopeTables:
 
     def __len__(self) -> int:
         return 2
+
+
+def angles_end_to_end(ropes: Sequence[RopeTables], shapes: tuple[tuple[int, int], ...]) -> torch.Tensor:
+    """(sum of tokens, P) fp32 angles of crops of `shapes` (samples, tokens): 0 for prefix tokens, the same for every
+    sample of a crop."""
+    rows = []
+    for (b, n), rope in zip(shapes, ropes, strict=True):
+        one = F.pad(rope.angles.float(), (0, 0, n - rope.angles.shape[-2], 0))
+        rows.append(one.expand(b, *one.shape).reshape(b * n, -1))
+    return torch.cat(rows)
+
+
+class CropRopes(list):
+    """The `RopeTables` of a list of crops as a model gives them to its blocks in one forward pass, made anew in each. The
+    first block that packs the crops has their angles laid end to end, the others use the same."""
+
+    def __init__(self, ropes: Iterable[RopeTables]) -> None:
+        super().__init__(ropes)
+        self._packed: dict[tuple, torch.Tensor] = {}
+
+    def end_to_end(self, shapes: tuple[tuple[int, int], ...]) -> torch.Tensor:
+        if shapes not in self._packed:
+            self._packed[shapes] = angles_end_to_end(self, shapes)
+        return self._packed[shapes]
 
 
 def _axis_coords(sizes: tuple[int, ...], mode: str, dtype, device) -> list[torch.Tensor]:

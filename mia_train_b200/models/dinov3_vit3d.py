@@ -36,7 +36,7 @@ from ..layers.dinov3.block import SelfAttentionBlock, _norm
 from ..layers.dinov3.config import dtype_dict, ffn_layer_dict, init_weights_vit, norm_layer_dict
 from ..layers.dinov3.ffn import SwiGLUFFN
 from ..layers.dinov3.patch_embed import PatchEmbed3D
-from ..layers.dinov3.rope import RopePositionEmbedding3D, RopePositionEmbedding3DSuperposition
+from ..layers.dinov3.rope import CropRopes, RopePositionEmbedding3D, RopePositionEmbedding3DSuperposition
 from ..utils.module_ops import named_apply
 from .base import BaseModel
 from .registry import ModelRegistry
@@ -233,13 +233,13 @@ class DinoVisionTransformer3D(BaseModel):
 
     def _run_blocks(self, tokens_list: list[torch.Tensor], grids: list[tuple[int, int, int]],
                     take: set[int] | None = None) -> tuple[list[torch.Tensor], list[list[torch.Tensor]]]:
-        shared = None if self._rope_augmented() else [self._rope(g) for g in grids]
+        shared = None if self._rope_augmented() else CropRopes(self._rope(g) for g in grids)
         sp = getattr(self, "_sequence_parallel", None)
         if sp is not None:
             return self._run_blocks_sequence_parallel(sp, tokens_list, grids, shared, take)
         taken: list[list[torch.Tensor]] = []
         for i, blk in enumerate(self.blocks):
-            ropes = shared if shared is not None else [self._rope(g) for g in grids]
+            ropes = shared if shared is not None else CropRopes(self._rope(g) for g in grids)
             if self.is_windowed(i):
                 tokens_list = [
                     self._windowed_block(blk, t, g, r) for t, g, r in zip(tokens_list, grids, ropes, strict=True)

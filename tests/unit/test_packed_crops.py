@@ -8,6 +8,8 @@ from copy import deepcopy
 import pytest
 import torch
 
+from mia_train_b200.layers.dinov3.attention import SelfAttention
+from mia_train_b200.layers.dinov3.rope import CropRopes, RopeTables
 from mia_train_b200.models.dinov3_vit import DinoVisionTransformer
 from mia_train_b200.models.dinov3_vit3d import DinoVisionTransformer3D
 from mia_train_b200.ops.packed_attention import PackedSequences
@@ -139,3 +141,39 @@ def test_channel_pairs_made_in_inference_mode_serve_training():
     with torch.inference_mode():
         model.forward_features([x.float() for x in _crops()], [None, None])
     assert not model.blocks[0].attn._pairs.is_inference()
+
+
+def test_angles_are_those_of_the_call():
+    """One rotation in several lists, or changed in place between two calls."""
+    torch.manual_seed(0)
+    attn = SelfAttention(48, num_heads=2).double()
+    attn.packed_crops = True
+    x = [torch.randn(2, 9, 48).double(), torch.randn(3, 5, 48).double()]
+    first, *second = (RopeTables(3 * torch.randn(n, 12)) for n in (8, 4, 4))
+
+    def check(ropes):
+        packed = attn.forward_list(x, rope_list=ropes)
+        for a, b in zip(packed, (attn(t, rope=r) for t, r in zip(x, ropes, strict=True)), strict=True):
+            _same(a, b)
+        return packed[1]
+
+    outs = [check([first, r]) for r in second]
+    second[1].angles.mul_(0.5)
+    outs.append(check([first, second[1]]))
+    outs.append(check(CropRopes([first, second[0]])))
+    assert torch.equal(outs[0], outs[3]) and not any(torch.equal(outs[0], y) for y in outs[1:3])
+    given = [RopeTables(torch.randn(b, n, 12)) for b, n in ((2, 9), (3, 5))]  # angles of every sample: crop by crop
+    check(given)
+
+
+@pytest.mark.parametrize("kw", [{}, {"drop_path_rate": 0.4}], ids=str)
+def test_the_blocks_of_a_forward_pass_share_their_angles(kw, monkeypatch):
+    from mia_train_b200.layers.dinov3 import rope as module
+
+    calls = []
+    real = module.angles_end_to_end
+    monkeypatch.setattr(module, "angles_end_to_end", lambda *a: calls.append(a[1]) or real(*a))
+    model = DinoVisionTransformer3D(img_size=16, packed_crops=True, **KW, **kw).train()
+    for n in (1, 2):
+        model.forward_features([x.float() for x in _crops()], [None, None])
+        assert len(calls) == n
