@@ -71,15 +71,15 @@ def top_logit_distillation_reference(student, values, indices, tau, teacher_tau,
     log_q = torch.log_softmax(torch.where(read, student.to(acc), 0.0) / tau, 1)
     t = torch.where(given, values.double(), -math.inf) / teacher_tau
     lse = torch.logsumexp(t, 1, keepdim=True) if teacher_lse is None else teacher_lse.double().unsqueeze(1)
-    p = torch.where(given & (t > -math.inf), (t - lse).exp(), 0.0)
-    some = p > 0
+    p = torch.where(given & (t != -math.inf), (t - lse).exp(), 0.0)
+    some = p != 0  # a NaN among them stays one
     log_p = torch.where(some, t - lse, 0.0)
     rows = torch.where(some, p * (log_p - log_q.gather(1, at).double()), 0.0).sum(1)
     if teacher_lse is not None:
         outside = torch.ones_like(log_q, dtype=torch.int32).scatter_reduce(1, at, (~given).int(), "amin") > 0
         rest = torch.where(outside.any(1), (1 - p.sum(1)).clamp(min=0), 0.0)
         others = torch.logsumexp(torch.where(outside, log_q, -math.inf), 1).double()
-        has = rest > 0
+        has = rest != 0
         rows = rows + torch.where(has, rest * (torch.where(has, rest, 1.0).log() - torch.where(has, others, 0.0)), 0.0)
     return (torch.where(read[:, 0], rows * w.double(), 0.0).sum() / norm).float()
 

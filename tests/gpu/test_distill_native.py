@@ -344,3 +344,20 @@ def test_distill_types_of_lse_and_weights(kind):
     _check_distill(s, values, indices, 1.0, 1.0, lse, w)
     both = torch.stack([lse, w], 1)  # strided
     _check_distill(s, values, indices, 1.0, 1.0, both[:, 0], both[:, 1])
+
+
+@pytest.mark.parametrize("where", ["value", "inf", "lse"])
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_teacher_that_is_not_finite_shows_in_the_loss(where, tail):
+    values = torch.tensor([[0.5, 0.0], [0.0, -1.0]], device=DEV)
+    lse = torch.tensor([1.0, 1.0], device=DEV) if tail else None
+    if where == "lse" and not tail:
+        return
+    if where == "lse":
+        lse[0] = math.nan
+    else:
+        values[0, 1] = math.nan if where == "value" else math.inf
+    s = _logits(2, 5, F32).requires_grad_(True)
+    loss = top_logit_distillation(s, values, torch.tensor([[0, 1], [2, 3]], device=DEV), teacher_lse=lse)
+    grad, = torch.autograd.grad(loss, s)
+    assert not loss.isfinite() and not grad[0].isfinite().any() and grad[1].isfinite().all()

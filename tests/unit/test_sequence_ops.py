@@ -270,3 +270,19 @@ def test_plans_made_in_inference_mode_serve_training():
         own = PackedSequences([5, 0, 3], [700, 2, 9], device="cpu")
     assert own.items is not None
     assert not any(t.is_inference() for t in (own.q_bounds, own.k_bounds, own.items, own.pieces))
+
+
+@pytest.mark.parametrize("where", ["value", "inf", "lse"])
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_teacher_that_is_not_finite_shows_in_the_loss(where, tail):
+    values, lse = torch.tensor([[0.5, 0.0], [0.0, -1.0]]), torch.tensor([1.0, 1.0]) if tail else None
+    if where == "lse" and not tail:
+        return
+    if where == "lse":
+        lse[0] = math.nan
+    else:
+        values[0, 1] = math.nan if where == "value" else math.inf
+    s = torch.randn(2, 5, requires_grad=True)
+    loss = top_logit_distillation(s, values, torch.tensor([[0, 1], [2, 3]]), teacher_lse=lse)
+    grad, = torch.autograd.grad(loss, s)
+    assert not loss.isfinite() and not grad[0].isfinite().any() and grad[1].isfinite().all()
