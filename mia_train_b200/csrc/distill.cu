@@ -15,8 +15,8 @@
 //   L   = sum_j p_j (log p_j - log q_{i_j}) [+ p_T (log p_T - log q_T)]
 //   dL/ds_i = (q_i S - p_i) / tau for the given classes, S = sum p_j (+ p_T);
 //             (q_i / q_T) (q_T S - p_T) / tau for the others  (q_i S / tau where there is no p_T).
-// The loss is sum_r w_r L_r / norm. A class named twice has the sum of its shares, an index outside the row is left
-// out, and a row of weight 0 is not read and gives zeros.
+// The loss is sum_r w_r L_r / norm. A class named twice has the sum of its shares in the gradient and both entries in the sum
+// of the loss, an index outside the row is left out, and a row of weight 0 is not read and gives zeros.
 //
 // What is normalised directly in the pass over the logits are the classes outside the teacher's (a bitmap in shared
 // memory tells them apart): a student that has nearly all its mass on the teacher's classes leaves a q_T that could

@@ -13,8 +13,10 @@ of a student (R, V) from the teacher's shares p of the classes `indices` (R, K),
   teacher_lse), and the classes that are not given count as one more, with the rest of 1 for p and the student's
   mass outside the given classes for q.
 
-An index outside 0 .. V - 1 is left out (lists of different lengths are filled up with -1), a class named twice has
-the sum of its shares, and a row of weight 0 is not read and gives zeros, whatever it holds. `norm` defaults to R.
+An index outside 0 .. V - 1 is left out (lists of different lengths are filled up with -1), and a row of weight 0 is not
+read and gives zeros, whatever it holds. `norm` defaults to R. A class that a row names twice has the sum of its shares in
+the gradient; the loss adds p_j log p_j entry by entry, as the formula has it, which is less than with both entries in
+one by a number that does not depend on the student (such a loss can be negative).
 The teacher and the weights get no gradient. A teacher logit of -inf has no share. Shares, their rest of 1 and the loss are
 computed in 64 bits; `values` and `teacher_lse` are taken as precise as they come, so a rest that is far below 1 needs them
 in fp64 (an fp32 lse of 20 moves it by 1e-6).

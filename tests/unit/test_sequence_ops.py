@@ -286,3 +286,20 @@ def test_a_teacher_that_is_not_finite_shows_in_the_loss(where, tail):
     loss = top_logit_distillation(s, values, torch.tensor([[0, 1], [2, 3]]), teacher_lse=lse)
     grad, = torch.autograd.grad(loss, s)
     assert not loss.isfinite() and not grad[0].isfinite().any() and grad[1].isfinite().all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_class_named_twice(tail):
+    """The gradient of one entry with both shares; the loss of two, less by sum p_j log(P / p_j)."""
+    torch.manual_seed(0)
+    s = torch.randn(1, 6, requires_grad=True)
+    values, indices = torch.tensor([[0.3, 0.3, -0.2]]), torch.tensor([[4, 4, 1]])
+    lse = torch.tensor([1.6]) if tail else None
+    twice = top_logit_distillation(s, values, indices, teacher_lse=lse)
+    once = top_logit_distillation(s, torch.tensor([[0.3 + math.log(2), -0.2]]), indices[:, 1:], teacher_lse=lse)
+    base = 1.6 if tail else math.log(2 * math.exp(0.3) + math.exp(-0.2))
+    assert twice.item() == pytest.approx(once.item() - 2 * math.exp(0.3 - base) * math.log(2), abs=1e-6)
+    grads = [torch.autograd.grad(x, s)[0] for x in (twice, once)]
+    assert torch.allclose(*grads, atol=1e-7)
+    sure = top_logit_distillation(torch.tensor([[50.0, 0.0, 0.0]]), torch.zeros(1, 2), torch.zeros(1, 2, dtype=torch.int64))
+    assert sure.item() == pytest.approx(-math.log(2))
