@@ -33,12 +33,19 @@ from ._native import native, use_native
 MAX_TOP = 256
 MAX_GIVEN = 1024
 MAX_CLASSES = 1 << 20  # a bit for every class fits the shared memory of a block
+TAUS = 1e-28, 1e28  # log2(e) / tau and what fp32 leaves of it are fp32 numbers
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _positive(value: float, name: str) -> float:
     if not (math.isfinite(value) and value > 0):
         raise ValueError(f"{name} must be positive and finite, got {value}")
+    return float(value)
+
+
+def _temperature(value: float, name: str) -> float:
+    if not TAUS[0] <= value <= TAUS[1]:
+        raise ValueError(f"{name} must be within {TAUS[0]} .. {TAUS[1]}, got {value}")
     return float(value)
 
 
@@ -55,7 +62,7 @@ def top_logits(logits: torch.Tensor, k: int, *, tau: float = 1.0) -> tuple[torch
         raise ValueError(f"logits must be a floating-point (R, V), got {logits.dtype} {tuple(logits.shape)}")
     if not 1 <= k <= min(MAX_TOP, logits.shape[1]):
         raise ValueError(f"k must be in 1 .. {min(MAX_TOP, logits.shape[1])}, got {k}")
-    _positive(tau, "tau")
+    _temperature(tau, "tau")
     if use_native(logits):
         if logits.dtype not in _DTYPES or logits.shape[1] >= 2**31 - 1024 or logits.shape[0] >= 2**31:
             raise ValueError(f"on CUDA, top_logits takes bf16, fp16 and fp32, got {logits.dtype} {tuple(logits.shape)}")
@@ -112,7 +119,7 @@ def top_logit_distillation(
     for name, x in (("values", values), ("indices", indices), ("teacher_lse", teacher_lse), ("weights", weights)):
         if x is not None and x.device != student.device:
             raise ValueError(f"student is on {student.device}, {name} on {x.device}")
-    tau, teacher_tau = _positive(tau, "tau"), _positive(teacher_tau, "teacher_tau")
+    tau, teacher_tau = _temperature(tau, "tau"), _temperature(teacher_tau, "teacher_tau")
     norm = _positive(float(max(r, 1)) if norm is None else float(norm), "norm")
     values, teacher_lse, weights = (x.detach() if x is not None else None for x in (values, teacher_lse, weights))
     if use_native(student):

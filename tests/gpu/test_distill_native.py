@@ -361,3 +361,26 @@ def test_a_teacher_that_is_not_finite_shows_in_the_loss(where, tail):
     loss = top_logit_distillation(s, values, torch.tensor([[0, 1], [2, 3]], device=DEV), teacher_lse=lse)
     grad, = torch.autograd.grad(loss, s)
     assert not loss.isfinite() and not grad[0].isfinite().any() and grad[1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau", [1e-28, 1e-10, 1e10, 1e28])
+def test_temperatures_at_the_ends_of_their_range(tau, dtype):
+    """Where one logit stands for all, and where all are the same; logits of -inf have no share in either."""
+    x = _logits(3, 1001, dtype)
+    x[1, 5:900] = -math.inf
+    x[2] = -math.inf
+    x[2, 77] = 0.5
+    values, indices, lse = top_logits(x, 3, tau=tau)
+    want = torch.logsumexp(x.double() / tau, 1)
+    top = (x.double() / tau).amax(1).abs()
+    # as in _check_top; the sum itself is rounded to fp32
+    assert ((lse.double() - want).abs() <= 2.0**-17 + 2.0**-22 * top).all()
+    leaf = x.requires_grad_(True)
+    loss = top_logit_distillation(leaf, values[:, :1], indices[:, :1], tau=tau)
+    grad, = torch.autograd.grad(loss, leaf)
+    # -log of the largest logit's probability: 0 where it stands for all, log of the number of others where all are the same
+    count = torch.isfinite(x.detach()).sum(1).double()
+    rows = torch.log(count) if tau > 1 else torch.zeros_like(count)
+    assert (loss.double() - rows.mean()).abs() <= 2.0**-16
+    assert grad.isfinite().all() and (grad[2] == 0).all()

@@ -303,3 +303,12 @@ def test_a_class_named_twice(tail):
     assert torch.allclose(*grads, atol=1e-7)
     sure = top_logit_distillation(torch.tensor([[50.0, 0.0, 0.0]]), torch.zeros(1, 2), torch.zeros(1, 2, dtype=torch.int64))
     assert sure.item() == pytest.approx(-math.log(2))
+
+
+@pytest.mark.parametrize("tau", [0.0, -1.0, math.nan, math.inf, 9e-29, 1.1e28])
+def test_temperatures_that_are_refused(tau):
+    s, values, indices = torch.randn(3, 6), torch.randn(3, 2), torch.zeros(3, 2, dtype=torch.int64)
+    for bad in (lambda: top_logits(s, 2, tau=tau), lambda: top_logit_distillation(s, values, indices, tau=tau),
+                lambda: top_logit_distillation(s, values, indices, teacher_tau=tau)):
+        with pytest.raises(ValueError, match="tau must be within"):
+            bad()
