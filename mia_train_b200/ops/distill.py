@@ -108,6 +108,8 @@ def top_logit_distillation(
     if student.dim() != 2 or student.shape[1] == 0 or not student.is_floating_point():
         raise ValueError(f"student must be a floating-point (R, V), got {student.dtype} {tuple(student.shape)}")
     r, v = student.shape
+    if r >= 2**31:
+        raise ValueError(f"at most {2**31 - 1} rows, got {r}")
     if values.dim() != 2 or values.shape != indices.shape or values.shape[0] != r or not 1 <= values.shape[1] <= MAX_GIVEN:
         raise ValueError(f"values and indices must be ({r}, 1 .. {MAX_GIVEN}), got {tuple(values.shape)} and "
                          f"{tuple(indices.shape)}")

@@ -116,6 +116,8 @@ def rotary(
                          f"{q.device} and {k.dtype} {tuple(k.shape)} on {k.device}")
     batched = q.dim() == 4
     b, t, hq, d = q.shape if batched else (1, *q.shape)
+    if t >= 2**31:
+        raise ValueError(f"at most {2**31 - 1} tokens in a row of the batch, got {t}")
     if frequencies is None:
         if positions.dim() not in (2, 3) or positions.dtype != torch.float32:
             raise ValueError(f"angles must be fp32 (T, P) or (B, T, P), got {positions.dtype} {tuple(positions.shape)}")

@@ -312,3 +312,12 @@ def test_temperatures_that_are_refused(tau):
                 lambda: top_logit_distillation(s, values, indices, teacher_tau=tau)):
         with pytest.raises(ValueError, match="tau must be within"):
             bad()
+
+
+def test_more_tokens_or_rows_than_a_kernel_counts_are_refused():
+    many = 2**31
+    q, one = torch.zeros(1, 1, 8).expand(many, 1, 8), torch.zeros(1, 1).expand(many, 1)
+    with pytest.raises(ValueError, match="tokens"):
+        rotary(q, None, torch.zeros(1, dtype=torch.int32).expand(many), torch.ones(4))
+    with pytest.raises(ValueError, match="rows"):
+        top_logit_distillation(one, one, torch.zeros(1, 1, dtype=torch.int32).expand(many, 1))
