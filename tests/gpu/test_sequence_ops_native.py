@@ -123,3 +123,28 @@ def test_blocks_train_after_an_evaluation_in_inference_mode(packed, qk_norm):
         out = model.forward_features(crops, [None, None])
         sum(o["x_norm_patchtokens"].float().sin().mean() for o in out).backward()
     assert model.blocks[0].attn.qkv.weight.grad.isfinite().all()
+
+
+def test_saved_tensors_may_go_through_hooks():
+    """Kept on the host between the passes (save_on_cpu), where strided views come back contiguous: the same bits."""
+    torch.manual_seed(0)
+    lengths, hq, hk, d = [130, 40, 1], 4, 2, 64
+    t = sum(lengths)
+    base = torch.randn(t, hq + 2 * hk, d, device=DEV).half()
+    freq = torch.rand(3, 16, device=DEV)
+    positions = torch.randn(t, 3, device=DEV)
+    seq = PackedSequences(lengths, causal=True, device=DEV)
+    wide = torch.randn(t, 2 * 300, device=DEV)
+    values, indices, lse = top_logits(torch.randn(t, 300, device=DEV), 8)
+
+    def step():
+        x, f, s = (y.detach().clone().requires_grad_(True) for y in (base, freq, wide))
+        q, k = rotary(x[:, :hq], x[:, hq:hq + hk], positions, f)
+        o = packed_attention(q, k, x[:, hq + hk:], seq)
+        loss = top_logit_distillation(s[:, ::2], values, indices, teacher_lse=lse)
+        return torch.autograd.grad(o.float().sin().sum() + top_logit_distillation(s[:, 300:], values, indices) + loss, (x, f, s))
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
