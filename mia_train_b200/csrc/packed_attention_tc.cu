@@ -252,10 +252,8 @@ struct FwdLayout {
   static constexpr int kK = kQ + NT * Tile<DP>::kBytes;
   static constexpr int kV = kK + kStages * Tile<DP>::kBytes;
   static constexpr int kBar = kV + kStages * Tile<DP>::kBytes;
-  // Where rows are computed again: a single tile is through with K by then; of two the other one may still load and read it.
-  static constexpr int kOwnScratch = kBar + 256;
-  static constexpr int kScratch = NT == 1 ? kK : kOwnScratch;
-  static constexpr int kBytes = kOwnScratch + (NT == 1 ? 0 : NT * 4 * kRowScratch * 4) + 1024;
+  static constexpr int kBytes = kBar + 256 + 1024;
+  static_assert(4 * kRowScratch * 4 <= Tile<DP>::kBytes, "a tile's four warps have their scratch in its queries' place");
   static constexpr int kThreads = NT == 2 ? 384 : 192;
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
   static constexpr bool kApart = DP == 64;  // P next to S instead of over it
@@ -550,7 +548,9 @@ __global__ void __launch_bounds__(NT == 2 ? 384 : 192, NT == 1 ? 2 : 1)
       uint32_t again = __ballot_sync(0xffffffffu, real && partly && bad != bad && inv == inv);
       if (again != 0) {
         __syncwarp();
-        float* scratch = reinterpret_cast<float*>(smem + L::kScratch) + warp * kRowScratch;
+        // in the place of this tile's queries: its last scores are done, and no load and no other tile comes there (K and V
+        // may still be loaded and read for the block's other tile)
+        float* scratch = reinterpret_cast<float*>(smem + L::kQ + t * Tile<DP>::kBytes) + (warp % 4) * kRowScratch;
         while (again != 0) {
           const int who = __ffs(again) - 1;
           again &= again - 1;
