@@ -25,7 +25,7 @@
 #include <type_traits>
 
 #include "pair_math.cuh"
-#include "sequence_kernels.h"
+#include "sequence_types.cuh"
 #include "vec8.cuh"
 
 namespace mia {
@@ -38,12 +38,6 @@ constexpr int kMany = 256, kFew = 512;
 int threads_for(int rows, int classes) { return rows < 2 * 148 && classes >= 16384 ? kFew : kMany; }
 
 constexpr int kCandidates = 2048;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Calls f(index, values) for the row's elements, eight aligned ones at a time, and f(index, value) for those at both ends.
 template <int NT, typename T, typename F>
@@ -111,15 +105,15 @@ struct Soft {
   float m = -INFINITY, l = 0.f;
   __device__ __forceinline__ void add(float s, Rate c) {
     if (s > m) {
-      l *= m == -INFINITY ? 0.f : ex2(c(m - s));
+      l *= m == -INFINITY ? 0.f : exp2_approx(c(m - s));
       m = s;
     }
-    l += s == -INFINITY ? 0.f : ex2(c(s - m));
+    l += s == -INFINITY ? 0.f : exp2_approx(c(s - m));
   }
   // `top` is the largest of the eight, or NaN
   __device__ __forceinline__ void add8(const float (&v)[8], float top, Rate c) {
     if (top > m) {
-      l *= m == -INFINITY ? 0.f : ex2(c(m - top));
+      l *= m == -INFINITY ? 0.f : exp2_approx(c(m - top));
       m = top;
     }
     // with m = -inf (all of them, or NaN next to them) the differences would be NaN: 0 stands in for m, the terms of
@@ -131,7 +125,7 @@ struct Soft {
     for (int e = 0; e < 8; e += 2) {
       float a, b;
       split(c(add2(pair_of(v[e], v[e + 1]), ref2)), a, b);
-      sum = add2(sum, pair_of(ex2(a), ex2(b)));
+      sum = add2(sum, pair_of(exp2_approx(a), exp2_approx(b)));
     }
     float a, b;
     split(sum, a, b);
@@ -140,7 +134,7 @@ struct Soft {
   __device__ __forceinline__ void join(float m2, float l2, Rate c) {
     const float top = fmaxf(m, m2);
     const float ref = top == -INFINITY ? 0.f : top;
-    l = l * ex2(c(m - ref)) + l2 * ex2(c(m2 - ref));
+    l = l * exp2_approx(c(m - ref)) + l2 * exp2_approx(c(m2 - ref));
     m = top;
   }
 };
@@ -504,17 +498,17 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
       for (int e = 0; e < 8; e += 2) {
         float a, b;
         split(c(add2(pair_of(v[e], v[e + 1]), ref2)), a, b);
-        split(mul2(pair_of(ex2(a), ex2(b)), coef2), v[e], v[e + 1]);
+        split(mul2(pair_of(exp2_approx(a), exp2_approx(b)), coef2), v[e], v[e + 1]);
       }
       store8<T>(out + vec_ahead + i * 8, v);
     }
     const int end = vec_ahead + vecs * 8;
     for (int i = threadIdx.x; i < vec_ahead + (p.V - end); i += NT) {
       const int at = i < vec_ahead ? i : end + i - vec_ahead;
-      out[at] = from_f32<T>(ex2(c(to_f32(row[at]) - ref)) * coef);
+      out[at] = from_f32<T>(exp2_approx(c(to_f32(row[at]) - ref)) * coef);
     }
   } else {
-    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(ex2(c(to_f32(row[i]) - ref)) * coef);
+    for (int i = threadIdx.x; i < p.V; i += NT) out[i] = from_f32<T>(exp2_approx(c(to_f32(row[i]) - ref)) * coef);
   }
   __syncthreads();  // the given classes replace what the pass wrote in their places
   const double inv_l = 1.0 / st[kAllL], all_m = st[kAllM], mass = st[kMass];
@@ -532,13 +526,6 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(DistillParams p, const 
     const double q = exp(((double)to_f32(row[at]) - all_m) * inv_tau) * inv_l;
     out[at] = from_f32<T>((float)(scale * (q * mass - share)));
   }
-}
-
-template <typename F>
-void by_type(SequenceType type, F&& f) {
-  if (type == kSeqBf16) f((__nv_bfloat16*)nullptr);
-  else if (type == kSeqF16) f((__half*)nullptr);
-  else f((float*)nullptr);
 }
 
 }  // namespace

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "packed_attention.h"
+#include "sequence_types.cuh"
 
 namespace mia {
 namespace {
@@ -272,13 +273,6 @@ __global__ void __launch_bounds__(128) packed_few_join_kernel(PackedProblem P, P
 int64_t blocks_of(int64_t items, int per) { return (items + per - 1) / per; }
 unsigned grid_of(int64_t items, int per) { return (unsigned)blocks_of(items, per); }
 
-template <typename F>
-void by_type(SequenceType type, F&& f) {
-  if (type == kSeqBf16) f((__nv_bfloat16*)nullptr);
-  else if (type == kSeqF16) f((__half*)nullptr);
-  else f((float*)nullptr);
-}
-
 }  // namespace
 
 cudaError_t packed_fwd_rows(const PackedProblem& P, void* o, float* lse, cudaStream_t stream) {
@@ -311,15 +305,11 @@ cudaError_t packed_bwd_rows(const PackedProblem& P, const void* o, const void* d
   by_type(P.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const T* go = (const T*)dout;
-    if (P.Tq > 0) {
-      packed_delta_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, 8), 256, 0, stream>>>(
-          (const T*)o, (const T*)P.o_low, go, ds, P.Tq, P.Hq, P.D, P.lse_stride, delta);
-      packed_dq_rows_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, kWarps), kWarps * 32, 0, stream>>>(P, go, ds, lse, delta,
-                                                                                                 (T*)dq);
-    }
-    if (P.Tk > 0)
-      packed_dkv_rows_kernel<T><<<grid_of((int64_t)P.Tk * P.Hk, kWarps), kWarps * 32, 0, stream>>>(
-          P, go, ds, lse, delta, (T*)dk, (T*)dv);
+    packed_delta_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, 8), 256, 0, stream>>>(
+        (const T*)o, (const T*)P.o_low, go, ds, P.Tq, P.Hq, P.D, P.lse_stride, delta);
+    packed_dq_rows_kernel<T><<<grid_of((int64_t)P.Tq * P.Hq, kWarps), kWarps * 32, 0, stream>>>(P, go, ds, lse, delta, (T*)dq);
+    packed_dkv_rows_kernel<T><<<grid_of((int64_t)P.Tk * P.Hk, kWarps), kWarps * 32, 0, stream>>>(P, go, ds, lse, delta, (T*)dk,
+                                                                                               (T*)dv);
   });
   return cudaGetLastError();
 }

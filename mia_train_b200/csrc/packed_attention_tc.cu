@@ -102,13 +102,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// exp2 of the multi-function unit: relative error 2^-22, far below the rounding of P; results under 2^-126 are 0.
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // max of three; NaN if any is
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
@@ -1390,13 +1383,12 @@ cudaError_t fwd(const PackedProblem& P, void* o, float* lse, int* err, cudaStrea
   CUtensorMap q, k, v;
   const cudaError_t ready = context_current();
   if (ready != cudaSuccess) return ready;
-  const int keys = P.Tk > 0 ? P.Tk : 1;  // without a key nothing is read
-  if (!map_rows(&q, P.q, P.qs, P.Tq, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, keys, P.Hk, P.D, P.type) ||
-      !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type))
+  if (!map_rows(&q, P.q, P.qs, P.Tq, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, P.Tk, P.Hk, P.D, P.type) ||
+      !map_rows(&v, P.v, P.vs, P.Tk, P.Hk, P.D, P.type))
     return cudaErrorInvalidValue;
   const int64_t pairs = (int64_t)((P.Tq + 2 * kRows - 1) / (2 * kRows)) * P.Hq;
   // Heads of up to 64 channels: a tile a CTA and two CTAs an SM, whose softmax fall into turns by themselves (4 x 4101
-  // tokens, 16 heads of 64: 437 us against 492 with two tiles in one CTA, which run in step). Wider heads have room for
+  // tokens, 16 heads of 64: 446 us; 492 with two tiles in one CTA, which ran in step, when one a CTA took 437). Wider heads have room for
   // one CTA, with two tiles that share the loads of K and V unless that would leave SMs without work.
   if constexpr (DP == 128) if (pairs >= 148)
     return launch(packed_fwd_tc_kernel<T, DP, 2>, pairs, FwdLayout<DP, 2>::kThreads, FwdLayout<DP, 2>::kBytes, stream, q,
@@ -1411,23 +1403,19 @@ cudaError_t bwd(const PackedProblem& P, const void* o, const void* dout, HeadRow
   CUtensorMap q, k, v, g;
   const cudaError_t ready = context_current();
   if (ready != cudaSuccess) return ready;
-  const int keys = P.Tk > 0 ? P.Tk : 1, queries = P.Tq > 0 ? P.Tq : 1;
-  if (!map_rows(&q, P.q, P.qs, queries, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, keys, P.Hk, P.D, P.type) ||
-      !map_rows(&v, P.v, P.vs, keys, P.Hk, P.D, P.type) || !map_rows(&g, dout, ds, queries, P.Hq, P.D, P.type))
+  if (!map_rows(&q, P.q, P.qs, P.Tq, P.Hq, P.D, P.type) || !map_rows(&k, P.k, P.ks, P.Tk, P.Hk, P.D, P.type) ||
+      !map_rows(&v, P.v, P.vs, P.Tk, P.Hk, P.D, P.type) || !map_rows(&g, dout, ds, P.Tq, P.Hq, P.D, P.type))
     return cudaErrorInvalidValue;
   const int64_t q_tiles = ((int64_t)P.Tq + kRows - 1) / kRows, k_tiles = ((int64_t)P.Tk + kRows - 1) / kRows;
   if (q_tiles * P.Hq > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (q_tiles > 0) {
-    packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>(
-        (const T*)o, (const T*)P.o_low, (const T*)dout, ds, P.Tq, P.Hq, P.D, P.lse_stride, lse, 1.f / (P.scale * kLog2e), delta,
-        (uint4*)channels, norms);
-    cudaError_t status = cudaGetLastError();
-    if (status != cudaSuccess) return status;
-    status = launch(packed_dq_tc_kernel<T, DP>, q_tiles * P.Hq, kBwdThreads, DqLayout<DP>::kBytes, stream, q, k, v, g, P,
-                    (const T*)dout, ds, lse, (const float*)delta, (const float*)norms, (T*)dq, err);
-    if (status != cudaSuccess) return status;
-  }
-  if (k_tiles == 0) return cudaSuccess;
+  packed_delta_tc_kernel<T><<<(unsigned)(q_tiles * P.Hq), 256, 0, stream>>>(
+      (const T*)o, (const T*)P.o_low, (const T*)dout, ds, P.Tq, P.Hq, P.D, P.lse_stride, lse, 1.f / (P.scale * kLog2e), delta,
+      (uint4*)channels, norms);
+  cudaError_t status = cudaGetLastError();
+  if (status != cudaSuccess) return status;
+  status = launch(packed_dq_tc_kernel<T, DP>, q_tiles * P.Hq, kBwdThreads, DqLayout<DP>::kBytes, stream, q, k, v, g, P,
+                  (const T*)dout, ds, lse, (const float*)delta, (const float*)norms, (T*)dq, err);
+  if (status != cudaSuccess) return status;
   return launch(packed_dkv_tc_kernel<T, DP>, k_tiles * P.Hk, kBwdThreads, DkvLayout<DP>::kBytes, stream, q, k, v, g, P,
                 (const T*)dout, ds, lse, (const float*)delta, (const uint4*)channels, (const float*)norms, (T*)dk, (T*)dv, err);
 }

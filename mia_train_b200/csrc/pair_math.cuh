@@ -1,4 +1,4 @@
-// Arithmetic on two fp32 values at a time: one issue slot for both on sm_100.
+// Arithmetic on two fp32 values at a time (one issue slot for both on sm_100), and exp2 of the multi-function unit.
 #pragma once
 
 namespace mia {
@@ -25,6 +25,13 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// Relative error 2^-22; results under 2^-126 are 0.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 }  // namespace mia
