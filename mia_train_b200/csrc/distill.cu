@@ -3,10 +3,11 @@
 // Top logits of a row: the k largest, largest first, equal ones by the lower index, and logsumexp(x / tau). A NaN
 // counts as larger than every number. One block owns a row. Pass 1 reads it once: running maximum and sum of the
 // log-sum-exp, and the largest value of each of 512 (or 1024) interleaved groups. The k-th largest of those group maxima is a
-// value that at least k elements reach, and few more do (65536 normal values and k = 64: about 66). Pass 2 finds the
-// row in L2 and collects what reaches it; every candidate then counts how many come before it. A row in which too
-// many elements are equal takes the exact k-th value by bisection over the bits instead, and its ties in order of
-// their index.
+// value that at least k elements reach, and few more do (65536 normal values and k = 64: about 66). Pass 2 reads the
+// row again, from L2 where the rows under way fit there (888 bf16 rows of 65536 are 116 MB, fp32 rows twice that), and
+// collects what reaches it; every candidate then counts how many come before it. A row in which too many elements are
+// equal takes the exact k-th value by bisection over the bits instead, 32 more passes, and its ties in order of their index
+// (1229 x 65536 bf16 logits within a few steps of each other: 1.3 ms; 69 us where they differ).
 //
 // Distillation: with the teacher's values t_j at classes i_j,
 //   p_j = exp(t_j / tau_t - lse_t), lse_t = logsumexp over the given classes, or over all of the teacher's (given):

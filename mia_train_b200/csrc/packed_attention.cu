@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kWarps * 32) packed_dkv_rows_kernel(PackedProb
 // masked, and there are fewer tiles than SMs. Here a CTA takes up to R rows (queries and heads that share a key head)
 // of one sequence and a piece of its keys, and the pieces' sums are joined by a second kernel. It is bound by reading
 // K and V: LP lanes hold a row's channels, eight each, and a warp has eight 16-byte loads of K and of V a lane under way.
-// 16 sequences of 1029 .. 4101 keys, one query, 16 heads of 64 fp16: 805 us by tiles, 47 us here (39 us at 5.6 TB/s and 7 us for joining).
+// 16 sequences of 1029 .. 4101 keys, one query, 16 heads of 64 fp16: 805 us by tiles, 46 us here (40 us at 5.4 TB/s and 6 us for joining).
 constexpr int kFewThreads = 128;
 
 template <typename T>

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, kLearn ? 2 : 3) rotary_kernel(const 
       }
       if (h0 == h_begin && rotates) {
         // While the first loads are under way. By way of shared memory, so that the code of one angle is there once:
-        // fetching eight copies took longer than a small call's work (6.1 us against 3.0 for nine tokens).
+        // fetching eight copies took longer than a small call's work (3 us more for nine tokens, which take 5).
         float2* mine = angles + threadIdx.x;
 #pragma unroll 1
         for (int e = 0; e < kPairs; ++e) mine[e * kThreads] = turn(p, table, at, v * kPairs + e);

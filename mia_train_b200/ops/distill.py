@@ -1,8 +1,8 @@
 """Distillation from a teacher of which only every row's top logits are kept.
 
 `top_logits(logits, k, tau)` gives the k largest logits of every row (largest first, equal ones by the lower index;
-a NaN counts as larger than every number), their classes (int64) and logsumexp(logits / tau) in fp32, in one pass
-over the logits. `top_logit_distillation(student, values, indices, ...)` is the Kullback-Leibler divergence
+a NaN counts as larger than every number), their classes (int64) and logsumexp(logits / tau) in fp32, in one
+kernel that sorts no row. `top_logit_distillation(student, values, indices, ...)` is the Kullback-Leibler divergence
 
     sum_r weights_r * sum_j p_rj (log p_rj - log q_rj) / norm,    q = softmax(student / tau)
 

@@ -8,7 +8,8 @@ less: query i of Lq sees the keys j <= i + Lk - Lq of Lk. A query that sees no k
 the gradients, and so do rows behind the last sequence, which are not read. A query whose scores are all -inf is 0 / 0: NaN.
 
 On CUDA in bf16 and fp16 with D % 8 == 0 and D <= 128 this is the native kernel, in fp32 a native kernel without
-tensor cores; statistics and sums are held in fp32. The probabilities and their gradients are rounded to the inputs'
+tensor cores, a warp per row, for checks and small problems (2 x 1029 tokens, 16 heads of 64: 3.2 ms forward, 10.3 ms
+backward); statistics and sums are held in fp32. The probabilities and their gradients are rounded to the inputs'
 type on their way into the second matrix products; what rounding takes from the output is kept for the backward pass (a
 second tensor of its size). Sums have a fixed order: the same inputs give the same bits. What a
 sequence holds reaches no other sequence's results, not even an infinity or NaN. On the CPU it is PyTorch math,

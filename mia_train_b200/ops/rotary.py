@@ -12,6 +12,8 @@ with the pairs (p, p + P) for `layout="half"` and (2 p, 2 p + 1) for `"interleav
 fp32 (T, P) or (B, T, P). Angles are reduced to a turn with at least 48 bits, of integer positions with 53, so that
 those of far positions are as good as of near ones; the rest is fp32, rounded once. q and k may be strided views of a packed projection;
 the outputs share one contiguous buffer. `k` may be None. Gradients go to q, k and the frequencies, not to positions or angles.
+A frequency that is not finite makes its pairs NaN. On CUDA bf16, fp16 and fp32 heads of up to 256 channels are rotated by
+the native kernel, other types and wider heads by PyTorch math, as everything on the CPU.
 
 `rotary_frequencies(rotary_dim, base, scaling=...)` gives the frequencies base^(-p / P) in fp64 and the amplitude:
 
