@@ -985,7 +985,7 @@ template <int DP>
 struct DkvLayout {
   static constexpr bool kTurns = DP == 64;
   static constexpr int kStages = kTurns ? 4 : 2;
-  static constexpr uint32_t kX = 0, kXStep = kTurns ? 192 : 0, kP = 128, kDS = kTurns ? 0 : 192;  // columns
+  static constexpr uint32_t kXStep = kTurns ? 192 : 0, kP = 128, kDS = kTurns ? 0 : 192;  // columns
   static constexpr uint32_t kDV = kTurns ? 384 : 256, kDK = kDV + DP;
   static constexpr int kK = 0;
   static constexpr int kV = kK + Tile<DP>::kBytes;
@@ -1389,7 +1389,8 @@ cudaError_t fwd(const PackedProblem& P, void* o, float* lse, int* err, cudaStrea
   const int64_t pairs = (int64_t)((P.Tq + 2 * kRows - 1) / (2 * kRows)) * P.Hq;
   // Heads of up to 64 channels: a tile a CTA and two CTAs an SM, whose softmax fall into turns by themselves (4 x 4101
   // tokens, 16 heads of 64: 446 us; 492 with two tiles in one CTA, which ran in step, when one a CTA took 437). Wider heads have room for
-  // one CTA, with two tiles that share the loads of K and V unless that would leave SMs without work.
+  // one CTA, with two tiles that share the loads of K and V unless that would leave SMs without work (heads of 128, one tile a
+  // CTA against two: 38 and 41 us at 64 pairs, 72 and 44 at 128, 104 and 80 at 160, 248 and 147 at 256).
   if constexpr (DP == 128) if (pairs >= 148)
     return launch(packed_fwd_tc_kernel<T, DP, 2>, pairs, FwdLayout<DP, 2>::kThreads, FwdLayout<DP, 2>::kBytes, stream, q,
                   k, v, P, (T*)o, lse, err);
